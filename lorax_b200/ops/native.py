@@ -121,6 +121,8 @@ def load() -> ctypes.CDLL:
     }
     from . import native_mixers
     sigs.update(native_mixers.SIGNATURES)
+    from . import native_steps
+    sigs.update(native_steps.SIGNATURES)
     for name, (argtypes, restype) in sigs.items():
         fn = getattr(lib, name, None)
         if fn is None:
@@ -130,6 +132,7 @@ def load() -> ctypes.CDLL:
         fn.argtypes = argtypes
         fn.restype = restype
     native_mixers.check_layouts(lib)
+    native_steps.check_limits(lib)
     for name, st in (("lx_moe_select_bytes", MoeSelectParams), ("lx_moe_place_bytes", MoePlaceParams)):
         if getattr(lib, name)() != ctypes.sizeof(st):
             raise NativeError(f"{name}: C++ says {getattr(lib, name)()} bytes, ctypes says {ctypes.sizeof(st)}")
@@ -846,12 +849,15 @@ from .native_mixers import (causal_conv, conv_rope_kvwrite, embed_stream, gate_n
                             latent_attn, latent_prefill, latent_prep, linear_attn, norm_add, norm_gate, norm_stream, qk_norm_kvwrite, rope_pairs,
                             ssd, tanh_, token_shift, wkv)
 
+# ------------------------------------------------------------------------------------------------ short ragged steps
+from .native_steps import moe_few, step_tables, token_scores  # noqa: E402
+
 # ------------------------------------------------------------------------------------------------ per-op timing
 _TIMED_OPS = ("gemm", "gemm_fp8", "norm_residual", "rope_kvwrite", "act_mul", "embed", "argmax_logprob", "advance_decode", "attn_decode",
               "attn_prefill", "lora_shrink", "lora_expand", "lora_shrink_tiles", "lora_expand_tiles",
               "embed_stream", "norm_stream", "norm_gate", "tanh_", "gemm_heads", "linear_attn", "wkv", "token_shift", "latent_prep", "rope_pairs",
               "latent_attn", "latent_prefill", "norm_add", "qk_norm_kvwrite", "conv_rope_kvwrite", "causal_conv", "ssd",
-              "gate_norm", "gqa_attn", "moe_route", "moe_grouped_gemm", "moe_combine")
+              "gate_norm", "gqa_attn", "moe_route", "moe_grouped_gemm", "moe_combine", "step_tables", "moe_few", "token_scores")
 _timing_records = None
 _timing_originals = {}
 

@@ -978,3 +978,166 @@ def moe_grouped_gemm(xg, w, seg, avg_rows: int, out=None, shared: int = 0, token
         z = xg[s[e] - back: s[e + 1] - back].float() @ w[e].float().t()
         y[s[e]: s[e + 1]] = (F.silu(z[:, 0::2]) * z[:, 1::2] if act == "swiglu" else _act(z, act) if act else z).to(xg.dtype)
     return y
+
+
+# ------------------------------------------------------------------------------------------------ short ragged steps
+MOE_FEW_TOKENS = 16         # tokens that `moe_few` takes at most
+TOP_MAX = 32                # alternatives that `token_scores` returns at most
+STEP_SEQS_MAX = 4096        # sequences of `step_tables`
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise ValueError(what)
+
+
+class StepTables(NamedTuple):
+    cu_q: torch.Tensor           # [B + 1] first token of every sequence, and their number
+    positions: torch.Tensor      # [T]
+    slots: torch.Tensor          # [T] place in the paged cache, -1: none
+    tok_slot: torch.Tensor       # [T] adapter slot, -1: none
+    block_tables: torch.Tensor   # [B, max_blocks]
+    tiles: tuple                 # for every list asked for: (sequence, first query) of its tiles
+    lora_tiles: torch.Tensor     # [n, 4] (adapter slot, first row, rows, 0)
+
+
+def check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, lead) -> int:
+    """-> number of sequences."""
+    _need(seqs.dtype == torch.int32 and seqs.dim() == 2 and seqs.shape[0] == 4 and (seqs.shape[1] <= 1 or seqs.stride(1) == 1),
+          "step_tables: seqs is [4, sequences] int32 (tokens, cached tokens, adapter slot, pages)")
+    _need(seqs.shape[1] <= STEP_SEQS_MAX, f"step_tables: {seqs.shape[1]} sequences, at most {STEP_SEQS_MAX}")
+    _need(pages.dtype == torch.int32 and pages.dim() == 1 and pages.is_contiguous() and pages.device == seqs.device,
+          "step_tables: pages is one contiguous int32 list on the device of seqs")
+    _need(tokens >= 0 and max_blocks > 0 and page > 0 and window >= 0, "step_tables: tokens and window from 0 on, max_blocks and page from 1 on")
+    _need(len(tiles) <= 4 and all(h > 0 and n >= 0 for h, n in tiles), "step_tables: up to four lists of tiles (height, count)")
+    _need(lora_tiles >= 0 and lora_rows > 0, "step_tables: lora_tiles from 0 on, lora_rows from 1 on")
+    _need(lead is None or (lead.dtype == torch.int32 and lead.dim() == 2 and lead.shape[1] == 4 and lead.is_contiguous() and lead.device == seqs.device
+                           and lead.data_ptr() % 16 == 0), "step_tables: lead is [n, 4] int32, contiguous, on a 16-byte boundary")
+    return seqs.shape[1]
+
+
+def step_tables(seqs, pages, tokens: int, max_blocks: int, page: int, window: int = 0, tiles=(), lora_tiles: int = 0, lora_rows: int = 32,
+                row_offset: int = 0, lead=None) -> StepTables:
+    """Tables of a ragged step.  `seqs` [4, B] int32: tokens, cached tokens, adapter slot (-1: none) and pages of every sequence; `pages`: the
+    sequences' page lists end to end.  The sequences' tokens follow one another.
+
+    A block table is a sequence's pages (`max_blocks` of them at most), then zeros; with a sliding `window` whose pages are recycled (fewer than
+    `max_blocks`, and a window and a page of them) the pages over and over.  Positions count from a sequence's cached tokens.  `tiles`:
+    (height, count) of lists of tiles, first queries 0, height, 2 height .. of every sequence in turn.  Adapter tiles hold up to `lora_rows`
+    rows of one sequence with an adapter; rows are counted from `row_offset`, and the tiles `lead` [n, 4] come first.
+
+    The caller states how much there is (`tokens`, the counts, `lora_tiles`).  Entries past what the lengths make are filled: position 0, slots
+    and tiles' sequences and adapters -1; what they make beyond is left out."""
+    B = check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, lead)
+    dev = seqs.device
+    n, cached, adapter, held = seqs.tolist() if B else ([], [], [], [])
+    n, cached, held, flat = [max(v, 0) for v in n], [max(v, 0) for v in cached], [max(v, 0) for v in held], pages.tolist()
+    cu, tables, off = [0], [], 0
+    for b in range(B):
+        cu.append(cu[-1] + n[b])
+        own = [flat[i] if i < len(flat) else 0 for i in range(off, off + held[b])]
+        off += held[b]
+        if window > 0 and 0 < held[b] < max_blocks and held[b] * page >= window + page:
+            tables.append([own[j % held[b]] for j in range(max_blocks)])
+        else:
+            tables.append((own + [0] * max_blocks)[:max_blocks])
+    pos, slots, tok = [], [], []
+    for b in range(B):
+        for p in range(cached[b], cached[b] + n[b]):
+            pos.append(p)
+            slots.append(tables[b][min(p // page, max_blocks - 1)] * page + p % page)
+        tok += [adapter[b]] * n[b]
+
+    def t(values, count, fill):
+        return torch.tensor((values + [fill] * count)[:count], dtype=torch.int32, device=dev)
+    lists = []
+    for height, count in tiles:
+        seq, q0 = prefill_tiles(n, height)
+        lists.append((t(seq, count, -1), t(q0, count, 0)))
+    rows = [[adapter[b], row_offset + cu[b] + r, min(lora_rows, n[b] - r), 0] for b in range(B) if adapter[b] >= 0 for r in range(0, n[b], lora_rows)]
+    rows = (rows + [[-1, 0, 0, 0]] * lora_tiles)[:lora_tiles]
+    lora = torch.tensor(rows, dtype=torch.int32, device=dev).view(-1, 4)
+    return StepTables(torch.tensor(cu, dtype=torch.int32, device=dev), t(pos, tokens, 0), t(slots, tokens, -1), t(tok, tokens, -1),
+                      torch.tensor(tables, dtype=torch.int32, device=dev).view(B, max_blocks), tuple(lists),
+                      lora if lead is None else torch.cat([lead, lora]))
+
+
+MOE_FEW_ACTS = ("silu", "swish", "gelu", "gelu_new", "gelu_pytorch_tanh", "gelu_fast", "gelu_tanh", "relu", "relu2")
+
+
+def check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out):
+    """-> (tokens, experts, width, features)."""
+    _need(x.dim() == 2 and router_w.dim() == 2 and w13.dim() == 3 and w2.dim() == 3, "moe_few: x [T, H], router_w [E, H], w13 [e, 2 I, H], w2 [e, H, I]")
+    (T, H), E, e_local, inter = x.shape, router_w.shape[0], w13.shape[0], w2.shape[2]
+    _need(T <= MOE_FEW_TOKENS, f"moe_few: {T} tokens, at most {MOE_FEW_TOKENS} (moe_ffn takes any number)")
+    _need(router_w.shape[1] == H and w13.shape == (e_local, 2 * inter, H) and w2.shape == (e_local, H, inter), "moe_few: the shapes of the weights do not fit")
+    _need(1 <= k <= min(E, 32) and E <= 256, f"moe_few: {k} of {E} experts; at most 32 of 256")
+    _need(0 <= e0 and e0 + e_local <= E, f"moe_few: experts {e0} .. {e0 + e_local} of {E}")
+    _need(H > 0 and inter > 0 and H % 8 == 0 and inter % 8 == 0, "moe_few: width and features are multiples of 8")
+    _need(act in MOE_FEW_ACTS, f"moe_few: activation {act!r}")
+    _need(all(t.dtype == x.dtype and t.device == x.device for t in (router_w, w13, w2)), "moe_few: the weights have another type or device than x")
+    _need(x.stride(1) == 1 and x.stride(0) % 8 == 0 and router_w.stride(1) == 1 and router_w.stride(0) % 8 == 0 and w13.is_contiguous() and w2.is_contiguous()
+          and all(t.data_ptr() % 16 == 0 for t in (x, router_w, w13, w2)), "moe_few: rows on 16-byte boundaries, experts stacked without gaps")
+    _need(out is None or (out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and out.stride(1) == 1), "moe_few: out is like x")
+    return T, E, H, inter
+
+
+def moe_few(x, router_w, w13, w2, k: int, e0: int = 0, act: str = "silu", renorm: bool = True, scale: float = 1.0, out=None):
+    """Mixture-of-experts feed-forward of a few tokens: x [T, H], router_w [E, H], w13 [e_local, 2 I, H] (gate rows, then up rows), w2 [e_local, H, I];
+    this rank owns the experts [e0, e0 + e_local), and the others' share is left out.  A token goes to the `k` experts with the largest logits (the
+    lower number on ties), with softmax weights over those (`renorm`) or over all, times `scale`."""
+    T, E, H, inter = check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out)
+    z = x.float() @ router_w.float().t()
+    ids = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :k]
+    w = torch.softmax(z.gather(1, ids), 1) if renorm else torch.softmax(z, 1).gather(1, ids)
+    w = torch.zeros_like(z).scatter_(1, ids, w * scale)
+    chosen = torch.zeros_like(z, dtype=torch.bool).scatter_(1, ids, True)
+    y = torch.zeros(T, H, dtype=torch.float32, device=x.device)
+    for e in range(w13.shape[0]):
+        rows = chosen[:, e0 + e].nonzero()[:, 0]
+        if rows.numel():
+            g = x[rows].float() @ w13[e].float().t()
+            y[rows] += w[rows, e0 + e, None] * ((_act(g[:, :inter], act) * g[:, inter:]) @ w2[e].float().t())
+    y = y.to(x.dtype)
+    if out is not None:
+        out.copy_(y)
+        return out
+    return y
+
+
+class TokenScores(NamedTuple):
+    logprobs: Optional[torch.Tensor]      # [T] of the given tokens (None without)
+    entropy: torch.Tensor                 # [T]
+    top_ids: torch.Tensor                 # [T, k] int32
+    top_logprobs: torch.Tensor            # [T, k]
+
+
+def check_token_scores(logits, targets, k, softcap):
+    """-> (rows, vocabulary)."""
+    _need(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1) and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1]),
+          "token_scores: logits are [rows, vocabulary], the logits of a row side by side")
+    T, V = logits.shape
+    _need(0 <= k <= min(TOP_MAX, V), f"token_scores: {k} alternatives of {V} tokens, at most {TOP_MAX}")
+    _need(softcap >= 0.0, "token_scores: softcap from 0 on (0: none)")
+    _need(targets is None or (targets.shape == (T,) and targets.dtype in (torch.int32, torch.int64) and targets.device == logits.device),
+          "token_scores: one int32 or int64 target a row, on the device of the logits")
+    return T, V
+
+
+def token_scores(logits, targets=None, k: int = 0, softcap: float = 0.0) -> TokenScores:
+    """Scores of tokens under softmax(logits), or softmax(softcap * tanh(logits / softcap)): the log-probability of `targets` (outside the
+    vocabulary: NaN), the entropy, and the `k` best tokens, best first, the lower id on ties (a NaN orders as -inf).  A logit of -inf
+    has no probability; a row with no other, with a NaN or with +inf (and no cap) has no distribution: its scores are NaN."""
+    T, V = check_token_scores(logits, targets, k, softcap)
+    raw = logits.float()
+    x = softcap * torch.tanh(raw / softcap) if softcap > 0 else raw
+    lp = torch.log_softmax(x, -1)
+    p = lp.exp()
+    entropy = -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(-1)
+    got = None
+    if targets is not None:
+        at = targets.long()
+        ok = (at >= 0) & (at < V)
+        got = torch.where(ok, lp.gather(1, at.clamp(0, V - 1)[:, None])[:, 0], torch.full_like(entropy, float("nan")))
+    ids = torch.sort(torch.where(raw.isnan(), torch.full_like(raw, float("-inf")), raw), dim=1, descending=True, stable=True).indices[:, :k]
+    return TokenScores(got, entropy, ids.to(torch.int32), lp.gather(1, ids))

@@ -1,0 +1,148 @@
+"""Operators of short ragged steps on the CPU: what they refuse, and the plain statements against the code that built these arrays before."""
+import random
+
+import pytest
+import torch
+
+from lorax_b200.ops import native, reference
+
+BF16 = torch.bfloat16
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def _refused(call, *a, **kw):
+    """By both forms, and by the CUDA one in front of everything that needs a GPU."""
+    for ops in (reference, native):
+        with pytest.raises(ValueError):
+            getattr(ops, call)(*a, **kw)
+
+
+# ------------------------------------------------------------------------------------------------ tables
+def _tables_args(**over):
+    a = dict(seqs=ints([3], [0], [-1], [1]), pages=ints(5), tokens=3, max_blocks=2, page=32)
+    a.update(over)
+    return a
+
+
+@pytest.mark.parametrize("over", [
+    dict(seqs=ints([3], [0], [-1], [1]).long()), dict(seqs=ints([3], [0], [-1])), dict(seqs=ints(3, 0, -1, 1)), dict(seqs=torch.zeros(4, 6, dtype=torch.int32)[:, ::2]),
+    dict(seqs=torch.zeros(4, reference.STEP_SEQS_MAX + 1, dtype=torch.int32)), dict(pages=ints(5).long()), dict(pages=ints([5])), dict(pages=ints(5, 6, 7, 8)[::2]),
+    dict(tokens=-1), dict(max_blocks=0), dict(page=0), dict(window=-1), dict(tiles=((0, 1),)), dict(tiles=((64, -1),)), dict(tiles=((64, 1),) * 5),
+    dict(lora_tiles=-1), dict(lora_rows=0), dict(lead=ints(1, 2, 3, 4)), dict(lead=ints([1, 2, 3])), dict(lead=ints([1, 2, 3, 4]).long()),
+    dict(lead=torch.zeros(5, 4, dtype=torch.int32).view(-1)[1:17].view(4, 4))])
+def test_tables_refuse(over):
+    _refused("step_tables", **_tables_args(**over))
+
+
+@pytest.mark.parametrize("window", [0, 64])
+def test_tables_are_the_ones_of_the_step_assembly(window):
+    """Positions, slots and adapter slots as `prefill_metadata` makes them from cumulative lengths and padded tables; tables, tiles and adapter
+    tiles as the runner's lists were."""
+    rng = random.Random(window)
+    B, M, page = 9, 7, 32
+    n = [rng.choice([0, 1, 31, 32, 33, 70, 130]) for _ in range(B)]
+    cached = [rng.randint(0, 90) for _ in range(B)]
+    slot = [rng.choice([-1, 0, 3]) for _ in range(B)]
+    pages = [[rng.randint(1, 99) for _ in range(rng.choice([1, 2, 3, 7, 9]))] for _ in range(B)]
+
+    def row(blocks):
+        k = len(blocks)
+        if k >= M:
+            return blocks[:M]
+        if window and k * page >= window + page:
+            return [blocks[i % k] for i in range(M)]
+        return blocks + [0] * (M - k)
+    T = sum(n)
+    cu = [sum(n[:b]) for b in range(B + 1)]
+    bt = ints(*[row(p) for p in pages])
+    want = reference.prefill_metadata(ints(*cu), ints(*cached), ints(*slot), bt, page, T)
+    lora = [[slot[b], 5 + cu[b] + a, min(32, n[b] - a), 0] for b in range(B) if slot[b] >= 0 for a in range(0, n[b], 32)]
+    t64, t128 = reference.prefill_tiles(n), reference.prefill_tiles(n, 128)
+    lead = ints([7, 0, 5, 0])
+    got = reference.step_tables(ints(n, cached, slot, [len(p) for p in pages]), ints(*[x for p in pages for x in p]), T, M, page, window=window,
+                                tiles=((64, len(t64[0])), (128, len(t128[0]) + 2)), lora_tiles=len(lora) + 1, row_offset=5, lead=lead)
+    assert got.cu_q.tolist() == cu and torch.equal(got.block_tables, bt)
+    assert torch.equal(got.positions, want[0]) and torch.equal(got.slots, want[1]) and torch.equal(got.tok_slot, want[2])
+    assert [x.tolist() for x in got.tiles[0]] == list(t64)
+    assert [x.tolist() for x in got.tiles[1]] == [t128[0] + [-1, -1], t128[1] + [0, 0]]
+    assert got.lora_tiles.tolist() == [[7, 0, 5, 0]] + lora + [[-1, 0, 0, 0]]
+
+
+def test_tables_fill_what_the_lengths_do_not_reach_and_leave_out_what_they_pass():
+    seqs, pages = ints([3, 2], [31, 0], [4, -1], [2, 1]), ints(9, 8, 7)
+    got = reference.step_tables(seqs, pages, 7, 2, 32, tiles=((2, 5),), lora_tiles=2)
+    assert got.slots.tolist() == [9 * 32 + 31, 8 * 32, 8 * 32 + 1, 7 * 32, 7 * 32 + 1, -1, -1] and got.tok_slot.tolist() == [4, 4, 4, -1, -1, -1, -1]
+    assert got.positions.tolist() == [31, 32, 33, 0, 1, 0, 0] and got.lora_tiles.tolist() == [[4, 0, 3, 0], [-1, 0, 0, 0]]
+    assert [x.tolist() for x in got.tiles[0]] == [[0, 0, 1, -1, -1], [0, 2, 0, 0, 0]]
+    short = reference.step_tables(seqs, pages, 2, 2, 32, tiles=((2, 1),), lora_tiles=0)
+    assert short.slots.tolist() == [9 * 32 + 31, 8 * 32] and short.cu_q.tolist() == [0, 3, 5] and short.lora_tiles.shape == (0, 4)
+
+
+# ------------------------------------------------------------------------------------------------ experts
+def _moe_args(T=2, E=4, k=2, H=64, I=32, **over):
+    a = dict(x=torch.zeros(T, H, dtype=BF16), router_w=torch.zeros(E, H, dtype=BF16), w13=torch.zeros(E, 2 * I, H, dtype=BF16),
+             w2=torch.zeros(E, H, I, dtype=BF16), k=k)
+    a.update(over)
+    return a
+
+
+@pytest.mark.parametrize("over", [
+    dict(T=17), dict(k=0), dict(k=5), dict(E=40, k=33), dict(E=257), dict(H=60), dict(I=12), dict(e0=1), dict(e0=-1), dict(act="tanh"),
+    dict(x=torch.zeros(2, 64)), dict(x=torch.zeros(64, dtype=BF16)), dict(x=torch.zeros(2, 128, dtype=BF16)[:, ::2]), dict(x=torch.zeros(2, 68, dtype=BF16)[:, :64]),
+    dict(x=torch.zeros(130, dtype=BF16)[1:129].view(2, 64)), dict(router_w=torch.zeros(4, 32, dtype=BF16)), dict(router_w=torch.zeros(4, 64)),
+    dict(w13=torch.zeros(4, 48, 64, dtype=BF16)), dict(w13=torch.zeros(8, 64, 64, dtype=BF16)[::2]), dict(w2=torch.zeros(4, 32, 64, dtype=BF16).transpose(1, 2)),
+    dict(out=torch.zeros(3, 64, dtype=BF16)), dict(out=torch.zeros(2, 64)), dict(out=torch.zeros(64, 2, dtype=BF16).t())])
+def test_experts_refuse(over):
+    _refused("moe_few", **_moe_args(**over))
+
+
+def test_experts_of_the_kernels_are_bf16():
+    a = {k: v.float() if isinstance(v, torch.Tensor) else v for k, v in _moe_args().items()}
+    reference.moe_few(**a)
+    with pytest.raises(ValueError, match="bf16"):
+        native.moe_few(**a)
+
+
+@pytest.mark.parametrize("renorm,e0,e_local", [(True, 0, 6), (False, 0, 6), (True, 2, 3)])
+def test_experts_as_a_dense_sum(renorm, e0, e_local):
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g)
+    x, wr, w13, w2 = r(5, 32), r(6, 32), r(e_local, 48, 32) / 6, r(e_local, 32, 24) / 5
+    z = (x.double() @ wr.double().t())
+    want = torch.zeros(5, 32, dtype=torch.float64)
+    for t in range(5):
+        best = sorted(range(6), key=lambda e: -z[t, e])[:2]
+        p = torch.softmax(z[t, best] if renorm else z[t], 0)
+        for j, e in enumerate(best):
+            if e0 <= e < e0 + e_local:
+                a = w13[e - e0].double() @ x[t].double()
+                want[t] += 1.5 * p[j if renorm else e] * (w2[e - e0].double() @ (torch.nn.functional.silu(a[:24]) * a[24:]))
+    got = reference.moe_few(x, wr, w13, w2, 2, e0, renorm=renorm, scale=1.5)
+    assert torch.allclose(got.double(), want, rtol=1e-4, atol=1e-5)
+
+
+# ------------------------------------------------------------------------------------------------ scores
+@pytest.mark.parametrize("over", [
+    dict(logits=torch.zeros(8)), dict(logits=torch.zeros(2, 0)), dict(logits=torch.zeros(2, 16)[:, ::2]), dict(logits=torch.zeros(1, 8).expand(2, 8)),
+    dict(k=-1), dict(k=9), dict(logits=torch.zeros(2, 64), k=33), dict(softcap=-1.0), dict(targets=ints(1)), dict(targets=torch.zeros(2)), dict(targets=ints([1], [2]))])
+def test_scores_refuse(over):
+    _refused("token_scores", **{**dict(logits=torch.zeros(2, 8)), **over})
+
+
+def test_scores_of_the_kernels_are_bf16_or_fp32():
+    with pytest.raises(ValueError, match="float16"):
+        native.token_scores(torch.zeros(2, 8, dtype=torch.float16))
+
+
+def test_scores_of_rows_with_masks():
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[1.0, -inf, 1.0, 0.0], [-inf] * 4, [0.0, nan, 1.0, 2.0], [0.0, inf, 1.0, 2.0], [-inf, 3.0, -inf, -inf]])
+    s = reference.token_scores(x, torch.tensor([2, 0, 0, 1, 4]), k=3)
+    assert s.top_ids.tolist() == [[0, 2, 3], [0, 1, 2], [3, 2, 0], [1, 3, 2], [1, 0, 2]]
+    z = 2 * torch.e + 1
+    assert torch.allclose(s.logprobs[0], torch.tensor(1 - torch.log(torch.tensor(z)).item()))
+    assert s.entropy[4] == 0 and s.top_logprobs[4].tolist() == [0.0, -inf, -inf]
+    assert s.logprobs[1:].isnan().all() and s.entropy[1:4].isnan().all()
