@@ -358,6 +358,9 @@ LX_DEVICE uint32_t cluster_rank() {
 LX_DEVICE void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Its two halves.
+LX_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+LX_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 LX_DEVICE void cluster_store_f32(uint32_t smem_addr, uint32_t rank, float v) {
   asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\tst.shared::cluster.f32 [ra], %2;\n\t}"
                ::"r"(smem_addr), "r"(rank), "f"(v) : "memory");

@@ -32,7 +32,9 @@ enum FewAct : int { kFewSilu = 0, kFewGelu = 1, kFewGeluTanh = 2, kFewRelu = 3, 
 struct MoeFewParams {
   const __nv_bfloat16* x;      // [T, H]
   long long ldx;
-  const float* logits;         // [T, E]
+  const __nv_bfloat16* wr;     // [E, H]
+  long long ldr;
+  const float* logits;         // [T, E], or null: the up kernel forms them itself
   const __nv_bfloat16* w13;    // [e_local, 2 I, H]: gate rows, then up rows
   const __nv_bfloat16* w2;     // [e_local, H, I]
   int* ids;                    // [T, k]: the chosen experts, for the second kernel
@@ -100,12 +102,59 @@ struct FewPlan {
   int reached;
 };
 
+// z[t, e] for all experts, by every CTA for itself: the router's rows stand where the up kernel has its tiles.
+template <int NT>
+LX_DEVICE void few_route(float* z, float4* red, const MoeFewParams& p) {
+  constexpr int kBatch = 8 / NT;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c8 = (lane & 3) * 8;
+  const int steps = (p.H + 31) / 32, tiles = (p.E + 15) / 16;
+  for (int i = 0; i < tiles; ++i) {
+    float acc[NT][4];
+#pragma unroll
+    for (int m = 0; m < NT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+    for (int s0 = warp; s0 < steps; s0 += kFewWarps * kBatch) {
+      uint4 a[kBatch][2], b[kBatch][NT];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int k = (s0 + j * kFewWarps) * 32 + c8, e = i * 16 + g;
+        const bool ok = k < p.H;
+        a[j][0] = few_load(p.wr + e * p.ldr + k, ok && e < p.E);
+        a[j][1] = few_load(p.wr + (e + 8) * p.ldr + k, ok && e + 8 < p.E);
+#pragma unroll
+        for (int m = 0; m < NT; ++m) b[j][m] = few_load(p.x + (m * 8 + g) * p.ldx + k, ok && m * 8 + g < p.T);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int m = 0; m < NT; ++m) few_mma32(acc[m], a[j][0], a[j][1], b[j][m]);
+    }
+#pragma unroll
+    for (int m = 0; m < NT; ++m) red[((warp * tiles + i) * NT + m) * 32 + lane] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+  }
+  __syncthreads();
+  for (int q = tid; q < tiles * NT * 32; q += kFewThreads) {
+    const int i = q / (NT * 32), m = q / 32 % NT, l = q & 31;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float4 part = red[((w * tiles + i) * NT + m) * 32 + l];
+      v.x += part.x; v.y += part.y; v.z += part.z; v.w += part.w;
+    }
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      const int t = m * 8 + (l & 3) * 2 + (o & 1), e = i * 16 + (l >> 2) + (o >> 1) * 8;
+      if (t < p.T && e < p.E) z[t * p.E + e] = o == 0 ? v.x : o == 1 ? v.y : o == 2 ? v.z : v.w;
+    }
+  }
+  __syncthreads();
+}
+
 // One warp per token.  A NaN orders as -inf (its weight is NaN all the same); no expert is chosen twice.
-LX_DEVICE void few_select(FewPlan& plan, const MoeFewParams& p) {
+LX_DEVICE void few_select(FewPlan& plan, const float* logits, const MoeFewParams& p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kPer = kFewExperts / 32;
   for (int t = warp; t < p.T; t += kFewWarps) {
-    const float* row = p.logits + (long long)t * p.E;
+    const float* row = logits + t * p.E;
     float z[kPer];
     uint32_t taken = 0;
 #pragma unroll
@@ -195,7 +244,13 @@ __global__ void __launch_bounds__(kFewThreads) moe_few_up_kernel(const __grid_co
   __shared__ FewPlan plan;
   extern __shared__ float4 red[];              // [warps][kTiles][NT][32 lanes]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c8 = (lane & 3) * 8;
-  few_select(plan, p);
+  const float* logits = p.logits;
+  if (logits == nullptr) {
+    __shared__ float z[kFewTokens * kFewExperts];
+    few_route<NT>(z, red, p);
+    logits = z;
+  }
+  few_select(plan, logits, p);
   __syncthreads();
   few_reached(plan, p);
   if (blockIdx.x == 0)
@@ -403,19 +458,26 @@ extern "C" {
 
 int lx_moe_few_max_tokens() { return lx::kFewTokens; }
 
-// `logits` [T, E] fp32 of lx_moe_router_logits; `ids` [T, k] and `h` [2, T k, I] are scratch of the call.
-int lx_moe_few(const void* x, long long ldx, const float* logits, const void* w13, const void* w2, int* ids, void* h, void* out, long long ldo, int T,
+int lx_moe_router_logits(const void* x, long long ldx, const void* wr, long long ldw, float* logits, int T, int E, int H, int* counts, int ncounts,
+                         void* stream);
+
+// `logits` [T, E], `ids` [T, k] and `h` [2, T k, I] are scratch of the call.
+int lx_moe_few(const void* x, long long ldx, const void* wr, long long ldw, const void* w13, const void* w2, float* logits, int* ids, void* h, void* out, long long ldo, int T,
                int E, int k, int e0, int e_local, int H, int I, int act, int renorm, float scale, int num_sms, void* stream) {
   using namespace lx;
   if (T < 0 || T > kFewTokens || E <= 0 || E > kFewExperts || k <= 0 || k > kFewTop || k > E || e_local < 0 || e_local > kFewExperts || H <= 0 || H % 8 != 0 ||
       I <= 0 || I % 8 != 0 || act < 0 || act > kFewRelu2 || num_sms <= 0)
     return -1;
-  for (const void* q : {x, w13, w2, (const void*)h})
+  for (const void* q : {x, wr, w13, w2, (const void*)h})
     if ((reinterpret_cast<uintptr_t>(q) & 15) != 0) return -2;
-  if (ldx % 8 != 0) return -2;
+  if (ldx % 8 != 0 || ldw % 8 != 0) return -2;
   if (T == 0) return 0;
+  const bool by_itself = getenv("FEW_ROUTE") ? atoi(getenv("FEW_ROUTE")) : E * (long long)H <= 65536;
+  if (!by_itself)
+    if (const int rc = lx_moe_router_logits(x, ldx, wr, ldw, logits, T, E, H, nullptr, 0, stream)) return rc;
   MoeFewParams p{};
-  p.x = reinterpret_cast<const __nv_bfloat16*>(x); p.ldx = ldx; p.logits = logits;
+  p.x = reinterpret_cast<const __nv_bfloat16*>(x); p.ldx = ldx; p.logits = by_itself ? nullptr : logits;
+  p.wr = reinterpret_cast<const __nv_bfloat16*>(wr); p.ldr = ldw;
   p.w13 = reinterpret_cast<const __nv_bfloat16*>(w13); p.w2 = reinterpret_cast<const __nv_bfloat16*>(w2);
   p.ids = ids; p.h = reinterpret_cast<__nv_bfloat16*>(h); p.out = reinterpret_cast<__nv_bfloat16*>(out); p.ldo = ldo;
   p.T = T; p.E = E; p.k = k; p.e0 = e0; p.e_local = e_local; p.H = H; p.I = I; p.act = act; p.renorm = renorm; p.scale = scale;

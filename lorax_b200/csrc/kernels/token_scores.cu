@@ -8,9 +8,9 @@
 // alone do not fill the GPU, the CTAs of a cluster that share a row.  The sums are fp32: a thread adds some hundred terms of at most one, the
 // rest is a tree.  A logit of -inf adds nothing; a row of nothing else, one with a NaN and one with +inf have no distribution and score NaN.
 //
-// The k best come from the threads' own best elements: the k-th best of those, by (value, index), is a lower bound of the row's k-th best, so
-// only the elements of the k threads at or above it can take part.  Those threads' elements are read again (one in 512 / k of the row, from
-// L2), what is at or above the bound is listed, and the list is ranked by counting.  The order of (value, index) pairs is total, so the outcome
+// The k best: of 64 groups of threads, each has a best element; the k-th best of those, by (value, index), is a lower bound of the row's k-th
+// best, so only threads whose own best is at or above it can hold any (k 64 / (64 - k) or so of 512).  Their elements are read again (from L2),
+// what is at or above the bound is listed, and the list is ranked by counting.  The order of (value, index) pairs is total, so the outcome
 // depends on no order of execution.
 #include "common.cuh"
 
@@ -20,6 +20,7 @@ constexpr int kScoreThreads = 512;
 constexpr int kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreMaxParts = 8;         // CTAs of a row (the portable cluster)
 constexpr int kScoreMaxTop = 32;
+constexpr int kScoreGroups = 64;          // of threads whose best elements set the bound: twice the most alternatives
 constexpr int kScoreList = 2048;          // candidates that are ranked at once
 constexpr int kScoreUnroll = 4;           // 16-byte loads of a thread in flight
 
@@ -69,217 +70,275 @@ LX_DEVICE float max_nan(float a, float b) {
   return r;
 }
 
-template <typename L>
+LX_DEVICE uint64_t pack_f32x2(float lo, float hi) { return ((uint64_t)__float_as_uint(hi) << 32) | __float_as_uint(lo); }
+LX_DEVICE float2 unpack_f32x2(uint64_t v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
+LX_DEVICE uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+LX_DEVICE uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+LX_DEVICE uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+LX_DEVICE float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// 16 bytes of logits (VEC), or one.  What lies past the end reads as -inf: it adds nothing.
+template <typename L, bool VEC>
 struct ScoreLoad;
 template <>
-struct ScoreLoad<__nv_bfloat16> {
-  static constexpr int kVec = 8;
-  LX_DEVICE static void vec(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
+struct ScoreLoad<__nv_bfloat16, true> {
+  static constexpr int kN = 8;
+  using Raw = uint4;
+  LX_DEVICE static Raw load(const __nv_bfloat16* p, bool ok) { return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  LX_DEVICE static void values(const Raw& v, float (&x)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float2 f = unpack_bf16x2(w[q]);
-      x[2 * q] = f.x;
-      x[2 * q + 1] = f.y;
+      x[2 * q] = __uint_as_float(w[q] << 16);
+      x[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
     }
   }
-  LX_DEVICE static float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  LX_DEVICE static float top(const Raw& v) {      // passes over NaN
+    auto two = [](uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); };
+    const __nv_bfloat162 m = __hmax2(__hmax2(two(v.x), two(v.y)), __hmax2(two(v.z), two(v.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
 };
 template <>
-struct ScoreLoad<float> {
-  static constexpr int kVec = 4;
-  LX_DEVICE static void vec(const float* p, float (&x)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-  }
-  LX_DEVICE static float one(const float* p) { return *p; }
+struct ScoreLoad<float, true> {
+  static constexpr int kN = 4;
+  using Raw = float4;
+  LX_DEVICE static Raw load(const float* p, bool ok) { return ok ? *reinterpret_cast<const float4*>(p) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
+  LX_DEVICE static void values(const Raw& v, float (&x)[4]) { x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+  LX_DEVICE static float top(const Raw& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+};
+template <>
+struct ScoreLoad<__nv_bfloat16, false> {
+  static constexpr int kN = 1;
+  using Raw = float;
+  LX_DEVICE static Raw load(const __nv_bfloat16* p, bool ok) { return ok ? __bfloat162float(*p) : -INFINITY; }
+  LX_DEVICE static void values(const Raw& v, float (&x)[1]) { x[0] = v; }
+  LX_DEVICE static float top(const Raw& v) { return v; }
+};
+template <>
+struct ScoreLoad<float, false> {
+  static constexpr int kN = 1;
+  using Raw = float;
+  LX_DEVICE static Raw load(const float* p, bool ok) { return ok ? *p : -INFINITY; }
+  LX_DEVICE static void values(const Raw& v, float (&x)[1]) { x[0] = v; }
+  LX_DEVICE static float top(const Raw& v) { return v; }
 };
 
 struct ScoreThread {
-  ScoreSums sums;
+  float m;                 // running maximum of the (capped) logits
+  uint64_t s, u;           // running sums, of even and odd elements
   float best;              // of the raw logits, with the lowest index that has it
   int index;
 };
 
-// N logits from index i on (indices only grow).
-template <int N, bool TOP, bool CAP>
-LX_DEVICE void score_take(ScoreThread& t, float (&x)[N], int i, float cap) {
-  float top = x[0];
+// R loads of a thread, the first from index i on, the others `step` further each (indices only grow); from `end` on they are not of the row.
+template <typename Load, int R, bool TOP, bool CAP>
+LX_DEVICE void score_take(ScoreThread& t, const typename Load::Raw (&raw)[R], int i, int step, int end, float cap) {
+  constexpr int N = Load::kN;
+  float top = Load::top(raw[0]);
 #pragma unroll
-  for (int q = 1; q < N; ++q) top = fmaxf(top, x[q]);      // (passes over NaN)
+  for (int r = 1; r < R; ++r) top = fmaxf(top, Load::top(raw[r]));
   if (TOP && top > t.best) {
     t.best = top;
 #pragma unroll
-    for (int q = N - 1; q >= 0; --q)
-      if (x[q] == top) t.index = i + q;
-  }
-  if constexpr (CAP) {
+    for (int r = R - 1; r >= 0; --r) {
+      float x[N];
+      Load::values(raw[r], x);
 #pragma unroll
-    for (int q = 0; q < N; ++q) x[q] = cap * tanhf(x[q] / cap);
-    top = cap * tanhf(top / cap);
-  }
-  ScoreSums& a = t.sums;
-  if (top > a.m) {
-    if (a.m != -INFINITY) {
-      const float d = fmaxf(a.m - top, kScoreFloor), f = __expf(d);
-      a.u = (a.u + d * a.s) * f;
-      a.s *= f;
+      for (int q = N - 1; q >= 0; --q)
+        if (x[q] == top) t.index = i + r * step + q;
     }
-    a.m = top;
   }
-  const float m = a.m == -INFINITY ? 0.f : a.m;      // (logits of -inf only, so far: they add zeros)
+  if constexpr (CAP) top = cap * tanhf(top / cap);
+  if (top > t.m) {
+    if (t.m != -INFINITY) {
+      const float d = fmaxf(t.m - top, kScoreFloor), f = __expf(d);
+      const uint64_t d2 = pack_f32x2(d, d), f2 = pack_f32x2(f, f);
+      t.u = mul_f32x2(fma_f32x2(d2, t.s, t.u), f2);
+      t.s = mul_f32x2(t.s, f2);
+    }
+    t.m = top;
+  }
+  const float m = t.m == -INFINITY ? 0.f : t.m;      // (logits of -inf only, so far: they add zeros)
+  const uint64_t m2 = pack_f32x2(-m, -m), log2e = pack_f32x2(1.4426950408889634f, 1.4426950408889634f);
+  auto add = [&](float a, float b) {
+    float2 d = unpack_f32x2(add_f32x2(pack_f32x2(a, b), m2));
+    d.x = max_nan(d.x, kScoreFloor);
+    d.y = max_nan(d.y, kScoreFloor);
+    const uint64_t d2 = pack_f32x2(d.x, d.y);
+    const float2 l = unpack_f32x2(mul_f32x2(d2, log2e));
+    const uint64_t e = pack_f32x2(exp2_fast(l.x), exp2_fast(l.y));
+    t.s = add_f32x2(t.s, e);
+    t.u = fma_f32x2(d2, e, t.u);
+  };
+  auto capped = [&](float x, int r) { return !CAP ? x : r == 0 || i + r * step < end ? cap * tanhf(x / cap) : -INFINITY; };
+  // (all values of the batch are formed before the chains of adds: N R is even but for the last element of a row)
+  float x[R][N];
 #pragma unroll
-  for (int q = 0; q < N; ++q) {
-    const float d = max_nan(x[q] - m, kScoreFloor);
-    const float e = __expf(d);
-    a.s += e;
-    a.u = fmaf(d, e, a.u);
+  for (int r = 0; r < R; ++r) Load::values(raw[r], x[r]);
+  if constexpr (N > 1) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int q = 0; q < N; q += 2) add(capped(x[r][q], r), capped(x[r][q + 1], r));
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; r += 2) add(capped(x[r][0], r), r + 1 < R ? capped(x[r + 1][0], r + 1) : -INFINITY);
   }
 }
 
 struct ScoreShared {
   ScoreSums warps[kScoreWarps];
   ScoreSums parts[kScoreMaxParts];                             // (of the cluster's first CTA)
-  unsigned long long best[kScoreMaxParts * kScoreMaxTop];      // the parts' best pairs, 0: none (of the cluster's first CTA)
+  unsigned long long best[kScoreMaxParts * kScoreMaxTop];      // the parts' best pairs (of the cluster's first CTA)
+  unsigned long long group[kScoreGroups];
   unsigned long long list[kScoreList];
   unsigned long long own[kScoreMaxTop];
+  unsigned long long bound;
   int cand[kScoreThreads];
   int ncand, n;
 };
 
-// The pairs list[0 .. n), ranked: own[r] = the r-th best, r < k; 0 where there are fewer.
+// The pairs list[0 .. n), ranked by counting: own[r] = the r-th best, r < k; 0 where there are fewer.  Several neighbouring lanes share a pair's
+// comparisons where there are threads for it.
 LX_DEVICE void score_rank(const unsigned long long* list, int n, int k, unsigned long long* own) {
-  if (threadIdx.x < k && (int)threadIdx.x >= n) own[threadIdx.x] = 0;
-  for (int i = threadIdx.x; i < n; i += kScoreThreads) {
-    const unsigned long long a = list[i];
-    int r = 0;
-    for (int j = 0; j < n && r < k; ++j) r += list[j] > a;
-    if (r < k) own[r] = a;
+  if ((int)threadIdx.x < k && (int)threadIdx.x >= n) own[threadIdx.x] = 0;
+  int share = 32;
+  while (share > 1 && share * n > kScoreThreads) share >>= 1;
+  const int at = threadIdx.x & (share - 1), rounds = (n * share + kScoreThreads - 1) / kScoreThreads;
+  for (int r = 0; r < rounds; ++r) {
+    const int i = (threadIdx.x + r * kScoreThreads) / share;
+    const unsigned long long a = i < n ? list[i] : 0;
+    int above = 0;
+    for (int j = at; j < n; j += share) above += list[j] > a;
+    for (int o = share >> 1; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (i < n && at == 0 && above < k) own[above] = a;
   }
 }
 
 template <typename L, bool VEC, bool TOP, bool CAP>
-__global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __grid_constant__ TokenScoresParams p) {
-  pdl_wait();
-  pdl_trigger();
-  constexpr int kVec = VEC ? ScoreLoad<L>::kVec : 1;
+__global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __grid_constant__ TokenScoresParams p) {
+  using Load = ScoreLoad<L, VEC>;
+  constexpr int kVec = Load::kN, kStep = kScoreThreads * kVec;
   __shared__ ScoreShared sh;
   const int t = blockIdx.x, part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
+  if (parts > 1) cluster_arrive();      // (waited for in front of the first write to another CTA: it has started by then)
+  pdl_wait();
+  pdl_trigger();
   const L* row = reinterpret_cast<const L*>(p.logits) + (long long)t * p.ld;
   const int chunk = ((p.V + parts - 1) / parts + 7) & ~7;
   const int lo = min(part * chunk, p.V), hi = min(lo + chunk, p.V);
   const int whole = lo + (hi - lo) / kVec * kVec;      // a thread's elements: kVec from lo + (it * threads + tid) * kVec on, and one from `whole` on
-  ScoreThread me{{-INFINITY, 0.f, 0.f}, -INFINITY, -1};
+  ScoreThread me{-INFINITY, 0, 0, -INFINITY, -1};
   if (lo + tid * kVec < whole) me.index = lo + tid * kVec;
   else if (whole + tid < hi) me.index = whole + tid;
-  constexpr int kStep = kScoreThreads * kVec;
-  int i = lo + tid * kVec;
-  for (; i + (kScoreUnroll - 1) * kStep < whole; i += kScoreUnroll * kStep) {
-    float x[kScoreUnroll][kVec];
+  for (int i = lo + tid * kVec; i < whole; i += kScoreUnroll * kStep) {
+    typename Load::Raw raw[kScoreUnroll];
 #pragma unroll
-    for (int r = 0; r < kScoreUnroll; ++r) {
-      if constexpr (VEC) ScoreLoad<L>::vec(row + i + r * kStep, x[r]);
-      else x[r][0] = ScoreLoad<L>::one(row + i + r * kStep);
-    }
-#pragma unroll
-    for (int r = 0; r < kScoreUnroll; ++r) score_take<kVec, TOP, CAP>(me, x[r], i + r * kStep, p.softcap);
+    for (int r = 0; r < kScoreUnroll; ++r) raw[r] = Load::load(row + i + r * kStep, i + r * kStep < whole);
+    score_take<Load, kScoreUnroll, TOP, CAP>(me, raw, i, kStep, whole, p.softcap);
   }
-  for (; i < whole; i += kStep) {
-    float x[kVec];
-    if constexpr (VEC) ScoreLoad<L>::vec(row + i, x);
-    else x[0] = ScoreLoad<L>::one(row + i);
-    score_take<kVec, TOP, CAP>(me, x, i, p.softcap);
-  }
-  if (whole + tid < hi) {
-    float x[1] = {ScoreLoad<L>::one(row + whole + tid)};
-    score_take<1, TOP, CAP>(me, x, whole + tid, p.softcap);
+  if (VEC && whole + tid < hi) {
+    using One = ScoreLoad<L, false>;
+    const float raw[1] = {One::load(row + whole + tid, true)};
+    score_take<One, 1, TOP, CAP>(me, raw, whole + tid, 0, hi, p.softcap);
   }
 
   // sums of the CTA
   auto from_lane = [](const ScoreSums& a, int o) {
     return ScoreSums{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
   };
-  ScoreSums a = me.sums;
+  const float2 s2 = unpack_f32x2(me.s), u2 = unpack_f32x2(me.u);
+  ScoreSums a{me.m, s2.x + s2.y, u2.x + u2.y};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) score_merge(a, from_lane(a, o));
   if ((tid & 31) == 0) sh.warps[tid >> 5] = a;
-  if (tid == 0) sh.ncand = sh.n = 0;
+  const bool live = me.index >= 0;
+  const unsigned long long mine = TOP && live ? score_pair(score_key(me.best), me.index) : 0;
+  if constexpr (TOP) {
+    unsigned long long g = mine;
+#pragma unroll
+    for (int o = 1; o < kScoreThreads / kScoreGroups; o <<= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, g, o);
+      g = other > g ? other : g;
+    }
+    if ((tid & (kScoreThreads / kScoreGroups - 1)) == 0) sh.group[tid / (kScoreThreads / kScoreGroups)] = g;
+    if (tid == 0) {
+      sh.ncand = sh.n = 0;
+      sh.bound = 0;
+    }
+  }
   __syncthreads();
-  if (parts > 1) cluster_sync();      // every CTA of the cluster has started: its shared memory may be written
   if (tid < 32) {
     a = sh.warps[tid & (kScoreWarps - 1)];
 #pragma unroll
     for (int o = kScoreWarps / 2; o > 0; o >>= 1) score_merge(a, from_lane(a, o));
-    if (tid == 0) {
-      if (parts > 1) {
-        const uint32_t to = smem_u32(&sh.parts[part]);
-        cluster_store_f32(to, 0, a.m);
-        cluster_store_f32(to + 4, 0, a.s);
-        cluster_store_f32(to + 8, 0, a.u);
-      } else {
-        sh.parts[0] = a;
-      }
-    }
   }
 
   if constexpr (TOP) {
-    // the bound: the k-th best (value, index) of the threads' own best
+    // the bound: the k-th best of the groups' best, or none where there are fewer
     const int k = p.k;
-    const bool live = me.index >= 0;
-    const uint32_t key = score_key(me.best);
-    constexpr int kLow = sizeof(L) == 2 ? 16 : 0;      // a bf16's order is in the upper half
-    uint32_t bound = 0;
-    for (int b = 31; b >= kLow; --b) {
-      const uint32_t at = bound | (1u << b);
-      if (__syncthreads_count(live && key >= at) >= k) bound = at;
-    }
-    const int above = __syncthreads_count(live && (key >> kLow) > (bound >> kLow));
-    const bool tie = live && (key >> kLow) == (bound >> kLow);
-    const int ties = __syncthreads_count(tie);
-    int limit = 0x7fffffff;                            // of the elements that equal the bound, those up to this index take part
-    if (above + ties > k) {
-      limit = 0;
-      for (int b = 30; b >= 0; --b) {                  // the largest index with fewer than k - above ties below it is the last one
-        const int at = limit | (1 << b);
-        if (__syncthreads_count(tie && me.index < at) < k - above) limit = at;
-      }
-    }
-    auto takes = [&](uint32_t x, int idx) { return (x >> kLow) > (bound >> kLow) || ((x >> kLow) == (bound >> kLow) && idx <= limit); };
-    if (live && takes(key, me.index)) sh.cand[atomicAdd(&sh.ncand, 1)] = tid;
-    __syncthreads();
-    const int ncand = sh.ncand, warp = tid >> 5, lane = tid & 31;
-    const int its = (whole - lo + kStep - 1) / kStep;
-    auto push = [&](float x, int idx) {
-      const uint32_t kx = score_key(x);
-      if (takes(kx, idx)) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < kScoreList) sh.list[at] = score_pair(kx, idx);
-      }
-    };
-    // elements of thread c in its rounds [it0, it1), one round a lane; its last element with round `its`
-    auto collect = [&](int c, int it0, int it1) {
-      for (int it = it0 + lane; it < it1; it += 32) {
-        if (it == its) {
-          if (whole + c < hi) push(ScoreLoad<L>::one(row + whole + c), whole + c);
-          continue;
-        }
-        const int from = lo + (it * kScoreThreads + c) * kVec;
-        if (from >= whole) continue;
-        float x[kVec];
-        if constexpr (VEC) ScoreLoad<L>::vec(row + from, x);
-        else x[0] = ScoreLoad<L>::one(row + from);
+    {
+      constexpr int kShare = kScoreThreads / kScoreGroups;
+      const unsigned long long g = sh.group[tid / kShare];
+      int above = 0;
 #pragma unroll
-        for (int q = 0; q < kVec; ++q) push(x[q], from + q);
+      for (int j = 0; j < kScoreGroups / kShare; ++j) above += sh.group[(tid & (kShare - 1)) + j * kShare] > g;
+#pragma unroll
+      for (int o = kShare / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+      if (g != 0 && above == k - 1 && (tid & (kShare - 1)) == 0) sh.bound = g;
+    }
+    __syncthreads();
+    const unsigned long long bound = sh.bound;
+    if (live && mine >= bound) sh.cand[atomicAdd(&sh.ncand, 1)] = tid;
+    __syncthreads();
+    const int ncand = sh.ncand;
+    const int its = (whole - lo + kStep - 1) / kStep;      // loads of a thread; its single element counts as one more
+    auto push = [&](float x, int idx) {
+      const unsigned long long pair = score_pair(score_key(x), idx);
+      if (pair >= bound) {
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < kScoreList) sh.list[at] = pair;
       }
     };
-    for (int c = warp; c < ncand; c += kScoreWarps) collect(sh.cand[c], 0, its + 1);
+    auto collect = [&](int c, int it) {
+      if (it == its) {
+        if (VEC && whole + c < hi) push(ScoreLoad<L, false>::load(row + whole + c, true), whole + c);
+        return;
+      }
+      const int from = lo + (it * kScoreThreads + c) * kVec;
+      if (from >= whole) return;
+      float x[kVec];
+      Load::values(Load::load(row + from, true), x);
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) push(x[q], from + q);
+    };
+    for (int q = tid; q < ncand * (its + 1); q += kScoreThreads) {
+      const int c = q / (its + 1);
+      collect(sh.cand[c], q - c * (its + 1));
+    }
     __syncthreads();
     if (sh.n <= kScoreList) {
       score_rank(sh.list, sh.n, k, sh.own);
     } else {
       // more than the list holds (large logits side by side in the threads' strides): portions that fit, with the best so far among them
-      constexpr int kPortion = (kScoreList - kScoreMaxTop) / kVec / 32 * 32;
+      constexpr int kPortion = (kScoreList - kScoreMaxTop) / kVec;
       int have = 0;
       for (int c = 0; c < ncand; ++c) {
         for (int it = 0; it <= its; it += kPortion) {
@@ -287,7 +346,7 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
           if (tid < have) sh.list[tid] = sh.own[tid];
           if (tid == 0) sh.n = have;
           __syncthreads();
-          if (warp == 0) collect(sh.cand[c], it, min(it + kPortion, its + 1));
+          for (int q = it + tid; q < min(it + kPortion, its + 1); q += kScoreThreads) collect(sh.cand[c], q);
           __syncthreads();
           score_rank(sh.list, sh.n, k, sh.own);
           have = min(k, sh.n);
@@ -295,24 +354,29 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
       }
     }
     __syncthreads();
-    if (parts > 1) {
-      if (tid < k) {
-        const uint32_t to = smem_u32(&sh.best[part * kScoreMaxTop + tid]);
-        cluster_store_f32(to, 0, __uint_as_float((uint32_t)sh.own[tid]));
-        cluster_store_f32(to + 4, 0, __uint_as_float((uint32_t)(sh.own[tid] >> 32)));
-      }
-      cluster_sync();      // (the parts have arrived)
-      if (part != 0) return;
-      // empty places are zeros and rank behind every pair
-      for (int j = tid; j < parts * kScoreMaxTop; j += kScoreThreads) sh.list[j] = (j & (kScoreMaxTop - 1)) < k ? sh.best[j] : 0;
-      __syncthreads();
-      score_rank(sh.list, parts * kScoreMaxTop, k, sh.own);
+  }
+
+  if (parts > 1) {
+    cluster_wait();
+    if (tid == 0) {
+      const uint32_t to = smem_u32(&sh.parts[part]);
+      cluster_store_f32(to, 0, a.m);
+      cluster_store_f32(to + 4, 0, a.s);
+      cluster_store_f32(to + 8, 0, a.u);
+    }
+    if (TOP && tid < p.k) {
+      const uint32_t to = smem_u32(&sh.best[part * p.k + tid]);
+      cluster_store_f32(to, 0, __uint_as_float((uint32_t)sh.own[tid]));
+      cluster_store_f32(to + 4, 0, __uint_as_float((uint32_t)(sh.own[tid] >> 32)));
+    }
+    cluster_sync();      // (the parts have arrived)
+    if (part != 0) return;
+    if constexpr (TOP) {
+      score_rank(sh.best, parts * p.k, p.k, sh.own);      // (empty places are zeros and rank behind every pair)
       __syncthreads();
     }
-  } else if (parts > 1) {
-    cluster_sync();
-    if (part != 0) return;
   } else {
+    if (tid == 0) sh.parts[0] = a;
     __syncthreads();
   }
 
@@ -328,7 +392,7 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
                                : p.wide_targets     ? reinterpret_cast<const long long*>(p.targets)[t]
                                                     : reinterpret_cast<const int*>(p.targets)[t];
       float lp = NAN;
-      if (target >= 0 && target < p.V) lp = (capped(ScoreLoad<L>::one(row + target)) - all.m) - logs;
+      if (target >= 0 && target < p.V) lp = (capped(ScoreLoad<L, false>::load(row + target, true)) - all.m) - logs;
       p.logprobs[t] = lp;
     }
   }

@@ -6,7 +6,7 @@ Arguments that do not fit raise ValueError in front of any launch.  Outputs and 
 
 from __future__ import annotations
 
-import ctypes
+import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Sequence, Tuple
 
@@ -21,7 +21,7 @@ SIGNATURES = {
     "lx_step_tables_max_seqs": ([], I),
     "lx_step_tables": ([P, L, P, I, I, I, I, I, I, I, P, P, I, P, I, I, I, P, P], I),
     "lx_moe_few_max_tokens": ([], I),
-    "lx_moe_few": ([P, L, P, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, I, P], I),
+    "lx_moe_few": ([P, L, P, L, P, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, I, P], I),
     "lx_token_scores_max_top": ([], I),
     "lx_token_scores": ([P, L, I, I, I, P, I, I, F, P, P, P, P, P], I),
 }
@@ -33,11 +33,18 @@ def check_limits(lib):
             raise nv.NativeError(f"{name}: C++ says {getattr(lib, name)()}, Python says {here}")
 
 
-def _on_current_device(*tensors: Optional[torch.Tensor]):
-    here = torch.cuda.current_device()
+def _stream_for(*tensors: Optional[torch.Tensor]) -> int:
+    """The current stream of the current device, which has to be the tensors' one."""
+    here = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and t.device.index != here:
+        if t is not None and t.get_device() != here:
             raise ValueError(f"a tensor on {t.device} while cuda:{here} is the current device")
+    return torch._C._cuda_getCurrentRawStream(here)
+
+
+@functools.lru_cache(maxsize=None)
+def _num_sms(device: int) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
 
 
 def step_tables(seqs: torch.Tensor, pages: torch.Tensor, tokens: int, max_blocks: int, page: int, window: int = 0,
@@ -45,7 +52,7 @@ def step_tables(seqs: torch.Tensor, pages: torch.Tensor, tokens: int, max_blocks
                 lead: Optional[torch.Tensor] = None) -> StepTables:
     """Tables of a ragged step from its sequences' lengths (`reference.step_tables` states them), in one launch."""
     B = check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, lead)
-    _on_current_device(seqs, pages, lead)
+    stream = _stream_for(seqs, pages, lead)
     M, n_lead, n_lists = max_blocks, 0 if lead is None else lead.shape[0], len(tiles)
     sizes = [4 * (n_lead + lora_tiles), B + 1, tokens, tokens, tokens, B * M]
     for _, n in tiles:
@@ -53,7 +60,7 @@ def step_tables(seqs: torch.Tensor, pages: torch.Tensor, tokens: int, max_blocks
     out = torch.empty(sum(sizes), dtype=torch.int32, device=seqs.device)
     heights, counts = (I * n_lists)(*[h for h, _ in tiles]), (I * n_lists)(*[n for _, n in tiles])
     rc = nv.load().lx_step_tables(seqs.data_ptr(), seqs.stride(0), pages.data_ptr(), pages.shape[0], B, tokens, M, page, window, row_offset, heights, counts,
-                                  n_lists, None if lead is None else lead.data_ptr(), n_lead, lora_rows, lora_tiles, out.data_ptr(), nv._stream())
+                                  n_lists, None if lead is None else lead.data_ptr(), n_lead, lora_rows, lora_tiles, out.data_ptr(), stream)
     nv._check(rc, "lx_step_tables")
     lora, cu, pos, slots, tok, bt, *lists = out.split(sizes)
     return StepTables(cu, pos, slots, tok, bt.view(B, M), tuple(zip(lists[::2], lists[1::2])), lora.view(-1, 4))
@@ -65,21 +72,20 @@ def moe_few(x: torch.Tensor, router_w: torch.Tensor, w13: torch.Tensor, w2: torc
     T, E, H, inter = check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"moe_few: the kernels are bf16; got {x.dtype}")
-    _on_current_device(x, router_w, w13, w2, out)
+    stream = _stream_for(x, router_w, w13, w2, out)
     if out is None:
         out = torch.empty(T, H, dtype=x.dtype, device=x.device)
     if T == 0:
         return out
-    lib, stream = nv.load(), nv._stream()
-    logits = torch.empty(T, E, dtype=torch.float32, device=x.device)
-    nv._check(lib.lx_moe_router_logits(x.data_ptr(), x.stride(0), router_w.data_ptr(), router_w.stride(0), logits.data_ptr(), T, E, H, None, 0, stream),
-              "lx_moe_router_logits")
-    ids = torch.empty(T * k, dtype=torch.int32, device=x.device)
-    h = torch.empty(2 * T * k * inter, dtype=torch.bfloat16, device=x.device)
-    rc = lib.lx_moe_few(x.data_ptr(), x.stride(0), logits.data_ptr(), w13.data_ptr(), w2.data_ptr(), ids.data_ptr(), h.data_ptr(), out.data_ptr(), out.stride(0),
-                        T, E, k, e0, w13.shape[0], H, inter, nv._ACTS[act], int(renorm), scale, nv.workspace(x.device).num_sms, stream)
+    # scratch: h (two planes), then the logits, then the choice of experts
+    h_bytes, logits_bytes = (4 * T * k * inter + 15) // 16 * 16, 4 * T * E
+    scratch = torch.empty(h_bytes + logits_bytes + 4 * T * k, dtype=torch.uint8, device=x.device)
+    at = scratch.data_ptr()
+    rc = nv.load().lx_moe_few(x.data_ptr(), x.stride(0), router_w.data_ptr(), router_w.stride(0), w13.data_ptr(), w2.data_ptr(), at + h_bytes,
+                              at + h_bytes + logits_bytes, at, out.data_ptr(), out.stride(0), T, E, k, e0, w13.shape[0], H, inter, nv._ACTS[act], int(renorm),
+                              scale, _num_sms(x.get_device()), stream)
     nv._check(rc, "lx_moe_few")
-    nv.launch_count += 1                 # (two kernels)
+    nv.launch_count += 2                 # (three kernels)
     return out
 
 
@@ -89,13 +95,14 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, k
     T, V = check_token_scores(logits, targets, k, softcap)
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"token_scores: the kernels take bf16 and fp32 logits; got {logits.dtype}")
-    _on_current_device(logits, targets)
-    if targets is not None and not targets.is_contiguous():
+    stream = _stream_for(logits, targets)
+    t_ptr = wide = 0
+    if targets is not None:
         targets = targets.contiguous()
-    out = torch.empty(T * (2 + 2 * k), dtype=torch.float32, device=logits.device)
-    lp, ent, top, ids = out.split([T, T, T * k, T * k])
-    rc = nv.load().lx_token_scores(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), T, V, None if targets is None else targets.data_ptr(),
-                                   int(targets is not None and targets.dtype == torch.int64), k, softcap, None if targets is None else lp.data_ptr(), ent.data_ptr(),
-                                   ids.data_ptr(), top.data_ptr(), nv._stream())
+        t_ptr, wide = targets.data_ptr(), int(targets.dtype == torch.int64)
+    lp, ent, best = torch.empty(T * (2 + k), dtype=torch.float32, device=logits.device).split([T, T, T * k])
+    ids = torch.empty(T, k, dtype=torch.int32, device=logits.device)
+    rc = nv.load().lx_token_scores(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), T, V, t_ptr, wide, k, softcap,
+                                   lp.data_ptr() if t_ptr else 0, ent.data_ptr(), ids.data_ptr(), best.data_ptr(), stream)
     nv._check(rc, "lx_token_scores")
-    return TokenScores(None if targets is None else lp, ent, ids.view(torch.int32).view(T, k), top.view(T, k))
+    return TokenScores(lp if targets is not None else None, ent, ids, best.view(T, k))

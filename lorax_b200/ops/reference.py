@@ -986,11 +986,6 @@ TOP_MAX = 32                # alternatives that `token_scores` returns at most
 STEP_SEQS_MAX = 4096        # sequences of `step_tables`
 
 
-def _need(ok: bool, what: str):
-    if not ok:
-        raise ValueError(what)
-
-
 class StepTables(NamedTuple):
     cu_q: torch.Tensor           # [B + 1] first token of every sequence, and their number
     positions: torch.Tensor      # [T]
@@ -1003,16 +998,21 @@ class StepTables(NamedTuple):
 
 def check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, lead) -> int:
     """-> number of sequences."""
-    _need(seqs.dtype == torch.int32 and seqs.dim() == 2 and seqs.shape[0] == 4 and (seqs.shape[1] <= 1 or seqs.stride(1) == 1),
-          "step_tables: seqs is [4, sequences] int32 (tokens, cached tokens, adapter slot, pages)")
-    _need(seqs.shape[1] <= STEP_SEQS_MAX, f"step_tables: {seqs.shape[1]} sequences, at most {STEP_SEQS_MAX}")
-    _need(pages.dtype == torch.int32 and pages.dim() == 1 and pages.is_contiguous() and pages.device == seqs.device,
-          "step_tables: pages is one contiguous int32 list on the device of seqs")
-    _need(tokens >= 0 and max_blocks > 0 and page > 0 and window >= 0, "step_tables: tokens and window from 0 on, max_blocks and page from 1 on")
-    _need(len(tiles) <= 4 and all(h > 0 and n >= 0 for h, n in tiles), "step_tables: up to four lists of tiles (height, count)")
-    _need(lora_tiles >= 0 and lora_rows > 0, "step_tables: lora_tiles from 0 on, lora_rows from 1 on")
-    _need(lead is None or (lead.dtype == torch.int32 and lead.dim() == 2 and lead.shape[1] == 4 and lead.is_contiguous() and lead.device == seqs.device
-                           and lead.data_ptr() % 16 == 0), "step_tables: lead is [n, 4] int32, contiguous, on a 16-byte boundary")
+    if not (seqs.dtype == torch.int32 and seqs.dim() == 2 and seqs.shape[0] == 4 and (seqs.shape[1] <= 1 or seqs.stride(1) == 1)):
+        raise ValueError("step_tables: seqs is [4, sequences] int32 (tokens, cached tokens, adapter slot, pages)")
+    if not (seqs.shape[1] <= STEP_SEQS_MAX):
+        raise ValueError(f"step_tables: {seqs.shape[1]} sequences, at most {STEP_SEQS_MAX}")
+    if not (pages.dtype == torch.int32 and pages.dim() == 1 and pages.is_contiguous() and pages.device == seqs.device):
+        raise ValueError("step_tables: pages is one contiguous int32 list on the device of seqs")
+    if not (tokens >= 0 and max_blocks > 0 and page > 0 and window >= 0):
+        raise ValueError("step_tables: tokens and window from 0 on, max_blocks and page from 1 on")
+    if not (len(tiles) <= 4 and all(h > 0 and n >= 0 for h, n in tiles)):
+        raise ValueError("step_tables: up to four lists of tiles (height, count)")
+    if not (lora_tiles >= 0 and lora_rows > 0):
+        raise ValueError("step_tables: lora_tiles from 0 on, lora_rows from 1 on")
+    if not (lead is None or (lead.dtype == torch.int32 and lead.dim() == 2 and lead.shape[1] == 4 and lead.is_contiguous() and lead.device == seqs.device
+                           and lead.data_ptr() % 16 == 0)):
+        raise ValueError("step_tables: lead is [n, 4] int32, contiguous, on a 16-byte boundary")
     return seqs.shape[1]
 
 
@@ -1067,18 +1067,28 @@ MOE_FEW_ACTS = ("silu", "swish", "gelu", "gelu_new", "gelu_pytorch_tanh", "gelu_
 
 def check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out):
     """-> (tokens, experts, width, features)."""
-    _need(x.dim() == 2 and router_w.dim() == 2 and w13.dim() == 3 and w2.dim() == 3, "moe_few: x [T, H], router_w [E, H], w13 [e, 2 I, H], w2 [e, H, I]")
+    if not (x.dim() == 2 and router_w.dim() == 2 and w13.dim() == 3 and w2.dim() == 3):
+        raise ValueError("moe_few: x [T, H], router_w [E, H], w13 [e, 2 I, H], w2 [e, H, I]")
     (T, H), E, e_local, inter = x.shape, router_w.shape[0], w13.shape[0], w2.shape[2]
-    _need(T <= MOE_FEW_TOKENS, f"moe_few: {T} tokens, at most {MOE_FEW_TOKENS} (moe_ffn takes any number)")
-    _need(router_w.shape[1] == H and w13.shape == (e_local, 2 * inter, H) and w2.shape == (e_local, H, inter), "moe_few: the shapes of the weights do not fit")
-    _need(1 <= k <= min(E, 32) and E <= 256, f"moe_few: {k} of {E} experts; at most 32 of 256")
-    _need(0 <= e0 and e0 + e_local <= E, f"moe_few: experts {e0} .. {e0 + e_local} of {E}")
-    _need(H > 0 and inter > 0 and H % 8 == 0 and inter % 8 == 0, "moe_few: width and features are multiples of 8")
-    _need(act in MOE_FEW_ACTS, f"moe_few: activation {act!r}")
-    _need(all(t.dtype == x.dtype and t.device == x.device for t in (router_w, w13, w2)), "moe_few: the weights have another type or device than x")
-    _need(x.stride(1) == 1 and x.stride(0) % 8 == 0 and router_w.stride(1) == 1 and router_w.stride(0) % 8 == 0 and w13.is_contiguous() and w2.is_contiguous()
-          and all(t.data_ptr() % 16 == 0 for t in (x, router_w, w13, w2)), "moe_few: rows on 16-byte boundaries, experts stacked without gaps")
-    _need(out is None or (out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and out.stride(1) == 1), "moe_few: out is like x")
+    if not (T <= MOE_FEW_TOKENS):
+        raise ValueError(f"moe_few: {T} tokens, at most {MOE_FEW_TOKENS} (moe_ffn takes any number)")
+    if not (router_w.shape[1] == H and w13.shape == (e_local, 2 * inter, H) and w2.shape == (e_local, H, inter)):
+        raise ValueError("moe_few: the shapes of the weights do not fit")
+    if not (1 <= k <= min(E, 32) and E <= 256):
+        raise ValueError(f"moe_few: {k} of {E} experts; at most 32 of 256")
+    if not (0 <= e0 and e0 + e_local <= E):
+        raise ValueError(f"moe_few: experts {e0} .. {e0 + e_local} of {E}")
+    if not (H > 0 and inter > 0 and H % 8 == 0 and inter % 8 == 0):
+        raise ValueError("moe_few: width and features are multiples of 8")
+    if not (act in MOE_FEW_ACTS):
+        raise ValueError(f"moe_few: activation {act!r}")
+    if not (router_w.dtype == w13.dtype == w2.dtype == x.dtype and router_w.device == w13.device == w2.device == x.device):
+        raise ValueError("moe_few: the weights have another type or device than x")
+    if not (x.stride(1) == 1 and x.stride(0) % 8 == 0 and router_w.stride(1) == 1 and router_w.stride(0) % 8 == 0 and w13.is_contiguous() and w2.is_contiguous()
+            and (x.data_ptr() | router_w.data_ptr() | w13.data_ptr() | w2.data_ptr()) % 16 == 0):
+        raise ValueError("moe_few: rows on 16-byte boundaries, experts stacked without gaps")
+    if not (out is None or (out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and out.stride(1) == 1)):
+        raise ValueError("moe_few: out is like x")
     return T, E, H, inter
 
 
@@ -1114,13 +1124,15 @@ class TokenScores(NamedTuple):
 
 def check_token_scores(logits, targets, k, softcap):
     """-> (rows, vocabulary)."""
-    _need(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1) and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1]),
-          "token_scores: logits are [rows, vocabulary], the logits of a row side by side")
+    if not (logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1) and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1])):
+        raise ValueError("token_scores: logits are [rows, vocabulary], the logits of a row side by side")
     T, V = logits.shape
-    _need(0 <= k <= min(TOP_MAX, V), f"token_scores: {k} alternatives of {V} tokens, at most {TOP_MAX}")
-    _need(softcap >= 0.0, "token_scores: softcap from 0 on (0: none)")
-    _need(targets is None or (targets.shape == (T,) and targets.dtype in (torch.int32, torch.int64) and targets.device == logits.device),
-          "token_scores: one int32 or int64 target a row, on the device of the logits")
+    if not (0 <= k <= min(TOP_MAX, V)):
+        raise ValueError(f"token_scores: {k} alternatives of {V} tokens, at most {TOP_MAX}")
+    if not (softcap >= 0.0):
+        raise ValueError("token_scores: softcap from 0 on (0: none)")
+    if not (targets is None or (targets.shape == (T,) and targets.dtype in (torch.int32, torch.int64) and targets.device == logits.device)):
+        raise ValueError("token_scores: one int32 or int64 target a row, on the device of the logits")
     return T, V
 
 
