@@ -6,7 +6,6 @@ Arguments that do not fit raise ValueError in front of any launch.  Outputs and 
 
 from __future__ import annotations
 
-import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Sequence, Tuple
 
@@ -21,7 +20,7 @@ SIGNATURES = {
     "lx_step_tables_max_seqs": ([], I),
     "lx_step_tables": ([P, L, P, I, I, I, I, I, I, I, P, P, I, P, I, I, I, P, P], I),
     "lx_moe_few_max_tokens": ([], I),
-    "lx_moe_few": ([P, L, P, L, P, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, I, P], I),
+    "lx_moe_few": ([P, L, P, L, P, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, P, I, P], I),
     "lx_token_scores_max_top": ([], I),
     "lx_token_scores": ([P, L, I, I, I, P, I, I, F, P, P, P, P, P], I),
 }
@@ -40,11 +39,6 @@ def _stream_for(*tensors: Optional[torch.Tensor]) -> int:
         if t is not None and t.get_device() != here:
             raise ValueError(f"a tensor on {t.device} while cuda:{here} is the current device")
     return torch._C._cuda_getCurrentRawStream(here)
-
-
-@functools.lru_cache(maxsize=None)
-def _num_sms(device: int) -> int:
-    return torch.cuda.get_device_properties(device).multi_processor_count
 
 
 def step_tables(seqs: torch.Tensor, pages: torch.Tensor, tokens: int, max_blocks: int, page: int, window: int = 0,
@@ -80,10 +74,10 @@ def moe_few(x: torch.Tensor, router_w: torch.Tensor, w13: torch.Tensor, w2: torc
     # scratch: h (two planes), then the logits, then the choice of experts
     h_bytes, logits_bytes = (4 * T * k * inter + 15) // 16 * 16, 4 * T * E
     scratch = torch.empty(h_bytes + logits_bytes + 4 * T * k, dtype=torch.uint8, device=x.device)
-    at = scratch.data_ptr()
+    at, ws = scratch.data_ptr(), nv.workspace(x.device)
     rc = nv.load().lx_moe_few(x.data_ptr(), x.stride(0), router_w.data_ptr(), router_w.stride(0), w13.data_ptr(), w2.data_ptr(), at + h_bytes,
                               at + h_bytes + logits_bytes, at, out.data_ptr(), out.stride(0), T, E, k, e0, w13.shape[0], H, inter, nv._ACTS[act], int(renorm),
-                              scale, _num_sms(x.get_device()), stream)
+                              scale, ws.status.data_ptr(), ws.num_sms, stream)
     nv._check(rc, "lx_moe_few")
     nv.launch_count += 2                 # (three kernels)
     return out
