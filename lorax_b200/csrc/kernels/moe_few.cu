@@ -6,13 +6,14 @@
 //   up      h[t, j, i] = w[t, j] act(G_e[i] . x_t) (U_e[i] . x_t)    for the experts e = e(t, j) that this rank owns
 //   down    out[t, n] = sum_j D_e[n] . h[t, j]
 //
-// Both products are streams of weights against at most 16 columns.  A thread of a CTA keeps a ring of shared memory filled by TMA, some 100 KB of it
-// on their way.  A box is 64 of K x some rows x up to 16 times 64 of K further on: the tensor map takes a row's blocks of 64 as a dimension of
-// their own, so that one copy brings 16 to 32 KB (bulk copies of one row's 1 to 2 KB each took 50 ns apiece: 5.0 and 3.2 TB/s; 16-byte loads
-// into registers, 96 KB in flight, 5.4 and 4.1).  The tokens' side of a stage travels in it, a copy a token: loaded by the math warps it came through
-// the same queues as the weights, 2 to 4 us behind its request.  Eight warps multiply what has arrived by mma.sync: the weights are the A operand
-// (16 rows x 16 of K), read 16 bytes a lane in the order of K in which they lie (the other operand is read in the same order, so the sum is
-// the same); tokens stand in the columns, those that an expert does not serve as zeros.  What is left of K behind its last 64 is loaded directly.
+// Both products are streams of weights against at most 16 columns.  A thread of a CTA keeps a ring of shared memory filled by TMA, 200 KB of it.
+// A box is 64 of K x some rows x up to 32 times 64 of K further on: the tensor map takes a row's blocks of 64 as a dimension of their own, so
+// that one copy brings up to 32 KB (bulk copies of one row's 1 to 2 KB each took 50 ns apiece: 5.0 and 3.2 TB/s; 16-byte loads into registers,
+// 96 KB in flight, 5.4 and 4.1).  What a row has behind its last block comes through a second map, which ends with the row.  The tokens' side of
+// a stage travels in it, a copy a token: loaded by the math warps it came through the same queues as the weights, 2 to 4 us behind its request.
+// Eight warps multiply what has arrived by mma.sync: the weights are the A operand (16 rows x 16 of K), read 16 bytes a lane in the order of
+// K in which they lie (the other operand is read in the same order, so the sum is the same); tokens stand in the columns, those that an expert
+// does not serve as zeros.
 //   up:   the rows of all reached experts, eight features of gate and up to a tile, are dealt evenly to the CTAs; the warps split K and sum
 //         their parts through shared memory
 //   down: the rows of the output are dealt to the CTAs; K runs over the reached experts' features one expert behind the other, so the sum
@@ -33,11 +34,10 @@ constexpr int kFewMath = 8;                // warps that multiply; one more fill
 constexpr int kFewWarps = kFewMath + 1;
 constexpr int kFewThreads = 32 * kFewWarps;
 constexpr int kFewRowTiles = 4;            // tiles of 16 rows of a CTA (down)
-constexpr int kFewUpSteps = 4;             // steps of 32 of K of a stage and a math warp, at most (up)
+constexpr int kFewUpSteps = 8;             // steps of 32 of K of a stage and a math warp, at most (up): stages of 64 KB (of 32 KB: 110 -> 114 us for one token)
 constexpr int kFewMaxStages = 16;
-constexpr int kFewInFlight = 104 * 1024;   // bytes of weights on their way: more of them only wait longer (96 and 192 KB: 6.4 TB/s both)
-constexpr int kFewSums = 2;                // tiles whose sums over the math warps may wait (up)
-constexpr int kFewSmem = 232448 - 14 * 1024;      // (the rest: what is static)
+constexpr int kFewSums = 4;                // tiles of eight columns whose sums over the math warps may wait (up)
+constexpr int kFewSmem = 232448 - 17 * 1024;      // (the rest: what is static)
 
 enum FewAct : int { kFewSilu = 0, kFewGelu = 1, kFewGeluTanh = 2, kFewRelu = 3, kFewRelu2 = 4 };
 
@@ -49,15 +49,14 @@ struct MoeFewParams {
   const float* logits;         // [T, E], or null: the up kernel forms them itself
   const __nv_bfloat16* w13;    // [e_local, 2 I, H]: gate rows, then up rows
   const __nv_bfloat16* w2;     // [e_local, H, I]
-  int* ids;                    // [T, k]: the chosen experts, for the second kernel
   __nv_bfloat16* h;            // two planes of [T k, I], in the order of the experts
   __nv_bfloat16* out;          // [T, H]
   long long ldo;
   int* status;
   int T, E, k, e0, e_local, H, I, act, renorm;
   float scale;
-  // blocks of 64 of K of a stage of the up and the down kernel; rows of a stage of the latter
-  int up_blocks, down_blocks, down_rows;
+  // blocks of 64 of K of a copy of the up and of a stage of the down kernel; rows of a stage of the latter, and the logarithm of the rows of h that a copy brings
+  int up_blocks, down_blocks, down_rows, h_shift;
 };
 
 LX_DEVICE void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -69,7 +68,7 @@ LX_DEVICE void few_mma32(float (&d)[4], const uint4& p, const uint4& q, const ui
   few_mma(d, p.x, q.x, p.y, q.y, b.x, b.y);
   few_mma(d, p.z, q.z, p.w, q.w, b.z, b.w);
 }
-// Eight elements of K behind the last block, or zeros.
+// Eight elements, or zeros.
 LX_DEVICE uint4 few_load(const __nv_bfloat16* p, bool valid) {
   uint4 v;
   asm volatile(
@@ -95,13 +94,12 @@ LX_DEVICE float few_act(float x, int act) {
 
 // ------------------------------------------------------------------------------------------------ choice of experts, and who is reached
 struct FewPlan {
-  float w[kFewTokens * kFewTop];
-  int ids[kFewTokens * kFewTop];
+  float w[kFewTokens * kFewTop];                // of a token's choices
   uint32_t mask[kFewExperts];                   // tokens of a local expert
   uint8_t place[kFewTokens][kFewExperts];       // which of its choices a local expert is for a token
   short list[kFewExperts];                      // local experts that have a token, ascending
   short base[kFewExperts];                      // the first row of h of each of those
-  int warps[kFewWarps];
+  int4 warps[kFewWarps];
   int reached, most;                            // number of those, and the most tokens of one
 };
 
@@ -152,113 +150,124 @@ LX_DEVICE void few_route(float* z, float4* red, const MoeFewParams& p) {
   __syncthreads();
 }
 
-// One warp per token.  A NaN orders as -inf (its weight is NaN all the same); no expert is chosen twice.
+// One warp per token, PER experts a lane: its experts, their weights, and its mark with those that this rank owns (plan.mask is zero).  A NaN
+// orders as -inf (its weight is NaN all the same); no expert is chosen twice.
+template <int PER>
 LX_DEVICE void few_select(FewPlan& plan, const float* logits, const MoeFewParams& p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kPer = kFewExperts / 32;
   for (int t = warp; t < p.T; t += kFewWarps) {
     const float* row = logits + t * p.E;
-    float z[kPer];
-    uint32_t taken = 0;
+    float z[PER];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = lane + 32 * i;
-      z[i] = e < p.E ? row[e] : 0.f;
-      if (e >= p.E) taken |= 1u << i;
+    for (int i = 0; i < PER; ++i) z[i] = lane + 32 * i < p.E ? row[lane + 32 * i] : 0.f;
+    // logits as numbers whose order is theirs; 0: taken, or no expert
+    uint32_t key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float v = z[i] == z[i] ? z[i] + 0.f : -INFINITY;
+      const uint32_t b = __float_as_uint(v);
+      key[i] = lane + 32 * i < p.E ? ((b >> 31) ? ~b : b | 0x80000000u) : 0;
     }
-    float all = 0.f, top = 0.f, own = 0.f;
+    float top = 0.f, mine = 0.f;
     int id = 0;
     for (int j = 0; j < p.k; ++j) {
-      float bv = -INFINITY;
-      int bi = 0x7fffffff;
+      uint32_t best = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const float v = z[i] == z[i] ? z[i] : -INFINITY;
-        if (!((taken >> i) & 1) && (bi == 0x7fffffff || v > bv)) { bv = v; bi = lane + 32 * i; }
-      }
+      for (int i = 0; i < PER; ++i) best = max(best, key[i]);
+      best = __reduce_max_sync(0xffffffffu, best);
+      int lowest = kFewExperts;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-        const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-        if (oi != 0x7fffffff && (bi == 0x7fffffff || ov > bv || (ov == bv && oi < bi))) { bv = ov; bi = oi; }
-      }
+      for (int i = PER - 1; i >= 0; --i)
+        if (key[i] == best) lowest = lane + 32 * i;
+      const int e = __reduce_min_sync(0xffffffffu, lowest);
       float v = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i == (bi >> 5)) {
-          v = z[i];
-          if (lane == (bi & 31)) taken |= 1u << i;
-        }
-      v = __shfl_sync(0xffffffffu, v, bi & 31);
+      for (int i = 0; i < PER; ++i)
+        if (lane + 32 * i == e) { v = z[i]; key[i] = 0; }
+      v = __shfl_sync(0xffffffffu, v, e & 31);
       if (j == 0) top = v;
-      if (lane == j) { id = bi; own = expf(v - top); }
+      if (lane == j) { id = e; mine = v; }
     }
-    if (p.renorm) {
-      all = warp_sum(lane < p.k ? own : 0.f);
-    } else {
+    const float own = lane < p.k ? expf(mine - top) : 0.f;
+    float all = own;
+    if (!p.renorm) {
+      all = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
+      for (int i = 0; i < PER; ++i)
         if (lane + 32 * i < p.E) all += expf(z[i] - top);
-      all = warp_sum(all);
     }
-    if (lane < p.k) {
-      plan.ids[t * p.k + lane] = id;
+    all = warp_sum(all);
+    const int e = id - p.e0;
+    if (lane < p.k && e >= 0 && e < p.e_local) {
       plan.w[t * p.k + lane] = own / all * p.scale;
+      plan.place[t][e] = (uint8_t)lane;
+      atomicOr(&plan.mask[e], 1u << t);
     }
   }
 }
 
-// From plan.ids: which tokens every local expert serves, and the experts that serve any.
-LX_DEVICE void few_reached(FewPlan& plan, const MoeFewParams& p) {
+// The experts that serve any token, and where their rows of h begin: one thread an expert.
+LX_DEVICE void few_reached(FewPlan& plan) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   static_assert(kFewThreads >= kFewExperts, "a thread for every expert");
-  if (threadIdx.x < kFewExperts) plan.mask[threadIdx.x] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.T * p.k; i += kFewThreads) {
-    const int e = plan.ids[i] - p.e0, t = i / p.k;
-    if (e >= 0 && e < p.e_local) {
-      atomicOr(&plan.mask[e], 1u << t);
-      plan.place[t][e] = (uint8_t)(i - t * p.k);
-    }
+  const int n = threadIdx.x < kFewExperts ? __popc(plan.mask[threadIdx.x]) : 0;
+  const uint32_t votes = __ballot_sync(0xffffffffu, n > 0);
+  int v = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
   }
+  const int most = __reduce_max_sync(0xffffffffu, n);
+  if (lane == 31) plan.warps[warp] = make_int4(__popc(votes), v, most, 0);
   __syncthreads();
-  const bool has = threadIdx.x < kFewExperts && plan.mask[threadIdx.x] != 0;
-  const uint32_t votes = __ballot_sync(0xffffffffu, has);
-  if (lane == 0) plan.warps[warp] = __popc(votes);
-  __syncthreads();
-  int at = __popc(votes & ((1u << lane) - 1)), all = 0;
+  int at = __popc(votes & ((1u << lane) - 1)), row = v - n, all = 0, top = 0;
 #pragma unroll
   for (int i = 0; i < kFewWarps; ++i) {
-    if (i < warp) at += plan.warps[i];
-    all += plan.warps[i];
+    const int4 w = plan.warps[i];
+    if (i < warp) { at += w.x; row += w.y; }
+    all += w.x;
+    top = max(top, w.z);
   }
-  if (has) plan.list[at] = (short)threadIdx.x;
-  if (threadIdx.x == 0) plan.reached = all;
-  __syncthreads();
-  if (warp == 0) {
-    int sum = 0, most = 0;
-    for (int d0 = 0; d0 < all; d0 += 32) {
-      const int n = d0 + lane < all ? __popc(plan.mask[plan.list[d0 + lane]]) : 0;
-      most = max(most, n);
-      int v = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
-      if (d0 + lane < all) plan.base[d0 + lane] = (short)(sum + v - n);
-      sum += __shfl_sync(0xffffffffu, v, 31);
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) plan.most = most;
+  if (n > 0) {
+    plan.list[at] = (short)threadIdx.x;
+    plan.base[at] = (short)row;
+  }
+  if (threadIdx.x == 0) {
+    plan.reached = all;
+    plan.most = top;
   }
   __syncthreads();
+}
+
+// The plan of the launch, by every CTA for itself: from the logits that a kernel in front of the up kernel left, or from logits of its own.
+template <int NT>
+LX_DEVICE void few_choose(FewPlan& plan, uint8_t* smem, const MoeFewParams& p) {
+  const float* logits = p.logits;
+  if (threadIdx.x < kFewExperts) plan.mask[threadIdx.x] = 0;
+  __syncthreads();
+  if (logits == nullptr) {
+    float4* sums = reinterpret_cast<float4*>(smem);
+    float* z = reinterpret_cast<float*>(sums + kFewWarps * ((p.E + 15) / 16) * NT * 32);
+    few_route<NT>(z, sums, p);
+    logits = z;
+  }
+  if (p.E <= 64) few_select<2>(plan, logits, p);
+  else few_select<kFewExperts / 32>(plan, logits, p);
+  fence_proxy_async_smem();                    // (the ring lies where the sums and logits did)
+  __syncthreads();
+  few_reached(plan);
 }
 
 // Row of h of token t (one of `mask`) within its expert's.
 LX_DEVICE int few_slot(uint32_t mask, int t) { return __popc(mask & ((1u << t) - 1)); }
+// Copies of 2^shift rows of h that bring n of them.
+LX_DEVICE int few_copies(int n, int shift) { return (n + (1 << shift) - 1) >> shift; }
 // The i-th token of `mask`.
-LX_DEVICE int few_token(uint32_t mask, int i) { return __fns(mask, 0, i + 1); }
+LX_DEVICE int few_token(uint32_t mask, int i) {
+  for (; i > 0; --i) mask &= mask - 1;
+  return __ffs(mask) - 1;
+}
 
 // ------------------------------------------------------------------------------------------------ the ring
 // Stages of shared memory, filled by one warp and read by the math warps.  Waits are bounded: one that runs out is reported, the filling warp stops (and
@@ -277,9 +286,6 @@ LX_DEVICE void few_ring_init(FewRing& r) {
     mbar_fence_init();
   }
 }
-
-// Stages of `bytes` each, `weights` of them weights: as many as are worth having on their way.
-LX_DEVICE int few_stages(int ring, int bytes, int weights) { return min(min(max(3, kFewInFlight / weights), ring / bytes), kFewMaxStages); }
 
 struct FewCursor {
   int stage = 0;
@@ -343,11 +349,22 @@ LX_DEVICE uint4 few_row(uint32_t at) {
 }
 constexpr int kFewZeros = kFewUpSteps * 512;      // what the lanes of a column without a token read instead of one
 
+// Tensor maps of a product's operands: whole blocks of 64 of K, and what is behind them.  [1]: boxes of twice the blocks (up).
+struct FewMaps {
+  CUtensorMap weights[2], tokens[2], weights_rest, tokens_rest;
+};
+
+LX_DEVICE void few_prefetch(const FewMaps& maps) {
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&maps.weights[0]);
+    tma_prefetch_desc(&maps.tokens[0]);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ up
 // NT: columns of eight tokens.
 template <int NT>
-__global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid_constant__ CUtensorMap weights, const __grid_constant__ CUtensorMap tokens,
-                                                                    const __grid_constant__ MoeFewParams p) {
+__global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ MoeFewParams p) {
   __shared__ FewPlan plan;
   __shared__ FewRing ring;
   __shared__ __align__(16) uint8_t zeros[kFewZeros];
@@ -356,25 +373,20 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c8 = (lane & 3) * 8;
   few_ring_init(ring);
   for (int i = tid; i < kFewZeros / 4; i += kFewThreads) reinterpret_cast<uint32_t*>(zeros)[i] = 0;
+  few_prefetch(maps);
   pdl_wait();
   pdl_trigger();
-  const float* logits = p.logits;
-  if (logits == nullptr) {
-    float4* sums = reinterpret_cast<float4*>(smem);
-    float* z = reinterpret_cast<float*>(sums + kFewWarps * ((p.E + 15) / 16) * NT * 32);
-    few_route<NT>(z, sums, p);
-    logits = z;
-  }
-  few_select(plan, logits, p);
-  fence_proxy_async_smem();                    // (the ring lies where the sums and logits did)
-  __syncthreads();
-  few_reached(plan, p);
-  if (blockIdx.x == 0)
-    for (int i = tid; i < p.T * p.k; i += kFewThreads) p.ids[i] = plan.ids[i];
-  // a stage: gate rows, up rows, then the expert's tokens
-  const int units = p.I / 8, blocks = p.H / 64, chunks = (blocks + p.up_blocks - 1) / p.up_blocks, half = p.up_blocks * 1024;
-  const int token = p.up_blocks * 128, stage_bytes = (2 * half + plan.most * token + 1023) & ~1023;
-  const int stages = few_stages(kFewSmem - 1024 - kFewSums * kFewMath * NT * 32 * (int)sizeof(float4), stage_bytes, 2 * half);
+  few_choose<NT>(plan, smem, p);
+  // A stage: gate rows, up rows, the expert's tokens (in large boxes where two such stages fit); the same of what is behind the last block, for a
+  // tile's last stage.
+  const int units = p.I / 8, blocks = p.H / 64, most = plan.most;
+  const bool rest = p.H % 64 != 0;
+  constexpr int kSums = kFewSums / NT, kRoom = kFewSmem - 1024 - kSums * kFewMath * NT * 32 * (int)sizeof(float4);
+  const auto stage_of = [&](int b) { return ((b * (2048 + most * 128) + 1023) & ~1023) + (rest ? (2048 + most * 128 + 1023) & ~1023 : 0); };
+  const bool large = blocks > p.up_blocks && 2 * stage_of(2 * p.up_blocks) <= kRoom;
+  const int wide = p.up_blocks << large;
+  const int chunks = max(1, (blocks + wide - 1) / wide), half = wide * 1024, token = wide * 128;
+  const int rest_at = (2 * half + most * token + 1023) & ~1023, stage_bytes = stage_of(wide), stages = min(kRoom / stage_bytes, kFewMaxStages);
   const long long all = (long long)plan.reached * units;
   const int u0 = (int)(all * blockIdx.x / gridDim.x), u1 = (int)(all * (blockIdx.x + 1) / gridDim.x);
   FewCursor at;
@@ -383,16 +395,31 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
       const uint64_t policy = policy_evict_first();
       long long filled = 0;
       bool ok = true;
+      int d = u0 / units, c = (u0 - d * units) * 8 - 8, e = 0, n = 0;
+      uint32_t mask = 0;
       for (int u = u0; ok && u < u1; ++u) {
-        const int d = u / units, c = (u - d * units) * 8, e = plan.list[d];
-        const uint32_t mask = plan.mask[e], bytes = 2 * half + __popc(mask) * token;
+        if ((c += 8) == p.I) { c = 0; ++d; }
+        if (u == u0 || c == 0) {
+          e = plan.list[d];
+          mask = plan.mask[e];
+          n = __popc(mask);
+        }
         for (int ch = 0; ok && ch < chunks; ++ch, ++filled) {
           uint8_t* stage = smem + at.stage * stage_bytes;
-          ok = few_fill(ring, at, stages, bytes, p.status, [&](uint64_t* bar) {
-            tma_load_4d_hint(stage, &weights, bar, 0, c, ch * p.up_blocks, e, policy);
-            tma_load_4d_hint(stage + half, &weights, bar, 0, p.I + c, ch * p.up_blocks, e, policy);
-            uint8_t* to = stage + 2 * half;
-            for (uint32_t m = mask; m != 0; m &= m - 1, to += token) tma_load_4d(to, &tokens, bar, 0, __ffs(m) - 1, ch * p.up_blocks, 0);
+          const bool ends = rest && ch == chunks - 1;
+          ok = few_fill(ring, at, stages, (blocks > 0 ? 2 * half + n * token : 0) + (ends ? 2048 + n * 128 : 0), p.status, [&](uint64_t* bar) {
+            if (blocks > 0) {
+              tma_load_4d_hint(stage, &maps.weights[large], bar, 0, c, ch * wide, e, policy);
+              tma_load_4d_hint(stage + half, &maps.weights[large], bar, 0, p.I + c, ch * wide, e, policy);
+              uint8_t* to = stage + 2 * half;
+              for (uint32_t m = mask; m != 0; m &= m - 1, to += token) tma_load_4d(to, &maps.tokens[large], bar, 0, __ffs(m) - 1, ch * wide, 0);
+            }
+            if (ends) {
+              tma_load_4d_hint(stage + rest_at, &maps.weights_rest, bar, blocks * 64, c, 0, e, policy);
+              tma_load_4d_hint(stage + rest_at + 1024, &maps.weights_rest, bar, blocks * 64, p.I + c, 0, e, policy);
+              uint8_t* to = stage + rest_at + 2048;
+              for (uint32_t m = mask; m != 0; m &= m - 1, to += 128) tma_load_4d(to, &maps.tokens_rest, bar, blocks * 64, __ffs(m) - 1, 0, 0);
+            }
           });
         }
       }
@@ -400,36 +427,29 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
     }
     return;
   }
-  float4* red = reinterpret_cast<float4*>(smem + stages * stage_bytes);      // [kFewSums][math warps][NT][32 lanes]
-  const int steps = 2 * blocks, per = 2 * p.up_blocks, place = few_place(8, few_lane_row(g), warp, c8), column = 2 * half + (warp * 32 + c8) * 2;
-  const int rest = blocks * 64 + warp * 32 + c8;      // K of this lane behind the blocks
+  float4* red = reinterpret_cast<float4*>(smem + stages * stage_bytes);      // [kSums][math warps][NT][32 lanes]
+  const int steps = 2 * blocks, per = 2 * wide, place = few_place(8, few_lane_row(g), warp, c8), column = (warp * 32 + c8) * 2;
   bool ok = true;
   uint32_t sums_phase = 0;
   // A tile for an expert of up to 8 N tokens: they stand in the columns in their order.
+  int d = u0 / units, c = (u0 - d * units) * 8 - 8, e = 0, served = 0;
+  uint32_t mask = 0;
   auto tile = [&](auto n, int u) {
     constexpr int N = decltype(n)::value;
-    const int d = u / units, e = plan.list[d], col = (u - d * units) * 8 + few_lane_row(g), buf = (u - u0) % kFewSums;
-    const uint32_t mask = plan.mask[e];
-    const int served = __popc(mask);
+    const int col = c + few_lane_row(g), buf = (u - u0) % kSums;
     float acc[2][N][4];                        // (two chains of MMAs)
 #pragma unroll
     for (int o = 0; o < 2; ++o)
 #pragma unroll
       for (int m = 0; m < N; ++m) acc[o][m][0] = acc[o][m][1] = acc[o][m][2] = acc[o][m][3] = 0.f;
-    if (blocks * 64 + warp * 32 < p.H) {
-      const __nv_bfloat16* w = p.w13 + ((long long)e * 2 * p.I + col) * p.H + rest;
-      const uint4 gate = few_load(w, rest < p.H), up = few_load(w + (long long)p.I * p.H, rest < p.H);
-#pragma unroll
-      for (int m = 0; m < N; ++m) {
-        const bool on = m * 8 + g < served;
-        few_mma32(acc[0][m], gate, up, few_load(p.x + (on ? few_token(mask, m * 8 + g) * p.ldx : 0) + rest, on && rest < p.H));
-      }
-    }
     for (int ch = 0; ch < chunks; ++ch) {
       const uint32_t stage = smem_u32(smem) + at.stage * stage_bytes;
       uint32_t xt[N];
 #pragma unroll
-      for (int m = 0; m < N; ++m) xt[m] = m * 8 + g < served ? stage + column + (m * 8 + g) * token : smem_u32(zeros);
+      for (int m = 0; m < N; ++m) {
+        const int i = m * 8 + g;
+        xt[m] = i < served ? stage + 2 * half + column + i * token : smem_u32(zeros);
+      }
       few_await(ring, &ring.full[at.stage], at.phase, ok, p.status);
 #pragma unroll
       for (int j = 0; j < kFewUpSteps; ++j) {
@@ -439,6 +459,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
 #pragma unroll
           for (int m = 0; m < N; ++m) few_mma32(acc[j & 1][m], gate, up, few_row(xt[m] + j * 512));
         }
+      }
+      if (rest && ch == chunks - 1 && warp < 2) {
+        const uint4 gate = few_row(stage + rest_at + place), up = few_row(stage + rest_at + 1024 + place);
+#pragma unroll
+        for (int m = 0; m < N; ++m)
+          few_mma32(acc[0][m], gate, up, few_row(m * 8 + g < served ? stage + rest_at + 2048 + (m * 8 + g) * 128 + column : smem_u32(zeros)));
       }
       few_release(ring, at, stages);
     }
@@ -475,22 +501,27 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
       __syncwarp();
       if (lane == 0) mbar_arrive(&ring.read[buf]);
     }
-    if (buf == kFewSums - 1) sums_phase ^= 1;
+    if (buf == kSums - 1) sums_phase ^= 1;
   };
   for (int u = u0; u < u1; ++u) {
-    if (NT == 1 || __popc(plan.mask[plan.list[u / units]]) <= 8) tile(std::integral_constant<int, 1>{}, u);
+    if ((c += 8) == p.I) { c = 0; ++d; }
+    if (u == u0 || c == 0) {
+      e = plan.list[d];
+      mask = plan.mask[e];
+      served = __popc(mask);
+    }
+    if (NT == 1 || served <= 8) tile(std::integral_constant<int, 1>{}, u);
     else tile(std::integral_constant<int, NT>{}, u);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ down
-// MT: tiles of 16 rows; steps of 32 of K of a stage and a math warp: as many as make stages of up to 32 KB.
-template <int MT>
-constexpr int few_down_steps() { return MT == 1 ? 4 : MT == 2 ? 2 : 1; }
+// MT: tiles of 16 rows; steps of 32 of K of a stage and a math warp: as many as make stages of 32 to 64 KB (of half of that, 470 -> 490 us for 16 tokens).
+template <int MT, int NT>
+constexpr int few_down_steps() { return MT == 1 || MT + NT == 3 ? 4 : 2; }
 
 template <int MT, int NT>
-__global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __grid_constant__ CUtensorMap weights, const __grid_constant__ CUtensorMap tokens,
-                                                                      const __grid_constant__ MoeFewParams p) {
+__global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ MoeFewParams p) {
   __shared__ FewPlan plan;
   __shared__ FewRing ring;
   __shared__ __align__(16) uint8_t zeros[kFewZeros];
@@ -499,49 +530,70 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c8 = (lane & 3) * 8;
   few_ring_init(ring);
   for (int i = tid; i < kFewZeros / 4; i += kFewThreads) reinterpret_cast<uint32_t*>(zeros)[i] = 0;
-  pdl_wait();
-  pdl_trigger();
-  for (int i = tid; i < p.T * p.k; i += kFewThreads) plan.ids[i] = p.ids[i];
-  __syncthreads();
-  few_reached(plan, p);
-  // a stage: rows of the weights, then value and remainder of the expert's tokens
-  const int blocks = p.I / 64, chunks = (blocks + p.down_blocks - 1) / p.down_blocks, reached = plan.reached;
-  const int rows = p.down_rows, bytes = p.down_blocks * rows * 128, wide = (bytes + 1023) & ~1023, plane = p.down_blocks * 128;
-  const int stage_bytes = (wide + plan.most * 2 * plane + 1023) & ~1023;
-  const int stages = few_stages(kFewSmem - 1024 - kFewMath * MT * NT * 32 * (int)sizeof(float4), stage_bytes, wide);
+  few_prefetch(maps);
+  // In front of the wait for the up kernel: it has waited itself for what wrote the tokens, the router and the logits, and triggers behind that.
+  few_choose<NT>(plan, smem, p);
+  // A stage: rows of the weights, values and remainders of the expert's tokens; the same of what is behind the last block, for an expert's last stage.
+  const int blocks = p.I / 64, chunks = max(1, (blocks + p.down_blocks - 1) / p.down_blocks), reached = plan.reached, rows = p.down_rows;
+  const int bytes = p.down_blocks * rows * 128, wide = (bytes + 1023) & ~1023, plane = p.down_blocks * 128 << p.h_shift, plane_rest = 128 << p.h_shift;
+  const int copies = few_copies(plan.most, p.h_shift);
+  const bool rest = p.I % 64 != 0;
+  const int rest_at = (wide + copies * 2 * plane + 1023) & ~1023, rest_h = (rest_at + rows * 128 + 127) & ~127;
+  const int stage_bytes = rest ? (rest_h + copies * 2 * plane_rest + 1023) & ~1023 : rest_at;
+  const int stages = min((kFewSmem - 1024 - kFewMath * MT * NT * 32 * (int)sizeof(float4)) / stage_bytes, kFewMaxStages);
   FewCursor at;
   if (warp == kFewMath) {
     if (lane == 0) {
       const uint64_t policy = policy_evict_first();
       long long filled = 0;
       bool ok = true;
+      // the weights of the first round of stages go ahead of the wait; their tokens follow
+      bool waited = false;
+      auto copies_of = [&](int d) { return few_copies(__popc(plan.mask[plan.list[d]]), p.h_shift); };
+      auto tokens_of = [&](uint8_t* stage, uint64_t* bar, int row, int n, int ch) {
+        if (blocks > 0)
+          for (int i = 0; i < n; ++i) tma_load_4d(stage + wide + i * 2 * plane, &maps.tokens[0], bar, 0, row + (i << p.h_shift), ch * p.down_blocks, 0);
+        if (rest && ch == chunks - 1)
+          for (int i = 0; i < n; ++i) tma_load_4d(stage + rest_h + i * 2 * plane_rest, &maps.tokens_rest, bar, blocks * 64, row + (i << p.h_shift), 0, 0);
+      };
+      auto catch_up = [&]() {
+        pdl_wait();
+        waited = true;
+        int d = 0, ch = 0;
+        for (int i = 0; i < filled; ++i) {
+          tokens_of(smem + i * stage_bytes, &ring.full[i], plan.base[d], copies_of(d), ch);
+          if (++ch == chunks) { ch = 0; d = d + 1 == reached ? 0 : d + 1; }
+        }
+      };
       for (int r0 = blockIdx.x * rows; ok && r0 < p.H; r0 += gridDim.x * rows)
         for (int d = 0; ok && d < reached; ++d) {
-          const int n = __popc(plan.mask[plan.list[d]]);
+          const int e = plan.list[d], row = plan.base[d], n = copies_of(d), whole = blocks > 0 ? bytes + n * 2 * plane : 0;
           for (int ch = 0; ok && ch < chunks; ++ch, ++filled) {
+            if (!waited && filled == stages) catch_up();
             uint8_t* stage = smem + at.stage * stage_bytes;
-            ok = few_fill(ring, at, stages, bytes + n * 2 * plane, p.status, [&](uint64_t* bar) {
-              tma_load_4d_hint(stage, &weights, bar, 0, r0, ch * p.down_blocks, plan.list[d], policy);
-              for (int i = 0; i < n; ++i) tma_load_4d(stage + wide + i * 2 * plane, &tokens, bar, 0, plan.base[d] + i, ch * p.down_blocks, 0);
+            const bool ends = rest && ch == chunks - 1;
+            ok = few_fill(ring, at, stages, whole + (ends ? rows * 128 + n * 2 * plane_rest : 0), p.status, [&](uint64_t* bar) {
+              if (blocks > 0) tma_load_4d_hint(stage, &maps.weights[0], bar, 0, r0, ch * p.down_blocks, e, policy);
+              if (ends) tma_load_4d_hint(stage + rest_at, &maps.weights_rest, bar, blocks * 64, r0, 0, e, policy);
+              if (waited) tokens_of(stage, bar, row, n, ch);
             });
           }
         }
+      if (!waited) catch_up();
       few_drain(ring, at, stages, filled);
     }
     return;
   }
+  pdl_wait();
+  pdl_trigger();
   float4* red = reinterpret_cast<float4*>(smem + stages * stage_bytes);      // [math warps][MT][NT][32 lanes]
-  constexpr int kSteps = few_down_steps<MT>();
-  const int steps = 2 * blocks, per = 2 * p.down_blocks, column = wide + (warp * 32 + c8) * 2;
-  int row[MT][2], place[MT][2];
+  constexpr int kSteps = few_down_steps<MT, NT>();
+  const int steps = 2 * blocks, per = 2 * p.down_blocks;
+  int place[MT][2];                            // (rows past the last one are taken from it: nobody stores their sums)
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      row[m][o] = min(m * 16 + o * 8 + few_lane_row(g), rows - 1);      // rows past the last one are taken from it: nobody stores their sums
-      place[m][o] = few_place(rows, row[m][o], warp, c8);
-    }
-  const int rest = blocks * 64 + warp * 32 + c8;      // K of this lane behind the blocks
+    for (int o = 0; o < 2; ++o) place[m][o] = few_place(rows, min(m * 16 + o * 8 + few_lane_row(g), rows - 1), warp, c8);
   bool ok = true;
   for (int r0 = blockIdx.x * rows; r0 < p.H; r0 += gridDim.x * rows) {
     const int last = min(r0 + rows, p.H);
@@ -562,16 +614,24 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
     for (int d = 0; d < reached; ++d) {
       const int e = plan.list[d];
       const uint32_t mask = plan.mask[e];
-      int slot[NT];                            // where the lane's tokens lie in a stage
+      // where the lane's tokens lie in a stage: copies of some rows, in each the rows of a block side by side, the blocks of the values, those of
+      // the remainders
+      int slot[NT], slot_rest[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) slot[n] = ((mask >> (n * 8 + g)) & 1) ? column + few_slot(mask, n * 8 + g) * 2 * plane : -1;
+      for (int n = 0; n < NT; ++n) {
+        const int i = few_slot(mask, n * 8 + g);
+        slot_rest[n] = rest_h + (i >> p.h_shift) * 2 * plane_rest + (i & ((1 << p.h_shift) - 1)) * 128 + (warp & 1) * 64 + c8 * 2;
+        slot[n] = ((mask >> (n * 8 + g)) & 1) ? wide + (i >> p.h_shift) * 2 * plane + (((warp >> 1) << p.h_shift) + (i & ((1 << p.h_shift) - 1))) * 128 + (warp & 1) * 64 + c8 * 2 : -1;
+      }
       for (int ch = 0; ch < chunks; ++ch) {
         const uint32_t stage = smem_u32(smem) + at.stage * stage_bytes;
-        uint32_t ht[NT][2];
+        uint32_t ht[NT][2], step[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          ht[n][0] = slot[n] >= 0 ? stage + slot[n] : smem_u32(zeros);
-          ht[n][1] = slot[n] >= 0 ? ht[n][0] + plane : ht[n][0];
+          const bool on = slot[n] >= 0;
+          ht[n][0] = on ? stage + slot[n] : smem_u32(zeros);
+          ht[n][1] = ht[n][0] + (on ? plane : 0);
+          step[n] = on ? 512 << p.h_shift : 0;
         }
         few_await(ring, &ring.full[at.stage], at.phase, ok, p.status);
 #pragma unroll
@@ -581,30 +641,25 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
             uint4 h[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              h[n][0] = few_row(ht[n][0] + j * 512);
-              h[n][1] = few_row(ht[n][1] + j * 512);
+              h[n][0] = few_row(ht[n][0] + j * step[n]);
+              h[n][1] = few_row(ht[n][1] + j * step[n]);
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m) multiply(few_row(stage + place[m][0] + j * 512 * rows), few_row(stage + place[m][1] + j * 512 * rows), h, m);
           }
         }
-        few_release(ring, at, stages);
-      }
-      if (blocks * 64 + warp * 32 < p.I) {
-        const bool in = rest < p.I;
-        uint4 h[NT][2];
+        if (rest && ch == chunks - 1 && warp < 2) {
+          uint4 h[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int t = n * 8 + g;
-          const bool on = in && ((mask >> t) & 1);
-          const __nv_bfloat16* from = p.h + (long long)(on ? plan.base[d] + few_slot(mask, t) : 0) * p.I + rest;
-          h[n][0] = few_load(from, on);
-          h[n][1] = few_load(from + (long long)p.T * p.k * p.I, on);
+          for (int n = 0; n < NT; ++n) {
+            const bool on = slot[n] >= 0;
+            h[n][0] = few_row(on ? stage + slot_rest[n] : smem_u32(zeros));
+            h[n][1] = few_row(on ? stage + slot_rest[n] + plane_rest : smem_u32(zeros));
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m) multiply(few_row(stage + rest_at + place[m][0]), few_row(stage + rest_at + place[m][1]), h, m);
         }
-        const __nv_bfloat16* w = p.w2 + ((long long)e * p.H + r0) * p.I + rest;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          multiply(few_load(w + (long long)row[m][0] * p.I, in && r0 + row[m][0] < p.H), few_load(w + (long long)row[m][1] * p.I, in && r0 + row[m][1] < p.H), h, m);
+        few_release(ring, at, stages);
       }
     }
 #pragma unroll
@@ -633,10 +688,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
   }
 }
 
-// Matrices [outer, rows, K], rows `ld` and matrices `ldo` elements apart, as {64 of K, rows, blocks of 64, outer}; boxes of `box_rows` rows x
-// `box_blocks` blocks x `box_outer`.  K behind the last whole block is left out; what a box has past the rows or blocks reads as zero.
-static int few_tmap(CUtensorMap* out, const void* base, long long outer, long long rows, long long K, long long ld, long long ldo, int box_rows, int box_blocks,
-                    int box_outer, bool swizzle) {
+// Matrices [outer, rows, K], rows `ld` and matrices `ldo` elements apart.  `out`: {64 of K, rows, blocks of 64, outer}, boxes of `box_rows` rows x
+// `box_blocks` blocks x `box_outer`; `rest`: {K, rows, 1, outer}, boxes of 64 of K x `box_rows` rows x `box_outer`, for what a row has behind its last
+// whole block.  What a box has past the rows, the blocks or K reads as zero.
+static int few_tmap(CUtensorMap* out, CUtensorMap* rest, const void* base, long long outer, long long rows, long long K, long long ld, long long ldo, int box_rows,
+                    int box_blocks, int box_outer, bool swizzle) {
   typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static Encode encode = nullptr;
@@ -646,13 +702,18 @@ static int few_tmap(CUtensorMap* out, const void* base, long long outer, long lo
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return -4;
     encode = reinterpret_cast<Encode>(fn);
   }
-  if (outer == 0 || K < 64) return 0;          // (no copy is made)
-  const cuuint64_t dims[4] = {64, (cuuint64_t)rows, (cuuint64_t)(K / 64), (cuuint64_t)outer};
+  if (outer == 0) return 0;                    // (no copy is made)
   const cuuint64_t strides[3] = {(cuuint64_t)ld * 2, 128, (cuuint64_t)ldo * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, (cuuint32_t)box_outer}, each[4] = {1, 1, 1, 1};
-  return encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-             ? 0 : -5;
+  const cuuint32_t each[4] = {1, 1, 1, 1};
+  for (int r = 0; r < 2; ++r) {
+    if (r == 0 ? K < 64 : K % 64 == 0 || rest == nullptr) continue;
+    const cuuint64_t dims[4] = {r == 0 ? 64 : (cuuint64_t)K, (cuuint64_t)rows, r == 0 ? (cuuint64_t)(K / 64) : 1, (cuuint64_t)outer};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, r == 0 ? (cuuint32_t)box_blocks : 1, (cuuint32_t)box_outer};
+    if (encode(r == 0 ? out : rest, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return -5;
+  }
+  return 0;
 }
 
 // Blocks of a stage, of `all`: at most `most`, in equal parts.
@@ -678,11 +739,11 @@ template <int MT, int NT>
 static int moe_few_down(MoeFewParams& p, int num_sms, cudaStream_t s) {
   static bool set[64] = {};
   if (const int rc = few_opt_in(moe_few_down_kernel<MT, NT>, set)) return rc;
-  p.down_blocks = few_blocks(p.I / 64, few_down_steps<MT>() * kFewMath / 2);
-  CUtensorMap map{}, tokens{};
-  if (const int rc = few_tmap(&map, p.w2, p.e_local, p.H, p.I, p.I, (long long)p.H * p.I, p.down_rows, p.down_blocks, 1, true)) return rc;
-  if (const int rc = few_tmap(&tokens, p.h, 2, (long long)p.T * p.k, p.I, p.I, (long long)p.T * p.k * p.I, 1, p.down_blocks, 2, false)) return rc;
-  launch_pdl(moe_few_down_kernel<MT, NT>, dim3(num_sms), dim3(kFewThreads), kFewSmem, s, map, tokens, p);
+  p.down_blocks = few_blocks(p.I / 64, few_down_steps<MT, NT>() * kFewMath / 2);
+  FewMaps maps{};
+  if (const int rc = few_tmap(&maps.weights[0], &maps.weights_rest, p.w2, p.e_local, p.H, p.I, p.I, (long long)p.H * p.I, p.down_rows, p.down_blocks, 1, true)) return rc;
+  if (const int rc = few_tmap(&maps.tokens[0], &maps.tokens_rest, p.h, 2, (long long)p.T * p.k, p.I, p.I, (long long)p.T * p.k * p.I, 1 << p.h_shift, p.down_blocks, 2, false)) return rc;
+  launch_pdl(moe_few_down_kernel<MT, NT>, dim3(num_sms), dim3(kFewThreads), kFewSmem, s, maps, p);
   return -(int)cudaGetLastError();
 }
 
@@ -690,12 +751,15 @@ template <int NT>
 static int moe_few_launch(MoeFewParams& p, int num_sms, cudaStream_t s) {
   static bool set[64] = {};
   if (const int rc = few_opt_in(moe_few_up_kernel<NT>, set)) return rc;
-  p.up_blocks = few_blocks(p.H / 64, kFewUpSteps * kFewMath / 2);
-  CUtensorMap map{}, tokens{};
-  if (const int rc = few_tmap(&map, p.w13, p.e_local, 2LL * p.I, p.H, p.H, 2LL * p.I * p.H, 8, p.up_blocks, 1, true)) return rc;
-  if (const int rc = few_tmap(&tokens, p.x, 1, p.T, p.H, p.ldx, p.T * p.ldx, 1, p.up_blocks, 1, false)) return rc;
-  launch_pdl(moe_few_up_kernel<NT>, dim3(num_sms), dim3(kFewThreads), kFewSmem, s, map, tokens, p);
+  p.up_blocks = few_blocks(p.H / 64, kFewUpSteps * kFewMath / 4);
+  FewMaps maps{};
+  for (int i = 0; i < 2; ++i) {
+    if (const int rc = few_tmap(&maps.weights[i], i == 0 ? &maps.weights_rest : nullptr, p.w13, p.e_local, 2LL * p.I, p.H, p.H, 2LL * p.I * p.H, 8, p.up_blocks << i, 1, true)) return rc;
+    if (const int rc = few_tmap(&maps.tokens[i], i == 0 ? &maps.tokens_rest : nullptr, p.x, 1, p.T, p.H, p.ldx, p.T * p.ldx, 1, p.up_blocks << i, 1, false)) return rc;
+  }
+  launch_pdl(moe_few_up_kernel<NT>, dim3(num_sms), dim3(kFewThreads), kFewSmem, s, maps, p);
   const int rows = ((p.H + num_sms - 1) / num_sms + 1) & ~1;
+  p.h_shift = p.T <= 2 ? p.T - 1 : 2;           // (what a copy brings beyond the expert's tokens is not read)
   p.down_rows = rows < 16 * kFewRowTiles ? rows : 16 * kFewRowTiles;
   if (rows <= 16) return moe_few_down<1, NT>(p, num_sms, s);
   if (rows <= 32) return moe_few_down<2, NT>(p, num_sms, s);
@@ -712,8 +776,8 @@ int lx_moe_few_max_tokens() { return lx::kFewTokens; }
 int lx_moe_router_logits(const void* x, long long ldx, const void* wr, long long ldw, float* logits, int T, int E, int H, int* counts, int ncounts,
                          void* stream);
 
-// `logits` [T, E], `ids` [T, k] and `h` [2, T k, I] are scratch of the call.
-int lx_moe_few(const void* x, long long ldx, const void* wr, long long ldw, const void* w13, const void* w2, float* logits, int* ids, void* h, void* out, long long ldo, int T,
+// `logits` [T, E] and `h` [2, T k, I] are scratch of the call.
+int lx_moe_few(const void* x, long long ldx, const void* wr, long long ldw, const void* w13, const void* w2, float* logits, void* h, void* out, long long ldo, int T,
                int E, int k, int e0, int e_local, int H, int I, int act, int renorm, float scale, int* status, int num_sms, void* stream) {
   using namespace lx;
   if (T < 0 || T > kFewTokens || E <= 0 || E > kFewExperts || k <= 0 || k > kFewTop || k > E || e_local < 0 || e_local > kFewExperts || H <= 0 || H % 8 != 0 ||
@@ -723,14 +787,16 @@ int lx_moe_few(const void* x, long long ldx, const void* wr, long long ldw, cons
     if ((reinterpret_cast<uintptr_t>(q) & 15) != 0) return -2;
   if (ldx % 8 != 0 || ldw % 8 != 0) return -2;
   if (T == 0) return 0;
-  const bool by_itself = getenv("FEW_ROUTE") ? atoi(getenv("FEW_ROUTE")) : E * (long long)H <= 65536;
+  // Up to 128 KB of router and tokens, every CTA of both kernels forms the logits itself; beyond, they are a launch of their own in front (one token of 4096
+  // and 8 experts 116 -> 115 us, of 2048 and 64 experts 30 -> 37).
+  const bool by_itself = (E + T) * (long long)H <= 65536;
   if (!by_itself)
     if (const int rc = lx_moe_router_logits(x, ldx, wr, ldw, logits, T, E, H, nullptr, 0, stream)) return rc;
   MoeFewParams p{};
   p.x = reinterpret_cast<const __nv_bfloat16*>(x); p.ldx = ldx; p.logits = by_itself ? nullptr : logits;
   p.wr = reinterpret_cast<const __nv_bfloat16*>(wr); p.ldr = ldw;
   p.w13 = reinterpret_cast<const __nv_bfloat16*>(w13); p.w2 = reinterpret_cast<const __nv_bfloat16*>(w2);
-  p.ids = ids; p.h = reinterpret_cast<__nv_bfloat16*>(h); p.out = reinterpret_cast<__nv_bfloat16*>(out); p.ldo = ldo;
+  p.h = reinterpret_cast<__nv_bfloat16*>(h); p.out = reinterpret_cast<__nv_bfloat16*>(out); p.ldo = ldo;
   p.T = T; p.E = E; p.k = k; p.e0 = e0; p.e_local = e_local; p.H = H; p.I = I; p.act = act; p.renorm = renorm; p.scale = scale; p.status = status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return T <= 8 ? moe_few_launch<1>(p, num_sms, s) : moe_few_launch<2>(p, num_sms, s);

@@ -20,7 +20,7 @@ SIGNATURES = {
     "lx_step_tables_max_seqs": ([], I),
     "lx_step_tables": ([P, L, P, I, I, I, I, I, I, I, P, P, I, P, I, I, I, P, P], I),
     "lx_moe_few_max_tokens": ([], I),
-    "lx_moe_few": ([P, L, P, L, P, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, P, I, P], I),
+    "lx_moe_few": ([P, L, P, L, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, P, I, P], I),
     "lx_token_scores_max_top": ([], I),
     "lx_token_scores": ([P, L, I, I, I, P, I, I, F, P, P, P, P, P], I),
 }
@@ -71,12 +71,11 @@ def moe_few(x: torch.Tensor, router_w: torch.Tensor, w13: torch.Tensor, w2: torc
         out = torch.empty(T, H, dtype=x.dtype, device=x.device)
     if T == 0:
         return out
-    # scratch: h (two planes), then the logits, then the choice of experts
-    h_bytes, logits_bytes = (4 * T * k * inter + 15) // 16 * 16, 4 * T * E
-    scratch = torch.empty(h_bytes + logits_bytes + 4 * T * k, dtype=torch.uint8, device=x.device)
+    # scratch: h (two planes), then the logits
+    h_bytes = (4 * T * k * inter + 15) // 16 * 16
+    scratch = torch.empty(h_bytes + 4 * T * E, dtype=torch.uint8, device=x.device)
     at, ws = scratch.data_ptr(), nv.workspace(x.device)
-    rc = nv.load().lx_moe_few(x.data_ptr(), x.stride(0), router_w.data_ptr(), router_w.stride(0), w13.data_ptr(), w2.data_ptr(), at + h_bytes,
-                              at + h_bytes + logits_bytes, at, out.data_ptr(), out.stride(0), T, E, k, e0, w13.shape[0], H, inter, nv._ACTS[act], int(renorm),
+    rc = nv.load().lx_moe_few(x.data_ptr(), x.stride(0), router_w.data_ptr(), router_w.stride(0), w13.data_ptr(), w2.data_ptr(), at + h_bytes, at, out.data_ptr(), out.stride(0), T, E, k, e0, w13.shape[0], H, inter, nv._ACTS[act], int(renorm),
                               scale, ws.status.data_ptr(), ws.num_sms, stream)
     nv._check(rc, "lx_moe_few")
     nv.launch_count += 2                 # (three kernels)
