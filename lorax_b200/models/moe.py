@@ -11,6 +11,8 @@ gather, a grouped tcgen05 GEMM over (expert, feature tile, token tile) work item
 for w2 and the weighted combine.  Only the k experts of a token do work for it, every count stays on the device and every
 launch has static shapes, so a decode step with experts is captured in a CUDA graph like a dense one.
 
+Steps of up to sixteen tokens take `moe_few` (`csrc/kernels/moe_few.cu`): routing, both products and the combine in two launches.
+
 Elsewhere (CPU, packed / quantised experts) two PyTorch shapes remain:
   * decode-sized batches: every local expert runs over all tokens and the routing weight (zero for unrouted tokens)
     scales its output;
@@ -21,7 +23,16 @@ from __future__ import annotations
 
 import torch
 
+from ..ops.reference import MOE_FEW_TOKENS
+
 DENSE_MAX_TOKENS = 256
+
+
+def few_tokens(T: int, k: int, hidden: int, inter: int) -> bool:
+    """Whether a layer takes `moe_few` instead of `moe_ffn`: up to its 16 tokens, unless they reach many small experts, whose turns then cost more than
+    their bytes.  Measured (us, `moe_ffn` / `moe_few`): 8 experts of 4096 x 14336, two a token: 181 / 108 for one token, 469 / 406 for 16; 64 of 2048 x 1024,
+    eight a token: 55 / 28 and 149 / 134; 128 of 1024 x 512, eight a token: 41 / 21 for one, 58 / 54 for six, 60 / 66 for eight, 77 / 110 for 16."""
+    return T <= MOE_FEW_TOKENS and (T * k <= 48 or hidden * inter >= 1 << 20)
 
 
 def route(router_logits: torch.Tensor, k: int):
@@ -44,8 +55,9 @@ def moe_forward(model, x: torch.Tensor, lw, li: int, inp) -> torch.Tensor:
     if (x.is_cuda and x.dtype == torch.bfloat16 and isinstance(lw.experts_w13, torch.Tensor) and isinstance(lw.experts_w2, torch.Tensor)
             and lw.experts_w13.dtype == torch.bfloat16 and lw.experts_w13.shape[1] % 128 == 0 and lw.experts_w2.shape[1] % 128 == 0
             and model.hidden % 8 == 0 and c.intermediate_size % 8 == 0 and E <= 256 and c.num_experts_per_tok <= 32 and hasattr(ops, "moe_ffn")):
-        out = ops.moe_ffn(x, lw.router_w.to(torch.bfloat16) if lw.router_w.dtype != torch.bfloat16 else lw.router_w, lw.experts_w13,
-                          lw.experts_w2, c.num_experts_per_tok, e0, c.hidden_act)
+        ffn = ops.moe_few if few_tokens(T, c.num_experts_per_tok, model.hidden, c.intermediate_size) else ops.moe_ffn
+        out = ffn(x, lw.router_w.to(torch.bfloat16) if lw.router_w.dtype != torch.bfloat16 else lw.router_w, lw.experts_w13,
+                  lw.experts_w2, c.num_experts_per_tok, e0, c.hidden_act)
         if ws > 1 and e_local < E:
             out = model.tp.all_reduce(out)
         return out

@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import math
 import time
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -178,17 +178,16 @@ class ModelRunner:
 
     # ------------------------------------------------------------------ prefill
     def _prefill_inputs(self, items: Sequence[PrefillItem], row_offset: int = 0, lead_tiles: Sequence[Tuple[int, int, int, int]] = ()):
-        """Assembly of a ragged prefill.  The host packs what it alone knows (token ids, per-sequence lengths, block tables, the
-        rows that want logits, the LoRA tile table) into one pinned buffer and one H2D transfer; the per-token positions, cache
-        slots and adapter slots are computed from the per-sequence arrays on the device (`ops.prefill_metadata`).  Returns the
+        """Assembly of a ragged prefill.  The host packs what it alone knows (token ids, lengths and pages of every sequence, the rows that
+        want logits) into one pinned buffer and one H2D transfer; block tables, positions, cache slots, adapter slots and the lists of
+        attention tiles and LoRA tiles are made from the lengths on the device (`ops.step_tables`).  Returns the
         StepInputs and whether any prefill row has an adapter.  In the LoRA tile table the prefill rows are numbered from
         `row_offset` and `lead_tiles` (tiles of rows that precede them in a mixed step) come first."""
         import numpy as np
         page = self.page
         id_parts: List = []
         cu = [0]
-        cache_lens, tables, head_idx, head_slot, q_lens, seq_slot = [], [], [], [], [], []
-        tl: List[Tuple[int, int, int, int]] = list(lead_tiles)
+        cache_lens, pages, held, head_idx, head_slot, q_lens, seq_slot = [], [], [], [], [], [], []
         any_lora = False
         state_slots: List[int] = []
         over_rows: List[int] = []
@@ -204,13 +203,11 @@ class ModelRunner:
             base = cu[-1]
             cu.append(base + n)
             cache_lens.append(it.cache_len)
-            tables.append(self._table_row(it.blocks))
+            pages.append(np.asarray(it.blocks, dtype=np.int32))
+            held.append(len(it.blocks))
             q_lens.append(n)
             seq_slot.append(slot_id)
             state_slots.append(it.state_slot)
-            if slot_id >= 0:
-                # rows of one adapter in tiles of at most 32 (a run that continues the previous sequence's adapter starts a new tile)
-                tl += [(slot_id, base + a + row_offset, min(32, n - a), 0) for a in range(0, n, 32)]
             if it.want_logits:
                 if it.logit_rows is not None:
                     head_idx += [base + int(r) for r in it.logit_rows]
@@ -224,13 +221,11 @@ class ModelRunner:
         T = cu[-1]
         if T > self.max_prefill_tokens:
             raise ValueError(f"prefill of {T} tokens exceeds max_prefill_tokens={self.max_prefill_tokens}")
-        ts, tq = reference.prefill_tiles(q_lens)
-        if not any_lora:
-            tl = list(lead_tiles)
-        seg_len, sgs, sgq = 0, [], []
-        q8s, q8q, ctx_offs = [], [], {}
+        tiles_of = lambda h, rows=q_lens: sum((n + h - 1) // h for n in rows)
+        lists = [(64, tiles_of(64))]
+        seg_len, ctx_offs = 0, {}
         if self.model.context_windows:
-            q8s, q8q = reference.prefill_tiles(q_lens, 128)
+            lists.append((128, tiles_of(128)))
             ctx_offs = {w: reference.context_offsets(cache_lens, q_lens, w) for w in self.model.context_windows}
         if self.model.recurrent:
             # the recurrence kernels carry the state through segments of this many tokens: long enough that the states between
@@ -240,28 +235,30 @@ class ModelRunner:
             longest = max(q_lens + [1])
             if T * self.model.state_parallelism >= 200 * longest:
                 seg_len = (longest + 63) // 64 * 64
-            sgs, sgq = reference.prefill_tiles(q_lens, seg_len)
+            lists.append((seg_len, tiles_of(seg_len)))
+        # rows of one adapter in tiles of at most 32 (a run that continues the previous sequence's adapter starts a new tile)
+        n_lora = tiles_of(32, [n for n, sl in zip(q_lens, seq_slot) if sl >= 0])
         i32 = lambda v: np.asarray(v, dtype=np.int32).reshape(-1)
-        segs = [np.concatenate(id_parts) if id_parts else i32([]), i32(cu), i32(cache_lens), i32(seq_slot), i32(ts), i32(tq), i32(head_idx),
-                i32(head_slot), i32(tl), i32(tables), i32(state_slots), i32(sgs), i32(sgq), i32(q8s), i32(q8q)] + \
-            [i32(o) for o in ctx_offs.values()]
+        segs = [i32(lead_tiles), np.concatenate(id_parts) if id_parts else i32([]), i32([q_lens, cache_lens, seq_slot, held]),
+                np.concatenate(pages) if pages else i32([]), i32(head_idx), i32(head_slot), i32(state_slots)] + [i32(o) for o in ctx_offs.values()]
         flat = torch.from_numpy(np.concatenate(segs))
         if self.is_cuda:
             flat = flat.pin_memory().to(self.device, non_blocking=True)
         self.h2d_bytes += flat.numel() * 4
-        views, o = [], 0
-        for sgm in segs:
-            views.append(flat[o:o + sgm.shape[0]])
-            o += sgm.shape[0]
-        d_ids, d_cu, d_cl, d_seqslot, d_ts, d_tq, d_head, d_headslot, d_tiles, d_bt, d_state, d_sgs, d_sgq, d_q8s, d_q8q, *d_off = views
-        bt = d_bt.view(len(items), self.max_blocks)
-        d_pos, d_slots, d_tokslot = self.model.ops.prefill_metadata(d_cu, d_cl, d_seqslot, bt, page, T)
+        d_lead, d_ids, d_seqs, d_pages, d_head, d_headslot, d_state, *d_off = flat.split([len(x) for x in segs])
+        d_seqs = d_seqs.view(4, len(items))
+        st = self.model.ops.step_tables(d_seqs, d_pages, T, self.max_blocks, page, window=self.model.config.sliding_window or 0, tiles=lists,
+                                        lora_tiles=n_lora, row_offset=row_offset, lead=d_lead.view(-1, 4) if lead_tiles else None)
+        (d_ts, d_tq), *more = st.tiles
+        none = (d_ids[:0], d_ids[:0])
+        d_q8s, d_q8q = more.pop(0) if self.model.context_windows else none
+        d_sgs, d_sgq = more.pop(0) if self.model.recurrent else none
         if any_lora and self.model.adapters is not None:
             self.model.adapters.fence()
-        tiles = LoraTiles(d_tiles.view(-1, 4), len(tl), 32) if tl else None
-        inp = StepInputs(input_ids=d_ids, positions=d_pos, slots=d_slots, is_prefill=True, block_tables=bt, cu_q=d_cu,
-                         cache_lens=d_cl, tile_seq=d_ts, tile_q0=d_tq, lm_head_indices=d_head if len(head_idx) else d_ids[:0],
-                         tok_slot=d_tokslot if any_lora else None, head_tok_slot=d_headslot if any_lora else None,
+        tiles = LoraTiles(st.lora_tiles, st.lora_tiles.shape[0], 32) if st.lora_tiles.shape[0] else None
+        inp = StepInputs(input_ids=d_ids, positions=st.positions, slots=st.slots, is_prefill=True, block_tables=st.block_tables, cu_q=st.cu_q,
+                         cache_lens=d_seqs[1], tile_seq=d_ts, tile_q0=d_tq, lm_head_indices=d_head if len(head_idx) else d_ids[:0],
+                         tok_slot=st.tok_slot if any_lora else None, head_tok_slot=d_headslot if any_lora else None,
                          lora_tiles=tiles, state_slots=d_state, seg_seq=d_sgs, seg_q0=d_sgq, seg_len=seg_len,
                          q128_seq=d_q8s, q128_q0=d_q8q, contexts={w: (t, o[-1]) for (w, o), t in zip(ctx_offs.items(), d_off)})
         if over_rows:
@@ -278,6 +275,17 @@ class ModelRunner:
             return None, None, logits
         next_ids, lps = self.model.ops.argmax_logprob(logits, softcap=self.model.config.final_logit_softcapping or 0.0)
         return next_ids, lps, self._cap(logits)
+
+    def score(self, items: Sequence[PrefillItem], k: int = 0):
+        """Scores of given tokens: one ragged step over the items (prompts, or continuations of cached ones: `cache_len`), their keys and
+        values written like a prefill's.  Returns `ops.TokenScores` on the device with a row for every token of the items in turn: under the
+        distribution behind that token, the log-probability of the item's next token (NaN behind the last), the entropy, and the `k` best
+        tokens with their log-probabilities."""
+        items = [replace(it, want_logits=True, all_logprobs=True, logit_rows=None) for it in items]
+        inp, _ = self._prefill_inputs(items)
+        targets = self._to_dev([t for it in items for t in [*it.token_ids[1:], -1][: len(it.token_ids)]])
+        return self.model.ops.token_scores(self.model.forward(inp, self.kv.layers), targets, k=k,
+                                           softcap=self.model.config.final_logit_softcapping or 0.0)
 
     def _cap(self, logits):
         """Logits as a sampler must see them: gemma2 squashes the head's output with cap * tanh(x / cap).  The greedy

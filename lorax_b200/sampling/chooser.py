@@ -15,6 +15,9 @@ from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..ops import get_ops
+from ..ops.reference import TOP_MAX
+
 
 @dataclass
 class NextTokenParams:
@@ -203,10 +206,15 @@ class HeterogeneousNextTokenChooser:
         """-> (next_ids [B] int64, logprobs [B] float32, alternatives or None)."""
         scores = self.warp(history, history_mask, logits.float(), last_tokens)
         next_ids = self._sample(scores)
-        logp = scores.log_softmax(-1)
-        lp = logp.gather(1, next_ids[:, None])[:, 0]
         alts = None
-        if self.max_alternatives > 0:
+        if self.max_alternatives <= TOP_MAX:
+            s = get_ops(self.device).token_scores(scores, next_ids, k=self.max_alternatives)
+            lp = s.logprobs
+            if self.max_alternatives > 0:
+                alts = (s.top_ids, s.top_logprobs)
+        else:                                    # (more alternatives than the kernel returns)
+            logp = scores.log_softmax(-1)
+            lp = logp.gather(1, next_ids[:, None])[:, 0]
             v, i = logp.topk(self.max_alternatives, dim=-1)
             alts = (i, v)
         if self.any_grammar:

@@ -613,9 +613,10 @@ class ShardRuntime:
             gen, stop = self._emit(s, int(tok), float(lp), alt)
             if gen is not None and it.all_logprobs:
                 n = len(it.token_ids)
-                plp = torch.log_softmax(logits[o:o + n].float(), -1)
-                tgt = torch.tensor(it.token_ids[1:], device=logits.device)
-                vals = [float("nan")] + plp[:-1].gather(1, tgt[:, None])[:, 0].tolist() if n > 1 else [float("nan")]
+                vals = [float("nan")]
+                if n > 1:
+                    tgt = torch.tensor(it.token_ids[1:], device=logits.device)
+                    vals += self.model.ops.token_scores(logits[o:o + n - 1], tgt).logprobs.tolist()
                 gen.prefill_tokens.CopyFrom(pb.NextTokens(ids=list(it.token_ids), logprobs=vals,
                                                           texts=[self._tok_text(i) for i in it.token_ids]))
             o += len(it.token_ids) if it.all_logprobs else 1

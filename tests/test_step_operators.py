@@ -146,3 +146,64 @@ def test_scores_of_rows_with_masks():
     assert torch.allclose(s.logprobs[0], torch.tensor(1 - torch.log(torch.tensor(z)).item()))
     assert s.entropy[4] == 0 and s.top_logprobs[4].tolist() == [0.0, -inf, -inf]
     assert s.logprobs[1:].isnan().all() and s.entropy[1:4].isnan().all()
+
+
+# ------------------------------------------------------------------------------------------------ where they are called
+def test_which_layers_take_the_operator_for_a_few_tokens():
+    from lorax_b200.models.moe import few_tokens
+    assert few_tokens(1, 2, 4096, 14336) and few_tokens(16, 2, 4096, 14336) and not few_tokens(17, 2, 4096, 14336)
+    assert few_tokens(16, 8, 2048, 1024) and few_tokens(6, 8, 1024, 512) and not few_tokens(7, 8, 1024, 512) and few_tokens(16, 3, 128, 64)
+
+
+def _tiny(device, dtype, **over):
+    from lorax_b200.config import ModelConfig
+    from lorax_b200.models.decoder import DecoderModel
+    from lorax_b200.runtime.kv_cache import KVCache
+    from lorax_b200.runtime.runner import ModelRunner
+    cfg = ModelConfig(**{**dict(model_type="mixtral", vocab_size=512, hidden_size=256, intermediate_size=384, num_hidden_layers=2, num_attention_heads=4,
+                                num_key_value_heads=2, head_dim=64, rope_theta=1e4, max_position_embeddings=1024, num_local_experts=4, num_experts_per_tok=2,
+                                torch_dtype="bfloat16"), **over})
+    m = DecoderModel.random_init(cfg, device, dtype, seed=2, std=0.05)
+    return m, ModelRunner(m, KVCache(cfg.num_hidden_layers, 32, m.nkv, m.d, m.dtype, m.device), max_batch=4, max_seq_tokens=512, max_prefill_tokens=512, use_graphs=False)
+
+
+@pytest.mark.parametrize("cap", [0.0, 2.0])
+def test_scores_of_prompts_by_the_runner(cap):
+    """Every token's score is that of the logits which a prefill of the same items returns; the last row of an item has no next token."""
+    from lorax_b200.runtime.runner import PrefillItem
+    m, r = _tiny("cpu", torch.float32, final_logit_softcapping=cap or None)
+    g = torch.Generator().manual_seed(5)
+    prompts = [torch.randint(0, 512, (n,), generator=g).tolist() for n in (5, 1, 40)]
+    items = [PrefillItem(p, 0, [1 + 2 * i, 2 + 2 * i]) for i, p in enumerate(prompts)]
+    got = r.score(items, k=3)
+    _, _, logits = r.prefill([PrefillItem(p, 0, [1 + 2 * i, 2 + 2 * i], all_logprobs=True) for i, p in enumerate(prompts)])
+    lp = torch.log_softmax(logits, -1)
+    row = 0
+    for p in prompts:
+        for i, _ in enumerate(p):
+            if i + 1 < len(p):
+                assert abs(got.logprobs[row].item() - lp[row, p[i + 1]].item()) < 1e-4
+            else:
+                assert got.logprobs[row].isnan()
+            best = lp[row].topk(3)
+            assert torch.allclose(got.top_logprobs[row], best.values, atol=1e-4) and got.top_ids[row].tolist() == best.indices.tolist()
+            assert abs(got.entropy[row].item() + (lp[row].exp() * lp[row]).sum().item()) < 1e-3
+            row += 1
+    assert row == got.entropy.shape[0]
+    # a continuation of a cached prompt: the scores behind its tokens are those of the whole prompt
+    whole = got.logprobs[6:46]
+    rest = r.score([PrefillItem(prompts[2][24:], 24, [5, 6])])
+    assert torch.allclose(rest.logprobs[:15], whole[24:39], atol=1e-4) and rest.top_ids.shape == (16, 0)
+
+
+def test_alternatives_beyond_the_kernels():
+    """The chooser answers with any number of alternatives: the operator's up to its most, the sorted row's beyond."""
+    from lorax_b200.sampling.chooser import HeterogeneousNextTokenChooser, NextTokenParams
+    logits = torch.randn(2, 100, generator=torch.Generator().manual_seed(1))
+    lp = torch.log_softmax(logits, -1)
+    for k in (1, reference.TOP_MAX, reference.TOP_MAX + 1, 100):
+        c = HeterogeneousNextTokenChooser([NextTokenParams(return_k_alternatives=k), NextTokenParams()], "cpu", 100)
+        ids, got, (alt, alp) = c(None, None, logits.clone())
+        best = lp.topk(k, -1)
+        assert ids.tolist() == logits.argmax(-1).tolist() and torch.allclose(got, lp.max(-1).values, atol=1e-6)
+        assert alt.tolist() == best.indices.tolist() and torch.allclose(alp, best.values, atol=1e-6)

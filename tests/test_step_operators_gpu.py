@@ -336,3 +336,67 @@ def test_inputs_of_the_kernel_in_front():
                 h.copy_(v)
             got = call(*held)
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------ a run of them together
+def test_a_short_ragged_step():
+    """Tables from lengths, keys and values to their slots, attention over the pages, a layer of experts, the head, the scores: every operator's result
+    against 64 bits from what it was given."""
+    nh, nkv, d, H, V, page, M = 8, 2, 128, 1024, 5003, 32, 4
+    n, cached, slot, held = [4, 1, 5], [30, 70, 0], [2, -1, 0], [2, 3, 1]
+    flat = [7, 3, 1, 9, 4, 6]
+    T = sum(n)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    r = lambda *s, std=1.0: (torch.randn(*s, generator=g, device="cuda") * std).to(BF16)
+    st = native.step_tables(ints(n, cached, slot, held).cuda(), ints(*flat).cuda(), T, M, page, tiles=((64, 3),), lora_tiles=2)
+    want = reference.step_tables(ints(n, cached, slot, held), ints(*flat), T, M, page, tiles=((64, 3),), lora_tiles=2)
+    assert torch.equal(st.slots.cpu(), want.slots) and torch.equal(st.lora_tiles.cpu(), want.lora_tiles)
+    qkv, cache = r(T, (nh + 2 * nkv) * d), r(12, nkv, 2, page, d)
+    before, raw = cache.clone(), qkv.clone()
+    table = reference.rope_cache(d, 256, 1e4, device="cuda")
+    native.rope_kvwrite(qkv, st.positions, table, cache, st.slots, nh, nkv, d, d)
+    written = torch.zeros(12, page, dtype=torch.bool)
+    for s in want.slots.tolist():
+        written[s // page, s % page] = True
+    assert torch.equal(cache.transpose(1, 3)[~written.cuda()], before.transpose(1, 3)[~written.cuda()])      # (pages of no request and rows behind the tokens stay)
+    for t, s in enumerate(want.slots.tolist()):
+        assert torch.equal(cache[s // page, :, 1, s % page], raw[t, (nh + nkv) * d:].view(nkv, d))
+    att = native.attn_prefill(qkv, cache, st.block_tables, st.cu_q, ints(*cached).cuda(), *st.tiles[0], nh, nkv, d, d ** -0.5)
+    at = 0
+    for b in range(3):
+        keys = cache[want.block_tables[b].long()].double()                       # [M, nkv, 2, page, d]
+        for i in range(n[b]):
+            for h in range(nh):
+                k, v = (keys[:, h // (nh // nkv), o].reshape(-1, d)[: cached[b] + i + 1] for o in (0, 1))
+                p = torch.softmax(k @ qkv[at, h * d:(h + 1) * d].double() * d ** -0.5, 0)
+                ref = p @ v
+                assert (att[at, h * d:(h + 1) * d].double() - ref).norm() <= 2.0 ** -7 * (p @ v.abs()).norm()      # weights and result rounded to bf16
+            at += 1
+    wr, w13, w2 = r(8, H, std=2 * H ** -0.5), r(8, 512, H, std=H ** -0.5), r(8, H, 256, std=256 ** -0.5)
+    y = _check_experts((att, wr, w13, w2), 2)
+    logits = native.gemm(y, r(V, H, std=0.2))
+    targets = torch.randint(0, V, (T,), generator=g, device="cuda")
+    _check_scores(logits, targets, 5, 30.0)
+    native.workspace().check_status()
+
+
+def test_scores_of_prompts_by_the_runner_with_experts():
+    """`ModelRunner.score` on the kernels (a step of ten tokens: `moe_few`) against the fp32 CPU path of the same weights, and against its own logits."""
+    from lorax_b200.runtime.runner import PrefillItem
+    from tests.test_step_operators import _tiny
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, 512, (n,), generator=g).tolist() for n in (6, 1, 3)]
+    outs = []
+    for device, dtype in (("cuda", BF16), ("cpu", F32)):
+        _, r = _tiny(device, dtype)
+        item = lambda p, i: PrefillItem(p, 0, [1 + i])
+        outs.append(r.score([item(p, i) for i, p in enumerate(prompts)], k=4))
+        if device == "cuda":
+            _, _, logits = r.prefill([PrefillItem(p, 0, [1 + i], all_logprobs=True) for i, p in enumerate(prompts)])
+            lp, ent, ids, best = _scores_oracle(logits, torch.tensor([t for p in prompts for t in [*p[1:], -1]], device="cuda"), 4, 0.0)
+            off = (512 / 512 + 80) * 2.0 ** -24
+            assert torch.equal(outs[0].top_ids.long(), ids)
+            _close(outs[0].logprobs, lp, off)
+            _close(outs[0].entropy, ent, off * (2 + 2 * math.log(513)))
+    a, b = outs[0].logprobs.cpu().double(), outs[1].logprobs.double()
+    assert torch.equal(a.isnan(), b.isnan()) and ((a - b)[~a.isnan()].norm() / b[~b.isnan()].norm()).item() < 4e-2      # (the bound of the model's logits in bf16)
