@@ -12,6 +12,10 @@
 // best, so only threads whose own best is at or above it can hold any (k 64 / (64 - k) or so of 512).  Their elements are read again (from L2),
 // what is at or above the bound is listed, and the list is ranked by counting.  The order of (value, index) pairs is total, so the outcome
 // depends on no order of execution.
+//
+// Without alternatives a kernel of its own has more rows on an SM (lean, below).  With them the pass over the row is bound by its instructions, not
+// by the HBM: 2048 rows of 128256 bf16 take 145 us with 20 alternatives (3.6 TB/s), 96 rows 12 us, one row of 32000 in eight CTAs 6.6 us, most of it
+// launch, cluster and merges.
 #include "common.cuh"
 
 namespace lx {
@@ -53,6 +57,13 @@ LX_DEVICE void score_merge(ScoreSums& a, const ScoreSums& b) {
   a.s = a.s * fa + b.s * fb;
   a.m = nm;
 }
+
+LX_DEVICE ScoreSums score_from_lane(const ScoreSums& a, int o) {
+  return ScoreSums{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
+}
+
+template <bool CAP>
+LX_DEVICE float score_cap(float x, float cap) { return CAP ? cap * tanhf(x / cap) : x; }
 
 // Order of logits as an unsigned number; -0 is 0, NaN is -inf.
 LX_DEVICE uint32_t score_key(float x) {
@@ -140,6 +151,17 @@ struct ScoreLoad<float, false> {
   LX_DEVICE static float top(const Raw& v) { return v; }
 };
 
+// Entropy of row t and the log-probability of its target, from the sums of the whole row.
+template <typename L, bool CAP>
+LX_DEVICE void score_row(const TokenScoresParams& p, int t, const L* row, const ScoreSums& all, float logs) {
+  p.entropy[t] = logs - all.u / all.s;
+  if (p.logprobs == nullptr) return;
+  const long long target = p.wide_targets ? reinterpret_cast<const long long*>(p.targets)[t] : reinterpret_cast<const int*>(p.targets)[t];
+  float lp = NAN;
+  if (target >= 0 && target < p.V) lp = (score_cap<CAP>(ScoreLoad<L, false>::load(row + target, true), p.softcap) - all.m) - logs;
+  p.logprobs[t] = lp;
+}
+
 struct ScoreThread {
   float m;                 // running maximum of the (capped) logits
   uint64_t s, u;           // running sums, of even and odd elements
@@ -148,13 +170,13 @@ struct ScoreThread {
 };
 
 // R loads of a thread, the first from index i on, the others `step` further each (indices only grow); from `end` on they are not of the row.
-template <typename Load, int R, bool TOP, bool CAP>
+template <typename Load, int R, bool CAP>
 LX_DEVICE void score_take(ScoreThread& t, const typename Load::Raw (&raw)[R], int i, int step, int end, float cap) {
   constexpr int N = Load::kN;
   float top = Load::top(raw[0]);
 #pragma unroll
   for (int r = 1; r < R; ++r) top = fmaxf(top, Load::top(raw[r]));
-  if (TOP && top > t.best) {
+  if (top > t.best) {
     t.best = top;
 #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
@@ -165,7 +187,7 @@ LX_DEVICE void score_take(ScoreThread& t, const typename Load::Raw (&raw)[R], in
         if (x[q] == top) t.index = i + r * step + q;
     }
   }
-  if constexpr (CAP) top = cap * tanhf(top / cap);
+  top = score_cap<CAP>(top, cap);
   if (top > t.m) {
     if (t.m != -INFINITY) {
       const float d = fmaxf(t.m - top, kScoreFloor), f = __expf(d);
@@ -187,7 +209,7 @@ LX_DEVICE void score_take(ScoreThread& t, const typename Load::Raw (&raw)[R], in
     t.s = add_f32x2(t.s, e);
     t.u = fma_f32x2(d2, e, t.u);
   };
-  auto capped = [&](float x, int r) { return !CAP ? x : r == 0 || i + r * step < end ? cap * tanhf(x / cap) : -INFINITY; };
+  auto capped = [&](float x, int r) { return r == 0 || i + r * step < end ? score_cap<CAP>(x, cap) : -INFINITY; };
   // (all values of the batch are formed before the chains of adds: N R is even but for the last element of a row)
   float x[R][N];
 #pragma unroll
@@ -232,7 +254,7 @@ LX_DEVICE void score_rank(const unsigned long long* list, int n, int k, unsigned
   }
 }
 
-template <typename L, bool VEC, bool TOP, bool CAP>
+template <typename L, bool VEC, bool CAP>
 __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __grid_constant__ TokenScoresParams p) {
   using Load = ScoreLoad<L, VEC>;
   constexpr int kVec = Load::kN, kStep = kScoreThreads * kVec;
@@ -252,109 +274,102 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
     typename Load::Raw raw[kScoreUnroll];
 #pragma unroll
     for (int r = 0; r < kScoreUnroll; ++r) raw[r] = Load::load(row + i + r * kStep, i + r * kStep < whole);
-    score_take<Load, kScoreUnroll, TOP, CAP>(me, raw, i, kStep, whole, p.softcap);
+    score_take<Load, kScoreUnroll, CAP>(me, raw, i, kStep, whole, p.softcap);
   }
   if (VEC && whole + tid < hi) {
     using One = ScoreLoad<L, false>;
     const float raw[1] = {One::load(row + whole + tid, true)};
-    score_take<One, 1, TOP, CAP>(me, raw, whole + tid, 0, hi, p.softcap);
+    score_take<One, 1, CAP>(me, raw, whole + tid, 0, hi, p.softcap);
   }
 
   // sums of the CTA
-  auto from_lane = [](const ScoreSums& a, int o) {
-    return ScoreSums{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
-  };
   const float2 s2 = unpack_f32x2(me.s), u2 = unpack_f32x2(me.u);
   ScoreSums a{me.m, s2.x + s2.y, u2.x + u2.y};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) score_merge(a, from_lane(a, o));
+  for (int o = 16; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
   if ((tid & 31) == 0) sh.warps[tid >> 5] = a;
   const bool live = me.index >= 0;
-  const unsigned long long mine = TOP && live ? score_pair(score_key(me.best), me.index) : 0;
-  if constexpr (TOP) {
-    unsigned long long g = mine;
+  const unsigned long long mine = live ? score_pair(score_key(me.best), me.index) : 0;
+  unsigned long long g = mine;
 #pragma unroll
-    for (int o = 1; o < kScoreThreads / kScoreGroups; o <<= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, g, o);
-      g = other > g ? other : g;
-    }
-    if ((tid & (kScoreThreads / kScoreGroups - 1)) == 0) sh.group[tid / (kScoreThreads / kScoreGroups)] = g;
-    if (tid == 0) {
-      sh.ncand = sh.n = 0;
-      sh.bound = 0;
-    }
+  for (int o = 1; o < kScoreThreads / kScoreGroups; o <<= 1) {
+    const unsigned long long other = __shfl_xor_sync(0xffffffffu, g, o);
+    g = other > g ? other : g;
+  }
+  if ((tid & (kScoreThreads / kScoreGroups - 1)) == 0) sh.group[tid / (kScoreThreads / kScoreGroups)] = g;
+  if (tid == 0) {
+    sh.ncand = sh.n = 0;
+    sh.bound = 0;
   }
   __syncthreads();
   if (tid < 32) {
     a = sh.warps[tid & (kScoreWarps - 1)];
 #pragma unroll
-    for (int o = kScoreWarps / 2; o > 0; o >>= 1) score_merge(a, from_lane(a, o));
+    for (int o = kScoreWarps / 2; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
   }
 
-  if constexpr (TOP) {
-    // the bound: the k-th best of the groups' best, or none where there are fewer
-    const int k = p.k;
-    {
-      constexpr int kShare = kScoreThreads / kScoreGroups;
-      const unsigned long long g = sh.group[tid / kShare];
-      int above = 0;
+  // the bound: the k-th best of the groups' best, or none where there are fewer
+  const int k = p.k;
+  {
+    constexpr int kShare = kScoreThreads / kScoreGroups;
+    const unsigned long long g = sh.group[tid / kShare];
+    int above = 0;
 #pragma unroll
-      for (int j = 0; j < kScoreGroups / kShare; ++j) above += sh.group[(tid & (kShare - 1)) + j * kShare] > g;
+    for (int j = 0; j < kScoreGroups / kShare; ++j) above += sh.group[(tid & (kShare - 1)) + j * kShare] > g;
 #pragma unroll
-      for (int o = kShare / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-      if (g != 0 && above == k - 1 && (tid & (kShare - 1)) == 0) sh.bound = g;
-    }
-    __syncthreads();
-    const unsigned long long bound = sh.bound;
-    if (live && mine >= bound) sh.cand[atomicAdd(&sh.ncand, 1)] = tid;
-    __syncthreads();
-    const int ncand = sh.ncand;
-    const int its = (whole - lo + kStep - 1) / kStep;      // loads of a thread; its single element counts as one more
-    auto push = [&](float x, int idx) {
-      const unsigned long long pair = score_pair(score_key(x), idx);
-      if (pair >= bound) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < kScoreList) sh.list[at] = pair;
-      }
-    };
-    auto collect = [&](int c, int it) {
-      if (it == its) {
-        if (VEC && whole + c < hi) push(ScoreLoad<L, false>::load(row + whole + c, true), whole + c);
-        return;
-      }
-      const int from = lo + (it * kScoreThreads + c) * kVec;
-      if (from >= whole) return;
-      float x[kVec];
-      Load::values(Load::load(row + from, true), x);
-#pragma unroll
-      for (int q = 0; q < kVec; ++q) push(x[q], from + q);
-    };
-    for (int q = tid; q < ncand * (its + 1); q += kScoreThreads) {
-      const int c = q / (its + 1);
-      collect(sh.cand[c], q - c * (its + 1));
-    }
-    __syncthreads();
-    if (sh.n <= kScoreList) {
-      score_rank(sh.list, sh.n, k, sh.own);
-    } else {
-      // more than the list holds (large logits side by side in the threads' strides): portions that fit, with the best so far among them
-      constexpr int kPortion = (kScoreList - kScoreMaxTop) / kVec;
-      int have = 0;
-      for (int c = 0; c < ncand; ++c) {
-        for (int it = 0; it <= its; it += kPortion) {
-          __syncthreads();
-          if (tid < have) sh.list[tid] = sh.own[tid];
-          if (tid == 0) sh.n = have;
-          __syncthreads();
-          for (int q = it + tid; q < min(it + kPortion, its + 1); q += kScoreThreads) collect(sh.cand[c], q);
-          __syncthreads();
-          score_rank(sh.list, sh.n, k, sh.own);
-          have = min(k, sh.n);
-        }
-      }
-    }
-    __syncthreads();
+    for (int o = kShare / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (g != 0 && above == k - 1 && (tid & (kShare - 1)) == 0) sh.bound = g;
   }
+  __syncthreads();
+  const unsigned long long bound = sh.bound;
+  if (live && mine >= bound) sh.cand[atomicAdd(&sh.ncand, 1)] = tid;
+  __syncthreads();
+  const int ncand = sh.ncand;
+  const int its = (whole - lo + kStep - 1) / kStep;      // loads of a thread; its single element counts as one more
+  auto push = [&](float x, int idx) {
+    const unsigned long long pair = score_pair(score_key(x), idx);
+    if (pair >= bound) {
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < kScoreList) sh.list[at] = pair;
+    }
+  };
+  auto collect = [&](int c, int it) {
+    if (it == its) {
+      if (VEC && whole + c < hi) push(ScoreLoad<L, false>::load(row + whole + c, true), whole + c);
+      return;
+    }
+    const int from = lo + (it * kScoreThreads + c) * kVec;
+    if (from >= whole) return;
+    float x[kVec];
+    Load::values(Load::load(row + from, true), x);
+#pragma unroll
+    for (int q = 0; q < kVec; ++q) push(x[q], from + q);
+  };
+  for (int q = tid; q < ncand * (its + 1); q += kScoreThreads) {
+    const int c = q / (its + 1);
+    collect(sh.cand[c], q - c * (its + 1));
+  }
+  __syncthreads();
+  if (sh.n <= kScoreList) {
+    score_rank(sh.list, sh.n, k, sh.own);
+  } else {
+    // more than the list holds (large logits side by side in the threads' strides): portions that fit, with the best so far among them
+    constexpr int kPortion = (kScoreList - kScoreMaxTop) / kVec;
+    int have = 0;
+    for (int c = 0; c < ncand; ++c) {
+      for (int it = 0; it <= its; it += kPortion) {
+        __syncthreads();
+        if (tid < have) sh.list[tid] = sh.own[tid];
+        if (tid == 0) sh.n = have;
+        __syncthreads();
+        for (int q = it + tid; q < min(it + kPortion, its + 1); q += kScoreThreads) collect(sh.cand[c], q);
+        __syncthreads();
+        score_rank(sh.list, sh.n, k, sh.own);
+        have = min(k, sh.n);
+      }
+    }
+  }
+  __syncthreads();
 
   if (parts > 1) {
     cluster_wait();
@@ -364,17 +379,15 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
       cluster_store_f32(to + 4, 0, a.s);
       cluster_store_f32(to + 8, 0, a.u);
     }
-    if (TOP && tid < p.k) {
+    if (tid < p.k) {
       const uint32_t to = smem_u32(&sh.best[part * p.k + tid]);
       cluster_store_f32(to, 0, __uint_as_float((uint32_t)sh.own[tid]));
       cluster_store_f32(to + 4, 0, __uint_as_float((uint32_t)(sh.own[tid] >> 32)));
     }
     cluster_sync();      // (the parts have arrived)
     if (part != 0) return;
-    if constexpr (TOP) {
-      score_rank(sh.best, parts * p.k, p.k, sh.own);      // (empty places are zeros and rank behind every pair)
-      __syncthreads();
-    }
+    score_rank(sh.best, parts * p.k, p.k, sh.own);      // (empty places are zeros and rank behind every pair)
+    __syncthreads();
   } else {
     if (tid == 0) sh.parts[0] = a;
     __syncthreads();
@@ -384,33 +397,143 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   ScoreSums all = sh.parts[0];
   for (int c = 1; c < parts; ++c) score_merge(all, sh.parts[c]);
   const float logs = logf(all.s);
-  auto capped = [&](float x) { return CAP ? p.softcap * tanhf(x / p.softcap) : x; };
-  if (tid == 0) {
-    p.entropy[t] = logs - all.u / all.s;
-    if (p.logprobs != nullptr) {
-      const long long target = p.targets == nullptr ? -1
-                               : p.wide_targets     ? reinterpret_cast<const long long*>(p.targets)[t]
-                                                    : reinterpret_cast<const int*>(p.targets)[t];
-      float lp = NAN;
-      if (target >= 0 && target < p.V) lp = (capped(ScoreLoad<L, false>::load(row + target, true)) - all.m) - logs;
-      p.logprobs[t] = lp;
+  if (tid == 0) score_row<L, CAP>(p, t, row, all, logs);
+  for (int j = tid; j < p.k; j += 32) {
+    const unsigned long long pair = sh.own[j];
+    p.top_ids[(long long)t * p.k + j] = (int)(0xffffffffu - (uint32_t)pair);
+    p.top_logprobs[(long long)t * p.k + j] = (score_cap<CAP>(score_value((uint32_t)(pair >> 32)), p.softcap) - all.m) - logs;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ without alternatives
+// Bound by the HBM, and by the instructions of a logit: 2048 rows of 128256 bf16 in 86 us (6.1 TB/s), 4001 of 32000 in 51 (5.0 TB/s; with 512 threads a
+// CTA, which reach the ends of their rows together, 63 to 72).  With a cap 1000 rows of 32000 take 50 us: tanhf.
+// exp(c - m) is formed as 2^(log2e c + shift) with shift = -log2e m rounded: one FMA a logit, whose product is not rounded.  What the rounding of the
+// shift leaves out is the same for all terms and put right where the sums change hands.  Where the maximum is too far out for that (masks of the
+// type's lowest value, infinities) the difference comes first.
+constexpr int kLeanThreads = 256;
+constexpr int kLeanWarps = kLeanThreads / 32;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Below 2048 the shift is rounded by at most 2^-13, and what the linear term of lean_sums leaves of that is under 2^-27.
+constexpr float kLeanFar = 2048.f;
+
+LX_DEVICE bool lean_far(float m) { return !(fabsf(m) < kLeanFar); }
+
+struct LeanThread {
+  float m, shift;          // running maximum of the (capped) logits
+  float s, u;              // running sums of e = 2^a and of a e, a = log2e c + shift
+};
+
+// The sums as they are for a shift that is not rounded, in natural logarithms.
+LX_DEVICE ScoreSums lean_sums(const LeanThread& t) {
+  const float off = lean_far(t.m) ? 0.f : fmaf(kLog2e, t.m, t.shift);      // (at most half a step of the shift)
+  const float f = 1.f - off * kLn2;                                        // 2^-off
+  return ScoreSums{t.m, t.s * f, (t.u - off * t.s) * f * kLn2};
+}
+
+// R loads of a thread, the first from index i on, the others `step` further each; from `end` on they are not of the row (GUARD: there may be such).
+template <typename Load, int R, bool CAP, bool GUARD>
+LX_DEVICE void lean_take(LeanThread& t, const typename Load::Raw (&raw)[R], int i, int step, int end, float cap) {
+  float top = Load::top(raw[0]);
+#pragma unroll
+  for (int r = 1; r < R; ++r) top = fmaxf(top, Load::top(raw[r]));
+  top = score_cap<CAP>(top, cap);
+  if (top > t.m) {
+    const float shift = lean_far(top) ? 0.f : -kLog2e * top;
+    if (t.m != -INFINITY) {
+      const float d = fmaxf(lean_far(top) || lean_far(t.m) ? (t.m - top) * kLog2e : shift - t.shift, kScoreFloor), f = exp2_fast(d);
+      t.u = fmaf(d, t.s, t.u) * f;
+      t.s *= f;
+    }
+    t.m = top;
+    t.shift = shift;
+  }
+  auto add = [&](float a) {
+    a = max_nan(a, kScoreFloor);
+    const float e = exp2_fast(a);
+    t.s += e;
+    t.u = fmaf(a, e, t.u);
+  };
+  const bool far = lean_far(t.m);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (GUARD && r > 0 && i + r * step >= end) continue;
+    float x[Load::kN];
+    Load::values(raw[r], x);
+    if (!far) {
+#pragma unroll
+      for (int q = 0; q < Load::kN; ++q) add(fmaf(score_cap<CAP>(x[q], cap), kLog2e, t.shift));
+    } else {                             // (logits of -inf only, so far: they add zeros)
+#pragma unroll 1
+      for (int q = 0; q < Load::kN; ++q) add((score_cap<CAP>(x[q], cap) - (t.m == -INFINITY ? 0.f : t.m)) * kLog2e);
     }
   }
-  if constexpr (TOP) {
-    for (int j = tid; j < p.k; j += 32) {
-      const unsigned long long pair = sh.own[j];
-      p.top_ids[(long long)t * p.k + j] = (int)(0xffffffffu - (uint32_t)pair);
-      p.top_logprobs[(long long)t * p.k + j] = (capped(score_value((uint32_t)(pair >> 32))) - all.m) - logs;
-    }
+}
+
+template <typename L, bool VEC, bool CAP>
+__global__ void __launch_bounds__(kLeanThreads, 6) token_logprobs_kernel(const __grid_constant__ TokenScoresParams p) {
+  using Load = ScoreLoad<L, VEC>;
+  constexpr int kVec = Load::kN, kStep = kLeanThreads * kVec;
+  __shared__ ScoreSums warps[kLeanWarps], ends[kScoreMaxParts];      // (the latter of the cluster's first CTA)
+  const int t = blockIdx.x, part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
+  if (parts > 1) cluster_arrive();      // (waited for in front of the first write to another CTA: it has started by then)
+  pdl_wait();
+  pdl_trigger();
+  const L* row = reinterpret_cast<const L*>(p.logits) + (long long)t * p.ld;
+  const int chunk = ((p.V + parts - 1) / parts + 7) & ~7;
+  const int lo = min(part * chunk, p.V), hi = min(lo + chunk, p.V), whole = lo + (hi - lo) / kVec * kVec;
+  LeanThread me{-INFINITY, 0.f, 0.f, 0.f};
+  int i = lo + tid * kVec;
+  for (; i + (kScoreUnroll - 1) * kStep < whole; i += kScoreUnroll * kStep) {
+    typename Load::Raw raw[kScoreUnroll];
+#pragma unroll
+    for (int r = 0; r < kScoreUnroll; ++r) raw[r] = Load::load(row + i + r * kStep, true);
+    lean_take<Load, kScoreUnroll, CAP, false>(me, raw, i, kStep, whole, p.softcap);
   }
+  if (i < whole) {
+    typename Load::Raw raw[kScoreUnroll];
+#pragma unroll
+    for (int r = 0; r < kScoreUnroll; ++r) raw[r] = Load::load(row + i + r * kStep, i + r * kStep < whole);
+    lean_take<Load, kScoreUnroll, CAP, true>(me, raw, i, kStep, whole, p.softcap);
+  }
+  if (VEC && whole + tid < hi) {
+    using One = ScoreLoad<L, false>;
+    const float raw[1] = {One::load(row + whole + tid, true)};
+    lean_take<One, 1, CAP, false>(me, raw, whole + tid, 0, hi, p.softcap);
+  }
+  ScoreSums a = lean_sums(me);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
+  if ((tid & 31) == 0) warps[tid >> 5] = a;
+  __syncthreads();
+  if (tid < 32) {
+    a = warps[tid & (kLeanWarps - 1)];
+#pragma unroll
+    for (int o = kLeanWarps / 2; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
+  }
+  if (parts > 1) {
+    cluster_wait();
+    if (tid == 0) {
+      const uint32_t to = smem_u32(&ends[part]);
+      cluster_store_f32(to, 0, a.m);
+      cluster_store_f32(to + 4, 0, a.s);
+      cluster_store_f32(to + 8, 0, a.u);
+    }
+    cluster_sync();      // (the parts have arrived)
+    if (part != 0 || tid != 0) return;
+    a = ends[0];
+    for (int c = 1; c < parts; ++c) score_merge(a, ends[c]);
+  }
+  if (tid == 0) score_row<L, CAP>(p, t, row, a, logf(a.s));
 }
 
 template <typename L, bool VEC>
 static int token_scores_launch(const TokenScoresParams& p, int T, int parts, cudaStream_t s) {
   void (*kernel)(TokenScoresParams);
-  if (p.softcap > 0.f) kernel = p.k > 0 ? token_scores_kernel<L, VEC, true, true> : token_scores_kernel<L, VEC, false, true>;
-  else kernel = p.k > 0 ? token_scores_kernel<L, VEC, true, false> : token_scores_kernel<L, VEC, false, false>;
-  const cudaError_t e = launch_pdl_cluster(kernel, dim3(T, parts), dim3(kScoreThreads), dim3(1, parts), 0, s, p);
+  if (p.k > 0) kernel = p.softcap > 0.f ? token_scores_kernel<L, VEC, true> : token_scores_kernel<L, VEC, false>;
+  else kernel = p.softcap > 0.f ? token_logprobs_kernel<L, VEC, true> : token_logprobs_kernel<L, VEC, false>;
+  const cudaError_t e = launch_pdl_cluster(kernel, dim3(T, parts), dim3(p.k > 0 ? kScoreThreads : kLeanThreads), dim3(1, parts), 0, s, p);
   return e != cudaSuccess ? -(int)e : -(int)cudaGetLastError();
 }
 
@@ -424,7 +547,7 @@ int lx_token_scores_max_top() { return lx::kScoreMaxTop; }
 int lx_token_scores(const void* logits, long long ld, int fp32, int T, int V, const void* targets, int wide_targets, int k, float softcap,
                     float* logprobs, float* entropy, int* top_ids, float* top_logprobs, void* stream) {
   using namespace lx;
-  if (T < 0 || V <= 0 || k < 0 || k > kScoreMaxTop || k > V || softcap < 0.f || (T > 1 && ld < V)) return -1;
+  if (T < 0 || V <= 0 || k < 0 || k > kScoreMaxTop || k > V || softcap < 0.f || (T > 1 && ld < V) || (logprobs != nullptr && targets == nullptr)) return -1;
   if (T == 0) return 0;
   TokenScoresParams p{logits, ld, V, targets, wide_targets, k, softcap, logprobs, entropy, top_ids, top_logprobs};
   // CTAs of a row: enough of them for two per SM, and at least one load per thread

@@ -152,6 +152,18 @@ def test_scores_of_rows_with_masks_ties_and_no_distribution(T, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("by", [700.0, -700.0, 1500.0, 2040.0, -2046.0, 5e4, -1e9, 1e30])
+def test_scores_of_logits_far_from_zero(dtype, by):
+    for T, V in ((2, 9001), (160, 4007)):
+        logits, targets = _logits(T, V, F32, 11)
+        x = (logits + by).to(dtype)
+        x[-1, : V // 2] = 0                     # (a maximum that leaves the range, or comes back into it, on the way)
+        x[0, V // 2:] = 0
+        for k in (0, 3):
+            _check_scores(x, targets, k)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_scores_when_more_candidates_than_the_list_holds(dtype):
     """Thirty-one threads whose strided elements are all above the bound that the thirty-second one sets."""
     T, V, k = 160, 512 * 8 * 17 + 5, 32
