@@ -56,7 +56,7 @@ def step_tables(seqs: torch.Tensor, pages: torch.Tensor, tokens: int, max_blocks
     rc = nv.load().lx_step_tables(seqs.data_ptr(), seqs.stride(0), pages.data_ptr(), pages.shape[0], B, tokens, M, page, window, row_offset, heights, counts,
                                   n_lists, None if lead is None else lead.data_ptr(), n_lead, lora_rows, lora_tiles, out.data_ptr(), stream)
     nv._check(rc, "lx_step_tables")
-    lora, cu, pos, slots, tok, bt, *lists = out.split(sizes)
+    lora, cu, pos, slots, tok, bt, *lists = out.split_with_sizes(sizes)
     return StepTables(cu, pos, slots, tok, bt.view(B, M), tuple(zip(lists[::2], lists[1::2])), lora.view(-1, 4))
 
 
@@ -93,7 +93,7 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, k
     if targets is not None:
         targets = targets.contiguous()
         t_ptr, wide = targets.data_ptr(), int(targets.dtype == torch.int64)
-    lp, ent, best = torch.empty(T * (2 + k), dtype=torch.float32, device=logits.device).split([T, T, T * k])
+    lp, ent, best = torch.empty(T * (2 + k), dtype=torch.float32, device=logits.device).split_with_sizes([T, T, T * k])
     ids = torch.empty(T, k, dtype=torch.int32, device=logits.device)
     rc = nv.load().lx_token_scores(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), T, V, t_ptr, wide, k, softcap,
                                    lp.data_ptr() if t_ptr else 0, ent.data_ptr(), ids.data_ptr(), best.data_ptr(), stream)
