@@ -87,6 +87,9 @@ LX_DEVICE int tables_find(const int* sums, int B, int i) {
 // Lengths, places and page counts below zero count as zero.
 LX_DEVICE int tables_len(const StepTablesParams& p, int row, int b) { return max(p.seqs[row * p.ld + b], 0); }
 
+// Tiles of `height` that n tokens make.
+LX_DEVICE int tables_up(int n, int height) { return n / height + (n % height != 0); }
+
 LX_DEVICE int tables_entry(const StepTablesParams& p, int off, int held, int j) {
   if (j < 0) return 0;                    // (a place past 32 bits)
   if (j >= held) {
@@ -94,7 +97,8 @@ LX_DEVICE int tables_entry(const StepTablesParams& p, int off, int held, int j) 
     if (!recycled) return 0;
     j %= held;
   }
-  return off + j < p.num_pages ? p.pages[off + j] : 0;
+  const unsigned at = (unsigned)off + (unsigned)j;      // (of page counts whose sum is past 32 bits nothing is read out of range)
+  return at < (unsigned)p.num_pages ? p.pages[at] : 0;
 }
 
 __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const __grid_constant__ StepTablesParams p) {
@@ -144,7 +148,7 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const __gri
   for (int l = 0; l < p.nlists; ++l) {
     if (block >= p.first[2 + l]) continue;
     const TileList list = p.lists[l];
-    tables_scan(cu, warps, p.B, [&](int b) { return (tokens(b) + list.height - 1) / list.height; });
+    tables_scan(cu, warps, p.B, [&](int b) { return tables_up(tokens(b), list.height); });
     for (int i = (block - p.first[1 + l]) * kTablesPer + threadIdx.x, end = min(list.count, i - (int)threadIdx.x + kTablesPer); i < end; i += kTablesThreads) {
       const bool live = i < cu[p.B];
       const int b = live ? tables_find(cu, p.B, i) : -1;
@@ -155,7 +159,7 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const __gri
   }
   tables_scan(cu, warps, p.B, tokens);    // adapter tiles
   int* const tiles = off;
-  tables_scan(tiles, warps, p.B, [&](int b) { return p.seqs[2 * p.ld + b] < 0 ? 0 : (tokens(b) + p.lora_rows - 1) / p.lora_rows; });
+  tables_scan(tiles, warps, p.B, [&](int b) { return p.seqs[2 * p.ld + b] < 0 ? 0 : tables_up(tokens(b), p.lora_rows); });
   const int n = p.nlead + p.lora_count;
   for (int i = (block - p.first[1 + p.nlists]) * kTablesPer + threadIdx.x, end = min(n, i - (int)threadIdx.x + kTablesPer); i < end; i += kTablesThreads) {
     int4 tile = make_int4(-1, 0, 0, 0);
@@ -182,7 +186,7 @@ int lx_step_tables(const int* seqs, long long ld, const int* pages, int num_page
                    const int* heights, const int* counts, int nlists, const int* lead, int nlead, int lora_rows, int lora_count, int* out,
                    void* stream) {
   using namespace lx;
-  if (B < 0 || B > kTablesMaxSeqs || T < 0 || M <= 0 || page <= 0 || num_pages < 0 || nlists < 0 || nlists > kTablesLists || nlead < 0 || lora_count < 0 ||
+  if (B < 0 || B > kTablesMaxSeqs || T < 0 || M <= 0 || page <= 0 || num_pages < 0 || nlists < 0 || nlists > kTablesLists || row_offset < 0 || nlead < 0 || lora_count < 0 ||
       (lora_count > 0 && lora_rows <= 0) || (nlead > 0 && lead == nullptr))
     return -1;
   if ((reinterpret_cast<uintptr_t>(out) & 15) != 0 || (reinterpret_cast<uintptr_t>(lead) & 15) != 0) return -2;

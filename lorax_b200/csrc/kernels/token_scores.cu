@@ -547,7 +547,7 @@ int lx_token_scores_max_top() { return lx::kScoreMaxTop; }
 int lx_token_scores(const void* logits, long long ld, int fp32, int T, int V, const void* targets, int wide_targets, int k, float softcap,
                     float* logprobs, float* entropy, int* top_ids, float* top_logprobs, void* stream) {
   using namespace lx;
-  if (T < 0 || V <= 0 || k < 0 || k > kScoreMaxTop || k > V || softcap < 0.f || (T > 1 && ld < V) || (logprobs != nullptr && targets == nullptr)) return -1;
+  if (T < 0 || V <= 0 || V >= 1 << 30 || k < 0 || k > kScoreMaxTop || k > V || !(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f)) || (T > 1 && ld < V) || (logprobs != nullptr && targets == nullptr)) return -1;
   if (T == 0) return 0;
   TokenScoresParams p{logits, ld, V, targets, wide_targets, k, softcap, logprobs, entropy, top_ids, top_logprobs};
   // CTAs of a row: enough of them for two per SM, and at least one load per thread

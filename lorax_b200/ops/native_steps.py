@@ -45,7 +45,7 @@ def step_tables(seqs: torch.Tensor, pages: torch.Tensor, tokens: int, max_blocks
                 tiles: Sequence[Tuple[int, int]] = (), lora_tiles: int = 0, lora_rows: int = 32, row_offset: int = 0,
                 lead: Optional[torch.Tensor] = None) -> StepTables:
     """Tables of a ragged step from its sequences' lengths (`reference.step_tables` states them), in one launch."""
-    B = check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, lead)
+    B = check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, row_offset, lead)
     stream = _stream_for(seqs, pages, lead)
     M, n_lead, n_lists = max_blocks, 0 if lead is None else lead.shape[0], len(tiles)
     sizes = [4 * (n_lead + lora_tiles), B + 1, tokens, tokens, tokens, B * M]
@@ -75,8 +75,8 @@ def moe_few(x: torch.Tensor, router_w: torch.Tensor, w13: torch.Tensor, w2: torc
     h_bytes = (4 * T * k * inter + 15) // 16 * 16
     scratch = torch.empty(h_bytes + 4 * T * E, dtype=torch.uint8, device=x.device)
     at, ws = scratch.data_ptr(), nv.workspace(x.device)
-    rc = nv.load().lx_moe_few(x.data_ptr(), x.stride(0), router_w.data_ptr(), router_w.stride(0), w13.data_ptr(), w2.data_ptr(), at + h_bytes, at, out.data_ptr(), out.stride(0), T, E, k, e0, w13.shape[0], H, inter, nv._ACTS[act], int(renorm),
-                              scale, ws.status.data_ptr(), ws.num_sms, stream)
+    rc = nv.load().lx_moe_few(x.data_ptr(), x.stride(0) if T > 1 else H, router_w.data_ptr(), router_w.stride(0) if E > 1 else H, w13.data_ptr(), w2.data_ptr(),
+                              at + h_bytes, at, out.data_ptr(), out.stride(0), T, E, k, e0, w13.shape[0], H, inter, nv._ACTS[act], int(renorm), scale, ws.status.data_ptr(), ws.num_sms, stream)
     nv._check(rc, "lx_moe_few")
     nv.launch_count += 2                 # (three kernels)
     return out

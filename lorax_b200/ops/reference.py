@@ -982,6 +982,7 @@ def moe_grouped_gemm(xg, w, seg, avg_rows: int, out=None, shared: int = 0, token
 
 # ------------------------------------------------------------------------------------------------ short ragged steps
 MOE_FEW_TOKENS = 16         # tokens that `moe_few` takes at most
+INT32_END = 1 << 31
 TOP_MAX = 32                # alternatives that `token_scores` returns at most
 STEP_SEQS_MAX = 4096        # sequences of `step_tables`
 
@@ -996,7 +997,7 @@ class StepTables(NamedTuple):
     lora_tiles: torch.Tensor     # [n, 4] (adapter slot, first row, rows, 0)
 
 
-def check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, lead) -> int:
+def check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, row_offset, lead) -> int:
     """-> number of sequences."""
     if not (seqs.dtype == torch.int32 and seqs.dim() == 2 and seqs.shape[0] == 4 and (seqs.shape[1] <= 1 or seqs.stride(1) == 1)):
         raise ValueError("step_tables: seqs is [4, sequences] int32 (tokens, cached tokens, adapter slot, pages)")
@@ -1004,12 +1005,12 @@ def check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora
         raise ValueError(f"step_tables: {seqs.shape[1]} sequences, at most {STEP_SEQS_MAX}")
     if not (pages.dtype == torch.int32 and pages.dim() == 1 and pages.is_contiguous() and pages.device == seqs.device):
         raise ValueError("step_tables: pages is one contiguous int32 list on the device of seqs")
-    if not (tokens >= 0 and max_blocks > 0 and page > 0 and window >= 0):
-        raise ValueError("step_tables: tokens and window from 0 on, max_blocks and page from 1 on")
-    if not (len(tiles) <= 4 and all(h > 0 and n >= 0 for h, n in tiles)):
+    if not (0 <= tokens < INT32_END and 0 < max_blocks < INT32_END and 0 < page < INT32_END and 0 <= window < INT32_END):
+        raise ValueError("step_tables: tokens and window from 0 on, max_blocks and page from 1 on, in 32 bits")
+    if not (len(tiles) <= 4 and all(0 < h < INT32_END and 0 <= n < INT32_END for h, n in tiles)):
         raise ValueError("step_tables: up to four lists of tiles (height, count)")
-    if not (lora_tiles >= 0 and lora_rows > 0):
-        raise ValueError("step_tables: lora_tiles from 0 on, lora_rows from 1 on")
+    if not (0 <= lora_tiles < INT32_END and 0 < lora_rows < INT32_END and 0 <= row_offset < INT32_END):
+        raise ValueError("step_tables: lora_tiles and row_offset from 0 on, lora_rows from 1 on, in 32 bits")
     if not (lead is None or (lead.dtype == torch.int32 and lead.dim() == 2 and lead.shape[1] == 4 and lead.is_contiguous() and lead.device == seqs.device
                            and lead.data_ptr() % 16 == 0)):
         raise ValueError("step_tables: lead is [n, 4] int32, contiguous, on a 16-byte boundary")
@@ -1026,10 +1027,16 @@ def step_tables(seqs, pages, tokens: int, max_blocks: int, page: int, window: in
     (height, count) of lists of tiles, first queries 0, height, 2 height .. of every sequence in turn.  Adapter tiles hold up to `lora_rows`
     rows of one sequence with an adapter; rows are counted from `row_offset`, and the tiles `lead` [n, 4] come first.
 
-    The caller states how much there is (`tokens`, the counts, `lora_tiles`).  Entries past what the lengths make are filled: position 0, slots
+    Sums of tokens and of pages stay below 2^31.  The caller states how much there is (`tokens`, the counts, `lora_tiles`).  Entries past what the lengths make are filled: position 0, slots
     and tiles' sequences and adapters -1; what they make beyond is left out."""
-    B = check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, lead)
-    dev = seqs.device
+    check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, row_offset, lead)
+    return step_tables_of_many(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, row_offset, lead)
+
+
+def step_tables_of_many(seqs, pages, tokens: int, max_blocks: int, page: int, window: int = 0, tiles=(), lora_tiles: int = 0, lora_rows: int = 32,
+                        row_offset: int = 0, lead=None) -> StepTables:
+    """`step_tables` of any number of sequences, on the host."""
+    B, dev = seqs.shape[1], seqs.device
     n, cached, adapter, held = seqs.tolist() if B else ([], [], [], [])
     n, cached, held, flat = [max(v, 0) for v in n], [max(v, 0) for v in cached], [max(v, 0) for v in held], pages.tolist()
     cu, tables, off = [0], [], 0
@@ -1084,10 +1091,12 @@ def check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out):
         raise ValueError(f"moe_few: activation {act!r}")
     if not (router_w.dtype == w13.dtype == w2.dtype == x.dtype and router_w.device == w13.device == w2.device == x.device):
         raise ValueError("moe_few: the weights have another type or device than x")
-    if not (x.stride(1) == 1 and x.stride(0) % 8 == 0 and router_w.stride(1) == 1 and router_w.stride(0) % 8 == 0 and w13.is_contiguous() and w2.is_contiguous()
-            and (x.data_ptr() | router_w.data_ptr() | w13.data_ptr() | w2.data_ptr()) % 16 == 0):
+    if not (x.stride(1) == 1 and (T <= 1 or (x.stride(0) >= H and x.stride(0) % 8 == 0)) and router_w.stride(1) == 1
+            and (E == 1 or (router_w.stride(0) >= H and router_w.stride(0) % 8 == 0)) and w13.is_contiguous()
+            and w2.is_contiguous() and (x.data_ptr() | router_w.data_ptr() | w13.data_ptr() | w2.data_ptr()) % 16 == 0):
         raise ValueError("moe_few: rows on 16-byte boundaries, experts stacked without gaps")
-    if not (out is None or (out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and out.stride(1) == 1)):
+    if not (out is None or (out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and out.stride(1) == 1
+                           and (T <= 1 or out.stride(0) >= H))):
         raise ValueError("moe_few: out is like x")
     return T, E, H, inter
 
@@ -1127,10 +1136,12 @@ def check_token_scores(logits, targets, k, softcap):
     if not (logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1) and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1])):
         raise ValueError("token_scores: logits are [rows, vocabulary], the logits of a row side by side")
     T, V = logits.shape
+    if not (V < 1 << 30):
+        raise ValueError(f"token_scores: a vocabulary of {V}, at most 2^30 - 1")
     if not (0 <= k <= min(TOP_MAX, V)):
         raise ValueError(f"token_scores: {k} alternatives of {V} tokens, at most {TOP_MAX}")
-    if not (softcap >= 0.0):
-        raise ValueError("token_scores: softcap from 0 on (0: none)")
+    if not (softcap == 0.0 or 1e-30 <= softcap <= 1e30):
+        raise ValueError("token_scores: softcap is 0 (none), or from 1e-30 to 1e30")
     if not (targets is None or (targets.shape == (T,) and targets.dtype in (torch.int32, torch.int64) and targets.device == logits.device)):
         raise ValueError("token_scores: one int32 or int64 target a row, on the device of the logits")
     return T, V
@@ -1151,5 +1162,8 @@ def token_scores(logits, targets=None, k: int = 0, softcap: float = 0.0) -> Toke
         at = targets.long()
         ok = (at >= 0) & (at < V)
         got = torch.where(ok, lp.gather(1, at.clamp(0, V - 1)[:, None])[:, 0], torch.full_like(entropy, float("nan")))
-    ids = torch.sort(torch.where(raw.isnan(), torch.full_like(raw, float("-inf")), raw), dim=1, descending=True, stable=True).indices[:, :k]
+    if k > 0:
+        ids = torch.sort(torch.where(raw.isnan(), torch.full_like(raw, float("-inf")), raw), dim=1, descending=True, stable=True).indices[:, :k]
+    else:
+        ids = torch.empty(T, 0, dtype=torch.long, device=logits.device)
     return TokenScores(got, entropy, ids.to(torch.int32), lp.gather(1, ids))

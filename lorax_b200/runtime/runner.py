@@ -247,8 +247,9 @@ class ModelRunner:
         self.h2d_bytes += flat.numel() * 4
         d_lead, d_ids, d_seqs, d_pages, d_head, d_headslot, d_state, *d_off = flat.split([len(x) for x in segs])
         d_seqs = d_seqs.view(4, len(items))
-        st = self.model.ops.step_tables(d_seqs, d_pages, T, self.max_blocks, page, window=self.model.config.sliding_window or 0, tiles=lists,
-                                        lora_tiles=n_lora, row_offset=row_offset, lead=d_lead.view(-1, 4) if lead_tiles else None)
+        make = self.model.ops.step_tables if len(items) <= reference.STEP_SEQS_MAX else reference.step_tables_of_many
+        st = make(d_seqs, d_pages, T, self.max_blocks, page, window=self.model.config.sliding_window or 0, tiles=lists,
+                  lora_tiles=n_lora, row_offset=row_offset, lead=d_lead.view(-1, 4) if lead_tiles else None)
         (d_ts, d_tq), *more = st.tiles
         none = (d_ids[:0], d_ids[:0])
         d_q8s, d_q8q = more.pop(0) if self.model.context_windows else none
@@ -280,7 +281,11 @@ class ModelRunner:
         """Scores of given tokens: one ragged step over the items (prompts, or continuations of cached ones: `cache_len`), their keys and
         values written like a prefill's.  Returns `ops.TokenScores` on the device with a row for every token of the items in turn: under the
         distribution behind that token, the log-probability of the item's next token (NaN behind the last), the entropy, and the `k` best
-        tokens with their log-probabilities."""
+        tokens with their log-probabilities (`k` up to 32).  An item has at least one token."""
+        if not all(len(it.token_ids) for it in items) or not items:
+            raise ValueError("score: items of at least one token")
+        if not 0 <= k <= min(reference.TOP_MAX, self.model.config.vocab_size):
+            raise ValueError(f"score: {k} alternatives, at most {reference.TOP_MAX}")
         items = [replace(it, want_logits=True, all_logprobs=True, logit_rows=None) for it in items]
         inp, _ = self._prefill_inputs(items)
         targets = self._to_dev([t for it in items for t in [*it.token_ids[1:], -1][: len(it.token_ids)]])

@@ -7,6 +7,7 @@ import torch
 from lorax_b200.ops import native, reference
 
 BF16 = torch.bfloat16
+INF, NAN = float("inf"), float("nan")
 
 
 def ints(*v):
@@ -34,6 +35,13 @@ def _tables_args(**over):
     dict(lora_tiles=-1), dict(lora_rows=0), dict(lead=ints(1, 2, 3, 4)), dict(lead=ints([1, 2, 3])), dict(lead=ints([1, 2, 3, 4]).long()),
     dict(lead=torch.zeros(5, 4, dtype=torch.int32).view(-1)[1:17].view(4, 4))])
 def test_tables_refuse(over):
+    _refused("step_tables", **_tables_args(**over))
+
+
+@pytest.mark.parametrize("over", [
+    dict(tokens=2 ** 31), dict(max_blocks=2 ** 31), dict(page=2 ** 32 + 32), dict(window=2 ** 31), dict(tiles=((2 ** 31, 1),)), dict(tiles=((64, 2 ** 31),)),
+    dict(lora_tiles=2 ** 31), dict(lora_rows=2 ** 31), dict(row_offset=-1), dict(row_offset=2 ** 31)])
+def test_tables_refuse_what_is_past_32_bits(over):
     _refused("step_tables", **_tables_args(**over))
 
 
@@ -96,6 +104,13 @@ def _moe_args(T=2, E=4, k=2, H=64, I=32, **over):
     dict(w13=torch.zeros(4, 48, 64, dtype=BF16)), dict(w13=torch.zeros(8, 64, 64, dtype=BF16)[::2]), dict(w2=torch.zeros(4, 32, 64, dtype=BF16).transpose(1, 2)),
     dict(out=torch.zeros(3, 64, dtype=BF16)), dict(out=torch.zeros(2, 64)), dict(out=torch.zeros(64, 2, dtype=BF16).t())])
 def test_experts_refuse(over):
+    _refused("moe_few", **_moe_args(**over))
+
+
+@pytest.mark.parametrize("over", [
+    dict(x=torch.zeros(1, 64, dtype=BF16).expand(2, -1)), dict(x=torch.zeros(88, dtype=BF16).as_strided((2, 64), (16, 1))),
+    dict(router_w=torch.zeros(1, 64, dtype=BF16).expand(4, -1)), dict(out=torch.zeros(1, 64, dtype=BF16).expand(2, -1))])
+def test_experts_refuse_rows_on_top_of_one_another(over):
     _refused("moe_few", **_moe_args(**over))
 
 
@@ -167,6 +182,24 @@ def _tiny(device, dtype, **over):
     return m, ModelRunner(m, KVCache(cfg.num_hidden_layers, 32, m.nkv, m.d, m.dtype, m.device), max_batch=4, max_seq_tokens=512, max_prefill_tokens=512, use_graphs=False)
 
 
+def test_scores_refuse_caps_that_are_no_fp32_numbers_and_vocabularies_past_30_bits():
+    logits = torch.zeros(2, 8)
+    for cap in (INF, NAN, -1.0, 1e39, 1e-50):
+        _refused("token_scores", logits, softcap=cap)
+    _refused("token_scores", torch.empty(1, 1 << 30, device="meta"))
+
+
+def test_the_runner_refuses_to_score_nothing_and_too_many_alternatives():
+    from lorax_b200.runtime.runner import PrefillItem
+    m, r = _tiny("cpu", torch.float32)
+    before = [t.clone() for layer in r.kv.layers for t in layer]
+    for items, k in (([], 0), ([PrefillItem([], 0, [1])], 0), ([PrefillItem([5], 0, [1]), PrefillItem([], 0, [2])], 0), ([PrefillItem([5], 0, [1])], 33),
+                     ([PrefillItem([5], 0, [1])], -1)):
+        with pytest.raises(ValueError, match="score"):
+            r.score(items, k=k)
+    assert all(torch.equal(a, b) for a, b in zip(before, (t for layer in r.kv.layers for t in layer)))
+
+
 @pytest.mark.parametrize("cap", [0.0, 2.0])
 def test_scores_of_prompts_by_the_runner(cap):
     """Every token's score is that of the logits which a prefill of the same items returns; the last row of an item has no next token."""
@@ -207,3 +240,12 @@ def test_alternatives_beyond_the_kernels():
         best = lp.topk(k, -1)
         assert ids.tolist() == logits.argmax(-1).tolist() and torch.allclose(got, lp.max(-1).values, atol=1e-6)
         assert alt.tolist() == best.indices.tolist() and torch.allclose(alp, best.values, atol=1e-6)
+
+
+def test_a_step_of_more_sequences_than_the_kernel_takes():
+    from lorax_b200.runtime.runner import PrefillItem
+    m, r = _tiny("cpu", torch.float32)
+    r.max_prefill_tokens = n = reference.STEP_SEQS_MAX + 5
+    inp, _ = r._prefill_inputs([PrefillItem([i % 512], i % 7, [1 + i % 9]) for i in range(n)])
+    assert inp.cu_q.tolist() == list(range(n + 1)) and inp.positions.tolist() == [i % 7 for i in range(n)]
+    assert inp.slots.tolist() == [(1 + i % 9) * r.page + i % 7 for i in range(n)] and inp.tile_seq.tolist() == list(range(n))

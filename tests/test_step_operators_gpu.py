@@ -66,6 +66,16 @@ def test_tables_without_sequences_and_with_bad_lengths():
     assert got.block_tables.tolist() == [[0] * 4, [11, 12, 0, 0], [0] * 4] and got.tiles[0][0].tolist() == [1, 1, 2] and got.lora_tiles.tolist() == [[2, 0, 3, 0]]
 
 
+def test_tables_of_sums_past_32_bits_and_of_high_tiles():
+    """Page counts whose sum wraps around read nothing out of range; a tile higher than any sequence is one a sequence."""
+    seqs, pages = ints([3, 4, 5, 6], [0, 0, 0, 0], [-1, 1, 1, -1], [2 ** 30, 2 ** 30, 2 ** 30, 2 ** 30 - 1]), ints(4, 5, 6)
+    got = native.step_tables(seqs.cuda(), pages.cuda(), 18, 5, 32, tiles=((2 ** 31 - 1, 5),), lora_tiles=3, lora_rows=2 ** 31 - 1)
+    want = reference.step_tables(seqs[:, :1], pages, 3, 5, 32)
+    assert torch.equal(got.block_tables[:1].cpu(), want.block_tables) and (got.block_tables[1:] == 0).all()
+    assert [x.tolist() for x in got.tiles[0]] == [[0, 1, 2, 3, -1], [0, 0, 0, 0, 0]]
+    assert got.lora_tiles.tolist() == [[1, 3, 4, 0], [1, 7, 5, 0], [-1, 0, 0, 0]]
+
+
 # ------------------------------------------------------------------------------------------------ scores
 def _scores_oracle(logits, targets, k, cap):
     raw = logits.double()
@@ -149,6 +159,21 @@ def test_scores_of_rows_with_masks_ties_and_no_distribution(T, dtype):
                    lambda x: (x.fill_(-INF), x[:, 0].fill_(NAN)), lambda x: x.copy_(x.round()), lambda x: x.mul_(1000), lambda x: (x.fill_(low), x[:, ::3].fill_(-INF))):
         for k in (0, 1, 6, 32):
             _check_scores(row(change), targets, k)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [2, 170])
+def test_scores_under_a_cap_of_rows_with_masks(T, dtype):
+    """A cap takes infinities and lowest values to its two ends: all tokens have a probability."""
+    V, low = 9001, torch.finfo(dtype).min
+    base, targets = _logits(T, V, dtype, 6)
+    for value in (-INF, INF, low, NAN):
+        for rows in (slice(None), slice(1)):
+            for cols in (slice(None), slice(0, V - 1), slice(4000, 4003)):
+                x = base.clone()
+                x[rows, cols] = value
+                for k in (0, 6):
+                    _check_scores(x, targets, k, 30.0)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -277,6 +302,19 @@ def test_experts_of_rows_apart_into_a_given_result():
     assert got.data_ptr() == out[:, 5:].data_ptr() and (out[:, :5] == 3).all() and (out[:, 517:] == 3).all()
     assert torch.equal(got, native.moe_few(x, wr, w13, w2, 2))
     assert native.moe_few(x[:0], wr, w13, w2, 2).shape == (0, 512)
+
+
+def test_one_token_and_one_expert_of_any_row_stride():
+    x, wr, w13, w2 = _experts(1, 1, 1, 128, 64)
+    want = native.moe_few(x, wr, w13, w2, 1)
+    assert torch.equal(native.moe_few(x[0].expand(1, -1), wr[0].expand(1, -1), w13, w2, 1), want)
+    assert torch.equal(native.moe_few(x.as_strided((1, 128), (1, 1)), wr.as_strided((1, 128), (1, 1)), w13, w2, 1), want)
+
+
+@pytest.mark.parametrize("T,E,k,H,I", [(16, 8, 4, 9480, 1000), (9, 4, 4, 8200, 520), (3, 3, 1, 4744, 584), (16, 16, 16, 7112, 72)])
+def test_experts_wider_than_a_round_of_rows_with_rests(T, E, k, H, I):
+    _check_experts(_experts(T, E, k, H, I), k)
+    native.workspace().check_status()
 
 
 def test_experts_choose_the_lower_number_on_ties_and_none_twice():
