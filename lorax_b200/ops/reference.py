@@ -1042,7 +1042,7 @@ def step_tables_of_many(seqs, pages, tokens: int, max_blocks: int, page: int, wi
     cu, tables, off = [0], [], 0
     for b in range(B):
         cu.append(cu[-1] + n[b])
-        own = [flat[i] if i < len(flat) else 0 for i in range(off, off + held[b])]
+        own = [flat[i] if i < len(flat) else 0 for i in range(off, off + min(held[b], max_blocks))]
         off += held[b]
         if window > 0 and 0 < held[b] < max_blocks and held[b] * page >= window + page:
             tables.append([own[j % held[b]] for j in range(max_blocks)])
