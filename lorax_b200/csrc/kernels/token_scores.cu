@@ -81,8 +81,16 @@ LX_DEVICE float max_nan(float a, float b) {
   return r;
 }
 
-LX_DEVICE uint64_t pack_f32x2(float lo, float hi) { return ((uint64_t)__float_as_uint(hi) << 32) | __float_as_uint(lo); }
-LX_DEVICE float2 unpack_f32x2(uint64_t v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
+LX_DEVICE uint64_t pack_f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+LX_DEVICE float2 unpack_f32x2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
 LX_DEVICE uint64_t add_f32x2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -104,13 +112,15 @@ LX_DEVICE float exp2_fast(float x) {
   return r;
 }
 
-// 16 bytes of logits (VEC), or one.  What lies past the end reads as -inf: it adds nothing.
-template <typename L, bool VEC>
+// 16 bytes of logits, or one (WIDE).  What lies past the end reads as -inf: it adds nothing.  values: those below `floor` are raised to it.  Tops pass over NaN.
+template <typename L, bool WIDE>
 struct ScoreLoad;
 template <>
 struct ScoreLoad<__nv_bfloat16, true> {
   static constexpr int kN = 8;
   using Raw = uint4;
+  using Top = __nv_bfloat162;      // of even and odd elements
+  LX_DEVICE static __nv_bfloat162 two(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
   LX_DEVICE static Raw load(const __nv_bfloat16* p, bool ok) { return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   LX_DEVICE static void values(const Raw& v, float (&x)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -120,35 +130,44 @@ struct ScoreLoad<__nv_bfloat16, true> {
       x[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
     }
   }
-  LX_DEVICE static float top(const Raw& v) {      // passes over NaN
-    auto two = [](uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); };
-    const __nv_bfloat162 m = __hmax2(__hmax2(two(v.x), two(v.y)), __hmax2(two(v.z), two(v.w)));
-    return fmaxf(__low2float(m), __high2float(m));
+  // (two elements an instruction; the floor is rounded: what is raised to it adds nothing all the same)
+  LX_DEVICE static void values(const Raw& v, float (&x)[8], float floor) {
+    const __nv_bfloat162 low = __float2bfloat162_rn(floor);
+    auto up = [&](uint32_t w) {
+      const __nv_bfloat162 r = __hmax2_nan(two(w), low);
+      return *reinterpret_cast<const uint32_t*>(&r);
+    };
+    values(make_uint4(up(v.x), up(v.y), up(v.z), up(v.w)), x);
   }
+  LX_DEVICE static Top top(const Raw& v) { return __hmax2(__hmax2(two(v.x), two(v.y)), __hmax2(two(v.z), two(v.w))); }
+  LX_DEVICE static Top top(const Top& a, const Top& b) { return __hmax2(a, b); }
+  LX_DEVICE static float value(const Top& a) { return fmaxf(__low2float(a), __high2float(a)); }
 };
 template <>
 struct ScoreLoad<float, true> {
   static constexpr int kN = 4;
   using Raw = float4;
+  using Top = float;
   LX_DEVICE static Raw load(const float* p, bool ok) { return ok ? *reinterpret_cast<const float4*>(p) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
   LX_DEVICE static void values(const Raw& v, float (&x)[4]) { x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-  LX_DEVICE static float top(const Raw& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+  LX_DEVICE static void values(const Raw& v, float (&x)[4], float floor) {
+    x[0] = max_nan(v.x, floor); x[1] = max_nan(v.y, floor); x[2] = max_nan(v.z, floor); x[3] = max_nan(v.w, floor);
+  }
+  LX_DEVICE static Top top(const Raw& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+  LX_DEVICE static Top top(Top a, Top b) { return fmaxf(a, b); }
+  LX_DEVICE static float value(Top a) { return a; }
 };
-template <>
-struct ScoreLoad<__nv_bfloat16, false> {
+template <typename L>
+struct ScoreLoad<L, false> {
   static constexpr int kN = 1;
   using Raw = float;
-  LX_DEVICE static Raw load(const __nv_bfloat16* p, bool ok) { return ok ? __bfloat162float(*p) : -INFINITY; }
+  using Top = float;
+  LX_DEVICE static Raw load(const L* p, bool ok) { return ok ? (float)*p : -INFINITY; }
   LX_DEVICE static void values(const Raw& v, float (&x)[1]) { x[0] = v; }
-  LX_DEVICE static float top(const Raw& v) { return v; }
-};
-template <>
-struct ScoreLoad<float, false> {
-  static constexpr int kN = 1;
-  using Raw = float;
-  LX_DEVICE static Raw load(const float* p, bool ok) { return ok ? *p : -INFINITY; }
-  LX_DEVICE static void values(const Raw& v, float (&x)[1]) { x[0] = v; }
-  LX_DEVICE static float top(const Raw& v) { return v; }
+  LX_DEVICE static void values(const Raw& v, float (&x)[1], float floor) { x[0] = max_nan(v, floor); }
+  LX_DEVICE static Top top(const Raw& v) { return v; }
+  LX_DEVICE static Top top(Top a, Top b) { return fmaxf(a, b); }
+  LX_DEVICE static float value(Top a) { return a; }
 };
 
 // Entropy of row t and the log-probability of its target, from the sums of the whole row.
@@ -162,68 +181,116 @@ LX_DEVICE void score_row(const TokenScoresParams& p, int t, const L* row, const 
   p.logprobs[t] = lp;
 }
 
+// exp(c - m) is formed as 2^(log2e c + shift) with shift = -log2e m rounded: one FMA for two logits, whose products are not rounded.  What the rounding of
+// the shift leaves out is the same for all terms and put right where the sums change hands.  Where the maximum is too far out for that (masks of the
+// type's lowest value, infinities) the difference comes first.
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Below 2048 the shift is rounded by at most 2^-13, and what the linear term of score_sums leaves of that is under 2^-27.
+constexpr float kScoreFar = 2048.f;
+
+LX_DEVICE bool score_far(float m) { return !(fabsf(m) < kScoreFar); }
+
 struct ScoreThread {
-  float m;                 // running maximum of the (capped) logits
-  uint64_t s, u;           // running sums, of even and odd elements
-  float best;              // of the raw logits, with the lowest index that has it
-  int index;
+  float m, shift;          // running maximum of the (capped) logits
+  uint64_t s, u;           // running sums of e = 2^a and of a e, a = log2e c + shift, of even and odd elements
+  float best;              // of the raw logits (TOP), and the first element of the first load that has it
+  int place;
 };
 
-// R loads of a thread, the first from index i on, the others `step` further each (indices only grow); from `end` on they are not of the row.
-template <typename Load, int R, bool CAP>
+// The sums as they are for a shift that is not rounded, in natural logarithms.
+LX_DEVICE ScoreSums score_sums(const ScoreThread& t) {
+  const float2 s2 = unpack_f32x2(t.s), u2 = unpack_f32x2(t.u);
+  const float s = s2.x + s2.y, u = u2.x + u2.y, off = score_far(t.m) ? 0.f : fmaf(kLog2e, t.m, t.shift);      // (at most half a step of the shift)
+  const float f = 1.f - off * kLn2;                                                                           // 2^-off
+  return ScoreSums{t.m, s * f, (u - off * s) * f * kLn2};
+}
+
+// R loads of a thread, the first from index i on, the others `step` further each; from `end` on they are not of the row (GUARD: there may be such).  Wide
+// loads come in the order of the row; a single one may be in front of them.
+template <typename Load, int R, bool TOP, bool CAP, bool GUARD>
 LX_DEVICE void score_take(ScoreThread& t, const typename Load::Raw (&raw)[R], int i, int step, int end, float cap) {
   constexpr int N = Load::kN;
-  float top = Load::top(raw[0]);
+  typename Load::Top tops[R], all = tops[0] = Load::top(raw[0]);
 #pragma unroll
-  for (int r = 1; r < R; ++r) top = fmaxf(top, Load::top(raw[r]));
-  if (top > t.best) {
-    t.best = top;
+  for (int r = 1; r < R; ++r) all = Load::top(all, tops[r] = Load::top(raw[r]));
+  float top = Load::value(all);
+  if (TOP && (top > t.best || (N == 1 && i < t.place && (top == top ? top : -INFINITY) == t.best))) {      // (NaN orders as -inf)
+    t.best = fmaxf(t.best, top);
 #pragma unroll
-    for (int r = R - 1; r >= 0; --r) {
-      float x[N];
-      Load::values(raw[r], x);
-#pragma unroll
-      for (int q = N - 1; q >= 0; --q)
-        if (x[q] == top) t.index = i + r * step + q;
-    }
+    for (int r = R - 1; r >= 0; --r)
+      if (N == 1 || Load::value(tops[r]) == top) t.place = i + r * step;
   }
   top = score_cap<CAP>(top, cap);
   if (top > t.m) {
+    const float shift = score_far(top) ? 0.f : -kLog2e * top;
     if (t.m != -INFINITY) {
-      const float d = fmaxf(t.m - top, kScoreFloor), f = __expf(d);
+      const float d = fmaxf(score_far(top) || score_far(t.m) ? (t.m - top) * kLog2e : shift - t.shift, kScoreFloor), f = exp2_fast(d);
       const uint64_t d2 = pack_f32x2(d, d), f2 = pack_f32x2(f, f);
       t.u = mul_f32x2(fma_f32x2(d2, t.s, t.u), f2);
       t.s = mul_f32x2(t.s, f2);
     }
     t.m = top;
+    t.shift = shift;
   }
-  const float m = t.m == -INFINITY ? 0.f : t.m;      // (logits of -inf only, so far: they add zeros)
-  const uint64_t m2 = pack_f32x2(-m, -m), log2e = pack_f32x2(1.4426950408889634f, 1.4426950408889634f);
-  auto add = [&](float a, float b) {
-    float2 d = unpack_f32x2(add_f32x2(pack_f32x2(a, b), m2));
-    d.x = max_nan(d.x, kScoreFloor);
-    d.y = max_nan(d.y, kScoreFloor);
-    const uint64_t d2 = pack_f32x2(d.x, d.y);
-    const float2 l = unpack_f32x2(mul_f32x2(d2, log2e));
-    const uint64_t e = pack_f32x2(exp2_fast(l.x), exp2_fast(l.y));
+  auto add = [&](uint64_t a2, bool low) {
+    float2 a = unpack_f32x2(a2);
+    if (low) {
+      a.x = max_nan(a.x, kScoreFloor);
+      a.y = max_nan(a.y, kScoreFloor);
+    }
+    const uint64_t e = pack_f32x2(exp2_fast(a.x), exp2_fast(a.y));
     t.s = add_f32x2(t.s, e);
-    t.u = fma_f32x2(d2, e, t.u);
+    t.u = fma_f32x2(pack_f32x2(a.x, a.y), e, t.u);
   };
-  auto capped = [&](float x, int r) { return r == 0 || i + r * step < end ? score_cap<CAP>(x, cap) : -INFINITY; };
-  // (all values of the batch are formed before the chains of adds: N R is even but for the last element of a row)
-  float x[R][N];
+  // two logits of a load; a single one has one of -inf beside it, which is raised to the floor
+  auto pair = [&](const float (&x)[N], int q) {
+    return pack_f32x2(score_cap<CAP>(x[q], cap), N > 1 ? score_cap<CAP>(x[(q + 1) % N], cap) : -INFINITY);
+  };
+  const uint64_t log2e = pack_f32x2(kLog2e, kLog2e);
+  if (!score_far(t.m)) {
+    const uint64_t shift = pack_f32x2(t.shift, t.shift);
 #pragma unroll
-  for (int r = 0; r < R; ++r) Load::values(raw[r], x[r]);
-  if constexpr (N > 1) {
+    for (int r = 0; r < R; ++r) {
+      if (GUARD && CAP && r > 0 && i + r * step >= end) continue;      // (without a cap they are -inf and add nothing)
+      float x[N];
+      if (CAP) Load::values(raw[r], x);
+      else Load::values(raw[r], x, t.m + kScoreFloor);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int q = 0; q < N; q += 2) add(capped(x[r][q], r), capped(x[r][q + 1], r));
+      for (int q = 0; q < N; q += 2) add(fma_f32x2(pair(x, q), log2e, shift), CAP || N == 1);
+    }
   } else {
+    const float m = t.m == -INFINITY ? 0.f : -t.m;      // (logits of -inf only, so far: they add zeros)
 #pragma unroll
-    for (int r = 0; r < R; r += 2) add(capped(x[r][0], r), r + 1 < R ? capped(x[r + 1][0], r + 1) : -INFINITY);
+    for (int r = 0; r < R; ++r) {
+      if (GUARD && CAP && r > 0 && i + r * step >= end) continue;
+      float x[N];
+      Load::values(raw[r], x);
+#pragma unroll
+      for (int q = 0; q < N; q += 2) add(mul_f32x2(add_f32x2(pair(x, q), pack_f32x2(m, m)), log2e), true);
+    }
   }
 }
+
+// A part [lo, hi) of a row: 16-byte loads from `body` to `whole`, where the row's alignment allows them; single logits in front and behind, one each for the
+// first threads of two warps.
+struct ScorePart {
+  int lo, hi, body, whole;
+  template <int N, typename L>
+  LX_DEVICE static ScorePart of(const L* row, int V) {
+    const int chunk = ((V + gridDim.y - 1) / gridDim.y + 7) & ~7;
+    ScorePart s;
+    s.lo = min((int)blockIdx.y * chunk, V);
+    s.hi = min(s.lo + chunk, V);
+    s.body = min(s.lo + (int)((0 - reinterpret_cast<uintptr_t>(row + s.lo) / sizeof(L)) & (N - 1)), s.hi);
+    s.whole = s.body + (s.hi - s.body) / N * N;
+    return s;
+  }
+  LX_DEVICE int single(int thread) const {
+    if (thread < body - lo) return lo + thread;
+    return thread >= 32 && thread - 32 < hi - whole ? whole + thread - 32 : -1;
+  }
+};
 
 struct ScoreShared {
   ScoreSums warps[kScoreWarps];
@@ -254,9 +321,10 @@ LX_DEVICE void score_rank(const unsigned long long* list, int n, int k, unsigned
   }
 }
 
-template <typename L, bool VEC, bool CAP>
+template <typename L, bool CAP>
 __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __grid_constant__ TokenScoresParams p) {
-  using Load = ScoreLoad<L, VEC>;
+  using Load = ScoreLoad<L, true>;
+  using One = ScoreLoad<L, false>;
   constexpr int kVec = Load::kN, kStep = kScoreThreads * kVec;
   __shared__ ScoreShared sh;
   const int t = blockIdx.x, part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
@@ -264,33 +332,38 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   pdl_wait();
   pdl_trigger();
   const L* row = reinterpret_cast<const L*>(p.logits) + (long long)t * p.ld;
-  const int chunk = ((p.V + parts - 1) / parts + 7) & ~7;
-  const int lo = min(part * chunk, p.V), hi = min(lo + chunk, p.V);
-  const int whole = lo + (hi - lo) / kVec * kVec;      // a thread's elements: kVec from lo + (it * threads + tid) * kVec on, and one from `whole` on
-  ScoreThread me{-INFINITY, 0, 0, -INFINITY, -1};
-  if (lo + tid * kVec < whole) me.index = lo + tid * kVec;
-  else if (whole + tid < hi) me.index = whole + tid;
-  for (int i = lo + tid * kVec; i < whole; i += kScoreUnroll * kStep) {
+  const ScorePart row_part = ScorePart::of<kVec>(row, p.V);
+  const int whole = row_part.whole, single = row_part.single(tid);
+  ScoreThread me{-INFINITY, 0.f, 0, 0, -INFINITY, -1};
+  int i = row_part.body + tid * kVec;
+  if (i < whole) me.place = i;
+  else if (single >= 0) me.place = single;
+  for (; i + (kScoreUnroll - 1) * kStep < whole; i += kScoreUnroll * kStep) {
+    typename Load::Raw raw[kScoreUnroll];
+#pragma unroll
+    for (int r = 0; r < kScoreUnroll; ++r) raw[r] = Load::load(row + i + r * kStep, true);
+    score_take<Load, kScoreUnroll, true, CAP, false>(me, raw, i, kStep, whole, p.softcap);
+  }
+  if (i < whole) {
     typename Load::Raw raw[kScoreUnroll];
 #pragma unroll
     for (int r = 0; r < kScoreUnroll; ++r) raw[r] = Load::load(row + i + r * kStep, i + r * kStep < whole);
-    score_take<Load, kScoreUnroll, CAP>(me, raw, i, kStep, whole, p.softcap);
+    score_take<Load, kScoreUnroll, true, CAP, true>(me, raw, i, kStep, whole, p.softcap);
   }
-  if (VEC && whole + tid < hi) {
-    using One = ScoreLoad<L, false>;
-    const float raw[1] = {One::load(row + whole + tid, true)};
-    score_take<One, 1, CAP>(me, raw, whole + tid, 0, hi, p.softcap);
+  if (single >= 0) {
+    const float raw[1] = {One::load(row + single, true)};
+    score_take<One, 1, true, CAP, false>(me, raw, single, 0, p.V, p.softcap);
   }
 
   // sums of the CTA
-  const float2 s2 = unpack_f32x2(me.s), u2 = unpack_f32x2(me.u);
-  ScoreSums a{me.m, s2.x + s2.y, u2.x + u2.y};
+  ScoreSums a = score_sums(me);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
   if ((tid & 31) == 0) sh.warps[tid >> 5] = a;
-  const bool live = me.index >= 0;
-  const unsigned long long mine = live ? score_pair(score_key(me.best), me.index) : 0;
-  unsigned long long g = mine;
+  // A thread's best element is one of those from `place` on that came in one load: it ranks between these two pairs.
+  const bool live = me.place >= 0;
+  const unsigned long long mine = live ? score_pair(score_key(me.best), me.place) : 0;
+  unsigned long long g = live ? score_pair(score_key(me.best), me.place + (me.place == single ? 0 : kVec - 1)) : 0;
 #pragma unroll
   for (int o = 1; o < kScoreThreads / kScoreGroups; o <<= 1) {
     const unsigned long long other = __shfl_xor_sync(0xffffffffu, g, o);
@@ -325,7 +398,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   if (live && mine >= bound) sh.cand[atomicAdd(&sh.ncand, 1)] = tid;
   __syncthreads();
   const int ncand = sh.ncand;
-  const int its = (whole - lo + kStep - 1) / kStep;      // loads of a thread; its single element counts as one more
+  const int its = (whole - row_part.body + kStep - 1) / kStep;      // wide loads of a thread; its single element counts as one more
   auto push = [&](float x, int idx) {
     const unsigned long long pair = score_pair(score_key(x), idx);
     if (pair >= bound) {
@@ -335,10 +408,11 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   };
   auto collect = [&](int c, int it) {
     if (it == its) {
-      if (VEC && whole + c < hi) push(ScoreLoad<L, false>::load(row + whole + c, true), whole + c);
+      const int one = row_part.single(c);
+      if (one >= 0) push(One::value(One::load(row + one, true)), one);
       return;
     }
-    const int from = lo + (it * kScoreThreads + c) * kVec;
+    const int from = row_part.body + (it * kScoreThreads + c) * kVec;
     if (from >= whole) return;
     float x[kVec];
     Load::values(Load::load(row + from, true), x);
@@ -408,72 +482,12 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
 // ------------------------------------------------------------------------------------------------ without alternatives
 // Bound by the HBM, and by the instructions of a logit: 2048 rows of 128256 bf16 in 86 us (6.1 TB/s), 4001 of 32000 in 51 (5.0 TB/s; with 512 threads a
 // CTA, which reach the ends of their rows together, 63 to 72).  With a cap 1000 rows of 32000 take 50 us: tanhf.
-// exp(c - m) is formed as 2^(log2e c + shift) with shift = -log2e m rounded: one FMA a logit, whose product is not rounded.  What the rounding of the
-// shift leaves out is the same for all terms and put right where the sums change hands.  Where the maximum is too far out for that (masks of the
-// type's lowest value, infinities) the difference comes first.
 constexpr int kLeanThreads = 256;
 constexpr int kLeanWarps = kLeanThreads / 32;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-// Below 2048 the shift is rounded by at most 2^-13, and what the linear term of lean_sums leaves of that is under 2^-27.
-constexpr float kLeanFar = 2048.f;
-
-LX_DEVICE bool lean_far(float m) { return !(fabsf(m) < kLeanFar); }
-
-struct LeanThread {
-  float m, shift;          // running maximum of the (capped) logits
-  float s, u;              // running sums of e = 2^a and of a e, a = log2e c + shift
-};
-
-// The sums as they are for a shift that is not rounded, in natural logarithms.
-LX_DEVICE ScoreSums lean_sums(const LeanThread& t) {
-  const float off = lean_far(t.m) ? 0.f : fmaf(kLog2e, t.m, t.shift);      // (at most half a step of the shift)
-  const float f = 1.f - off * kLn2;                                        // 2^-off
-  return ScoreSums{t.m, t.s * f, (t.u - off * t.s) * f * kLn2};
-}
-
-// R loads of a thread, the first from index i on, the others `step` further each; from `end` on they are not of the row (GUARD: there may be such).
-template <typename Load, int R, bool CAP, bool GUARD>
-LX_DEVICE void lean_take(LeanThread& t, const typename Load::Raw (&raw)[R], int i, int step, int end, float cap) {
-  float top = Load::top(raw[0]);
-#pragma unroll
-  for (int r = 1; r < R; ++r) top = fmaxf(top, Load::top(raw[r]));
-  top = score_cap<CAP>(top, cap);
-  if (top > t.m) {
-    const float shift = lean_far(top) ? 0.f : -kLog2e * top;
-    if (t.m != -INFINITY) {
-      const float d = fmaxf(lean_far(top) || lean_far(t.m) ? (t.m - top) * kLog2e : shift - t.shift, kScoreFloor), f = exp2_fast(d);
-      t.u = fmaf(d, t.s, t.u) * f;
-      t.s *= f;
-    }
-    t.m = top;
-    t.shift = shift;
-  }
-  auto add = [&](float a) {
-    a = max_nan(a, kScoreFloor);
-    const float e = exp2_fast(a);
-    t.s += e;
-    t.u = fmaf(a, e, t.u);
-  };
-  const bool far = lean_far(t.m);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (GUARD && r > 0 && i + r * step >= end) continue;
-    float x[Load::kN];
-    Load::values(raw[r], x);
-    if (!far) {
-#pragma unroll
-      for (int q = 0; q < Load::kN; ++q) add(fmaf(score_cap<CAP>(x[q], cap), kLog2e, t.shift));
-    } else {                             // (logits of -inf only, so far: they add zeros)
-#pragma unroll 1
-      for (int q = 0; q < Load::kN; ++q) add((score_cap<CAP>(x[q], cap) - (t.m == -INFINITY ? 0.f : t.m)) * kLog2e);
-    }
-  }
-}
-
-template <typename L, bool VEC, bool CAP>
+template <typename L, bool CAP>
 __global__ void __launch_bounds__(kLeanThreads, 6) token_logprobs_kernel(const __grid_constant__ TokenScoresParams p) {
-  using Load = ScoreLoad<L, VEC>;
+  using Load = ScoreLoad<L, true>;
+  using One = ScoreLoad<L, false>;
   constexpr int kVec = Load::kN, kStep = kLeanThreads * kVec;
   __shared__ ScoreSums warps[kLeanWarps], ends[kScoreMaxParts];      // (the latter of the cluster's first CTA)
   const int t = blockIdx.x, part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
@@ -481,28 +495,27 @@ __global__ void __launch_bounds__(kLeanThreads, 6) token_logprobs_kernel(const _
   pdl_wait();
   pdl_trigger();
   const L* row = reinterpret_cast<const L*>(p.logits) + (long long)t * p.ld;
-  const int chunk = ((p.V + parts - 1) / parts + 7) & ~7;
-  const int lo = min(part * chunk, p.V), hi = min(lo + chunk, p.V), whole = lo + (hi - lo) / kVec * kVec;
-  LeanThread me{-INFINITY, 0.f, 0.f, 0.f};
-  int i = lo + tid * kVec;
+  const ScorePart row_part = ScorePart::of<kVec>(row, p.V);
+  const int whole = row_part.whole, single = row_part.single(tid);
+  ScoreThread me{-INFINITY, 0.f, 0, 0, -INFINITY, -1};
+  int i = row_part.body + tid * kVec;
   for (; i + (kScoreUnroll - 1) * kStep < whole; i += kScoreUnroll * kStep) {
     typename Load::Raw raw[kScoreUnroll];
 #pragma unroll
     for (int r = 0; r < kScoreUnroll; ++r) raw[r] = Load::load(row + i + r * kStep, true);
-    lean_take<Load, kScoreUnroll, CAP, false>(me, raw, i, kStep, whole, p.softcap);
+    score_take<Load, kScoreUnroll, false, CAP, false>(me, raw, i, kStep, whole, p.softcap);
   }
   if (i < whole) {
     typename Load::Raw raw[kScoreUnroll];
 #pragma unroll
     for (int r = 0; r < kScoreUnroll; ++r) raw[r] = Load::load(row + i + r * kStep, i + r * kStep < whole);
-    lean_take<Load, kScoreUnroll, CAP, true>(me, raw, i, kStep, whole, p.softcap);
+    score_take<Load, kScoreUnroll, false, CAP, true>(me, raw, i, kStep, whole, p.softcap);
   }
-  if (VEC && whole + tid < hi) {
-    using One = ScoreLoad<L, false>;
-    const float raw[1] = {One::load(row + whole + tid, true)};
-    lean_take<One, 1, CAP, false>(me, raw, whole + tid, 0, hi, p.softcap);
+  if (single >= 0) {
+    const float raw[1] = {One::load(row + single, true)};
+    score_take<One, 1, false, CAP, false>(me, raw, single, 0, p.V, p.softcap);
   }
-  ScoreSums a = lean_sums(me);
+  ScoreSums a = score_sums(me);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
   if ((tid & 31) == 0) warps[tid >> 5] = a;
@@ -528,11 +541,11 @@ __global__ void __launch_bounds__(kLeanThreads, 6) token_logprobs_kernel(const _
   if (tid == 0) score_row<L, CAP>(p, t, row, a, logf(a.s));
 }
 
-template <typename L, bool VEC>
+template <typename L>
 static int token_scores_launch(const TokenScoresParams& p, int T, int parts, cudaStream_t s) {
   void (*kernel)(TokenScoresParams);
-  if (p.k > 0) kernel = p.softcap > 0.f ? token_scores_kernel<L, VEC, true> : token_scores_kernel<L, VEC, false>;
-  else kernel = p.softcap > 0.f ? token_logprobs_kernel<L, VEC, true> : token_logprobs_kernel<L, VEC, false>;
+  if (p.k > 0) kernel = p.softcap > 0.f ? token_scores_kernel<L, true> : token_scores_kernel<L, false>;
+  else kernel = p.softcap > 0.f ? token_logprobs_kernel<L, true> : token_logprobs_kernel<L, false>;
   const cudaError_t e = launch_pdl_cluster(kernel, dim3(T, parts), dim3(p.k > 0 ? kScoreThreads : kLeanThreads), dim3(1, parts), 0, s, p);
   return e != cudaSuccess ? -(int)e : -(int)cudaGetLastError();
 }
@@ -554,10 +567,8 @@ int lx_token_scores(const void* logits, long long ld, int fp32, int T, int V, co
   const int vec = fp32 ? 4 : 8;
   int parts = 1;
   while (parts < kScoreMaxParts && (long long)T * parts * 2 <= 2 * 148 && V >= parts * kScoreThreads * vec) parts *= 2;
-  const bool aligned = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && (T == 1 || ld % vec == 0);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (fp32) return aligned ? token_scores_launch<float, true>(p, T, parts, s) : token_scores_launch<float, false>(p, T, parts, s);
-  return aligned ? token_scores_launch<__nv_bfloat16, true>(p, T, parts, s) : token_scores_launch<__nv_bfloat16, false>(p, T, parts, s);
+  return fp32 ? token_scores_launch<float>(p, T, parts, s) : token_scores_launch<__nv_bfloat16>(p, T, parts, s);
 }
 
 }  // extern "C"
