@@ -4,7 +4,7 @@
 //   log p_i = (c_i - m) - log s;  entropy = -sum p_i log p_i = log s - u / s
 //   best: by x descending, then by index ascending (the cap is monotone: it changes no order); a NaN orders as -inf
 //
-// One pass over the row with running m, s, u (a thread rescales its sums when its maximum grows), merged over lanes, warps and, where the rows
+// One pass over the row with running m, s, u (a thread rescales its sums when its maximum grows), joined over lanes, warps and, where the rows
 // alone do not fill the GPU, the CTAs of a cluster that share a row.  The sums are fp32: a thread adds some hundred terms of at most one, the
 // rest is a tree.  A logit of -inf adds nothing; a row of nothing else, one with a NaN and one with +inf have no distribution and score NaN.
 //
@@ -13,9 +13,10 @@
 // what is at or above the bound is listed, and the list is ranked by counting.  The order of (value, index) pairs is total, so the outcome
 // depends on no order of execution.
 //
-// Without alternatives a kernel of its own has more rows on an SM (lean, below).  With them the pass over the row is bound by its instructions, not
-// by the HBM: 2048 rows of 128256 bf16 take 145 us with 20 alternatives (3.6 TB/s), 96 rows 12 us, one row of 32000 in eight CTAs 6.6 us, most of it
-// launch, cluster and merges.
+// Without alternatives a kernel of its own has more rows on an SM (below).  With them a CTA is through with its row by some 5 us of joining, listing
+// and ranking, beside one other CTA on its SM, and the pass itself is bound by its instructions, not by the HBM: 2048 rows of 128256 bf16 take 127 us
+// with 20 alternatives (4.1 TB/s; 117 with one), 4001 rows of 32000 104 us, 96 rows of 32000 fp32 8.3 us, one row of 32000 in four CTAs 6.3 us, most of
+// it launch, cluster and joins.
 #include "common.cuh"
 
 namespace lx {
@@ -48,20 +49,6 @@ struct ScoreSums { float m, s, u; };
 // (masks of -inf or of the type's lowest value).
 constexpr float kScoreFloor = -200.f;
 
-LX_DEVICE void score_merge(ScoreSums& a, const ScoreSums& b) {
-  const float nm = fmaxf(a.m, b.m);
-  // (a side without a logit above -inf has s = u = 0, or NaN, which stays)
-  const float da = a.m == -INFINITY ? 0.f : fmaxf(a.m - nm, kScoreFloor), db = b.m == -INFINITY ? 0.f : fmaxf(b.m - nm, kScoreFloor);
-  const float fa = __expf(da), fb = __expf(db);
-  a.u = (a.u + da * a.s) * fa + (b.u + db * b.s) * fb;
-  a.s = a.s * fa + b.s * fb;
-  a.m = nm;
-}
-
-LX_DEVICE ScoreSums score_from_lane(const ScoreSums& a, int o) {
-  return ScoreSums{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
-}
-
 template <bool CAP>
 LX_DEVICE float score_cap(float x, float cap) { return CAP ? cap * tanhf(x / cap) : x; }
 
@@ -74,6 +61,25 @@ LX_DEVICE uint32_t score_key(float x) {
 LX_DEVICE float score_value(uint32_t key) { return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key); }
 // (value, index) pairs as one number, larger is better.
 LX_DEVICE unsigned long long score_pair(uint32_t key, int i) { return ((unsigned long long)key << 32) | (0xffffffffu - (uint32_t)i); }
+
+// The lanes' sums joined, in every lane.  (A side without a logit above -inf has s = u = 0, or NaN, which stays.)
+LX_DEVICE ScoreSums score_join(ScoreSums a) {
+  const float m = score_value(__reduce_max_sync(0xffffffffu, score_key(a.m)));
+  const float d = a.m == -INFINITY ? 0.f : fmaxf(a.m - m, kScoreFloor), f = __expf(d);
+  a.u = (a.u + d * a.s) * f;
+  a.s *= f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
+  return ScoreSums{m, a.s, a.u};
+}
+// The first n of a list of at most 32.
+LX_DEVICE ScoreSums score_join(const ScoreSums* list, int n) {
+  const int lane = threadIdx.x & 31;
+  return score_join(lane < n ? list[lane] : ScoreSums{-INFINITY, 0.f, 0.f});
+}
 
 LX_DEVICE float max_nan(float a, float b) {
   float r;
@@ -170,15 +176,17 @@ struct ScoreLoad<L, false> {
   LX_DEVICE static float value(Top a) { return a; }
 };
 
-// Entropy of row t and the log-probability of its target, from the sums of the whole row.
-template <typename L, bool CAP>
-LX_DEVICE void score_row(const TokenScoresParams& p, int t, const L* row, const ScoreSums& all, float logs) {
-  p.entropy[t] = logs - all.u / all.s;
-  if (p.logprobs == nullptr) return;
+// The target of row t, -1 where there is none.
+LX_DEVICE int score_target(const TokenScoresParams& p, int t) {
+  if (p.logprobs == nullptr) return -1;
   const long long target = p.wide_targets ? reinterpret_cast<const long long*>(p.targets)[t] : reinterpret_cast<const int*>(p.targets)[t];
-  float lp = NAN;
-  if (target >= 0 && target < p.V) lp = (score_cap<CAP>(ScoreLoad<L, false>::load(row + target, true), p.softcap) - all.m) - logs;
-  p.logprobs[t] = lp;
+  return target >= 0 && target < p.V ? (int)target : -1;
+}
+// Entropy of row t and the log-probability of its target, a logit (NaN: none), from the sums of the whole row.
+template <bool CAP>
+LX_DEVICE void score_row(const TokenScoresParams& p, int t, float given, const ScoreSums& all, float logs) {
+  p.entropy[t] = logs - all.u / all.s;
+  if (p.logprobs != nullptr) p.logprobs[t] = (score_cap<CAP>(given, p.softcap) - all.m) - logs;
 }
 
 // exp(c - m) is formed as 2^(log2e c + shift) with shift = -log2e m rounded: one FMA for two logits, whose products are not rounded.  What the rounding of
@@ -356,10 +364,10 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   }
 
   // sums of the CTA
-  ScoreSums a = score_sums(me);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
+  const int target = tid == 0 ? score_target(p, t) : -1;      // (its loads are on their way while the sums are joined)
+  ScoreSums a = score_join(score_sums(me));
   if ((tid & 31) == 0) sh.warps[tid >> 5] = a;
+  const float given = target >= 0 ? One::value(One::load(row + target, true)) : NAN;
   // A thread's best element is one of those from `place` on that came in one load: it ranks between these two pairs.
   const bool live = me.place >= 0;
   const unsigned long long mine = live ? score_pair(score_key(me.best), me.place) : 0;
@@ -375,11 +383,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
     sh.bound = 0;
   }
   __syncthreads();
-  if (tid < 32) {
-    a = sh.warps[tid & (kScoreWarps - 1)];
-#pragma unroll
-    for (int o = kScoreWarps / 2; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
-  }
+  if (tid < 32) a = score_join(sh.warps, kScoreWarps);
 
   // the bound: the k-th best of the groups' best, or none where there are fewer
   const int k = p.k;
@@ -468,10 +472,9 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   }
 
   if (tid >= 32) return;
-  ScoreSums all = sh.parts[0];
-  for (int c = 1; c < parts; ++c) score_merge(all, sh.parts[c]);
+  const ScoreSums all = score_join(sh.parts, parts);
   const float logs = logf(all.s);
-  if (tid == 0) score_row<L, CAP>(p, t, row, all, logs);
+  if (tid == 0) score_row<CAP>(p, t, given, all, logs);
   for (int j = tid; j < p.k; j += 32) {
     const unsigned long long pair = sh.own[j];
     p.top_ids[(long long)t * p.k + j] = (int)(0xffffffffu - (uint32_t)pair);
@@ -480,8 +483,8 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
 }
 
 // ------------------------------------------------------------------------------------------------ without alternatives
-// Bound by the HBM, and by the instructions of a logit: 2048 rows of 128256 bf16 in 86 us (6.1 TB/s), 4001 of 32000 in 51 (5.0 TB/s; with 512 threads a
-// CTA, which reach the ends of their rows together, 63 to 72).  With a cap 1000 rows of 32000 take 50 us: tanhf.
+// Bound by the HBM, and by the instructions of a logit (nine, one of them the exponential): 2048 rows of 128256 bf16 in 87 us (6.1 TB/s), 4001 of 32000
+// in 45 (5.7 TB/s; with 512 threads a CTA, which reach the ends of their rows together, half as long again).  With a cap 1000 rows of 32000 take 49 us: tanhf.
 constexpr int kLeanThreads = 256;
 constexpr int kLeanWarps = kLeanThreads / 32;
 template <typename L, bool CAP>
@@ -515,16 +518,12 @@ __global__ void __launch_bounds__(kLeanThreads, 6) token_logprobs_kernel(const _
     const float raw[1] = {One::load(row + single, true)};
     score_take<One, 1, false, CAP, false>(me, raw, single, 0, p.V, p.softcap);
   }
-  ScoreSums a = score_sums(me);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
+  const int target = tid == 0 ? score_target(p, t) : -1;      // (its loads are on their way while the sums are joined)
+  ScoreSums a = score_join(score_sums(me));
   if ((tid & 31) == 0) warps[tid >> 5] = a;
+  const float given = target >= 0 ? One::value(One::load(row + target, true)) : NAN;
   __syncthreads();
-  if (tid < 32) {
-    a = warps[tid & (kLeanWarps - 1)];
-#pragma unroll
-    for (int o = kLeanWarps / 2; o > 0; o >>= 1) score_merge(a, score_from_lane(a, o));
-  }
+  if (tid < 32) a = score_join(warps, kLeanWarps);
   if (parts > 1) {
     cluster_wait();
     if (tid == 0) {
@@ -534,11 +533,10 @@ __global__ void __launch_bounds__(kLeanThreads, 6) token_logprobs_kernel(const _
       cluster_store_f32(to + 8, 0, a.u);
     }
     cluster_sync();      // (the parts have arrived)
-    if (part != 0 || tid != 0) return;
-    a = ends[0];
-    for (int c = 1; c < parts; ++c) score_merge(a, ends[c]);
+    if (part != 0 || tid >= 32) return;
+    a = score_join(ends, parts);
   }
-  if (tid == 0) score_row<L, CAP>(p, t, row, a, logf(a.s));
+  if (tid == 0) score_row<CAP>(p, t, given, a, logf(a.s));
 }
 
 template <typename L>
