@@ -15,7 +15,7 @@
 //
 // Without alternatives a kernel of its own has more rows on an SM (below).  With them a CTA is through with its row by some 5 us of joining, listing
 // and ranking, beside one other CTA on its SM, and the pass itself is bound by its instructions, not by the HBM: 2048 rows of 128256 bf16 take 127 us
-// with 20 alternatives (4.1 TB/s; 117 with one), 4001 rows of 32000 104 us, 96 rows of 32000 fp32 8.3 us, one row of 32000 in four CTAs 6.3 us, most of
+// with 20 alternatives (4.1 TB/s; 117 with one), 4001 rows of 32000 104 us, 96 rows of 32000 fp32 8.3 us, one row of 32000 in eight CTAs 6.3 us, most of
 // it launch, cluster and joins.
 #include "common.cuh"
 
