@@ -130,6 +130,28 @@ def test_scores(T, V, dtype, cap):
         _check_scores(logits, targets, k, cap)
 
 
+@pytest.mark.parametrize("T", [100, 140, 200, 256, 300])      # (seven, six, four, three and two CTAs a row)
+def test_scores_of_long_rows_in_any_number_of_parts(T):
+    logits, targets = _logits(T, 120001, BF16, T)
+    _check_scores(logits, targets, 0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [1, 5, 8, 9, 15, 16, 17, 23, 4099])
+def test_scores_of_rows_at_every_place_of_a_load(dtype, V):
+    """Rows that start and end anywhere between two 16-byte boundaries; ties and masks in what lies in front of and behind the wide loads."""
+    whole, _ = _logits(12, V + 8, dtype, V)
+    for at in range(8):
+        x = whole[:, at:at + V].clone() if V == 1 else whole[:, at:at + V]
+        targets = torch.arange(12, device="cuda") % V
+        for k in {0, min(V, 3), min(V, 32)}:
+            _check_scores(x, targets, k)
+            _check_scores(torch.zeros_like(whole)[:, at:at + V], targets, k)
+            masked = torch.full_like(whole, -INF)[:, at:at + V]
+            masked[:, [0, -1]] = 1.0
+            _check_scores(masked, targets, k)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("wide", [1, 3, 64])
 def test_scores_of_rows_apart_and_off_their_alignment(dtype, wide):
