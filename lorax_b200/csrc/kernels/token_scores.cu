@@ -13,10 +13,10 @@
 // what is at or above the bound is listed, and the list is ranked by counting.  The order of (value, index) pairs is total, so the outcome
 // depends on no order of execution.
 //
-// Without alternatives a kernel of its own has more rows on an SM (below).  With them a CTA is through with its row by some 5 us of joining, listing
-// and ranking, beside one other CTA on its SM, and the pass itself is bound by its instructions, not by the HBM: 2048 rows of 128256 bf16 take 127 us
-// with 20 alternatives (4.1 TB/s; 117 with one), 4001 rows of 32000 104 us, 96 rows of 32000 fp32 8.3 us, one row of 32000 in eight CTAs 6.3 us, most of
-// it launch, cluster and joins.
+// Without alternatives a kernel of its own has more rows on an SM (below).  With them a CTA is through with its row by some 4 us of joining, listing
+// and ranking, beside one other CTA on its SM, and the pass itself is bound by its instructions (ten a logit), not by the HBM: 2048 rows of 128256 bf16
+// take 124 us with 20 alternatives (4.3 TB/s; 115 with one), 4001 rows of 32000 101 us, 48 rows of 128256 fp32 12.4 us, one row of 32000 in eight CTAs
+// 6.0 us, most of it launch, cluster and joins.
 #include <algorithm>
 
 #include "common.cuh"
@@ -318,11 +318,11 @@ struct ScoreShared {
 // comparisons where there are threads for it.
 LX_DEVICE void score_rank(const unsigned long long* list, int n, int k, unsigned long long* own) {
   if ((int)threadIdx.x < k && (int)threadIdx.x >= n) own[threadIdx.x] = 0;
-  int share = 32;
-  while (share > 1 && share * n > kScoreThreads) share >>= 1;
-  const int at = threadIdx.x & (share - 1), rounds = (n * share + kScoreThreads - 1) / kScoreThreads;
+  int shift = 5;
+  while (shift > 0 && n << shift > kScoreThreads) --shift;
+  const int share = 1 << shift, at = threadIdx.x & (share - 1), rounds = ((n << shift) + kScoreThreads - 1) / kScoreThreads;
   for (int r = 0; r < rounds; ++r) {
-    const int i = (threadIdx.x + r * kScoreThreads) / share;
+    const int i = (threadIdx.x + r * kScoreThreads) >> shift;
     const unsigned long long a = i < n ? list[i] : 0;
     int above = 0;
     for (int j = at; j < n; j += share) above += list[j] > a;
@@ -412,6 +412,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
       if (at < kScoreList) sh.list[at] = pair;
     }
   };
+  const float low = score_value((uint32_t)(bound >> 32));      // (no number where there is no bound: nothing is below it)
   auto collect = [&](int c, int it) {
     if (it == its) {
       const int one = row_part.single(c);
@@ -420,15 +421,17 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
     }
     const int from = row_part.body + (it * kScoreThreads + c) * kVec;
     if (from >= whole) return;
+    const typename Load::Raw raw = Load::load(row + from, true);
+    if (Load::value(Load::top(raw)) < low) return;
     float x[kVec];
-    Load::values(Load::load(row + from, true), x);
+    Load::values(raw, x);
 #pragma unroll
     for (int q = 0; q < kVec; ++q) push(x[q], from + q);
   };
-  for (int q = tid; q < ncand * (its + 1); q += kScoreThreads) {
-    const int c = q / (its + 1);
-    collect(sh.cand[c], q - c * (its + 1));
-  }
+  const int lanes = its > 1 ? min(32 - __clz(its - 1), 5) : 0;      // (a power of two of neighbours for a candidate)
+  for (int c = tid >> lanes; c < ncand; c += kScoreThreads >> lanes)
+    for (int it = tid & ((1 << lanes) - 1); it < its; it += 1 << lanes) collect(sh.cand[c], it);
+  if (tid < ncand) collect(sh.cand[tid], its);
   __syncthreads();
   if (sh.n <= kScoreList) {
     score_rank(sh.list, sh.n, k, sh.own);
@@ -485,8 +488,9 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
 }
 
 // ------------------------------------------------------------------------------------------------ without alternatives
-// Bound by the HBM, and by the instructions of a logit (nine, one of them the exponential): 2048 rows of 128256 bf16 in 87 us (6.1 TB/s), 4001 of 32000
-// in 45 (5.7 TB/s; with 512 threads a CTA, which reach the ends of their rows together, half as long again).  With a cap 1000 rows of 32000 take 49 us: tanhf.
+// Bound by the HBM, and by the instructions of a logit (six, one of them the exponential, whose unit is busy for three quarters of the time): 2048 rows of
+// 128256 bf16 in 87 us (6.1 TB/s), 4001 of 32000 in 45 (5.7 TB/s; with 512 threads a CTA, which reach the ends of their rows together, half as long
+// again).  With a cap 1000 rows of 32000 take 49 us: tanhf.
 constexpr int kLeanThreads = 256;
 constexpr int kLeanWarps = kLeanThreads / 32;
 template <typename L, bool CAP>
