@@ -182,6 +182,38 @@ def bench_moe(results, peaks):
         print(results[-1], flush=True)
 
 
+def bench_steps(results, peaks):
+    """Operators of short ragged steps: tables from lengths (bound by the call), an expert layer of few tokens (the reached experts' bytes), scores of tokens
+    (the logits' bytes)."""
+    def put(kernel, shape, ms, nbytes):
+        results.append({"kernel": kernel, "shape": shape, "ms": round(ms, 4), "gbs": round(nbytes / ms / 1e6, 1),
+                        "frac_of_measured_hbm": round(nbytes / ms / 1e6 / peaks["hbm_gbs"], 3)})
+        print(results[-1], flush=True)
+
+    for B, n, c, M in ((1, 137, 0, 65), (96, 4, 4000, 258), (512, 32, 2000, 128)):
+        p = min((c + n + 31) // 32, M)
+        seqs = torch.tensor([[n] * B, [c] * B, [0] * B, [p] * B], dtype=torch.int32, device="cuda")
+        pages = torch.arange(B * p, dtype=torch.int32, device="cuda")
+        tiles = ((64, B * ((n + 63) // 64)),)
+        ms = _time(lambda i: native.step_tables(seqs, pages, B * n, M, 32, tiles=tiles, lora_tiles=B * ((n + 31) // 32)), 1)
+        put("step_tables", f"B={B} n={n} blocks={M}", ms, 4 * (B * p + B * M + 3 * B * n))
+    for T, E, k, H, I in ((1, 8, 2, 4096, 14336), (16, 8, 2, 4096, 14336), (1, 64, 8, 2048, 1024), (16, 64, 8, 2048, 1024)):
+        sets = [((torch.randn(T, H, device="cuda")).to(torch.bfloat16), (torch.randn(E, H, device="cuda") * 0.3).to(torch.bfloat16),
+                 torch.randn(E, 2 * I, H, device="cuda", dtype=torch.bfloat16) / math.sqrt(H),
+                 torch.randn(E, H, I, device="cuda", dtype=torch.bfloat16) / math.sqrt(I)) for _ in range(1 if H > 2048 else 3)]
+        reached = sum(torch.topk(x.float() @ wr.float().t(), k, 1).indices.unique().numel() for x, wr, _, _ in sets) / len(sets)
+        ms = _time(lambda i: native.moe_few(*sets[i], k), len(sets))
+        native.workspace().check_status()
+        put("moe_few", f"T={T} E={E} top{k} H={H} I={I}", ms, reached * 6 * H * I)
+        del sets
+    for T, V, k in ((1, 32000, 5), (4001, 32000, 0), (2048, 128256, 0), (2048, 128256, 20)):
+        x = [torch.randn(T, V, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+        t = torch.zeros(T, dtype=torch.int32, device="cuda")
+        ms = _time(lambda i: native.token_scores(x[i], t, k=k), 2)
+        put("token_scores", f"T={T} V={V} k={k}", ms, 2 * T * V)
+        del x
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--json", default=None)
@@ -195,7 +227,7 @@ def main():
         pass
     results = []
     for name, fn in (("gemm", bench_gemm), ("lora", bench_lora), ("moe", bench_moe), ("attn_decode", bench_attn_decode), ("attn_prefill", bench_attn_prefill),
-                     ("small", bench_small)):
+                     ("small", bench_small), ("steps", bench_steps)):
         if a.only and a.only != name:
             continue
         fn(results, peaks)

@@ -153,6 +153,23 @@ def moe_case(T):
         native.moe_ffn(x, wr, w13, w2, k, 0, "silu")
 
 
+def few_case():
+    """One token through two of eight experts of 4096 x 14336 (0.7 GB of weights a call)."""
+    E, H, I = 8, 4096, 14336
+    std = lambda *s, a: torch.randn(*s, device="cuda", dtype=torch.bfloat16) * a
+    x, wr, w13, w2 = std(1, H, a=1.0), std(E, H, a=0.3), std(E, 2 * I, H, a=H ** -0.5), std(E, H, I, a=I ** -0.5)
+    for _ in range(3):
+        native.moe_few(x, wr, w13, w2, 2)
+
+
+def scores_case(k):
+    """2048 rows of 128256 logits (0.5 GB)."""
+    x = torch.randn(2048, 128256, device="cuda", dtype=torch.bfloat16)
+    t = torch.zeros(2048, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        native.token_scores(x, t, k=k)
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--case", required=True)
@@ -164,6 +181,7 @@ def main():
      "gemm_fp8_decode": lambda: gemm_fp8_case(64), "gemm_fp8_prefill": lambda: gemm_fp8_case(2048), "gemm_mid": lambda: gemm_case(256),
      "gemm_int4_decode": lambda: gemm_int4_case(8),
      "lora_shrink": lambda: lora_case("shrink"), "lora_expand": lambda: lora_case("expand"),
+     "moe_few": few_case, "token_logprobs": lambda: scores_case(0), "token_scores": lambda: scores_case(20),
      "moe_decode": lambda: moe_case(256), "moe_prefill": lambda: moe_case(2048)}[a.case]()
     torch.cuda.synchronize()
     native.workspace().check_status()
