@@ -357,13 +357,16 @@ def _each():
     l1, l2 = (_logits(3, 32000, BF16, s) for s in (1, 2))
     t1 = [ints([5, 70], [3, 0], [1, -1], [1, 3]).cuda(), ints(4, 5, 6, 7).cuda()]
     t2 = [ints([70, 5], [0, 90], [-1, 0], [3, 1]).cuda(), ints(9, 8, 7, 6).cuda()]
+    many = [_experts(3, 64, 8, 2048, 128, seed=s) for s in (3, 4)]      # (a router in a launch of its own)
     flat = lambda r: [x for f in r if f is not None for x in ([f] if isinstance(f, torch.Tensor) else [y for p in f for y in p])]
     return [(lambda *v: [native.moe_few(*v, 2)], list(a), list(b)),
             (lambda x, t: flat(native.token_scores(x, t, k=7)), list(l1), list(l2)),
-            (lambda s, p: flat(native.step_tables(s, p, 75, 4, 32, tiles=((64, 3),), lora_tiles=3)), t1, t2)]
+            (lambda s, p: flat(native.step_tables(s, p, 75, 4, 32, tiles=((64, 3),), lora_tiles=3)), t1, t2),
+            (lambda x, t: flat(native.token_scores(x, t)), list(l1), list(l2)),
+            (lambda *v: [native.moe_few(*v, 8)], list(many[0]), list(many[1]))]
 
 
-@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("which", [0, 1, 2, 3, 4])
 def test_captured_and_replayed(which):
     call, first, second = _each()[which]
     want1, want2 = ([x.clone() for x in call(*v)] for v in (first, second))
@@ -382,7 +385,7 @@ def test_captured_and_replayed(which):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
-@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("which", [0, 1, 2, 3, 4])
 def test_on_two_streams_at_once_and_again(which):
     call, first, second = _each()[which]
     want1, want2 = ([x.clone() for x in call(*v)] for v in (first, second))
