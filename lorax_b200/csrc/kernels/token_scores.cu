@@ -235,7 +235,9 @@ LX_DEVICE void score_take(ScoreThread& t, const typename Load::Raw (&raw)[R], in
   if (top > t.m) {
     const float shift = score_far(top) ? 0.f : -kLog2e * top;
     if (t.m != -INFINITY) {
-      const float d = fmaxf(score_far(top) || score_far(t.m) ? (t.m - top) * kLog2e : shift - t.shift, kScoreFloor), f = exp2_fast(d);
+      const float by = score_far(top) ? (score_far(t.m) ? (t.m - top) * kLog2e : -fmaf(kLog2e, top, t.shift))
+                                      : (score_far(t.m) ? fmaf(kLog2e, t.m, shift) : shift - t.shift);
+      const float d = fmaxf(by, kScoreFloor), f = exp2_fast(d);
       const uint64_t d2 = pack_f32x2(d, d), f2 = pack_f32x2(f, f);
       t.u = mul_f32x2(fma_f32x2(d2, t.s, t.u), f2);
       t.s = mul_f32x2(t.s, f2);

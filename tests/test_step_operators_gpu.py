@@ -210,6 +210,15 @@ def test_scores_of_logits_far_from_zero(dtype, by):
             _check_scores(x, targets, k)
 
 
+@pytest.mark.parametrize("around", [-2048.0, 2048.0])
+@pytest.mark.parametrize("T", [1, 900])
+def test_scores_of_maxima_that_grow_past_the_end_of_a_range(around, T):
+    """Half of a row's weight on either side of where the form of the exponents changes, in the order of the row."""
+    x = torch.linspace(around - 0.5, around + 0.5, 70001, device="cuda").expand(T, -1).contiguous()
+    for k in (0, 2):
+        _check_scores(x, torch.arange(T, device="cuda") * 77, k)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_scores_when_more_candidates_than_the_list_holds(dtype):
     """Thirty-one threads whose strided elements are all above the bound that the thirty-second one sets."""
