@@ -484,3 +484,40 @@ def test_scores_of_prompts_by_the_runner_with_experts():
             _close(outs[0].entropy, ent, off * (2 + 2 * math.log(513)))
     a, b = outs[0].logprobs.cpu().double(), outs[1].logprobs.double()
     assert torch.equal(a.isnan(), b.isnan()) and ((a - b)[~a.isnan()].norm() / b[~b.isnan()].norm()).item() < 4e-2      # (the bound of the model's logits in bf16)
+
+
+def test_decoding_with_experts_in_graphs_and_without():
+    """Six rows through `moe_few`: a captured step and an eager one run the same kernels on the same data."""
+    from lorax_b200.runtime.engine import Engine, EngineConfig
+    from tests.test_step_operators import _tiny
+    m, _ = _tiny("cuda", BF16)
+    g = torch.Generator().manual_seed(8)
+    prompts = [torch.randint(0, 512, (3 + i,), generator=g).tolist() for i in range(6)]
+    outs = [Engine(m, EngineConfig(max_total_tokens=128, max_batch_prefill_tokens=256), num_blocks=64, max_batch=8, use_graphs=graphs).generate(prompts, max_new_tokens=12)
+            for graphs in (True, False)]
+    assert outs[0] == outs[1] and all(len(o) == 12 for o in outs[0])
+    native.workspace().check_status()
+
+
+@pytest.mark.parametrize("k", [0, 5, 32, 40])      # (40: more than the kernel returns)
+def test_scores_of_the_chooser(k):
+    """Log-probabilities and alternatives of filtered, cooled and penalised rows against log_softmax of the same scores."""
+    from lorax_b200.sampling.chooser import HeterogeneousNextTokenChooser, NextTokenParams
+    V = 3001
+    params = [NextTokenParams(return_k_alternatives=k), NextTokenParams(temperature=1e-4, do_sample=True, seed=1), NextTokenParams(top_k=3, do_sample=True, seed=2),
+              NextTokenParams(repetition_penalty=1.3, top_p=0.4, do_sample=True, seed=3)]
+    c = HeterogeneousNextTokenChooser(params, "cuda", V)
+    logits, _ = _logits(4, V, BF16, 17)
+    history = torch.randint(0, V, (4, 9), device="cuda")
+    mask = torch.ones(4, 9, dtype=torch.bool, device="cuda")
+    scores = c.warp(history, mask, logits.float(), history[:, -1])
+    ids, lp, alts = HeterogeneousNextTokenChooser(params, "cuda", V)(history, mask, logits, history[:, -1])
+    want, _, best, best_lp = _scores_oracle(scores, ids, max(k, 1), 0.0)
+    # (a thread adds V / 256 terms at most; the form of log_softmax for more than 32 alternatives is PyTorch's own in fp32: as long a sum, in another order)
+    off = (V / 256 + 80) * 2.0 ** -24
+    _close(lp, want, off)
+    assert (alts is None) == (k == 0)
+    if k:
+        _close(alts[1], best_lp, off)
+        if k <= 32:
+            assert torch.equal(alts[0].long(), best)
