@@ -31,7 +31,8 @@ constexpr int kFewTokens = 16;
 constexpr int kFewExperts = 256;
 constexpr int kFewTop = 32;
 constexpr int kFewMath = 8;                // warps that multiply; one more fills the ring
-constexpr int kFewWarps = kFewMath + 1;
+constexpr int kFewSumWarps = 2;            // and two sum up the others' parts of a tile (up; by the math warps in turn, nine experts of 512 x 10752 took 145 us, now 111)
+constexpr int kFewWarps = kFewMath + 1 + kFewSumWarps;
 constexpr int kFewThreads = 32 * kFewWarps;
 constexpr int kFewRowTiles = 4;            // tiles of 16 rows of a CTA (down)
 constexpr int kFewUpSteps = 8;             // steps of 32 of K of a stage and a math warp, at most (up): stages of 64 KB (of 32 KB: 110 -> 114 us for one token)
@@ -428,6 +429,48 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
     return;
   }
   float4* red = reinterpret_cast<float4*>(smem + stages * stage_bytes);      // [kSums][math warps][NT][32 lanes]
+  if (warp > kFewMath) {
+    bool ok = true;
+    int d = u0 / units, c = (u0 - d * units) * 8 - 8, e = 0, served = 0, row = 0;
+    uint32_t mask = 0;
+    for (int u = u0; u < u1; ++u) {
+      if ((c += 8) == p.I) { c = 0; ++d; }
+      if (u == u0 || c == 0) {
+        e = plan.list[d];
+        mask = plan.mask[e];
+        served = __popc(mask);
+        row = plan.base[d];
+      }
+      const int turn = u - u0, buf = turn % kSums, n = NT == 1 || served <= 8 ? 1 : NT;
+      if (turn % kFewSumWarps != warp - kFewMath - 1) continue;
+      const int col = c + few_lane_row(g);
+      const float4* part = red + buf * kFewMath * NT * 32;
+      few_await(ring, &ring.sums[buf], (turn / kSums) & 1, ok, p.status);
+      for (int m = 0; m < n; ++m) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kFewMath; ++w) {
+          const float4 a = part[(w * n + m) * 32 + lane];
+          v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+        }
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {          // (gate and up of the lane's column, tokens 2 (lane % 4) and the next)
+          const int i = m * 8 + (lane & 3) * 2 + o;
+          if (i >= served) continue;
+          const int t = few_token(mask, i);
+          const float h = few_act(o ? v.y : v.x, p.act) * (o ? v.w : v.z) * plan.w[t * p.k + plan.place[t][e]];
+          const __nv_bfloat16 hi = __float2bfloat16(h);
+          const float back = __bfloat162float(hi);
+          const long long at = (long long)(row + i) * p.I + col;
+          p.h[at] = hi;
+          p.h[at + (long long)p.T * p.k * p.I] = __float2bfloat16(fabsf(back) < INFINITY ? h - back : 0.f);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring.read[buf]);
+    }
+    return;
+  }
   const int steps = 2 * blocks, per = 2 * wide, place = few_place(8, few_lane_row(g), warp, c8), column = (warp * 32 + c8) * 2;
   bool ok = true;
   uint32_t sums_phase = 0;
@@ -436,7 +479,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
   uint32_t mask = 0;
   auto tile = [&](auto n, int u) {
     constexpr int N = decltype(n)::value;
-    const int col = c + few_lane_row(g), buf = (u - u0) % kSums;
+    const int buf = (u - u0) % kSums;
     float acc[2][N][4];                        // (two chains of MMAs)
 #pragma unroll
     for (int o = 0; o < 2; ++o)
@@ -475,32 +518,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
       part[(warp * N + m) * 32 + lane] = make_float4(acc[0][m][0] + acc[1][m][0], acc[0][m][1] + acc[1][m][1], acc[0][m][2] + acc[1][m][2], acc[0][m][3] + acc[1][m][3]);
     __syncwarp();
     if (lane == 0) mbar_arrive(&ring.sums[buf]);
-    if ((u - u0) % kFewMath == warp) {         // one warp a tile, in turn, sums up the warps' parts
-      few_await(ring, &ring.sums[buf], sums_phase, ok, p.status);
-#pragma unroll
-      for (int m = 0; m < N; ++m) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kFewMath; ++w) {
-          const float4 a = part[(w * N + m) * 32 + lane];
-          v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-        }
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {          // (gate and up of the lane's column, tokens 2 (lane % 4) and the next)
-          const int i = m * 8 + (lane & 3) * 2 + o;
-          if (i >= served) continue;
-          const int t = few_token(mask, i);
-          const float h = few_act(o ? v.y : v.x, p.act) * (o ? v.w : v.z) * plan.w[t * p.k + plan.place[t][e]];
-          const __nv_bfloat16 hi = __float2bfloat16(h);
-          const float back = __bfloat162float(hi);
-          const long long row = plan.base[d] + i;
-          p.h[row * p.I + col] = hi;
-          p.h[(row + p.T * p.k) * p.I + col] = __float2bfloat16(fabsf(back) < INFINITY ? h - back : 0.f);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ring.read[buf]);
-    }
     if (buf == kSums - 1) sums_phase ^= 1;
   };
   for (int u = u0; u < u1; ++u) {
@@ -584,6 +601,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
     }
     return;
   }
+  if (warp > kFewMath) return;
   pdl_wait();
   pdl_trigger();
   float4* red = reinterpret_cast<float4*>(smem + stages * stage_bytes);      // [math warps][MT][NT][32 lanes]
