@@ -430,6 +430,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
   }
   float4* red = reinterpret_cast<float4*>(smem + stages * stage_bytes);      // [kSums][math warps][NT][32 lanes]
   if (warp > kFewMath) {
+    // (a buffer is always the same warp's: one that waited for another's phase could take the last but one of the same parity for it)
+    static_assert(kSums % kFewSumWarps == 0, "whole turns");
     bool ok = true;
     int d = u0 / units, c = (u0 - d * units) * 8 - 8, e = 0, served = 0, row = 0;
     uint32_t mask = 0;
