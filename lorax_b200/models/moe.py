@@ -28,11 +28,13 @@ from ..ops.reference import MOE_FEW_TOKENS
 DENSE_MAX_TOKENS = 256
 
 
-def few_tokens(T: int, k: int, hidden: int, inter: int) -> bool:
-    """Whether a layer takes `moe_few` instead of `moe_ffn`: up to its 16 tokens, unless they reach many small experts, whose turns then cost more than
-    their bytes.  Measured (us, `moe_ffn` / `moe_few`): 8 experts of 4096 x 14336, two a token: 181 / 108 for one token, 469 / 406 for 16; 64 of 2048 x 1024,
-    eight a token: 55 / 28 and 149 / 134; 128 of 1024 x 512, eight a token: 41 / 21 for one, 58 / 54 for six, 60 / 66 for eight, 77 / 110 for 16."""
-    return T <= MOE_FEW_TOKENS and (T * k <= 48 or hidden * inter >= 1 << 20)
+def few_tokens(T: int, k: int, experts: int, hidden: int) -> bool:
+    """Whether a layer takes `moe_few` instead of `moe_ffn`: up to its 16 tokens on wide layers; up to eight on narrower ones, and on narrow ones if they
+    reach few experts, since turns of short rows then cost more than their bytes.  Measured (us, `moe_ffn` / `moe_few`): 8 experts of 4096 x 14336,
+    two a token: 179 / 107 for one token, 463 / 399 for 16; 64 of 2048 x 1024, eight a token: 54 / 28 and 155 / 128; 128 of 2048 x 192: 46 / 19 and 78 / 76;
+    64 of 1024 x 1408, six a token: 39 / 24 for one, 75 / 74 for eight, 94 / 115 for 16; 32 of 512 x 2048, four a token: 32 / 22 for one, 37 / 34 for
+    three, 43 / 53 for six; 8 of 512 x 8192, two a token: 61 / 29 for one, 75 / 75 for eight, 76 / 94 for 16."""
+    return T <= MOE_FEW_TOKENS and (hidden >= 2048 or (T <= 8 and (hidden >= 1024 or min(experts, T * k) <= 12)))
 
 
 def route(router_logits: torch.Tensor, k: int):
@@ -55,7 +57,7 @@ def moe_forward(model, x: torch.Tensor, lw, li: int, inp) -> torch.Tensor:
     if (x.is_cuda and x.dtype == torch.bfloat16 and isinstance(lw.experts_w13, torch.Tensor) and isinstance(lw.experts_w2, torch.Tensor)
             and lw.experts_w13.dtype == torch.bfloat16 and lw.experts_w13.shape[1] % 128 == 0 and lw.experts_w2.shape[1] % 128 == 0
             and model.hidden % 8 == 0 and c.intermediate_size % 8 == 0 and E <= 256 and c.num_experts_per_tok <= 32 and hasattr(ops, "moe_ffn")):
-        ffn = ops.moe_few if few_tokens(T, c.num_experts_per_tok, model.hidden, c.intermediate_size) else ops.moe_ffn
+        ffn = ops.moe_few if few_tokens(T, c.num_experts_per_tok, E, model.hidden) else ops.moe_ffn
         out = ffn(x, lw.router_w.to(torch.bfloat16) if lw.router_w.dtype != torch.bfloat16 else lw.router_w, lw.experts_w13,
                   lw.experts_w2, c.num_experts_per_tok, e0, c.hidden_act)
         if ws > 1 and e_local < E:

@@ -166,8 +166,9 @@ def test_scores_of_rows_with_masks():
 # ------------------------------------------------------------------------------------------------ where they are called
 def test_which_layers_take_the_operator_for_a_few_tokens():
     from lorax_b200.models.moe import few_tokens
-    assert few_tokens(1, 2, 4096, 14336) and few_tokens(16, 2, 4096, 14336) and not few_tokens(17, 2, 4096, 14336)
-    assert few_tokens(16, 8, 2048, 1024) and few_tokens(6, 8, 1024, 512) and not few_tokens(7, 8, 1024, 512) and few_tokens(16, 3, 128, 64)
+    assert few_tokens(1, 2, 8, 4096) and few_tokens(16, 2, 8, 4096) and not few_tokens(17, 2, 8, 4096) and few_tokens(16, 8, 128, 2048)
+    assert few_tokens(8, 8, 128, 1024) and not few_tokens(9, 8, 128, 1024)
+    assert few_tokens(3, 4, 32, 512) and not few_tokens(4, 4, 32, 512) and few_tokens(8, 2, 8, 512) and not few_tokens(9, 2, 8, 512)
 
 
 def _tiny(device, dtype, **over):

@@ -465,11 +465,11 @@ def test_a_short_ragged_step():
 
 
 def test_scores_of_prompts_by_the_runner_with_experts():
-    """`ModelRunner.score` on the kernels (a step of ten tokens: `moe_few`) against the fp32 CPU path of the same weights, and against its own logits."""
+    """`ModelRunner.score` on the kernels (a step of eight tokens: `moe_few`) against the fp32 CPU path of the same weights, and against its own logits."""
     from lorax_b200.runtime.runner import PrefillItem
     from tests.test_step_operators import _tiny
     g = torch.Generator().manual_seed(3)
-    prompts = [torch.randint(0, 512, (n,), generator=g).tolist() for n in (6, 1, 3)]
+    prompts = [torch.randint(0, 512, (n,), generator=g).tolist() for n in (4, 1, 3)]
     outs = []
     for device, dtype in (("cuda", BF16), ("cpu", F32)):
         _, r = _tiny(device, dtype)
