@@ -14,8 +14,8 @@
 // Eight warps multiply what has arrived by mma.sync: the weights are the A operand (16 rows x 16 of K), read 16 bytes a lane in the order of
 // K in which they lie (the other operand is read in the same order, so the sum is the same); tokens stand in the columns, those that an expert
 // does not serve as zeros.
-//   up:   the rows of all reached experts, eight features of gate and up to a tile, are dealt evenly to the CTAs; the warps split K and sum
-//         their parts through shared memory
+//   up:   the rows of all reached experts, eight features of gate and up to a tile, are dealt evenly to the CTAs; the warps split K and
+//         leave their parts in shared memory, where two warps of their own sum them up, so that nobody waits for activations and stores
 //   down: the rows of the output are dealt to the CTAs; K runs over the reached experts' features one expert behind the other, so the sum
 //         over a token's experts forms in the accumulators (their weights are in h), in the order of the experts' numbers
 // h is held as two bf16 terms, value and remainder, which take two MMAs: it is as exact as the fp32 sums, and the tensor cores have room.  Its
