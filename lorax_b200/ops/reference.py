@@ -1072,6 +1072,22 @@ def step_tables_of_many(seqs, pages, tokens: int, max_blocks: int, page: int, wi
 MOE_FEW_ACTS = ("silu", "swish", "gelu", "gelu_new", "gelu_pytorch_tanh", "gelu_fast", "gelu_tanh", "relu", "relu2")
 
 
+def _share_memory(a, b) -> bool:
+    """Whether any row of one tensor (rows along the last dimension, without gaps in it) lies on a row of the other.  Rows that take turns do not."""
+    def rows(t):
+        t = t.detach()
+        if t.is_contiguous():
+            return [(t.data_ptr(), t.numel() * t.element_size())]
+        t = t.reshape(1, -1) if t.dim() < 2 else t
+        return [(t[i].data_ptr(), t.shape[1] * t.element_size()) for i in range(t.shape[0])]
+    if not a.numel() or not b.numel():
+        return False
+    ra, rb = rows(a), rows(b)
+    if max(p + n for p, n in ra) <= min(p for p, _ in rb) or max(p + n for p, n in rb) <= min(p for p, _ in ra):
+        return False
+    return any(p < q + m and q < p + n for p, n in ra for q, m in rb)
+
+
 def check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out):
     """-> (tokens, experts, width, features)."""
     if not (x.dim() == 2 and router_w.dim() == 2 and w13.dim() == 3 and w2.dim() == 3):
@@ -1098,13 +1114,15 @@ def check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out):
     if not (out is None or (out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and out.stride(1) == 1
                            and (T <= 1 or out.stride(0) >= H))):
         raise ValueError("moe_few: out is like x")
+    if out is not None and any(_share_memory(out, t) for t in (x, router_w, w13, w2)):
+        raise ValueError("moe_few: out lies apart from the inputs (rows are still routed when others are written)")
     return T, E, H, inter
 
 
 def moe_few(x, router_w, w13, w2, k: int, e0: int = 0, act: str = "silu", renorm: bool = True, scale: float = 1.0, out=None):
     """Mixture-of-experts feed-forward of a few tokens: x [T, H], router_w [E, H], w13 [e_local, 2 I, H] (gate rows, then up rows), w2 [e_local, H, I];
     this rank owns the experts [e0, e0 + e_local), and the others' share is left out.  A token goes to the `k` experts with the largest logits (the
-    lower number on ties), with softmax weights over those (`renorm`) or over all, times `scale`."""
+    lower number on ties), with softmax weights over those (`renorm`) or over all, times `scale`.  `out` shares no memory with the inputs."""
     T, E, H, inter = check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out)
     z = x.float() @ router_w.float().t()
     ids = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :k]
