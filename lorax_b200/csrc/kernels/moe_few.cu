@@ -152,7 +152,7 @@ LX_DEVICE void few_route(float* z, float4* red, const MoeFewParams& p) {
 }
 
 // One warp per token, PER experts a lane: its experts, their weights, and its mark with those that this rank owns (plan.mask is zero).  A NaN
-// orders as -inf (its weight is NaN all the same); no expert is chosen twice.
+// orders as -inf, and a token with one among its logits has weights that are NaN, whichever experts it goes to; no expert is chosen twice.
 template <int PER>
 LX_DEVICE void few_select(FewPlan& plan, const float* logits, const MoeFewParams& p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -163,8 +163,10 @@ LX_DEVICE void few_select(FewPlan& plan, const float* logits, const MoeFewParams
     for (int i = 0; i < PER; ++i) z[i] = lane + 32 * i < p.E ? row[lane + 32 * i] : 0.f;
     // logits as numbers whose order is theirs; 0: taken, or no expert
     uint32_t key[PER];
+    bool odd = false;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
+      odd |= z[i] != z[i];
       const float v = z[i] == z[i] ? z[i] + 0.f : -INFINITY;
       const uint32_t b = __float_as_uint(v);
       key[i] = lane + 32 * i < p.E ? ((b >> 31) ? ~b : b | 0x80000000u) : 0;
@@ -197,7 +199,7 @@ LX_DEVICE void few_select(FewPlan& plan, const float* logits, const MoeFewParams
       for (int i = 0; i < PER; ++i)
         if (lane + 32 * i < p.E) all += expf(z[i] - top);
     }
-    all = warp_sum(all);
+    all = __any_sync(0xffffffffu, odd) ? NAN : warp_sum(all);
     const int e = id - p.e0;
     if (lane < p.k && e >= 0 && e < p.e_local) {
       plan.w[t * p.k + lane] = own / all * p.scale;
@@ -268,6 +270,36 @@ LX_DEVICE int few_copies(int n, int shift) { return (n + (1 << shift) - 1) >> sh
 LX_DEVICE int few_token(uint32_t mask, int i) {
   for (; i > 0; --i) mask &= mask - 1;
   return __ffs(mask) - 1;
+}
+
+// Feature `row` of token t from the experts that serve it alone, by one warp.  A column of the down product has zeros where an expert does not serve its token, and
+// an h that one bf16 term holds has a remainder of zero: times a weight that is infinite or no number, both are NaN.  Sums that are not finite are formed again here,
+// unless the token's own weights are NaN.  (Not inlined: no call of finite numbers comes by.)
+__device__ __noinline__ float few_alone(const FewPlan& plan, const MoeFewParams& p, int t, int row) {
+  const int lane = threadIdx.x & 31;
+  float sum = 0.f;
+  for (int d = 0; d < plan.reached; ++d) {
+    const int e = plan.list[d];
+    const uint32_t mask = plan.mask[e];
+    if (((mask >> t) & 1) == 0) continue;
+    const float w = plan.w[t * p.k + plan.place[t][e]];
+    if (w != w) return NAN;
+    const __nv_bfloat16* weights = p.w2 + ((long long)e * p.H + row) * p.I;
+    const __nv_bfloat16* value = p.h + (long long)(plan.base[d] + few_slot(mask, t)) * p.I;
+    const __nv_bfloat16* remainder = value + (long long)p.T * p.k * p.I;
+    for (int i = lane * 8; i < p.I; i += 256) {
+      const uint4 a = few_load(weights + i, true), b = few_load(value + i, true), c = few_load(remainder + i, true);
+      const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
+      float part = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        part += __uint_as_float(av[q] << 16) * (__uint_as_float(bv[q] << 16) + __uint_as_float(cv[q] << 16));
+        part += __uint_as_float(av[q] & 0xffff0000u) * (__uint_as_float(bv[q] & 0xffff0000u) + __uint_as_float(cv[q] & 0xffff0000u));
+      }
+      sum += part;
+    }
+  }
+  return warp_sum(sum);
 }
 
 // ------------------------------------------------------------------------------------------------ the ring
@@ -701,7 +733,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
 #pragma unroll
       for (int o = 0; o < 4; ++o) {              // (the row of lane group l / 4 and 8 behind it, tokens 2 (l % 4) and the next)
         const int t = n * 8 + (l & 3) * 2 + (o & 1), r = m * 16 + (o >> 1) * 8 + few_lane_row(l >> 2);
-        if (t < p.T && r < rows && r0 + r < last) p.out[(long long)t * p.ldo + r0 + r] = __float2bfloat16(o == 0 ? v.x : o == 1 ? v.y : o == 2 ? v.z : v.w);
+        const bool live = t < p.T && r < rows && r0 + r < last;
+        float y = o == 0 ? v.x : o == 1 ? v.y : o == 2 ? v.z : v.w;
+        for (uint32_t odd = __ballot_sync(0xffffffffu, live && !(fabsf(y) < INFINITY)); odd != 0; odd &= odd - 1) {
+          const int from = __ffs(odd) - 1;
+          const float again = few_alone(plan, p, __shfl_sync(0xffffffffu, t, from), r0 + __shfl_sync(0xffffffffu, r, from));
+          if (lane == from) y = again;
+        }
+        if (live) p.out[(long long)t * p.ldo + r0 + r] = __float2bfloat16(y);
       }
     }
     few_math_sync();

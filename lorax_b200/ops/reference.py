@@ -1122,11 +1122,13 @@ def check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out):
 def moe_few(x, router_w, w13, w2, k: int, e0: int = 0, act: str = "silu", renorm: bool = True, scale: float = 1.0, out=None):
     """Mixture-of-experts feed-forward of a few tokens: x [T, H], router_w [E, H], w13 [e_local, 2 I, H] (gate rows, then up rows), w2 [e_local, H, I];
     this rank owns the experts [e0, e0 + e_local), and the others' share is left out.  A token goes to the `k` experts with the largest logits (the
-    lower number on ties), with softmax weights over those (`renorm`) or over all, times `scale`.  `out` shares no memory with the inputs."""
+    lower number on ties), with softmax weights over those (`renorm`) or over all, times `scale`.  A NaN among its logits orders as -inf, and a token that
+    has one has no weights: its result is NaN.  Other numbers that are not finite stay with the tokens of the expert that they come from.  `out` shares no memory with the inputs."""
     T, E, H, inter = check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out)
     z = x.float() @ router_w.float().t()
-    ids = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :k]
+    ids = torch.sort(torch.where(z.isnan(), torch.full_like(z, float("-inf")), z), dim=1, descending=True, stable=True).indices[:, :k]
     w = torch.softmax(z.gather(1, ids), 1) if renorm else torch.softmax(z, 1).gather(1, ids)
+    w = torch.where(z.isnan().any(1, keepdim=True), torch.full_like(w, float("nan")), w)
     w = torch.zeros_like(z).scatter_(1, ids, w * scale)
     chosen = torch.zeros_like(z, dtype=torch.bool).scatter_(1, ids, True)
     y = torch.zeros(T, H, dtype=torch.float32, device=x.device)

@@ -34,3 +34,23 @@ def test_experts_into_a_result_between_the_rows_of_their_inputs():
     lines = torch.zeros(8, 64)
     lines[::2] = buf[:, :64]
     assert torch.equal(reference.moe_few(lines[::2], wr, w13, w2, 2, out=lines[1::2]), want)
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+def test_a_token_with_a_logit_that_is_no_number_has_no_weights(renorm):
+    """Whether or not the expert whose logit it is would be chosen, on the rank that has it and on the others."""
+    g = torch.Generator().manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g)
+    x, wr, w13, w2 = r(3, 32), r(6, 32), r(6, 48, 32), r(6, 32, 24)
+    bad = wr.clone()
+    bad[4, 0] = float("nan")
+    assert reference.moe_few(x, bad, w13, w2, 2, renorm=renorm).isnan().all()
+    ids = torch.sort(torch.where(torch.arange(6) == 4, float("-inf"), x @ wr.t()), dim=1, descending=True, stable=True).indices[:, :2]
+    for e in range(6):
+        part = reference.moe_few(x, bad, w13[e:e + 1], w2[e:e + 1], 2, e, renorm=renorm)
+        for t in range(3):
+            assert part[t].isnan().all() if e in ids[t] else (part[t] == 0).all()
+    x[1, 3] = float("nan")                                   # one token's numbers are its own
+    clean = reference.moe_few(x[[0, 2]], wr, w13, w2, 2, renorm=renorm)
+    got = reference.moe_few(x, wr, w13, w2, 2, renorm=renorm)
+    assert got[1].isnan().all() and torch.allclose(got[[0, 2]], clean)
