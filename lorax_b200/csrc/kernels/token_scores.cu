@@ -31,6 +31,19 @@ constexpr int kScoreGroups = 64;          // of threads whose best elements set 
 constexpr int kScoreList = 2048;          // candidates that are ranked at once
 constexpr int kScoreUnroll = 4;           // 16-byte loads of a thread in flight
 
+// What the kernel with alternatives takes for granted of these numbers.  A row's single logits are read by the first threads of two warps, up to seven each
+// (ScorePart::single); the warps' sums, and the parts', are joined by one warp.
+static_assert(kScoreThreads % 32 == 0 && kScoreThreads >= 64 && kScoreWarps <= 32 && kScoreMaxParts <= 32, "whole warps, two of them, and no more sums than lanes");
+// The threads of a group are neighbours within a warp, and so many threads share the comparisons of its best element, each with as many others.
+constexpr int kScoreShare = kScoreThreads / kScoreGroups;
+static_assert(kScoreShare * kScoreGroups == kScoreThreads && (kScoreShare & (kScoreShare - 1)) == 0 && kScoreShare <= 32 && kScoreGroups % kScoreShare == 0,
+              "groups are a power of two of lanes");
+// A bound exists only with as many groups as alternatives, an alternative has a thread of its own to write its place, and the list takes the best so far beside a
+// portion of at least one wide load (eight elements).
+static_assert(kScoreMaxTop <= kScoreGroups && kScoreMaxTop <= kScoreThreads && kScoreMaxTop + 8 <= kScoreList, "places for the alternatives");
+// A pair's comparisons are shared by up to 32 neighbouring lanes of the same warp in rounds of all threads (score_rank).
+static_assert(kScoreMaxParts * kScoreMaxTop <= kScoreList, "the parts' best are ranked like a list");
+
 struct TokenScoresParams {
   const void* logits;
   long long ld;            // elements
@@ -377,11 +390,11 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   const unsigned long long mine = live ? score_pair(score_key(me.best), me.place) : 0;
   unsigned long long g = live ? score_pair(score_key(me.best), me.place + (me.place == single ? 0 : kVec - 1)) : 0;
 #pragma unroll
-  for (int o = 1; o < kScoreThreads / kScoreGroups; o <<= 1) {
+  for (int o = 1; o < kScoreShare; o <<= 1) {
     const unsigned long long other = __shfl_xor_sync(0xffffffffu, g, o);
     g = other > g ? other : g;
   }
-  if ((tid & (kScoreThreads / kScoreGroups - 1)) == 0) sh.group[tid / (kScoreThreads / kScoreGroups)] = g;
+  if ((tid & (kScoreShare - 1)) == 0) sh.group[tid / kScoreShare] = g;
   if (tid == 0) {
     sh.ncand = sh.n = 0;
     sh.bound = 0;
@@ -392,14 +405,13 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   // the bound: the k-th best of the groups' best, or none where there are fewer
   const int k = p.k;
   {
-    constexpr int kShare = kScoreThreads / kScoreGroups;
-    const unsigned long long g = sh.group[tid / kShare];
+    const unsigned long long g = sh.group[tid / kScoreShare];
     int above = 0;
 #pragma unroll
-    for (int j = 0; j < kScoreGroups / kShare; ++j) above += sh.group[(tid & (kShare - 1)) + j * kShare] > g;
+    for (int j = 0; j < kScoreGroups / kScoreShare; ++j) above += sh.group[(tid & (kScoreShare - 1)) + j * kScoreShare] > g;
 #pragma unroll
-    for (int o = kShare / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-    if (g != 0 && above == k - 1 && (tid & (kShare - 1)) == 0) sh.bound = g;
+    for (int o = kScoreShare / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (g != 0 && above == k - 1 && (tid & (kScoreShare - 1)) == 0) sh.bound = g;
   }
   __syncthreads();
   const unsigned long long bound = sh.bound;
@@ -440,6 +452,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const __
   } else {
     // more than the list holds (large logits side by side in the threads' strides): portions that fit, with the best so far among them
     constexpr int kPortion = (kScoreList - kScoreMaxTop) / kVec;
+    static_assert(kPortion >= 1 && kPortion * kVec + kScoreMaxTop <= kScoreList, "a portion and the best so far fit the list");
     int have = 0;
     for (int c = 0; c < ncand; ++c) {
       for (int it = 0; it <= its; it += kPortion) {
