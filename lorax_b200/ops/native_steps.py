@@ -82,9 +82,10 @@ def moe_few(x: torch.Tensor, router_w: torch.Tensor, w13: torch.Tensor, w2: torc
     return out
 
 
-def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, k: int = 0, softcap: float = 0.0) -> TokenScores:
+def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, k: int = 0, softcap: float = 0.0,
+                 entropy: bool = True) -> TokenScores:
     """Log-probability of a given token of every row, entropy of the row, and its `k` best tokens with their log-probabilities
-    (`reference.token_scores` states them): one pass over the logits, one launch."""
+    (`reference.token_scores` states them): one pass over the logits, one launch.  (`entropy` saves the kernel nothing.)"""
     T, V = check_token_scores(logits, targets, k, softcap)
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"token_scores: the kernels take bf16 and fp32 logits; got {logits.dtype}")
@@ -98,4 +99,4 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, k
     rc = nv.load().lx_token_scores(logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), T, V, t_ptr, wide, k, softcap,
                                    lp.data_ptr() if t_ptr else 0, ent.data_ptr(), ids.data_ptr(), best.data_ptr(), stream)
     nv._check(rc, "lx_token_scores")
-    return TokenScores(lp if targets is not None else None, ent, ids, best.view(T, k))
+    return TokenScores(lp if targets is not None else None, ent if entropy else None, ids, best.view(T, k))

@@ -1146,7 +1146,7 @@ def moe_few(x, router_w, w13, w2, k: int, e0: int = 0, act: str = "silu", renorm
 
 class TokenScores(NamedTuple):
     logprobs: Optional[torch.Tensor]      # [T] of the given tokens (None without)
-    entropy: torch.Tensor                 # [T]
+    entropy: Optional[torch.Tensor]       # [T] (None without)
     top_ids: torch.Tensor                 # [T, k] int32
     top_logprobs: torch.Tensor            # [T, k]
 
@@ -1167,23 +1167,37 @@ def check_token_scores(logits, targets, k, softcap):
     return T, V
 
 
-def token_scores(logits, targets=None, k: int = 0, softcap: float = 0.0) -> TokenScores:
+def _best(raw, k: int):
+    """-> ids [T, k] of the largest values of every row, the lower id on ties; a NaN orders as -inf.  No sort of whole rows: the `k` largest, put in order, and the
+    first of those that are equal to the last where there are more of them."""
+    raw = torch.where(raw.isnan(), torch.full_like(raw, float("-inf")), raw) if bool(raw.isnan().any()) else raw
+    ids = torch.sort(raw.topk(k, 1).indices, dim=1).values
+    values = raw.gather(1, ids)
+    order = torch.sort(values, dim=1, descending=True, stable=True)
+    values, ids = order.values, ids.gather(1, order.indices)
+    last = values[:, -1:]
+    held, all_ = (values == last).sum(1), (raw == last).sum(1)
+    for t in (all_ > held).nonzero()[:, 0].tolist():
+        n = int(held[t])
+        ids[t, k - n:] = (raw[t] == last[t]).nonzero()[:n, 0]
+    return ids
+
+
+def token_scores(logits, targets=None, k: int = 0, softcap: float = 0.0, entropy: bool = True) -> TokenScores:
     """Scores of tokens under softmax(logits), or softmax(softcap * tanh(logits / softcap)): the log-probability of `targets` (outside the
-    vocabulary: NaN), the entropy, and the `k` best tokens, best first, the lower id on ties (a NaN orders as -inf).  A logit of -inf
+    vocabulary: NaN), with `entropy` the entropy, and the `k` best tokens, best first, the lower id on ties (a NaN orders as -inf).  A logit of -inf
     has no probability; a row with no other, with a NaN or with +inf (and no cap) has no distribution: its scores are NaN."""
     T, V = check_token_scores(logits, targets, k, softcap)
     raw = logits.float()
     x = softcap * torch.tanh(raw / softcap) if softcap > 0 else raw
     lp = torch.log_softmax(x, -1)
-    p = lp.exp()
-    entropy = -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(-1)
-    got = None
+    got = ent = None
+    if entropy:
+        p = lp.exp()
+        ent = -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(-1)
     if targets is not None:
         at = targets.long()
         ok = (at >= 0) & (at < V)
-        got = torch.where(ok, lp.gather(1, at.clamp(0, V - 1)[:, None])[:, 0], torch.full_like(entropy, float("nan")))
-    if k > 0:
-        ids = torch.sort(torch.where(raw.isnan(), torch.full_like(raw, float("-inf")), raw), dim=1, descending=True, stable=True).indices[:, :k]
-    else:
-        ids = torch.empty(T, 0, dtype=torch.long, device=logits.device)
-    return TokenScores(got, entropy, ids.to(torch.int32), lp.gather(1, ids))
+        got = lp.gather(1, at.clamp(0, V - 1)[:, None])[:, 0].masked_fill(~ok, float("nan"))
+    ids = _best(raw, k) if k > 0 and T > 0 else torch.empty(T, k, dtype=torch.long, device=logits.device)
+    return TokenScores(got, ent, ids.to(torch.int32), lp.gather(1, ids))

@@ -208,7 +208,7 @@ class HeterogeneousNextTokenChooser:
         next_ids = self._sample(scores)
         alts = None
         if self.max_alternatives <= TOP_MAX:
-            s = get_ops(self.device).token_scores(scores, next_ids, k=self.max_alternatives)
+            s = get_ops(self.device).token_scores(scores, next_ids, k=self.max_alternatives, entropy=False)
             lp = s.logprobs
             if self.max_alternatives > 0:
                 alts = (s.top_ids, s.top_logprobs)

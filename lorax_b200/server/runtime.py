@@ -616,7 +616,7 @@ class ShardRuntime:
                 vals = [float("nan")]
                 if n > 1:
                     tgt = torch.tensor(it.token_ids[1:], device=logits.device)
-                    vals += self.model.ops.token_scores(logits[o:o + n - 1], tgt).logprobs.tolist()
+                    vals += self.model.ops.token_scores(logits[o:o + n - 1], tgt, entropy=False).logprobs.tolist()
                 gen.prefill_tokens.CopyFrom(pb.NextTokens(ids=list(it.token_ids), logprobs=vals,
                                                           texts=[self._tok_text(i) for i in it.token_ids]))
             o += len(it.token_ids) if it.all_logprobs else 1

@@ -54,3 +54,43 @@ def test_a_token_with_a_logit_that_is_no_number_has_no_weights(renorm):
     clean = reference.moe_few(x[[0, 2]], wr, w13, w2, 2, renorm=renorm)
     got = reference.moe_few(x, wr, w13, w2, 2, renorm=renorm)
     assert got[1].isnan().all() and torch.allclose(got[[0, 2]], clean)
+
+
+# ------------------------------------------------------------------------------------------------ scores
+def test_the_best_of_rows_without_sorting_them(monkeypatch):
+    """As a stable sort of whole rows has them, whatever the ties and masks; no row of the vocabulary is sorted."""
+    inf, nan = float("inf"), float("nan")
+    g = torch.Generator().manual_seed(4)
+    rows = [torch.randn(300, generator=g), torch.randn(300, generator=g).round(), torch.zeros(300), torch.full((300,), -inf), torch.full((300,), nan),
+            torch.where(torch.rand(300, generator=g) < 0.95, -inf, torch.randn(300, generator=g)), torch.cat([torch.full((290,), 1.0), torch.arange(10.0)]),
+            torch.where(torch.rand(300, generator=g) < 0.5, nan, torch.randn(300, generator=g)), torch.tensor([-0.0, 0.0] * 150)]
+    x = torch.stack(rows)
+    order = torch.sort(torch.where(x.isnan(), -inf, x), dim=1, descending=True, stable=True).indices
+    lengths = []
+    sort = torch.sort
+    monkeypatch.setattr(torch, "sort", lambda t, *a, **kw: (lengths.append(t.shape[1]), sort(t, *a, **kw))[1])
+    for dtype in (torch.float32, BF16):
+        for k in (1, 2, 7, 32):
+            want = order if dtype == torch.float32 else torch.argsort(torch.where(x.isnan(), -inf, x).to(dtype).float(), dim=1, descending=True, stable=True)
+            assert torch.equal(reference.token_scores(x.to(dtype), k=k).top_ids.long(), want[:, :k])
+    assert max(lengths) <= 32
+    assert reference.token_scores(torch.zeros(0, 8), k=3).top_ids.shape == (0, 3)
+    assert reference.token_scores(torch.ones(2, 3), k=3).top_ids.tolist() == [[0, 1, 2]] * 2
+
+
+def test_scores_without_the_entropy():
+    x = torch.randn(3, 50, generator=torch.Generator().manual_seed(5))
+    whole, some = (reference.token_scores(x, ints(1, 2, 60), k=4, softcap=3.0, entropy=e) for e in (True, False))
+    assert some.entropy is None and whole.entropy.shape == (3,)
+    assert torch.equal(some.logprobs[:2], whole.logprobs[:2]) and some.logprobs[2].isnan()
+    assert torch.equal(some.top_ids, whole.top_ids) and torch.equal(some.top_logprobs, whole.top_logprobs)
+
+
+def test_sampling_asks_for_no_entropy(monkeypatch):
+    """Rows of a whole vocabulary are not gone over for what nobody reads."""
+    from lorax_b200.sampling.chooser import HeterogeneousNextTokenChooser, NextTokenParams
+    asked, scores = [], reference.token_scores
+    monkeypatch.setattr(reference, "token_scores", lambda *a, **kw: (asked.append(kw), scores(*a, **kw))[1])
+    c = HeterogeneousNextTokenChooser([NextTokenParams(return_k_alternatives=2), NextTokenParams()], "cpu", 50)
+    c(None, None, torch.randn(2, 50, generator=torch.Generator().manual_seed(6)))
+    assert [kw.get("entropy") for kw in asked] == [False]
