@@ -1,11 +1,12 @@
 """Bindings of the operators of short ragged steps: `csrc/kernels/step_tables.cu`, `moe_few.cu` and `token_scores.cu`.  Imported into
 :mod:`lorax_b200.ops.native`; `reference` states what they compute.
 
-Arguments that do not fit raise ValueError in front of any launch.  Outputs and scratch are allocated by the call, on the stream that is current
-(calls on several streams, and captured graphs, share nothing)."""
+Arguments that do not fit raise ValueError in front of any launch.  Outputs and scratch are allocated by the call, on the current stream of the tensors' device,
+whichever device is the current one (calls on several streams, and captured graphs, share nothing)."""
 
 from __future__ import annotations
 
+import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Sequence, Tuple
 
@@ -32,21 +33,35 @@ def check_limits(lib):
             raise nv.NativeError(f"{name}: C++ says {getattr(lib, name)()}, Python says {here}")
 
 
-def _stream_for(*tensors: Optional[torch.Tensor]) -> int:
-    """The current stream of the current device, which has to be the tensors' one."""
-    here = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"a tensor on {t.device} while cuda:{here} is the current device")
-    return torch._C._cuda_getCurrentRawStream(here)
+def _on_its_device(op):
+    """`op` with its first tensor's device as the current one: launches go to the current device.  (That the others are on the same one is among its checks.)"""
+    name = op.__code__.co_varnames[0]
+
+    @functools.wraps(op)
+    def call(*args, **kw):
+        t = args[0] if args else kw.get(name)
+        at = t.get_device() if isinstance(t, torch.Tensor) else -1
+        if at < 0 or at == torch._C._cuda_getDevice():
+            return op(*args, **kw)
+        with torch.cuda.device(at):
+            return op(*args, **kw)
+    return call
 
 
+def _stream_of(t: torch.Tensor) -> int:
+    at = t.get_device()
+    if at < 0:
+        raise ValueError(f"tensors on {t.device}: the kernels take those of a CUDA device")
+    return torch._C._cuda_getCurrentRawStream(at)
+
+
+@_on_its_device
 def step_tables(seqs: torch.Tensor, pages: torch.Tensor, tokens: int, max_blocks: int, page: int, window: int = 0,
                 tiles: Sequence[Tuple[int, int]] = (), lora_tiles: int = 0, lora_rows: int = 32, row_offset: int = 0,
                 lead: Optional[torch.Tensor] = None) -> StepTables:
     """Tables of a ragged step from its sequences' lengths (`reference.step_tables` states them), in one launch."""
     B = check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, row_offset, lead)
-    stream = _stream_for(seqs, pages, lead)
+    stream = _stream_of(seqs)
     M, n_lead, n_lists = max_blocks, 0 if lead is None else lead.shape[0], len(tiles)
     sizes = [4 * (n_lead + lora_tiles), B + 1, tokens, tokens, tokens, B * M]
     for _, n in tiles:
@@ -60,13 +75,14 @@ def step_tables(seqs: torch.Tensor, pages: torch.Tensor, tokens: int, max_blocks
     return StepTables(cu, pos, slots, tok, bt.view(B, M), tuple(zip(lists[::2], lists[1::2])), lora.view(-1, 4))
 
 
+@_on_its_device
 def moe_few(x: torch.Tensor, router_w: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, k: int, e0: int = 0, act: str = "silu", renorm: bool = True,
             scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The mixture-of-experts feed-forward of up to `MOE_FEW_TOKENS` tokens (`reference.moe_few` states it; `moe_ffn` takes any number)."""
     T, E, H, inter = check_moe_few(x, router_w, w13, w2, k, e0, act, scale, out)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"moe_few: the kernels are bf16; got {x.dtype}")
-    stream = _stream_for(x, router_w, w13, w2, out)
+    stream = _stream_of(x)
     if out is None:
         out = torch.empty(T, H, dtype=x.dtype, device=x.device)
     if T == 0:
@@ -82,6 +98,7 @@ def moe_few(x: torch.Tensor, router_w: torch.Tensor, w13: torch.Tensor, w2: torc
     return out
 
 
+@_on_its_device
 def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, k: int = 0, softcap: float = 0.0,
                  entropy: bool = True) -> TokenScores:
     """Log-probability of a given token of every row, entropy of the row, and its `k` best tokens with their log-probabilities
@@ -89,7 +106,7 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, k
     T, V = check_token_scores(logits, targets, k, softcap)
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"token_scores: the kernels take bf16 and fp32 logits; got {logits.dtype}")
-    stream = _stream_for(logits, targets)
+    stream = _stream_of(logits)
     t_ptr = wide = 0
     if targets is not None:
         targets = targets.contiguous()

@@ -94,3 +94,47 @@ def test_sampling_asks_for_no_entropy(monkeypatch):
     c = HeterogeneousNextTokenChooser([NextTokenParams(return_k_alternatives=2), NextTokenParams()], "cpu", 50)
     c(None, None, torch.randn(2, 50, generator=torch.Generator().manual_seed(6)))
     assert [kw.get("entropy") for kw in asked] == [False]
+
+
+# ------------------------------------------------------------------------------------------------ devices
+def test_operators_run_on_their_tensors_device_whichever_is_current(monkeypatch):
+    """Tensors of a second device while the first is current: launches, with the second device's stream, while it is the current one."""
+    from lorax_b200.ops import native_steps
+    current, launches = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: (launches.append((name, current[0], a[-1])), 0)[1]
+
+    class Space:
+        status, num_sms = torch.zeros(1, dtype=torch.int32), 148
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 100 + d, raising=False)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1)
+    monkeypatch.setattr(native_steps.nv, "load", Library)
+    monkeypatch.setattr(native_steps.nv, "workspace", lambda d: Space())
+    native.token_scores(torch.zeros(2, 8, dtype=BF16), k=2)
+    native.token_scores(logits=torch.zeros(2, 8), targets=ints(1, 2))
+    native.moe_few(**_moe_args())
+    native.step_tables(ints([3], [0], [-1], [1]), ints(5), 3, 2, 32)
+    current[0] = 1
+    native.token_scores(torch.zeros(2, 8, dtype=BF16))
+    assert launches == [(n, 1, 101) for n in ("lx_token_scores", "lx_token_scores", "lx_moe_few", "lx_step_tables", "lx_token_scores")] and current == [1]
+
+
+def test_kernels_refuse_tensors_that_are_on_no_device():
+    for call in (lambda: native.token_scores(torch.zeros(2, 8)), lambda: native.moe_few(**_moe_args()),
+                 lambda: native.step_tables(ints([3], [0], [-1], [1]), ints(5), 3, 2, 32)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
