@@ -69,7 +69,7 @@ LX_DEVICE void few_mma32(float (&d)[4], const uint4& p, const uint4& q, const ui
   few_mma(d, p.x, q.x, p.y, q.y, b.x, b.y);
   few_mma(d, p.z, q.z, p.w, q.w, b.z, b.w);
 }
-// Eight elements, or zeros.
+// Eight elements, or zeros.  From L2: the down kernel chooses in front of its own wait, so nothing has made its SM's L1 forget what stood there before.
 LX_DEVICE uint4 few_load(const __nv_bfloat16* p, bool valid) {
   uint4 v;
   asm volatile(
@@ -77,7 +77,7 @@ LX_DEVICE uint4 few_load(const __nv_bfloat16* p, bool valid) {
       ".reg .pred p;\n\t"
       "setp.ne.b32 p, %5, 0;\n\t"
       "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-      "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t"
+      "@p ld.relaxed.gpu.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t"
       "}\n"
       : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)valid));
   return v;
@@ -91,6 +91,12 @@ LX_DEVICE float few_act(float x, int act) {
     case kFewRelu: return fmaxf(x, 0.f);
     default: { const float r = fmaxf(x, 0.f); return r * r; }
   }
+}
+
+LX_DEVICE float few_logit(const float* p) {      // (the same, of the logits that a kernel in front of the up kernel left, or of shared memory)
+  float v;
+  asm volatile("ld.relaxed.gpu.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
 }
 
 // ------------------------------------------------------------------------------------------------ choice of experts, and who is reached
@@ -160,7 +166,7 @@ LX_DEVICE void few_select(FewPlan& plan, const float* logits, const MoeFewParams
     const float* row = logits + t * p.E;
     float z[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) z[i] = lane + 32 * i < p.E ? row[lane + 32 * i] : 0.f;
+    for (int i = 0; i < PER; ++i) z[i] = lane + 32 * i < p.E ? few_logit(row + lane + 32 * i) : 0.f;
     // logits as numbers whose order is theirs; 0: taken, or no expert
     uint32_t key[PER];
     bool odd = false;
@@ -582,7 +588,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
   few_ring_init(ring);
   for (int i = tid; i < kFewZeros / 4; i += kFewThreads) reinterpret_cast<uint32_t*>(zeros)[i] = 0;
   few_prefetch(maps);
-  // In front of the wait for the up kernel: it has waited itself for what wrote the tokens, the router and the logits, and triggers behind that.
+  // In front of the wait for the up kernel: every CTA of it has waited itself for what wrote the tokens, the router and the logits, and triggers behind that, so
+  // they are complete in L2, where few_load and few_logit read them.
   few_choose<NT>(plan, smem, p);
   // A stage: rows of the weights, values and remainders of the expert's tokens; the same of what is behind the last block, for an expert's last stage.
   const int blocks = p.I / 64, chunks = max(1, (blocks + p.down_blocks - 1) / p.down_blocks), reached = plan.reached, rows = p.down_rows;
