@@ -21,6 +21,7 @@
 // h is held as two bf16 terms, value and remainder, which take two MMAs: it is as exact as the fp32 sums, and the tensor cores have room.  Its
 // rows lie in the order of the experts, the tokens of one behind the other.
 // Every CTA chooses the experts for itself from the logits; no CTA waits for another.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -271,7 +272,7 @@ LX_DEVICE void few_choose(FewPlan& plan, uint8_t* smem, const MoeFewParams& p) {
 // Row of h of token t (one of `mask`) within its expert's.
 LX_DEVICE int few_slot(uint32_t mask, int t) { return __popc(mask & ((1u << t) - 1)); }
 // Copies of 2^shift rows of h that bring n of them.
-LX_DEVICE int few_copies(int n, int shift) { return (n + (1 << shift) - 1) >> shift; }
+__host__ __device__ inline int few_copies(int n, int shift) { return (n + (1 << shift) - 1) >> shift; }
 // The i-th token of `mask`.
 LX_DEVICE int few_token(uint32_t mask, int i) {
   for (; i > 0; --i) mask &= mask - 1;
@@ -388,7 +389,7 @@ LX_DEVICE uint4 few_row(uint32_t at) {
 }
 constexpr int kFewZeros = kFewUpSteps * 512;      // what the lanes of a column without a token read instead of one
 
-// Tensor maps of a product's operands: whole blocks of 64 of K, and what is behind them.  [1]: boxes of twice the blocks (up).
+// Tensor maps of a product's operands: whole blocks of 64 of K, and what is behind them.  [1]: boxes of twice the blocks (up), of half of them (down).
 struct FewMaps {
   CUtensorMap weights[2], tokens[2], weights_rest, tokens_rest;
 };
@@ -573,9 +574,31 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_up_kernel(const __grid
 }
 
 // ------------------------------------------------------------------------------------------------ down
-// MT: tiles of 16 rows; steps of 32 of K of a stage and a math warp: as many as make stages of 32 to 64 KB (of half of that, 470 -> 490 us for 16 tokens).
+// MT: tiles of 16 rows; steps of 32 of K of a stage and a math warp: as many as bring 32 to 64 KB of weights (of half of that, 470 -> 490 us for 16 tokens).
 template <int MT, int NT>
 constexpr int few_down_steps() { return MT == 1 || MT + NT == 3 ? 4 : 2; }
+static int few_down_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 ? 3 : kFewRowTiles; }
+
+// A stage: rows of the weights, values and remainders of the expert's tokens (at most `copies` copies); the same of what is behind the last block, for an expert's last
+// stage.  Where only one such stage fits beside the sums, it has half the blocks: filling and multiplying would take turns (wide layers whose 13 to 16 tokens
+// share an expert, and some with a rest of K and more than four or twelve: 16 tokens at two experts of 9472 x 8192 232 -> 207 us).
+struct FewDownStage {
+  int blocks, rest, wide, plane, plane_rest, rest_at, rest_h, bytes, stages;
+  bool half;
+  __host__ __device__ FewDownStage(int mt, int nt, int I, int rows, int all_blocks, int copies, int h_shift) : rest(I % 64 != 0), plane_rest(128 << h_shift) {
+    const int room = kFewSmem - 1024 - kFewMath * mt * nt * 32 * (int)sizeof(float4);
+    blocks = all_blocks;
+    for (half = false;; half = true, blocks = (all_blocks + 1) / 2) {
+      wide = (blocks * rows * 128 + 1023) & ~1023;
+      plane = blocks * 128 << h_shift;
+      rest_at = (wide + copies * 2 * plane + 1023) & ~1023;
+      rest_h = (rest_at + rows * 128 + 127) & ~127;
+      bytes = rest ? (rest_h + copies * 2 * plane_rest + 1023) & ~1023 : rest_at;
+      stages = room / bytes < kFewMaxStages ? room / bytes : kFewMaxStages;
+      if (stages > 1 || half) return;
+    }
+  }
+};
 
 template <int MT, int NT>
 __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ MoeFewParams p) {
@@ -591,14 +614,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
   // In front of the wait for the up kernel: every CTA of it has waited itself for what wrote the tokens, the router and the logits, and triggers behind that, so
   // they are complete in L2, where few_load and few_logit read them.
   few_choose<NT>(plan, smem, p);
-  // A stage: rows of the weights, values and remainders of the expert's tokens; the same of what is behind the last block, for an expert's last stage.
-  const int blocks = p.I / 64, chunks = max(1, (blocks + p.down_blocks - 1) / p.down_blocks), reached = plan.reached, rows = p.down_rows;
-  const int bytes = p.down_blocks * rows * 128, wide = (bytes + 1023) & ~1023, plane = p.down_blocks * 128 << p.h_shift, plane_rest = 128 << p.h_shift;
-  const int copies = few_copies(plan.most, p.h_shift);
-  const bool rest = p.I % 64 != 0;
-  const int rest_at = (wide + copies * 2 * plane + 1023) & ~1023, rest_h = (rest_at + rows * 128 + 127) & ~127;
-  const int stage_bytes = rest ? (rest_h + copies * 2 * plane_rest + 1023) & ~1023 : rest_at;
-  const int stages = min((kFewSmem - 1024 - kFewMath * MT * NT * 32 * (int)sizeof(float4)) / stage_bytes, kFewMaxStages);
+  const FewDownStage geo(MT, NT, p.I, p.down_rows, p.down_blocks, few_copies(plan.most, p.h_shift), p.h_shift);
+  const int blocks = p.I / 64, deep = geo.blocks, chunks = max(1, (blocks + deep - 1) / deep), reached = plan.reached, rows = p.down_rows;
+  const int bytes = deep * rows * 128, wide = geo.wide, plane = geo.plane, plane_rest = geo.plane_rest;
+  const bool rest = geo.rest;
+  const int rest_at = geo.rest_at, rest_h = geo.rest_h, stage_bytes = geo.bytes, stages = geo.stages;
   FewCursor at;
   if (warp == kFewMath) {
     if (lane == 0) {
@@ -610,7 +630,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
       auto copies_of = [&](int d) { return few_copies(__popc(plan.mask[plan.list[d]]), p.h_shift); };
       auto tokens_of = [&](uint8_t* stage, uint64_t* bar, int row, int n, int ch) {
         if (blocks > 0)
-          for (int i = 0; i < n; ++i) tma_load_4d(stage + wide + i * 2 * plane, &maps.tokens[0], bar, 0, row + (i << p.h_shift), ch * p.down_blocks, 0);
+          for (int i = 0; i < n; ++i) tma_load_4d(stage + wide + i * 2 * plane, &maps.tokens[geo.half], bar, 0, row + (i << p.h_shift), ch * deep, 0);
         if (rest && ch == chunks - 1)
           for (int i = 0; i < n; ++i) tma_load_4d(stage + rest_h + i * 2 * plane_rest, &maps.tokens_rest, bar, blocks * 64, row + (i << p.h_shift), 0, 0);
       };
@@ -631,7 +651,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
             uint8_t* stage = smem + at.stage * stage_bytes;
             const bool ends = rest && ch == chunks - 1;
             ok = few_fill(ring, at, stages, whole + (ends ? rows * 128 + n * 2 * plane_rest : 0), p.status, [&](uint64_t* bar) {
-              if (blocks > 0) tma_load_4d_hint(stage, &maps.weights[0], bar, 0, r0, ch * p.down_blocks, e, policy);
+              if (blocks > 0) tma_load_4d_hint(stage, &maps.weights[geo.half], bar, 0, r0, ch * deep, e, policy);
               if (ends) tma_load_4d_hint(stage + rest_at, &maps.weights_rest, bar, blocks * 64, r0, 0, e, policy);
               if (waited) tokens_of(stage, bar, row, n, ch);
             });
@@ -647,7 +667,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
   pdl_trigger();
   float4* red = reinterpret_cast<float4*>(smem + stages * stage_bytes);      // [math warps][MT][NT][32 lanes]
   constexpr int kSteps = few_down_steps<MT, NT>();
-  const int steps = 2 * blocks, per = 2 * p.down_blocks;
+  const int steps = 2 * blocks, per = 2 * deep;
   int place[MT][2];                            // (rows past the last one are taken from it: nobody stores their sums)
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -801,14 +821,24 @@ static int few_opt_in(K* kernel, bool (&set)[64]) {
   return 0;
 }
 
+// Rows of a CTA's stages of the down kernel, and the logarithm of the rows of h of a copy (what a copy brings beyond the expert's tokens is not read).
+static int few_down_rows(int H, int num_sms) { return std::min(((H + num_sms - 1) / num_sms + 1) & ~1, 16 * kFewRowTiles); }
+static int few_h_shift(int T) { return T <= 2 ? T - 1 : 2; }
+
 template <int MT, int NT>
 static int moe_few_down(MoeFewParams& p, int num_sms, cudaStream_t s) {
   static bool set[64] = {};
   if (const int rc = few_opt_in(moe_few_down_kernel<MT, NT>, set)) return rc;
   p.down_blocks = few_blocks(p.I / 64, few_down_steps<MT, NT>() * kFewMath / 2);
   FewMaps maps{};
-  if (const int rc = few_tmap(&maps.weights[0], &maps.weights_rest, p.w2, p.e_local, p.H, p.I, p.I, (long long)p.H * p.I, p.down_rows, p.down_blocks, 1, true)) return rc;
-  if (const int rc = few_tmap(&maps.tokens[0], &maps.tokens_rest, p.h, 2, (long long)p.T * p.k, p.I, p.I, (long long)p.T * p.k * p.I, 1 << p.h_shift, p.down_blocks, 2, false)) return rc;
+  // (the half ones are made where the most tokens an expert can have need them; the kernel goes by those that it has)
+  const int n = FewDownStage(MT, NT, p.I, p.down_rows, p.down_blocks, few_copies(p.T, p.h_shift), p.h_shift).half ? 2 : 1;
+  for (int i = 0; i < n; ++i) {
+    const int blocks = (p.down_blocks + i) >> i;
+    if (const int rc = few_tmap(&maps.weights[i], i == 0 ? &maps.weights_rest : nullptr, p.w2, p.e_local, p.H, p.I, p.I, (long long)p.H * p.I, p.down_rows, blocks, 1, true)) return rc;
+    if (const int rc = few_tmap(&maps.tokens[i], i == 0 ? &maps.tokens_rest : nullptr, p.h, 2, (long long)p.T * p.k, p.I, p.I, (long long)p.T * p.k * p.I, 1 << p.h_shift, blocks, 2,
+                                false)) return rc;
+  }
   launch_pdl(moe_few_down_kernel<MT, NT>, dim3(num_sms), dim3(kFewThreads), kFewSmem, s, maps, p);
   return -(int)cudaGetLastError();
 }
@@ -824,13 +854,14 @@ static int moe_few_launch(MoeFewParams& p, int num_sms, cudaStream_t s) {
     if (const int rc = few_tmap(&maps.tokens[i], i == 0 ? &maps.tokens_rest : nullptr, p.x, 1, p.T, p.H, p.ldx, p.T * p.ldx, 1, p.up_blocks << i, 1, false)) return rc;
   }
   launch_pdl(moe_few_up_kernel<NT>, dim3(num_sms), dim3(kFewThreads), kFewSmem, s, maps, p);
-  const int rows = ((p.H + num_sms - 1) / num_sms + 1) & ~1;
-  p.h_shift = p.T <= 2 ? p.T - 1 : 2;           // (what a copy brings beyond the expert's tokens is not read)
-  p.down_rows = rows < 16 * kFewRowTiles ? rows : 16 * kFewRowTiles;
-  if (rows <= 16) return moe_few_down<1, NT>(p, num_sms, s);
-  if (rows <= 32) return moe_few_down<2, NT>(p, num_sms, s);
-  if (rows <= 48) return moe_few_down<3, NT>(p, num_sms, s);
-  return moe_few_down<kFewRowTiles, NT>(p, num_sms, s);
+  p.h_shift = few_h_shift(p.T);
+  p.down_rows = few_down_rows(p.H, num_sms);
+  switch (few_down_tiles(p.down_rows)) {
+    case 1: return moe_few_down<1, NT>(p, num_sms, s);
+    case 2: return moe_few_down<2, NT>(p, num_sms, s);
+    case 3: return moe_few_down<3, NT>(p, num_sms, s);
+    default: return moe_few_down<kFewRowTiles, NT>(p, num_sms, s);
+  }
 }
 
 }  // namespace lx
@@ -841,6 +872,15 @@ int lx_moe_few_max_tokens() { return lx::kFewTokens; }
 
 int lx_moe_router_logits(const void* x, long long ldx, const void* wr, long long ldw, float* logits, int T, int E, int H, int* counts, int ncounts,
                          void* stream);
+
+// Stages of the down kernel's ring for T tokens, `most` of which one expert serves.
+int lx_moe_few_down_stages(int T, int H, int I, int most, int num_sms) {
+  using namespace lx;
+  if (T <= 0 || T > kFewTokens || most <= 0 || most > T || H <= 0 || I <= 0 || num_sms <= 0) return -1;
+  const int rows = few_down_rows(H, num_sms), mt = few_down_tiles(rows), nt = T <= 8 ? 1 : 2, shift = few_h_shift(T);
+  const int steps = mt == 1 ? few_down_steps<1, 1>() : mt == 2 ? (nt == 1 ? few_down_steps<2, 1>() : few_down_steps<2, 2>()) : mt == 3 ? few_down_steps<3, 1>() : few_down_steps<4, 1>();
+  return FewDownStage(mt, nt, I, rows, few_blocks(I / 64, steps * kFewMath / 2), few_copies(most, shift), shift).stages;
+}
 
 // `logits` [T, E] and `h` [2, T k, I] are scratch of the call.
 int lx_moe_few(const void* x, long long ldx, const void* wr, long long ldw, const void* w13, const void* w2, float* logits, void* h, void* out, long long ldo, int T,

@@ -21,6 +21,7 @@ SIGNATURES = {
     "lx_step_tables_max_seqs": ([], I),
     "lx_step_tables": ([P, L, P, I, I, I, I, I, I, I, P, P, I, P, I, I, I, P, P], I),
     "lx_moe_few_max_tokens": ([], I),
+    "lx_moe_few_down_stages": ([I, I, I, I, I], I),
     "lx_moe_few": ([P, L, P, L, P, P, P, P, P, L, I, I, I, I, I, I, I, I, I, F, P, I, P], I),
     "lx_token_scores_max_top": ([], I),
     "lx_token_scores": ([P, L, I, I, I, P, I, I, F, P, P, P, P, P], I),

@@ -56,6 +56,17 @@ def test_a_token_with_a_logit_that_is_no_number_has_no_weights(renorm):
     assert got[1].isnan().all() and torch.allclose(got[[0, 2]], clean)
 
 
+def test_the_ring_of_a_few_tokens_experts_has_more_than_one_stage():
+    """With one stage its copies and its products take turns: no width, features or number of an expert's tokens may leave just that."""
+    lib = native.load()
+    for H in (8, 512, 1024, 2048, 2304, 2368, 4096, 4600, 4736, 6144, 7104, 7168, 8192, 9216, 9472, 9480, 16384, 20000):
+        for inter in (8, 64, 200, 1024, 1032, 4096, 4104, 8192, 14336, 14344):
+            for T in range(1, 17):
+                for most in range(1, T + 1):
+                    for sms in (148, 132):
+                        assert lib.lx_moe_few_down_stages(T, H, inter, most, sms) > 1, (T, H, inter, most, sms)
+
+
 # ------------------------------------------------------------------------------------------------ scores
 def test_the_best_of_rows_without_sorting_them(monkeypatch):
     """As a stable sort of whole rows has them, whatever the ties and masks; no row of the vocabulary is sorted."""

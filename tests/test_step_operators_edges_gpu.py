@@ -125,3 +125,14 @@ def test_experts_of_squared_relu(T, E, k, H, I):
             off += p[j] * (D.abs() @ (herr + gamma(I * min(E, T * k)) * h.abs()))
         off = off + 2.0 ** -8 * (out.abs() + off)
         assert ((got[t] - out).abs() <= off).all()
+
+
+@pytest.mark.parametrize("T,E,k,H,I", [(16, 4, 2, 9480, 1024), (13, 8, 1, 9216, 1088), (16, 4, 2, 9480, 1160), (7, 8, 2, 4600, 2056), (16, 3, 3, 2304, 1096), (14, 8, 2, 2048, 4104)])
+def test_all_tokens_at_the_same_experts_of_wide_layers(T, E, k, H, I):
+    """What a stage of the second product's ring holds depends on the most tokens of an expert."""
+    x, wr, w13, w2 = _experts(T, E, k, H, I, seed=8)
+    x = (x[:1].float() + 0.02 * x.float()).to(BF16)
+    ids = _routes(x, wr, k)
+    assert max(sum(e in row for row in ids) for e in range(E)) == T
+    _check_experts((x, wr, w13, w2), k)
+    native.workspace().check_status()
