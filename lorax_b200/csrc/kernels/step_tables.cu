@@ -20,6 +20,7 @@ constexpr int kTablesThreads = 256;
 constexpr int kTablesPer = 1024;          // entries of an output that a block writes
 constexpr int kTablesMaxSeqs = 4096;
 constexpr int kTablesLists = 4;
+constexpr int kTablesMaxTiles = 1 << 30;  // entries of a list (its blocks count in 32 bits, past its end)
 
 struct TileList {
   int* seq;
@@ -186,7 +187,7 @@ int lx_step_tables(const int* seqs, long long ld, const int* pages, int num_page
                    const int* heights, const int* counts, int nlists, const int* lead, int nlead, int lora_rows, int lora_count, int* out,
                    void* stream) {
   using namespace lx;
-  if (B < 0 || B > kTablesMaxSeqs || T < 0 || M <= 0 || page <= 0 || num_pages < 0 || nlists < 0 || nlists > kTablesLists || row_offset < 0 || nlead < 0 || lora_count < 0 ||
+  if (B < 0 || B > kTablesMaxSeqs || T < 0 || M <= 0 || page <= 0 || num_pages < 0 || nlists < 0 || nlists > kTablesLists || row_offset < 0 || nlead < 0 || lora_count < 0 || nlead > kTablesMaxTiles || lora_count > kTablesMaxTiles - nlead ||
       (lora_count > 0 && lora_rows <= 0) || (nlead > 0 && lead == nullptr))
     return -1;
   if ((reinterpret_cast<uintptr_t>(out) & 15) != 0 || (reinterpret_cast<uintptr_t>(lead) & 15) != 0) return -2;
@@ -208,7 +209,7 @@ int lx_step_tables(const int* seqs, long long ld, const int* pages, int num_page
   p.first[1] = (int)grid;
   p.nlists = nlists;
   for (int l = 0; l < nlists; ++l) {
-    if (heights[l] <= 0 || counts[l] < 0) return -1;
+    if (heights[l] <= 0 || counts[l] < 0 || counts[l] > kTablesMaxTiles) return -1;
     p.lists[l] = TileList{out, out + counts[l], heights[l], counts[l]};
     out += 2LL * counts[l];
     grid += blocks(counts[l]);

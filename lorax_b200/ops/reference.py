@@ -985,6 +985,7 @@ MOE_FEW_TOKENS = 16         # tokens that `moe_few` takes at most
 INT32_END = 1 << 31
 TOP_MAX = 32                # alternatives that `token_scores` returns at most
 STEP_SEQS_MAX = 4096        # sequences of `step_tables`
+STEP_TILES_MAX = 1 << 30    # entries of one of its lists of tiles
 
 
 class StepTables(NamedTuple):
@@ -1007,13 +1008,13 @@ def check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora
         raise ValueError("step_tables: pages is one contiguous int32 list on the device of seqs")
     if not (0 <= tokens < INT32_END and 0 < max_blocks < INT32_END and 0 < page < INT32_END and 0 <= window < INT32_END):
         raise ValueError("step_tables: tokens and window from 0 on, max_blocks and page from 1 on, in 32 bits")
-    if not (len(tiles) <= 4 and all(0 < h < INT32_END and 0 <= n < INT32_END for h, n in tiles)):
-        raise ValueError("step_tables: up to four lists of tiles (height, count)")
-    if not (0 <= lora_tiles < INT32_END and 0 < lora_rows < INT32_END and 0 <= row_offset < INT32_END):
-        raise ValueError("step_tables: lora_tiles and row_offset from 0 on, lora_rows from 1 on, in 32 bits")
+    if not (len(tiles) <= 4 and all(0 < h < INT32_END and 0 <= n <= STEP_TILES_MAX for h, n in tiles)):
+        raise ValueError("step_tables: up to four lists of up to 2^30 tiles (height, count)")
+    if not (0 <= lora_tiles <= STEP_TILES_MAX and 0 < lora_rows < INT32_END and 0 <= row_offset < INT32_END):
+        raise ValueError("step_tables: lora_tiles from 0 to 2^30, row_offset from 0 on and lora_rows from 1 on, in 32 bits")
     if not (lead is None or (lead.dtype == torch.int32 and lead.dim() == 2 and lead.shape[1] == 4 and lead.is_contiguous() and lead.device == seqs.device
-                           and lead.data_ptr() % 16 == 0)):
-        raise ValueError("step_tables: lead is [n, 4] int32, contiguous, on a 16-byte boundary")
+                           and lead.data_ptr() % 16 == 0 and lead.shape[0] + lora_tiles <= STEP_TILES_MAX)):
+        raise ValueError("step_tables: lead is [n, 4] int32, contiguous, on a 16-byte boundary, and up to 2^30 tiles with lora_tiles")
     return seqs.shape[1]
 
 
@@ -1027,7 +1028,7 @@ def step_tables(seqs, pages, tokens: int, max_blocks: int, page: int, window: in
     (height, count) of lists of tiles, first queries 0, height, 2 height .. of every sequence in turn.  Adapter tiles hold up to `lora_rows`
     rows of one sequence with an adapter; rows are counted from `row_offset`, and the tiles `lead` [n, 4] come first.
 
-    Sums of tokens and of pages stay below 2^31.  The caller states how much there is (`tokens`, the counts, `lora_tiles`).  Entries past what the lengths make are filled: position 0, slots
+    Sums of tokens and of pages, positions and slots stay below 2^31.  The caller states how much there is (`tokens`, the counts, `lora_tiles`).  Entries past what the lengths make are filled: position 0, slots
     and tiles' sequences and adapters -1; what they make beyond is left out."""
     check_step_tables(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, row_offset, lead)
     return step_tables_of_many(seqs, pages, tokens, max_blocks, page, window, tiles, lora_tiles, lora_rows, row_offset, lead)

@@ -3,7 +3,14 @@ import pytest
 import torch
 
 from lorax_b200.ops import native, reference
-from tests.test_step_operators import BF16, _moe_args, _refused, ints
+from tests.test_step_operators import BF16, _moe_args, _refused, _tables_args, ints
+
+
+# ------------------------------------------------------------------------------------------------ tables
+@pytest.mark.parametrize("over", [dict(tiles=((64, 2 ** 31 - 1),)), dict(tiles=((64, 1), (64, 2 ** 30 + 1))), dict(lora_tiles=2 ** 31 - 1),
+                                  dict(lora_tiles=2 ** 30, lead=torch.zeros(1, 4, dtype=torch.int32))])
+def test_tables_refuse_lists_whose_blocks_would_count_past_32_bits(over):
+    _refused("step_tables", **_tables_args(**over))
 
 
 # ------------------------------------------------------------------------------------------------ experts
