@@ -1036,37 +1036,47 @@ def step_tables(seqs, pages, tokens: int, max_blocks: int, page: int, window: in
 
 def step_tables_of_many(seqs, pages, tokens: int, max_blocks: int, page: int, window: int = 0, tiles=(), lora_tiles: int = 0, lora_rows: int = 32,
                         row_offset: int = 0, lead=None) -> StepTables:
-    """`step_tables` of any number of sequences, on the host."""
+    """`step_tables` of any number of sequences: whole arrays at a time on the tensors' device, with nothing read back to the host."""
     B, dev = seqs.shape[1], seqs.device
-    n, cached, adapter, held = seqs.tolist() if B else ([], [], [], [])
-    n, cached, held, flat = [max(v, 0) for v in n], [max(v, 0) for v in cached], [max(v, 0) for v in held], pages.tolist()
-    cu, tables, off = [0], [], 0
-    for b in range(B):
-        cu.append(cu[-1] + n[b])
-        own = [flat[i] if i < len(flat) else 0 for i in range(off, off + min(held[b], max_blocks))]
-        off += held[b]
-        if window > 0 and 0 < held[b] < max_blocks and held[b] * page >= window + page:
-            tables.append([own[j % held[b]] for j in range(max_blocks)])
-        else:
-            tables.append((own + [0] * max_blocks)[:max_blocks])
-    pos, slots, tok = [], [], []
-    for b in range(B):
-        for p in range(cached[b], cached[b] + n[b]):
-            pos.append(p)
-            slots.append(tables[b][min(p // page, max_blocks - 1)] * page + p % page)
-        tok += [adapter[b]] * n[b]
+    n, cached, adapter, held = seqs.long()
+    n, cached, held = n.clamp(min=0), cached.clamp(min=0), held.clamp(min=0)
+    sums = lambda count: torch.cat([count.new_zeros(1), torch.cumsum(count, 0)])
+    cu, off = sums(n), sums(held)[:-1, None]
+    i32 = lambda x: x.to(torch.int32)
 
-    def t(values, count, fill):
-        return torch.tensor((values + [fill] * count)[:count], dtype=torch.int32, device=dev)
+    j = torch.arange(max_blocks, device=dev)[None]
+    kept = held[:, None]
+    recycled = (window > 0) & (kept > 0) & (kept < max_blocks) & (kept * page >= window + page)
+    at = torch.where(recycled, off + j % kept.clamp(min=1), torch.where(j < kept, off + j, -1))
+    flat = torch.cat([pages.long(), pages.new_zeros(1).long()])              # (behind the list, and for what is no entry: page 0)
+    tables = flat[torch.where((at >= 0) & (at < pages.shape[0]), at, pages.shape[0])]
+
+    def places(first, count):
+        """Entry i of `count` belongs to sequence b, the last one that begins at or before it; live: there is one."""
+        i = torch.arange(count, device=dev)
+        return i, torch.searchsorted(first[1:], i, right=True).clamp(max=max(B - 1, 0)), i < first[-1]
+
+    def pick(live, value, fill):
+        return i32(torch.where(live, value, torch.full_like(value, fill)))
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    if B == 0:
+        blank = lambda count, fill: torch.full((count,), fill, dtype=torch.int32, device=dev)
+        lora = none.view(0, 4) if lora_tiles == 0 else torch.tensor([[-1, 0, 0, 0]], dtype=torch.int32, device=dev).expand(lora_tiles, 4)
+        return StepTables(i32(cu), blank(tokens, 0), blank(tokens, -1), blank(tokens, -1), none.view(0, max_blocks),
+                          tuple((blank(count, -1), blank(count, 0)) for _, count in tiles), lora.clone() if lead is None else torch.cat([lead, lora]))
+    t, b, live = places(cu, tokens)
+    pos = cached[b] + t - cu[b]
+    slot = tables[b, torch.div(pos, page, rounding_mode="floor").clamp(0, max_blocks - 1)] * page + pos % page
     lists = []
     for height, count in tiles:
-        seq, q0 = prefill_tiles(n, height)
-        lists.append((t(seq, count, -1), t(q0, count, 0)))
-    rows = [[adapter[b], row_offset + cu[b] + r, min(lora_rows, n[b] - r), 0] for b in range(B) if adapter[b] >= 0 for r in range(0, n[b], lora_rows)]
-    rows = (rows + [[-1, 0, 0, 0]] * lora_tiles)[:lora_tiles]
-    lora = torch.tensor(rows, dtype=torch.int32, device=dev).view(-1, 4)
-    return StepTables(torch.tensor(cu, dtype=torch.int32, device=dev), t(pos, tokens, 0), t(slots, tokens, -1), t(tok, tokens, -1),
-                      torch.tensor(tables, dtype=torch.int32, device=dev).view(B, max_blocks), tuple(lists),
+        first = sums((n + height - 1) // height)
+        i, of, has = places(first, count)
+        lists.append((pick(has, of, -1), pick(has, (i - first[of]) * height, 0)))
+    first = sums(torch.where(adapter >= 0, (n + lora_rows - 1) // lora_rows, torch.zeros_like(n)))
+    i, of, has = places(first, lora_tiles)
+    row = (i - first[of]) * lora_rows
+    lora = torch.stack([pick(has, adapter[of], -1), pick(has, row_offset + cu[of] + row, 0), pick(has, (n[of] - row).clamp(max=lora_rows), 0), i32(torch.zeros_like(i))], 1)
+    return StepTables(i32(cu), pick(live, pos, 0), pick(live, slot, -1), pick(live, adapter[b], -1), i32(tables), tuple(lists),
                       lora if lead is None else torch.cat([lead, lora]))
 
 

@@ -1,4 +1,6 @@
 """Calls of the operators of short ragged steps that are easily answered wrongly, on the CPU: what they refuse, and what the plain forms say."""
+import random
+
 import pytest
 import torch
 
@@ -11,6 +13,50 @@ from tests.test_step_operators import BF16, _moe_args, _refused, _tables_args, i
                                   dict(lora_tiles=2 ** 30, lead=torch.zeros(1, 4, dtype=torch.int32))])
 def test_tables_refuse_lists_whose_blocks_would_count_past_32_bits(over):
     _refused("step_tables", **_tables_args(**over))
+
+
+def _tables_by_hand(n, cached, adapter, held, pages, tokens, M, page, window, tiles, lora_tiles, lora_rows, row_offset):
+    """Sequence by sequence, token by token."""
+    n, cached, held = ([max(v, 0) for v in row] for row in (n, cached, held))
+    B, at, cu, tables, rows, lora = len(n), 0, [0], [], [], []
+    for b in range(B):
+        entry = [pages[at + j] if at + j < len(pages) else 0 for j in range(held[b])]
+        at += held[b]
+        turns = 0 < held[b] < M and window > 0 and held[b] * page >= window + page
+        tables.append([entry[j % held[b]] if turns else entry[j] if j < held[b] else 0 for j in range(M)])
+        for p in range(cached[b], cached[b] + n[b]):
+            rows.append((p, tables[b][min(p // page, M - 1)] * page + p % page, adapter[b]))
+        if adapter[b] >= 0:
+            lora += [(adapter[b], row_offset + cu[b] + r, min(lora_rows, n[b] - r), 0) for r in range(0, n[b], lora_rows)]
+        cu.append(cu[-1] + n[b])
+    fill = lambda got, want, blank: (got + [blank] * want)[:want]
+    rows, lora = fill(rows, tokens, (0, -1, -1)), fill(lora, lora_tiles, (-1, 0, 0, 0))
+    lists = [fill([(b, q) for b in range(B) for q in range(0, n[b], h)], count, (-1, 0)) for h, count in tiles]
+    return cu, [list(c) for c in zip(*rows)] if rows else [[], [], []], tables, lists, [list(r) for r in lora]
+
+
+def test_tables_of_any_lengths_without_a_word_from_the_host(monkeypatch):
+    """Lengths below zero, page lists that end early, counts beyond and below what the lengths make; the arrays of any number of sequences are made whole."""
+    rng, tolist = random.Random(9), torch.Tensor.tolist
+    for case in range(300):
+        B = rng.choice([0, 1, 2, 5, 17])
+        n = [rng.choice([-2, 0, 1, rng.randint(1, 150)]) for _ in range(B)]
+        cached = [rng.choice([-1, 0, rng.randint(0, 300)]) for _ in range(B)]
+        adapter, held = [rng.randint(-2, 3) for _ in range(B)], [rng.choice([-1, 0, 1, 2, 5, 9]) for _ in range(B)]
+        pages = [rng.randint(0, 99) for _ in range(max(0, sum(max(v, 0) for v in held) + rng.choice([0, 0, -3, 4])))]
+        tokens = max(0, sum(max(v, 0) for v in n) + rng.choice([0, 0, -3, 5]))
+        M, page, window = rng.choice([1, 2, 5, 8, 12]), rng.choice([1, 16, 32, 7]), rng.choice([0, 0, 16, 64])
+        tiles = tuple((rng.choice([1, 3, 64, 128]), rng.randint(0, 30)) for _ in range(rng.randint(0, 4)))
+        lora_tiles, lora_rows, offset = rng.randint(0, 20), rng.choice([1, 8, 32]), rng.randint(0, 9)
+        lead = ints([1, 2, 3, 0]) if case % 3 == 0 else None
+        with monkeypatch.context() as m:
+            m.setattr(torch.Tensor, "tolist", lambda t: pytest.fail("read back"))
+            got = reference.step_tables(ints(n, cached, adapter, held).view(4, B), ints(*pages), tokens, M, page, window, tiles, lora_tiles, lora_rows, offset, lead)
+        cu, rows, tables, lists, lora = _tables_by_hand(n, cached, adapter, held, pages, tokens, M, page, window, tiles, lora_tiles, lora_rows, offset)
+        assert tolist(got.cu_q) == cu and [tolist(x) for x in (got.positions, got.slots, got.tok_slot)] == rows and tolist(got.block_tables) == tables
+        assert [list(zip(*map(tolist, pair))) for pair in got.tiles] == lists
+        assert tolist(got.lora_tiles) == (tolist(lead) if lead is not None else []) + lora
+        assert all(t.dtype == torch.int32 for t in (got.cu_q, got.positions, got.slots, got.tok_slot, got.block_tables, got.lora_tiles))
 
 
 # ------------------------------------------------------------------------------------------------ experts

@@ -136,3 +136,17 @@ def test_all_tokens_at_the_same_experts_of_wide_layers(T, E, k, H, I):
     assert max(sum(e in row for row in ids) for e in range(E)) == T
     _check_experts((x, wr, w13, w2), k)
     native.workspace().check_status()
+
+
+@pytest.mark.parametrize("B,window", [(0, 0), (1, 0), (300, 64), (4096, 0)])
+def test_tables_of_many_sequences_are_the_kernels(B, window):
+    """Steps of more sequences than the kernel takes are tabled by whole arrays on the device."""
+    g = torch.Generator().manual_seed(B)
+    draw = lambda lo, hi: torch.randint(lo, hi, (B,), generator=g, dtype=torch.int32)
+    seqs = torch.stack([draw(0, 40), draw(0, 200), draw(-1, 4), draw(0, 9)]).cuda()
+    pages = torch.randint(1, 10000, (int(seqs[3].sum()),), generator=g, dtype=torch.int32).cuda()
+    args = dict(tokens=int(seqs[0].sum()) + 3, max_blocks=8, page=16, window=window, tiles=((64, B + 2), (8, 4 * B)), lora_tiles=B + 1, lora_rows=32, row_offset=7,
+                lead=torch.tensor([[2, 0, 7, 0]], dtype=torch.int32, device="cuda"))
+    a, b = native.step_tables(seqs, pages, **args), reference.step_tables_of_many(seqs, pages, **args)
+    for x, y in zip(a, b):
+        assert all(torch.equal(p, q) for s, t in zip(x, y) for p, q in zip(s, t)) if isinstance(x, tuple) else torch.equal(x, y)
