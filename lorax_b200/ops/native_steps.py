@@ -13,7 +13,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import native as nv
-from .reference import MOE_FEW_TOKENS, TOP_MAX, StepTables, TokenScores, check_moe_few, check_step_tables, check_token_scores
+from .reference import MOE_FEW_TOKENS, STEP_SEQS_MAX, TOP_MAX, StepTables, TokenScores, check_moe_few, check_step_tables, check_token_scores
 
 P, I, L, F = c_void_p, c_int, c_longlong, c_float
 
@@ -29,7 +29,7 @@ SIGNATURES = {
 
 
 def check_limits(lib):
-    for name, here in (("lx_moe_few_max_tokens", MOE_FEW_TOKENS), ("lx_token_scores_max_top", TOP_MAX)):
+    for name, here in (("lx_step_tables_max_seqs", STEP_SEQS_MAX), ("lx_moe_few_max_tokens", MOE_FEW_TOKENS), ("lx_token_scores_max_top", TOP_MAX)):
         if getattr(lib, name)() != here:
             raise nv.NativeError(f"{name}: C++ says {getattr(lib, name)()}, Python says {here}")
 

@@ -202,3 +202,14 @@ def test_kernels_refuse_tensors_that_are_on_no_device():
                  lambda: native.step_tables(ints([3], [0], [-1], [1]), ints(5), 3, 2, 32)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+# ------------------------------------------------------------------------------------------------ bindings
+@pytest.mark.parametrize("name", ["STEP_SEQS_MAX", "MOE_FEW_TOKENS", "TOP_MAX"])
+def test_limits_that_drift_apart_are_found_when_the_library_is_loaded(monkeypatch, name):
+    from lorax_b200.ops import native_steps
+    lib = native.load()
+    native_steps.check_limits(lib)
+    monkeypatch.setattr(native_steps, name, getattr(reference, name) + 1)
+    with pytest.raises(native.NativeError, match="Python says"):
+        native_steps.check_limits(lib)
