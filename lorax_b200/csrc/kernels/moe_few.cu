@@ -882,7 +882,7 @@ int lx_moe_few_down_stages(int T, int H, int I, int most, int num_sms) {
   return FewDownStage(mt, nt, I, rows, few_blocks(I / 64, steps * kFewMath / 2), few_copies(most, shift), shift).stages;
 }
 
-// `logits` [T, E] and `h` [2, T k, I] are scratch of the call.
+// -> kernels launched, or an error below zero.  `logits` [T, E] and `h` [2, T k, I] are scratch of the call.
 int lx_moe_few(const void* x, long long ldx, const void* wr, long long ldw, const void* w13, const void* w2, float* logits, void* h, void* out, long long ldo, int T,
                int E, int k, int e0, int e_local, int H, int I, int act, int renorm, float scale, int* status, int num_sms, void* stream) {
   using namespace lx;
@@ -905,7 +905,8 @@ int lx_moe_few(const void* x, long long ldx, const void* wr, long long ldw, cons
   p.h = reinterpret_cast<__nv_bfloat16*>(h); p.out = reinterpret_cast<__nv_bfloat16*>(out); p.ldo = ldo;
   p.T = T; p.E = E; p.k = k; p.e0 = e0; p.e_local = e_local; p.H = H; p.I = I; p.act = act; p.renorm = renorm; p.scale = scale; p.status = status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return T <= 8 ? moe_few_launch<1>(p, num_sms, s) : moe_few_launch<2>(p, num_sms, s);
+  const int rc = T <= 8 ? moe_few_launch<1>(p, num_sms, s) : moe_few_launch<2>(p, num_sms, s);
+  return rc != 0 ? rc : by_itself ? 2 : 3;
 }
 
 }  // extern "C"

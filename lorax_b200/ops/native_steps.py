@@ -94,8 +94,8 @@ def moe_few(x: torch.Tensor, router_w: torch.Tensor, w13: torch.Tensor, w2: torc
     at, ws = scratch.data_ptr(), nv.workspace(x.device)
     rc = nv.load().lx_moe_few(x.data_ptr(), x.stride(0) if T > 1 else H, router_w.data_ptr(), router_w.stride(0) if E > 1 else H, w13.data_ptr(), w2.data_ptr(),
                               at + h_bytes, at, out.data_ptr(), out.stride(0), T, E, k, e0, w13.shape[0], H, inter, nv._ACTS[act], int(renorm), scale, ws.status.data_ptr(), ws.num_sms, stream)
-    nv._check(rc, "lx_moe_few")
-    nv.launch_count += 2                 # (three kernels)
+    nv._check(min(rc, 0), "lx_moe_few")
+    nv.launch_count += rc - 1            # (two or three)
     return out
 
 

@@ -213,3 +213,23 @@ def test_limits_that_drift_apart_are_found_when_the_library_is_loaded(monkeypatc
     monkeypatch.setattr(native_steps, name, getattr(reference, name) + 1)
     with pytest.raises(native.NativeError, match="Python says"):
         native_steps.check_limits(lib)
+
+
+@pytest.mark.parametrize("made", [2, 3])
+def test_the_launches_of_the_experts_are_counted_as_they_were_made(monkeypatch, made):
+    from lorax_b200.ops import native_steps
+
+    class Library:
+        def lx_moe_few(self, *a):
+            return made
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(native_steps.nv, "load", Library)
+    monkeypatch.setattr(native_steps.nv, "workspace", lambda d: type("", (), dict(status=torch.zeros(1), num_sms=148)))
+    before = native.launch_count
+    native.moe_few(**_moe_args())
+    assert native.launch_count - before == made
+    made = -5
+    with pytest.raises(native.NativeError, match="-5"):
+        native.moe_few(**_moe_args())

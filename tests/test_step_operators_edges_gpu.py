@@ -150,3 +150,12 @@ def test_tables_of_many_sequences_are_the_kernels(B, window):
     a, b = native.step_tables(seqs, pages, **args), reference.step_tables_of_many(seqs, pages, **args)
     for x, y in zip(a, b):
         assert all(torch.equal(p, q) for s, t in zip(x, y) for p, q in zip(s, t)) if isinstance(x, tuple) else torch.equal(x, y)
+
+
+@pytest.mark.parametrize("T,E,H,kernels", [(1, 8, 512, 2), (8, 8, 4096, 2), (9, 8, 4096, 3), (1, 64, 2048, 3)])
+def test_launches_of_small_and_of_large_routers(T, E, H, kernels):
+    a = _experts(T, E, 2, H, 64)
+    native.moe_few(*a, 2)
+    before = native.launch_count
+    native.moe_few(*a, 2)
+    assert native.launch_count - before == kernels
