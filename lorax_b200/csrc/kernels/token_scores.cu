@@ -560,6 +560,18 @@ __global__ void __launch_bounds__(kLeanThreads, 6) token_logprobs_kernel(const _
   if (tid == 0) score_row<CAP>(p, t, given, a, logf(a.s));
 }
 
+// SMs of the current device.
+static int score_sms() {
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (sms[dev] == 0) {
+    int n = 0;
+    sms[dev] = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
+  }
+  return sms[dev];
+}
+
 template <typename L>
 static int token_scores_launch(const TokenScoresParams& p, int T, int parts, cudaStream_t s) {
   void (*kernel)(TokenScoresParams);
@@ -585,9 +597,10 @@ int lx_token_scores(const void* logits, long long ld, int fp32, int T, int V, co
   // CTAs of a row: enough of them for two per SM, and at least one load per thread.  Without alternatives up to the six that an SM holds, of 16384 logits and
   // more (rows of 128256 bf16: 96 of them 12.4 -> 10.7 us, 200 19.7 -> 13.9, 440 24.4 -> 22.9; halves of 32000: 300 rows 7.6 -> 9.0).
   const int vec = fp32 ? 4 : 8;
+  const int sms = score_sms();
   int parts = 1;
-  while (parts < kScoreMaxParts && (long long)T * parts * 2 <= 2 * 148 && V >= parts * kScoreThreads * vec) parts *= 2;
-  if (k == 0) parts = std::max(parts, std::min({kScoreMaxParts, 6 * 148 / T, V / 16384}));
+  while (parts < kScoreMaxParts && (long long)T * parts * 2 <= 2 * sms && V >= parts * kScoreThreads * vec) parts *= 2;
+  if (k == 0) parts = std::max(parts, std::min({kScoreMaxParts, 6 * sms / T, V / 16384}));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return fp32 ? token_scores_launch<float>(p, T, parts, s) : token_scores_launch<__nv_bfloat16>(p, T, parts, s);
 }
