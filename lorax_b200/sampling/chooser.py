@@ -211,7 +211,7 @@ class HeterogeneousNextTokenChooser:
             s = get_ops(self.device).token_scores(scores, next_ids, k=self.max_alternatives, entropy=False)
             lp = s.logprobs
             if self.max_alternatives > 0:
-                alts = (s.top_ids, s.top_logprobs)
+                alts = (s.top_ids.long(), s.top_logprobs)
         else:                                    # (more alternatives than the kernel returns)
             logp = scores.log_softmax(-1)
             lp = logp.gather(1, next_ids[:, None])[:, 0]

@@ -160,6 +160,17 @@ def test_sampling_asks_for_no_entropy(monkeypatch):
     assert [kw.get("entropy") for kw in asked] == [False]
 
 
+@pytest.mark.parametrize("k", [1, reference.TOP_MAX, reference.TOP_MAX + 1])
+def test_alternatives_of_a_chooser_index_its_scores(k):
+    """Token ids as `topk` gave them, of one type however many there are."""
+    from lorax_b200.sampling.chooser import HeterogeneousNextTokenChooser, NextTokenParams
+    logits = torch.randn(2, 100, generator=torch.Generator().manual_seed(7))
+    c = HeterogeneousNextTokenChooser([NextTokenParams(return_k_alternatives=k), NextTokenParams()], "cpu", 100)
+    ids, _, (alt, lp) = c(None, None, logits.clone())
+    assert alt.dtype == ids.dtype == torch.int64
+    assert torch.allclose(torch.log_softmax(logits, -1).gather(1, alt), lp, atol=1e-6)
+
+
 # ------------------------------------------------------------------------------------------------ devices
 def test_operators_run_on_their_tensors_device_whichever_is_current(monkeypatch):
     """Tensors of a second device while the first is current: launches, with the second device's stream, while it is the current one."""
