@@ -280,9 +280,9 @@ LX_DEVICE int few_token(uint32_t mask, int i) {
 }
 
 // Feature `row` of token t from the experts that serve it alone, by one warp.  A column of the down product has zeros where an expert does not serve its token, and
-// an h that one bf16 term holds has a remainder of zero: times a weight that is infinite or no number, both are NaN.  Sums that are not finite are formed again here,
-// unless the token's own weights are NaN.  (Not inlined: no call of finite numbers comes by.)
-__device__ __noinline__ float few_alone(const FewPlan& plan, const MoeFewParams& p, int t, int row) {
+// an h that one bf16 term holds has a remainder of zero: times a weight that is infinite or no number, both are NaN.  Sums that are not finite are formed again by
+// this, unless the token's own weights are NaN.
+LX_DEVICE float few_alone(const FewPlan& plan, const MoeFewParams& p, int t, int row) {
   const int lane = threadIdx.x & 31;
   float sum = 0.f;
   for (int d = 0; d < plan.reached; ++d) {
@@ -316,13 +316,14 @@ struct FewRing {
   uint64_t full[kFewMaxStages], empty[kFewMaxStages];
   uint64_t sums[kFewSums], read[kFewSums];      // the math warps' sums of a tile: written, read
   int stop;
+  int odd;                                      // a result is not finite (down)
 };
 
 LX_DEVICE void few_ring_init(FewRing& r) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < kFewMaxStages; ++s) { mbar_init(&r.full[s], 1); mbar_init(&r.empty[s], kFewMath); }
     for (int s = 0; s < kFewSums; ++s) { mbar_init(&r.sums[s], kFewMath); mbar_init(&r.read[s], 1); }
-    r.stop = 0;
+    r.stop = r.odd = 0;
     mbar_fence_init();
   }
 }
@@ -760,17 +761,26 @@ __global__ void __launch_bounds__(kFewThreads, 1) moe_few_down_kernel(const __gr
 #pragma unroll
       for (int o = 0; o < 4; ++o) {              // (the row of lane group l / 4 and 8 behind it, tokens 2 (l % 4) and the next)
         const int t = n * 8 + (l & 3) * 2 + (o & 1), r = m * 16 + (o >> 1) * 8 + few_lane_row(l >> 2);
-        const bool live = t < p.T && r < rows && r0 + r < last;
-        float y = o == 0 ? v.x : o == 1 ? v.y : o == 2 ? v.z : v.w;
-        for (uint32_t odd = __ballot_sync(0xffffffffu, live && !(fabsf(y) < INFINITY)); odd != 0; odd &= odd - 1) {
-          const int from = __ffs(odd) - 1;
-          const float again = few_alone(plan, p, __shfl_sync(0xffffffffu, t, from), r0 + __shfl_sync(0xffffffffu, r, from));
-          if (lane == from) y = again;
+        const float y = o == 0 ? v.x : o == 1 ? v.y : o == 2 ? v.z : v.w;
+        if (t < p.T && r < rows && r0 + r < last) {
+          p.out[(long long)t * p.ldo + r0 + r] = __float2bfloat16(y);
+          if (!(fabsf(y) < INFINITY)) ring.odd = 1;
         }
-        if (live) p.out[(long long)t * p.ldo + r0 + r] = __float2bfloat16(y);
       }
     }
     few_math_sync();
+  }
+  // Results that are not finite, once more.  (Behind everything else: in the loop above, as a call, it cost the finite ones 2 % of narrow layers.)
+  if (ring.odd == 0) return;
+  for (int r0 = blockIdx.x * rows; r0 < p.H; r0 += gridDim.x * rows) {
+    const int n = min(rows, p.H - r0);
+    for (int i = warp; i < n * p.T; i += kFewMath) {
+      const int t = i / n, r = r0 + i % n;
+      __nv_bfloat16* out = p.out + (long long)t * p.ldo + r;
+      if (fabsf(__bfloat162float(*out)) < INFINITY) continue;
+      const float y = few_alone(plan, p, t, r);
+      if (lane == 0) *out = __float2bfloat16(y);
+    }
   }
 }
 
