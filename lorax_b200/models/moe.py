@@ -11,7 +11,8 @@ gather, a grouped tcgen05 GEMM over (expert, feature tile, token tile) work item
 for w2 and the weighted combine.  Only the k experts of a token do work for it, every count stays on the device and every
 launch has static shapes, so a decode step with experts is captured in a CUDA graph like a dense one.
 
-Steps of up to sixteen tokens take `moe_few` (`csrc/kernels/moe_few.cu`): routing, both products and the combine in two launches.
+Steps of up to sixteen tokens on wide layers, of up to eight on narrower ones (`few_tokens`), take `moe_few` (`csrc/kernels/moe_few.cu`): routing, both products and
+the combine in two launches, in three with a router and tokens of more than 128 KB.
 
 Elsewhere (CPU, packed / quantised experts) two PyTorch shapes remain:
   * decode-sized batches: every local expert runs over all tokens and the routing weight (zero for unrouted tokens)
@@ -28,13 +29,19 @@ from ..ops.reference import MOE_FEW_TOKENS
 DENSE_MAX_TOKENS = 256
 
 
-def few_tokens(T: int, k: int, experts: int, hidden: int) -> bool:
+def few_tokens(T: int, k: int, experts: int, hidden: int, features: int = 0) -> bool:
     """Whether a layer takes `moe_few` instead of `moe_ffn`: up to its 16 tokens on wide layers; up to eight on narrower ones, and on narrow ones if they
-    reach few experts, since turns of short rows then cost more than their bytes.  Measured (us, `moe_ffn` / `moe_few`): 8 experts of 4096 x 14336,
-    two a token: 179 / 107 for one token, 463 / 399 for 16; 64 of 2048 x 1024, eight a token: 54 / 28 and 155 / 128; 128 of 2048 x 192: 46 / 19 and 78 / 76;
-    64 of 1024 x 1408, six a token: 39 / 24 for one, 75 / 74 for eight, 94 / 115 for 16; 32 of 512 x 2048, four a token: 32 / 22 for one, 37 / 34 for
-    three, 43 / 53 for six; 8 of 512 x 8192, two a token: 61 / 29 for one, 75 / 75 for eight, 76 / 94 for 16."""
-    return T <= MOE_FEW_TOKENS and (hidden >= 2048 or (T <= 8 and (hidden >= 1024 or min(experts, T * k) <= 12)))
+    reach few experts, since turns of short rows then cost more than their bytes, and on the narrowest few features in all (90000, by the experts that tokens
+    reach on average).  Measured (us, `moe_ffn` / `moe_few`): 8 experts of 4096 x 14336,
+    two a token: 178 / 106 for one token, 466 / 408 for 16; 64 of 2048 x 1024, eight a token: 53 / 28 and 155 / 128; 128 of 2048 x 192: 46 / 19 and 77 / 74;
+    64 of 1024 x 1408, six a token: 39 / 25 for one, 77 / 77 for eight, 94 / 115 for 16; 32 of 512 x 2048, four a token: 32 / 22 for one, 38 / 38 for
+    three, 43 / 53 for six; 8 of 512 x 8192, two a token: 61 / 30 for one, 73 / 67 for eight, 76 / 94 for 16; of 512 x 14336: 104 / 83 for four, 115 / 120 for
+    eight; nine of nine of 512 x 10752: 101 / 110 for one.  (All 16 tokens at the same experts can be 2 % behind: two of 9472 x 8192 203 / 207.)"""
+    if T > MOE_FEW_TOKENS or hidden >= 2048:
+        return T <= MOE_FEW_TOKENS
+    if T > 8 or hidden >= 1024:
+        return T <= 8
+    return min(experts, T * k) <= 12 and (hidden >= 768 or experts * (1 - (1 - k / experts) ** T) * features <= 90000)
 
 
 def route(router_logits: torch.Tensor, k: int):
@@ -57,7 +64,7 @@ def moe_forward(model, x: torch.Tensor, lw, li: int, inp) -> torch.Tensor:
     if (x.is_cuda and x.dtype == torch.bfloat16 and isinstance(lw.experts_w13, torch.Tensor) and isinstance(lw.experts_w2, torch.Tensor)
             and lw.experts_w13.dtype == torch.bfloat16 and lw.experts_w13.shape[1] % 128 == 0 and lw.experts_w2.shape[1] % 128 == 0
             and model.hidden % 8 == 0 and c.intermediate_size % 8 == 0 and E <= 256 and c.num_experts_per_tok <= 32 and hasattr(ops, "moe_ffn")):
-        ffn = ops.moe_few if few_tokens(T, c.num_experts_per_tok, E, model.hidden) else ops.moe_ffn
+        ffn = ops.moe_few if few_tokens(T, c.num_experts_per_tok, E, model.hidden, c.intermediate_size) else ops.moe_ffn
         out = ffn(x, lw.router_w.to(torch.bfloat16) if lw.router_w.dtype != torch.bfloat16 else lw.router_w, lw.experts_w13,
                   lw.experts_w2, c.num_experts_per_tok, e0, c.hidden_act)
         if ws > 1 and e_local < E:

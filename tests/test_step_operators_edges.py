@@ -109,6 +109,13 @@ def test_a_token_with_a_logit_that_is_no_number_has_no_weights(renorm):
     assert got[1].isnan().all() and torch.allclose(got[[0, 2]], clean)
 
 
+def test_the_narrowest_layers_take_the_operator_for_a_few_tokens_by_their_features_too():
+    from lorax_b200.models.moe import few_tokens
+    assert few_tokens(1, 2, 8, 512, 14336) and few_tokens(4, 2, 8, 512, 14336) and not few_tokens(8, 2, 8, 512, 14336) and few_tokens(8, 2, 8, 512, 8192)
+    assert not few_tokens(1, 9, 9, 512, 10752) and few_tokens(1, 9, 9, 768, 10752) and few_tokens(16, 9, 9, 2048, 10752)
+    assert few_tokens(3, 4, 32, 512, 2048) and not few_tokens(4, 4, 32, 512, 2048) and not few_tokens(9, 2, 8, 1024, 64)
+
+
 def test_the_ring_of_a_few_tokens_experts_has_more_than_one_stage():
     """With one stage its copies and its products take turns: no width, features or number of an expert's tokens may leave just that."""
     lib = native.load()
