@@ -6,7 +6,7 @@
 //
 // One pass over the row with running m, s, u (a thread rescales its sums when its maximum grows), joined over lanes, warps and, where the rows
 // alone do not fill the GPU, the CTAs of a cluster that share a row.  The sums are fp32: a thread adds some hundred terms of at most one, the
-// rest is a tree.  A logit of -inf adds nothing; a row of nothing else, one with a NaN and one with +inf have no distribution and score NaN.
+// rest is a tree.  Exponentials are the approximate ones (ex2.approx, __expf: within about 2^-22), logarithms and the cap's tanh are full.  A logit of -inf adds nothing; a row of nothing else, one with a NaN and one with +inf have no distribution and score NaN.
 //
 // The k best: of 64 groups of threads, each has a best element; the k-th best of those, by (value, index), is a lower bound of the row's k-th
 // best, so only threads whose own best is at or above it can hold any (k 64 / (64 - k) or so of 512).  Their elements are read again (from L2),

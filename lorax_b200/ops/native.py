@@ -675,7 +675,8 @@ def advance_decode(input_ids, next_ids, positions, ctx_lens, slots, block_tables
 
 
 def prefill_metadata(cu_q: torch.Tensor, cache_lens: torch.Tensor, seq_slot: torch.Tensor, block_tables: torch.Tensor, page: int, T: int):
-    """Per-token (positions, slots, adapter slot) of a ragged prefill from its per-sequence description, on the device."""
+    """Per-token (positions, slots, adapter slot) of a ragged prefill from its per-sequence description, on the device: for callers with padded block tables
+    at hand.  (The runner's steps take `step_tables`, which makes the tables too.)"""
     dev = cu_q.device
     out = torch.empty(3, T, dtype=torch.int32, device=dev)
     rc = load().lx_prefill_metadata(_ptr(cu_q), _ptr(cache_lens), _ptr(seq_slot), _ptr(block_tables), block_tables.shape[1], cache_lens.shape[0],
