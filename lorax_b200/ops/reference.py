@@ -1084,13 +1084,12 @@ MOE_FEW_ACTS = ("silu", "swish", "gelu", "gelu_new", "gelu_pytorch_tanh", "gelu_
 
 
 def _share_memory(a, b) -> bool:
-    """Whether any row of one tensor (rows along the last dimension, without gaps in it) lies on a row of the other.  Rows that take turns do not."""
+    """Whether any row of one tensor lies on a row of the other (contiguous tensors, or matrices whose rows have no gaps).  Rows that take turns do not."""
     def rows(t):
-        t = t.detach()
+        at, size = t.data_ptr(), t.element_size()
         if t.is_contiguous():
-            return [(t.data_ptr(), t.numel() * t.element_size())]
-        t = t.reshape(1, -1) if t.dim() < 2 else t
-        return [(t[i].data_ptr(), t.shape[1] * t.element_size()) for i in range(t.shape[0])]
+            return [(at, t.numel() * size)]
+        return [(at + i * t.stride(0) * size, t.shape[1] * size) for i in range(t.shape[0])]
     if not a.numel() or not b.numel():
         return False
     ra, rb = rows(a), rows(b)
