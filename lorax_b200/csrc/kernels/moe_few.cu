@@ -89,8 +89,8 @@ LX_DEVICE float few_act(float x, int act) {
     case kFewSilu: return x / (1.f + expf(-x));
     case kFewGelu: return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
     case kFewGeluTanh: return 0.5f * x * (1.f + tanhf(0.79788456080286536f * (x + 0.044715f * x * x * x)));
-    case kFewRelu: return fmaxf(x, 0.f);
-    default: { const float r = fmaxf(x, 0.f); return r * r; }
+    case kFewRelu: return x < 0.f ? 0.f : x;      // (a NaN stays)
+    default: { const float r = x < 0.f ? 0.f : x; return r * r; }
   }
 }
 

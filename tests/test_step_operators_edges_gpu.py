@@ -73,6 +73,20 @@ def test_an_expert_without_numbers_spoils_its_own_tokens_only(T, E, k, H, I, val
     native.workspace().check_status()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu", "relu2"])
+@pytest.mark.parametrize("where", ["gate", "up"])
+def test_a_token_of_an_expert_with_a_nan_in_front_of_its_activation_has_no_result(act, where):
+    x, wr, w13, w2 = _experts(6, 8, 2, 512, 256, seed=9)
+    ids = _routes(x, wr, 2)
+    e = _one_expert(ids)
+    bad = w13.clone()
+    bad[e, 7 if where == "gate" else 263, 30] = NAN
+    got, clean = native.moe_few(x, wr, bad, w2, 2, act=act), native.moe_few(x, wr, w13, w2, 2, act=act)
+    plain = reference.moe_few(x.cpu(), wr.cpu(), bad.cpu(), w2.cpu(), 2, act=act)
+    for t in range(6):
+        assert got[t].isnan().all() and plain[t].isnan().all() if e in ids[t] else torch.equal(got[t], clean[t])
+
+
 @pytest.mark.parametrize("T,E,k,H,I", SHAPES + [(4, 4, 4, 64, 40)])
 @pytest.mark.parametrize("renorm", [True, False])
 def test_a_router_row_without_numbers(T, E, k, H, I, renorm):
