@@ -123,6 +123,8 @@ def load() -> ctypes.CDLL:
     sigs.update(native_mixers.SIGNATURES)
     from . import native_steps
     sigs.update(native_steps.SIGNATURES)
+    from . import native_int8
+    sigs.update(native_int8.SIGNATURES)
     for name, (argtypes, restype) in sigs.items():
         fn = getattr(lib, name, None)
         if fn is None:
@@ -133,6 +135,7 @@ def load() -> ctypes.CDLL:
         fn.restype = restype
     native_mixers.check_layouts(lib)
     native_steps.check_limits(lib)
+    native_int8.check_limits(lib)
     for name, st in (("lx_moe_select_bytes", MoeSelectParams), ("lx_moe_place_bytes", MoePlaceParams)):
         if getattr(lib, name)() != ctypes.sizeof(st):
             raise NativeError(f"{name}: C++ says {getattr(lib, name)()} bytes, ctypes says {ctypes.sizeof(st)}")
@@ -852,6 +855,7 @@ from .native_mixers import (causal_conv, conv_rope_kvwrite, embed_stream, gate_n
 
 # ------------------------------------------------------------------------------------------------ short ragged steps
 from .native_steps import moe_few, step_tables, token_scores  # noqa: E402
+from .native_int8 import act_mul_int8, gemm_int8, norm_block, quant_rows_int8  # noqa: E402
 
 # ------------------------------------------------------------------------------------------------ per-op timing
 _TIMED_OPS = ("gemm", "gemm_fp8", "norm_residual", "rope_kvwrite", "act_mul", "embed", "argmax_logprob", "advance_decode", "attn_decode",

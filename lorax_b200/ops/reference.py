@@ -1211,3 +1211,225 @@ def token_scores(logits, targets=None, k: int = 0, softcap: float = 0.0, entropy
         got = lp.gather(1, at.clamp(0, V - 1)[:, None])[:, 0].masked_fill(~ok, float("nan"))
     ids = _best(raw, k) if k > 0 and T > 0 else torch.empty(T, k, dtype=torch.long, device=logits.device)
     return TokenScores(got, ent, ids.to(torch.int32), lp.gather(1, ids))
+
+
+# ------------------------------------------------------------------------------------------------ layers in 8-bit integers
+INT8_MAX_K = 1 << 17               # products whose sums stay below 2^31
+NORM_BLOCK_MAX_WIDTH = 16384
+ROWS_INT8_MAX = 1 << 30            # values of a row
+INT8_ACTS = ("silu", "swish", "gelu", "gelu_new", "gelu_pytorch_tanh", "gelu_fast", "gelu_tanh", "relu", "relu2")
+
+
+class Int8Rows(NamedTuple):
+    """Rows in 8-bit integers: row t stands for q[t] * scale[t]."""
+    q: torch.Tensor                # [T, K] int8, rows 16 bytes apart or a multiple of that
+    scale: torch.Tensor            # [T] fp32
+
+
+def empty_int8_rows(T: int, K: int, device) -> Int8Rows:
+    return Int8Rows(torch.empty(T, (K + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :K], torch.empty(T, dtype=torch.float32, device=device))
+
+
+def _to_int8_rows(v) -> Int8Rows:
+    """scale = max |v| / 127 in 32 bits, q = v / scale to the nearest integer (ties to the even one).  A row whose largest magnitude is not finite has a NaN for
+    its scale; where the scale is zero, as for a row of zeros, and where it is a NaN, q is zero."""
+    top = v.abs().amax(1) if v.shape[1] else v.new_zeros(v.shape[0])
+    scale = torch.where(top.isfinite(), top / torch.full_like(top, 127.0), torch.full_like(top, float("nan")))      # (a division, not a product)
+    some = (scale > 0)[:, None]
+    q = torch.where(some, v.double() / torch.where(some, scale[:, None], 1.0).double(), 0.0)      # (64 bits: which of two integers is nearer)
+    r = empty_int8_rows(*v.shape, v.device)
+    r.q.copy_(q.round().clamp(-127, 127))
+    r.scale.copy_(scale)
+    return r
+
+
+def quantize_weight_int8(w: torch.Tensor):
+    """[N, K] -> (int8 [N, K], rows 16 bytes apart or a multiple of that; fp32 [N]): the weights of `gemm_int8`, a scale for each output channel."""
+    parts = [_to_int8_rows(p.float()) for p in w.split(max(1, (1 << 26) // max(1, w.shape[1])))]
+    if len(parts) == 1:
+        return tuple(parts[0])
+    whole = empty_int8_rows(*w.shape, w.device)
+    at = 0
+    for p in parts:
+        n = p.q.shape[0]
+        whole.q[at:at + n].copy_(p.q)
+        whole.scale[at:at + n].copy_(p.scale)
+        at += n
+    return tuple(whole)
+
+
+def _span(t):
+    """First byte, bytes of a row, bytes between two rows, rows."""
+    size = t.element_size()
+    if t.dim() < 2 or t.shape[0] == 1 or t.is_contiguous():
+        return t.data_ptr(), t.numel() * size, t.numel() * size, 1
+    return t.data_ptr(), t.shape[1] * size, t.stride(0) * size, t.shape[0]
+
+
+def _apart(a, b) -> bool:
+    """Whether no byte of one tensor (rows without gaps in them) is one of the other's, as far as their strides say: rows of the same distance may take turns, others
+    have to lie one tensor behind the other."""
+    if a is None or b is None or not a.numel() or not b.numel():
+        return True
+    (pa, na, sa, ra), (pb, nb, sb, rb) = _span(a), _span(b)
+    if pa + sa * (ra - 1) + na <= pb or pb + sb * (rb - 1) + nb <= pa:
+        return True
+    if sa != sb or ra == 1 or rb == 1:
+        return False
+    d = (pb - pa) % sa
+    return d >= na and sa - d >= nb
+
+
+def _same(a, b) -> bool:
+    return b is not None and a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
+
+
+def _rows_fit(t, T: int, n: int) -> bool:
+    return t.dim() == 2 and t.shape == (T, n) and (n <= 1 or t.stride(1) == 1) and (T <= 1 or t.stride(0) >= n)
+
+
+def check_quant_rows_int8(x):
+    if not (isinstance(x, torch.Tensor) and x.dim() == 2 and x.is_floating_point()):
+        raise ValueError("quant_rows_int8: x [T, K] of numbers")
+    T, K = x.shape
+    if not (1 <= K <= ROWS_INT8_MAX and _rows_fit(x, T, K)):
+        raise ValueError(f"quant_rows_int8: rows of 1 to {ROWS_INT8_MAX} neighbouring values; got {tuple(x.shape)}, strides {x.stride()}")
+    return T, K
+
+
+def quant_rows_int8(x) -> Int8Rows:
+    """Rows x [T, K] in 8-bit integers, with a scale for each row (`_to_int8_rows` states the numbers)."""
+    check_quant_rows_int8(x)
+    return _to_int8_rows(x.float())
+
+
+def check_act_mul_int8(x, inter, act, gated, out):
+    if not (isinstance(x, torch.Tensor) and x.dim() == 2 and x.is_floating_point()):
+        raise ValueError("act_mul_int8: x [T, gate and up] of numbers")
+    T, n = x.shape[0], inter * (2 if gated else 1)
+    if not (1 <= inter <= ROWS_INT8_MAX // 2 and x.shape[1] == n and _rows_fit(x, T, n)):
+        raise ValueError(f"act_mul_int8: rows of {n} neighbouring values; got {tuple(x.shape)}, strides {x.stride()}")
+    if act not in INT8_ACTS:
+        raise ValueError(f"act_mul_int8: activation {act!r}")
+    if out is not None and not (out.dtype == x.dtype and out.device == x.device and _rows_fit(out, T, inter) and _apart(out, x)):
+        raise ValueError("act_mul_int8: out [T, features] is of x's type and device, and lies apart from it")
+    return T
+
+
+def act_mul_int8(x, inter: int, act: str = "silu", gated: bool = True, out=None) -> Int8Rows:
+    """act(gate) * up of rows [gate | up], or act(gate), in 8-bit integers with a scale for each row.  `out` [T, inter] takes the values themselves, rounded to x's
+    type."""
+    check_act_mul_int8(x, inter, act, gated, out)
+    v = _act(x[:, :inter].float(), act)
+    if gated:
+        v = v * x[:, inter:].float()
+    if out is not None:
+        out.copy_(v)
+    return _to_int8_rows(v)
+
+
+def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8):
+    """-> (T, H, gate as [T, H] or None, what h is written to or None)."""
+    if not (isinstance(residual, torch.Tensor) and residual.dim() == 2 and residual.is_floating_point()):
+        raise ValueError("norm_block: residual [T, H] of numbers")
+    T, H = residual.shape
+    if not 1 <= H <= NORM_BLOCK_MAX_WIDTH:
+        raise ValueError(f"norm_block: rows of 1 to {NORM_BLOCK_MAX_WIDTH} values; got {H}")
+    rows = {"y": y, "residual": residual, "residual_out": residual_out, "out": out}
+    for name, t in rows.items():
+        if t is not None and not (t.dtype == residual.dtype and t.device == residual.device and _rows_fit(t, T, H)):
+            raise ValueError(f"norm_block: {name} is [T, H] with neighbouring values in a row, of the residual's type and device")
+    if y is None and not (post_weight is None and gate is None and scale == 1.0 and residual_out is None):
+        raise ValueError("norm_block: without y there is nothing to norm, gate, scale or write back")
+    if post_bias is not None and post_weight is None:
+        raise ValueError("norm_block: post_bias without post_weight")
+    vectors = {"weight": weight, "post_weight": post_weight, "bias": bias, "post_bias": post_bias}
+    for name, t in vectors.items():
+        if t is None and name != "weight":
+            continue
+        if not (isinstance(t, torch.Tensor) and t.shape == (H,) and t.is_contiguous() and t.dtype == residual.dtype and t.device == residual.device):
+            raise ValueError(f"norm_block: {name} is [H], contiguous, of the residual's type and device")
+    given = gate
+    if gate is not None:
+        if not (gate.dtype == residual.dtype and gate.device == residual.device and gate.dim() <= 2):
+            raise ValueError("norm_block: gate is of the residual's type and device")
+        try:
+            gate = gate.expand(T, H)
+        except RuntimeError:
+            raise ValueError(f"norm_block: a gate of {tuple(gate.shape)} for rows of {(T, H)}: one, [H], [T, 1] or [T, H]") from None
+    to = None if y is None else residual if residual_out is None else residual_out
+    for name, t in (("residual_out", to), ("out", out)):
+        if t is None:
+            continue
+        # a row's values are read before they are written, at the same places
+        if not (all(_apart(t, v) for v in vectors.values()) and all(_same(t, v) or _apart(t, v) for v in (y, residual))
+                and _apart(t, given)):
+            raise ValueError(f"norm_block: {name} lies apart from the inputs, or is y or the residual itself")
+    if gate is not None and H > 1 and T > 0 and gate.stride(1) not in (0, 1):
+        raise ValueError("norm_block: a row's gates are neighbours, or one for all")
+    if to is not None and out is not None and not _apart(to, out):
+        raise ValueError("norm_block: out and the residual lie apart")
+    return T, H, gate, to
+
+
+def norm_block(y, residual, weight, eps, post_weight=None, gate=None, scale: float = 1.0, bias=None, post_bias=None, weight_offset: float = 0.0,
+               layernorm: bool = False, residual_out=None, out=None, int8: bool = False):
+    """Norms on both sides of a block: h = residual + scale * gate * N_post(y), written over the residual (or to `residual_out`) in its type, and N(h), of h as it
+    was written.  N is the RMS norm, or the layer norm, times (weight + weight_offset), plus the bias; N_post is left out without a `post_weight`, h is the residual
+    without y.  `gate` is one value, [H], [T, 1] or [T, H].  Returns N(h) in the residual's type (in `out` where given), or with `int8` as `Int8Rows` made from the
+    32-bit values, and then writes `out` too where it is given."""
+    T, H, gate, to = check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
+
+    def norm(v, w, b):
+        if layernorm:
+            v = v - v.mean(1, keepdim=True)
+        v = v * torch.rsqrt((v * v).mean(1, keepdim=True) + eps) * (w.float() + weight_offset)
+        return v if b is None else v + b.float()
+    h = residual
+    if y is not None:
+        v = y.float() if post_weight is None else norm(y.float(), post_weight, post_bias)
+        if gate is not None:
+            v = v * gate.float()
+        h = (residual.float() + scale * v).to(residual.dtype)
+        to.copy_(h)
+    x = norm(h.float(), weight, bias)
+    if out is not None:
+        out.copy_(x)
+    if int8:
+        return _to_int8_rows(x)
+    return x.to(residual.dtype) if out is None else out
+
+
+def check_gemm_int8(x, w, w_scale, bias, out, dtype):
+    """-> (T, N, K)."""
+    if not isinstance(x, Int8Rows):
+        raise ValueError("gemm_int8: x is the Int8Rows of a quantiser")
+    q, scale = x
+    if not (q.dim() == 2 and w.dim() == 2 and q.dtype == w.dtype == torch.int8 and q.shape[1] == w.shape[1]):
+        raise ValueError(f"gemm_int8: int8 rows [T, K] and weights [N, K]; got {tuple(q.shape)} {q.dtype}, {tuple(w.shape)} {w.dtype}")
+    (T, K), N = q.shape, w.shape[0]
+    if not (1 <= K <= INT8_MAX_K):
+        raise ValueError(f"gemm_int8: K from 1 to {INT8_MAX_K}, whose sums stay whole; got {K}")
+    for name, t, n in (("rows", q, T), ("weights", w, N)):
+        if not ((K == 1 or t.stride(1) == 1) and (n <= 1 or (t.stride(0) >= K and t.stride(0) % 16 == 0)) and (n == 0 or t.data_ptr() % 16 == 0)):
+            raise ValueError(f"gemm_int8: {name} begin at 16 bytes and lie a multiple of 16 bytes apart; got strides {t.stride()}")
+    for name, t, n in (("the rows' scales", scale, T), ("w_scale", w_scale, N)):
+        if not (t.shape == (n,) and t.dtype == torch.float32 and t.is_contiguous() and t.device == q.device):
+            raise ValueError(f"gemm_int8: {name} are [{n}] fp32 on the rows' device")
+    if not (w.device == q.device and (bias is None or (bias.shape == (N,) and bias.dtype == dtype and bias.is_contiguous() and bias.device == q.device))):
+        raise ValueError(f"gemm_int8: weights and bias [{N}] {dtype} on the rows' device")
+    if out is not None and not (out.dtype == dtype and out.device == q.device and _rows_fit(out, T, N) and all(_apart(out, t) for t in (q, scale, w, w_scale, bias))):
+        raise ValueError(f"gemm_int8: out is [T, N] {dtype} on the rows' device, apart from the inputs")
+    return T, N, K
+
+
+def gemm_int8(x: Int8Rows, w, w_scale, bias=None, out=None, lora=None, dtype=torch.bfloat16, w_const: bool = False):
+    """out[t, n] = (sum over k of x.q[t, k] * w[n, k]) * w_scale[n] * x.scale[t] + bias[n]: the sums whole, the rest in 32 bits, one rounding to `dtype`."""
+    T, N, K = check_gemm_int8(x, w, w_scale, bias, out, dtype)
+    y = (x.q.double() @ w.double().t()).float() * w_scale * x.scale[:, None]
+    if bias is not None:
+        y = y + bias.float()
+    if out is None:
+        return y.to(dtype)
+    out.copy_(y)
+    return out

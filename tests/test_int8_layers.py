@@ -1,0 +1,205 @@
+"""Operators of layers in 8-bit integers on the CPU: what they compute, and what they refuse in front of any launch."""
+import pytest
+import torch
+
+from lorax_b200.ops import reference as ref
+from lorax_b200.ops.reference import Int8Rows
+
+BF = torch.bfloat16
+
+
+def _ops():
+    """The plain forms and the bindings: both check their arguments in the same way (the bindings raise before they look for a device)."""
+    from lorax_b200.ops import native
+    return (ref, native)
+
+
+def test_rows_are_rounded_to_the_nearest_step():
+    x = torch.randn(17, 259, generator=torch.Generator().manual_seed(1)) * 3
+    r = ref.quant_rows_int8(x)
+    assert r.q.dtype == torch.int8 and r.q.stride(0) == 272 and r.scale.dtype == torch.float32
+    top = x.abs().amax(1)
+    assert torch.equal(r.scale, top / torch.full_like(top, 127.0))
+    back = r.q.double() * r.scale.double()[:, None]
+    assert ((back - x.double()).abs() <= 0.5 * r.scale.double()[:, None] * (1 + 2 ** -20)).all()
+    assert (r.q.int().abs().amax(1) == 127).all()
+
+
+def test_ties_go_to_the_even_integer_and_neighbours_of_ties_do_not():
+    """A row whose scale is 1: halves are ties, and the numbers beside them are not."""
+    up = torch.nextafter(torch.tensor(2.5), torch.tensor(9.0))
+    x = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, up.item(), 126.5, -126.5]])
+    assert ref.quant_rows_int8(x).q.tolist() == [[127, 0, 2, 2, 0, -2, -2, 3, 126, -126]]
+
+
+def test_rows_without_a_scale():
+    x = torch.tensor([[0.0, -0.0, 0.0], [1.0, float("inf"), 2.0], [float("nan"), 1.0, 2.0], [3.0, 1.0, -3.0], [2.0 ** -149, 0.0, 0.0]])
+    r = ref.quant_rows_int8(x)
+    assert r.scale[0] == 0 and r.scale[1].isnan() and r.scale[2].isnan() and r.scale[4] == 0
+    assert r.q.tolist() == [[0, 0, 0], [0, 0, 0], [0, 0, 0], [127, 42, -127], [0, 0, 0]]
+    w, ws = ref.quantize_weight_int8(torch.randn(5, 3))
+    y = ref.gemm_int8(r, w, ws, bias=torch.ones(5), dtype=torch.float32)
+    assert (y[0] == 1).all() and y[1:3].isnan().all() and y[3:].isfinite().all()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu", "relu2"])
+@pytest.mark.parametrize("gated", [True, False])
+def test_activations(act, gated):
+    x = torch.randn(6, 2 * 33 if gated else 33, generator=torch.Generator().manual_seed(2))
+    out = torch.empty(6, 33)
+    r = ref.act_mul_int8(x, 33, act, gated, out=out)
+    assert torch.equal(out, ref.act_mul(x, 33, act, gated=gated))
+    s = ref.quant_rows_int8(out)
+    assert torch.equal(r.q, s.q) and torch.equal(r.scale, s.scale)
+
+
+@pytest.mark.parametrize("layernorm", [False, True])
+def test_a_norm_without_extras_is_norm_residual(layernorm):
+    g = torch.Generator().manual_seed(3)
+    y, res, w, b = torch.randn(4, 40, generator=g), torch.randn(4, 40, generator=g), torch.randn(40, generator=g), torch.randn(40, generator=g)
+    r0, r1 = res.clone(), res.clone()
+    a = ref.norm_residual(y, r0, w, 1e-5, bias=b, weight_offset=1.0, x_scale=0.22, layernorm=layernorm)
+    c = ref.norm_block(y, r1, w, 1e-5, bias=b, weight_offset=1.0, scale=0.22, layernorm=layernorm)
+    torch.testing.assert_close(c, a, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(r1, r0, rtol=1e-6, atol=1e-6)
+    assert torch.equal(ref.norm_block(None, res, w, 1e-5, layernorm=layernorm), ref.norm_residual(res, None, w, 1e-5, layernorm=layernorm)) or layernorm
+
+
+def test_gates_of_every_shape():
+    g = torch.Generator().manual_seed(4)
+    y, res, w, pw = torch.randn(5, 24, generator=g), torch.randn(5, 24, generator=g), torch.randn(24, generator=g), torch.randn(24, generator=g)
+    for gate in (torch.tensor(0.5), torch.tensor([0.5]), torch.randn(24, generator=g), torch.tensor([[1.0], [0.0], [1.0], [0.0], [0.0]]), torch.randn(5, 24, generator=g)):
+        h = torch.empty_like(res)
+        x = ref.norm_block(y, res, w, 1e-6, post_weight=pw, gate=gate, scale=0.5, residual_out=h)
+        n = y * torch.rsqrt((y * y).mean(1, keepdim=True) + 1e-6) * pw
+        torch.testing.assert_close(h, res + 0.5 * gate * n, rtol=1e-6, atol=1e-6)
+        torch.testing.assert_close(x, h * torch.rsqrt((h * h).mean(1, keepdim=True) + 1e-6) * w, rtol=1e-6, atol=1e-6)
+        if gate.dim() == 2 and gate.shape[1] == 1:
+            assert torch.equal(h[1], res[1])           # a token whose gate is shut keeps its stream
+    r = ref.norm_block(y, res.clone(), w, 1e-6, int8=True)
+    assert isinstance(r, Int8Rows) and torch.equal(r.q, ref.quant_rows_int8(ref.norm_block(y, res.clone(), w, 1e-6)).q)
+
+
+def test_products_are_whole():
+    g = torch.Generator().manual_seed(5)
+    q, w = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8) for s in ((3, 1 << 12), (7, 1 << 12)))
+    one = lambda n: torch.ones(n)
+    y = ref.gemm_int8(Int8Rows(q, one(3)), w, one(7), dtype=torch.float32)
+    assert torch.equal(y, (q.long() @ w.long().t()).float())
+
+
+def test_weights_in_pieces_are_those_in_one(monkeypatch):
+    w = torch.randn(300, 400, generator=torch.Generator().manual_seed(6))
+    whole = ref.quantize_weight_int8(w)
+    real = torch.Tensor.split
+    monkeypatch.setattr(torch.Tensor, "split", lambda t, n, dim=0: real(t, min(n, 77), dim))
+    parts = ref.quantize_weight_int8(w)
+    assert all(torch.equal(a, b) for a, b in zip(whole, parts)) and parts[0].stride() == whole[0].stride()
+
+
+def test_empty_calls():
+    w, ws = ref.quantize_weight_int8(torch.randn(5, 8))
+    r = ref.quant_rows_int8(torch.empty(0, 8))
+    assert ref.gemm_int8(r, w, ws).shape == (0, 5)
+    assert ref.norm_block(torch.empty(0, 8), torch.empty(0, 8), torch.ones(8), 1e-6).shape == (0, 8)
+    assert ref.act_mul_int8(torch.empty(0, 8), 4).q.shape == (0, 4)
+
+
+def _rows(T, K):
+    return ref.empty_int8_rows(T, K, "cpu")
+
+
+NORM = dict(y=torch.zeros(3, 16, dtype=BF), residual=torch.zeros(3, 16, dtype=BF), weight=torch.ones(16, dtype=BF), eps=1e-6)
+_BUF = torch.zeros(3, 64, dtype=BF)
+
+
+@pytest.mark.parametrize("change", [
+    dict(y=torch.zeros(2, 16, dtype=BF)), dict(y=torch.zeros(3, 16)), dict(residual=torch.zeros(16, dtype=BF)), dict(y=torch.zeros(16, 3, dtype=BF).t()),
+    dict(weight=torch.ones(8, dtype=BF)), dict(weight=torch.ones(16)), dict(weight=torch.ones(32, dtype=BF)[::2]), dict(weight=None),
+    dict(post_bias=torch.zeros(16, dtype=BF)), dict(post_weight=torch.ones(1, dtype=BF)), dict(gate=torch.ones(3, dtype=BF)), dict(gate=torch.ones(16)),
+    dict(gate=torch.ones(3, 32, dtype=BF)[:, ::2]), dict(gate=torch.ones(1, 1, 16, dtype=BF)), dict(y=None, scale=0.5), dict(y=None, gate=torch.ones(1, dtype=BF)),
+    dict(y=None, post_weight=torch.ones(16, dtype=BF)), dict(y=None, residual_out=torch.zeros(3, 16, dtype=BF)),
+    dict(y=_BUF[:, :16], residual=_BUF[:, 8:24]), dict(y=_BUF[:, :16], residual_out=_BUF[:, 8:24]), dict(residual_out=torch.zeros(3, 16)),
+    dict(residual=torch.zeros(2, 16385, dtype=BF), y=torch.zeros(2, 16385, dtype=BF), weight=torch.zeros(16385, dtype=BF)), dict(out=torch.zeros(3, 17, dtype=BF))])
+def test_norms_that_are_refused(change):
+    for ops in _ops():
+        with pytest.raises(ValueError, match="norm_block"):
+            ops.norm_block(**{**NORM, **change})
+
+
+def test_results_on_top_of_inputs():
+    """y and the residual may be written over, value by value; anything else may not, and rows of one buffer may take turns."""
+    buf = torch.zeros(3, 32, dtype=BF)
+    ok = [dict(out=NORM["y"]), dict(residual_out=NORM["y"]), dict(y=buf[:, :16], residual=buf[:, 16:]), dict(y=buf[:, :16], residual=buf[:, 16:], out=buf[:, :16])]
+    for change in ok:
+        ref.norm_block(**{**NORM, **change})
+    vec = torch.ones(48, dtype=BF)
+    bad = [dict(out=NORM["residual"]), dict(residual_out=vec.view(3, 16), weight=vec[:16]), dict(out=vec.view(3, 16), gate=vec[16:32]),
+           dict(out=vec[:48].view(3, 16), residual_out=vec[:48].view(3, 16)), dict(out=buf[:, :16], residual_out=buf[:, 8:24])]
+    for change in bad:
+        for ops in _ops():
+            with pytest.raises(ValueError, match="norm_block"):
+                ops.norm_block(**{**NORM, **change})
+
+
+GEMM = dict(x=_rows(3, 32), w=torch.zeros(5, 32, dtype=torch.int8), w_scale=torch.ones(5))
+
+
+@pytest.mark.parametrize("change", [
+    dict(x=torch.zeros(3, 32, dtype=torch.int8)), dict(x=_rows(3, 48)), dict(x=Int8Rows(torch.zeros(3, 32), torch.ones(3))), dict(x=Int8Rows(_rows(3, 32).q, torch.ones(4))),
+    dict(x=Int8Rows(torch.zeros(3, 40, dtype=torch.int8)[:, :32], torch.ones(3))), dict(x=Int8Rows(torch.zeros(3, 48, dtype=torch.int8)[:, 8:40], torch.ones(3))),
+    dict(x=Int8Rows(_rows(3, 32).q, torch.ones(3, dtype=torch.float64))), dict(w=torch.zeros(5, 32)), dict(w=torch.zeros(32, 5, dtype=torch.int8).t()),
+    dict(w_scale=torch.ones(5, 1)), dict(w_scale=torch.ones(10)[::2]), dict(bias=torch.ones(5)), dict(bias=torch.ones(4, dtype=BF)),
+    dict(out=torch.zeros(3, 6, dtype=BF)), dict(out=torch.zeros(3, 5)), dict(out=torch.zeros(5, 3, dtype=BF).t()), dict(x=_rows(3, 0), w=torch.zeros(5, 0, dtype=torch.int8)),
+    dict(x=_rows(1, (1 << 17) + 16), w=torch.zeros(1, (1 << 17) + 16, dtype=torch.int8), w_scale=torch.ones(1))])
+def test_products_that_are_refused(change):
+    for ops in _ops():
+        with pytest.raises(ValueError, match="gemm_int8"):
+            ops.gemm_int8(**{**GEMM, **change})
+
+
+def test_a_product_on_top_of_its_scales_is_refused():
+    x = Int8Rows(_rows(4, 32).q, torch.ones(4))
+    out = x.scale.view(BF)[:4].view(4, 1)
+    for ops in _ops():
+        with pytest.raises(ValueError, match="apart"):
+            ops.gemm_int8(x, torch.zeros(1, 32, dtype=torch.int8), torch.ones(1), out=out)
+
+
+@pytest.mark.parametrize("x", [torch.zeros(3, dtype=BF), torch.zeros(3, 0, dtype=BF), torch.zeros(8, 3, dtype=BF).t(), torch.zeros(1, 4, dtype=BF).expand(3, 4),
+                               torch.zeros(3, 4, dtype=torch.int32)])
+def test_rows_that_are_refused(x):
+    for ops in _ops():
+        with pytest.raises(ValueError, match="quant_rows_int8"):
+            ops.quant_rows_int8(x)
+
+
+def test_activations_that_are_refused():
+    x = torch.zeros(3, 16, dtype=BF)
+    for ops in _ops():
+        for args, kw in (((x, 7), {}), ((x, 8, "tanh"), {}), ((x, 0), {}), ((x, 8, "silu", False), {}), ((x[0], 8), {}), ((x, 8), dict(out=x[:, :8])),
+                         ((x, 8), dict(out=torch.zeros(3, 8))), ((x, 8), dict(out=torch.zeros(3, 9, dtype=BF)))):
+            with pytest.raises(ValueError, match="act_mul_int8"):
+                ops.act_mul_int8(*args, **kw)
+
+
+def test_the_bindings_take_bf16_on_a_gpu():
+    from lorax_b200.ops import native
+    for call in (lambda: native.quant_rows_int8(torch.zeros(3, 16)), lambda: native.act_mul_int8(torch.zeros(3, 16), 8),
+                 lambda: native.norm_block(torch.zeros(3, 16), torch.zeros(3, 16), torch.ones(16), 1e-6),
+                 lambda: native.gemm_int8(_rows(3, 32), torch.zeros(5, 32, dtype=torch.int8), torch.ones(5), dtype=torch.float32)):
+        with pytest.raises(ValueError, match="bf16"):
+            call()
+    for call in (lambda: native.quant_rows_int8(torch.zeros(3, 16, dtype=BF)), lambda: native.norm_block(**NORM), lambda: native.gemm_int8(**GEMM)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+def test_limits_of_the_library_and_of_python_agree(monkeypatch):
+    from lorax_b200.ops import native, native_int8
+    native_int8.check_limits(native.load())
+    for name in ("NORM_BLOCK_MAX_WIDTH", "INT8_MAX_K"):
+        monkeypatch.setattr(native_int8, name, getattr(ref, name) + 1)
+        with pytest.raises(native.NativeError, match="C\\+\\+ says"):
+            native_int8.check_limits(native.load())
+        monkeypatch.undo()

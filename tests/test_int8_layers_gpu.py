@@ -1,0 +1,353 @@
+"""Operators of layers in 8-bit integers on the GPU, against their definitions in 64 bits.
+
+Tolerances.  A result in bf16 is rounded once: 2^-8 of it.  What is computed in 32 bits loses some 2^-24 a step; the steps are counted beside each bound."""
+import pytest
+import torch
+
+from lorax_b200.ops import reference as ref
+from lorax_b200.ops.reference import Int8Rows
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+HALF, E = 2.0 ** -8, 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from lorax_b200.ops import native
+    native.load()
+    yield native
+    native.workspace().check_status()
+
+
+def _gen(*seed):
+    return torch.Generator(device="cuda").manual_seed(hash(seed) % (1 << 40))
+
+
+def _randn(g, *shape, dtype=BF, std=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+def _int8(g, rows, K, at=0):
+    """Random bytes; `at`: rows of a wider buffer that begin `at` bytes into it."""
+    wide = (K + at + 15) // 16 * 16
+    return torch.randint(-127, 128, (rows, wide), generator=g, device="cuda", dtype=torch.int8)[:, at:at + K]
+
+
+# ------------------------------------------------------------------------------------------------ rows
+def _check_rows(r, v, steps):
+    """`v`: the values in 64 bits, of which the kernel's differ by `steps` of 2^-24 of the row's largest at most."""
+    top = v.abs().amax(1)
+    assert ((r.scale.double() - top / 127).abs() <= top / 127 * (steps + 2) * E).all()
+    off = (r.q.double() * r.scale.double()[:, None] - v).abs()
+    assert (off <= r.scale.double()[:, None] * 0.5 * (1 + 4 * E) + top[:, None] * steps * E).all()
+    assert ((r.q.int().abs().amax(1) == 127) | (top == 0)).all()
+
+
+@pytest.mark.parametrize("T", [1, 3, 150, 1027])
+@pytest.mark.parametrize("K", [1, 7, 8, 64, 1021, 2048, 4096, 8200, 14336])
+def test_rows_equal_the_plain_form(ops, T, K):
+    x = _randn(_gen(T, K), T, K, std=3.0)
+    x[:, 0] = 127 * 2.0 ** -3                       # with scales of 2^-3 and quotients at halves in many rows
+    x[:, K // 2] = 2.5 * 2.0 ** -3
+    r, want = ops.quant_rows_int8(x), ref.quant_rows_int8(x.cpu())
+    assert torch.equal(r.scale.cpu(), want.scale) and torch.equal(r.q.cpu(), want.q)
+
+
+@pytest.mark.parametrize("T,K", [(2, 16392), (1, 40000), (149, 20001)])
+def test_rows_longer_than_a_block_holds(ops, T, K):
+    x = _randn(_gen(T, K), T, K)
+    r, want = ops.quant_rows_int8(x), ref.quant_rows_int8(x.cpu())
+    assert torch.equal(r.scale.cpu(), want.scale) and torch.equal(r.q.cpu(), want.q)
+
+
+@pytest.mark.parametrize("at,wide", [(0, 80), (1, 80), (8, 80), (3, 75)])
+def test_rows_of_a_wider_buffer(ops, at, wide):
+    x = _randn(_gen(at, wide), 40, wide)[:, at:at + 64]
+    r, want = ops.quant_rows_int8(x), ref.quant_rows_int8(x.cpu())
+    assert torch.equal(r.scale.cpu(), want.scale) and torch.equal(r.q.cpu(), want.q)
+
+
+@pytest.mark.parametrize("K", [24, 25])
+def test_rows_without_a_scale(ops, K):
+    x = _randn(_gen(K), 9, K)
+    x[0] = 0
+    x[1, 5] = float("inf")
+    x[2, 6] = float("-inf")
+    x[3, K - 1] = float("nan")
+    x[4] = 0
+    x[4, 3] = 2.0 ** -133                           # the least bf16
+    x[5] *= 2.0 ** -126
+    x[6] = torch.finfo(BF).max
+    x[7, 0] = torch.finfo(BF).min
+    r, want = ops.quant_rows_int8(x), ref.quant_rows_int8(x.cpu())
+    assert r.scale[1:4].isnan().all() and torch.equal(r.q.cpu(), want.q)
+    keep = [0, 4, 5, 6, 7, 8]
+    assert torch.equal(r.scale.cpu()[keep], want.scale[keep])
+    w, ws = ref.quantize_weight_int8(_randn(_gen(1), 33, K, dtype=torch.float32))
+    y = ops.gemm_int8(r, w, ws)
+    # (rows of the largest bf16 pass it where the sum of their products does, and nowhere else)
+    want = (r.q.double() @ w.double().t()) * r.scale.double()[:, None] * ws.double()
+    assert (y[0] == 0).all() and y[1:4].isnan().all() and torch.equal(y[keep].isfinite(), want[keep].to(BF).isfinite())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu", "relu2"])
+@pytest.mark.parametrize("T,I,gated", [(1, 14336, True), (5, 33, True), (200, 1000, True), (3, 17, False), (150, 512, False), (2, 20000, True)])
+def test_activations(ops, act, T, I, gated):
+    x = _randn(_gen(T, I), T, 2 * I if gated else I, std=2.0)
+    out = torch.full((T, I), 7.0, device="cuda", dtype=BF)
+    r = ops.act_mul_int8(x, I, act, gated, out=out)
+    v = ref._act(x[:, :I].double(), act)
+    if gated:
+        v = v * x[:, I:].double()
+    # of a value: exp within 2^-21 of itself for |x| below 10 or so, tanh and erf within some 2^-22 of 1, four roundings: 24 steps of the largest value
+    _check_rows(r, v, 24)
+    top = v.abs().amax(1, keepdim=True)
+    assert ((out.double() - v).abs() <= HALF * v.abs() + 24 * E * top).all()
+    assert torch.equal(ops.act_mul_int8(x, I, act, gated).q, r.q)
+
+
+def test_activations_keep_what_is_not_a_number(ops):
+    x = _randn(_gen(3), 4, 64)
+    x[1, 3] = float("nan")
+    x[2, 40] = float("inf")
+    for act in ("silu", "gelu", "gelu_tanh", "relu", "relu2"):
+        r = ops.act_mul_int8(x, 32, act)
+        assert r.scale.isfinite().tolist()[0::3] == [True, True] and r.scale[1].isnan(), act
+
+
+# ------------------------------------------------------------------------------------------------ norms
+def _norm64(v, w, b, eps, offset, layernorm):
+    if layernorm:
+        v = v - v.mean(1, keepdim=True)
+    r = (v * v).mean(1, keepdim=True).add(eps).rsqrt()
+    y = v * r * (w.double() + offset)
+    # 32-bit sums of a row's squares and values, a reciprocal root, three products: 64 steps of the largest normed value, and of the offset's mean
+    slack = 64 * E * ((v * r).abs().amax(1, keepdim=True) * (w.double().abs() + abs(offset)))
+    if b is not None:
+        y = y + b.double()
+        slack = slack + 2 * E * b.double().abs()
+    return y, slack
+
+
+def _check_norm(ops, T, H, post, gate, scale, layernorm, int8, bias=True, offset=0.0, eps=1e-5, at=0):
+    g = _gen(T, H, post, scale, layernorm)
+    wide = H + at
+    y, res = _randn(g, T, wide)[:, at:], _randn(g, T, wide, std=3.0)[:, at:]
+    w, pw = 1 + _randn(g, H, std=0.2), 1 + _randn(g, H, std=0.2)
+    b, pb = (_randn(g, H, std=0.3), _randn(g, H, std=0.3)) if bias else (None, None)
+    gates = dict(none=None, one=_randn(g, 1), zero=torch.tensor(0.0, device="cuda", dtype=BF), channel=_randn(g, H), token=_randn(g, T, 1), all=_randn(g, T, H))
+    gate = gates[gate]
+    h = torch.full((T, wide), 5.0, device="cuda", dtype=BF)[:, at:]
+    keep = res.clone()
+    kw = dict(post_weight=pw if post else None, gate=gate, scale=scale, bias=b, post_bias=pb if post else None, weight_offset=offset, layernorm=layernorm)
+    out = torch.full((T, H), 5.0, device="cuda", dtype=BF) if int8 == "both" else None
+    x = ops.norm_block(y, res, w, eps, residual_out=h, out=out, int8=bool(int8), **kw)
+    assert torch.equal(res, keep)
+    part, slack = (y.double(), 0.0) if not post else _norm64(y.double(), pw, kw["post_bias"], eps, offset, layernorm)
+    f = scale * (1.0 if gate is None else gate.double())
+    want = res.double() + f * part
+    assert ((h.double() - want).abs() <= HALF * want.abs() + torch.as_tensor(f, device="cuda").abs() * (slack + 4 * E * part.abs()) + 2 * E * want.abs()).all()
+    want, slack = _norm64(h.double(), w, b, eps, offset, layernorm)
+    if int8:
+        top = want.abs().amax(1)
+        assert ((x.scale.double() - top / 127).abs() <= slack.amax(1) / 127 + 4 * E * top / 127).all()
+        assert ((x.q.double() * x.scale.double()[:, None] - want).abs() <= x.scale.double()[:, None] * (0.5 + 2.0 ** -18) + 2 * slack.amax(1, keepdim=True)).all()
+    value = out if int8 == "both" else None if int8 else x
+    if value is not None:
+        assert ((value.double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
+    # in place, the same bits
+    again = ops.norm_block(y, res, w, eps, int8=bool(int8), **kw)
+    assert torch.equal(res, h) and (torch.equal(again.q, x.q) and torch.equal(again.scale, x.scale) if int8 else torch.equal(again, x))
+
+
+@pytest.mark.parametrize("T,H", [(1, 4096), (1, 1), (2, 7), (5, 8), (148, 1000), (149, 1000), (300, 2049), (3, 8192), (150, 8192), (2, 16384), (151, 16384), (2, 16383)])
+@pytest.mark.parametrize("layernorm", [False, True])
+@pytest.mark.parametrize("int8", [False, True])
+def test_norms(ops, T, H, layernorm, int8):
+    _check_norm(ops, T, H, True, "none", 1.0, layernorm, int8)
+
+
+@pytest.mark.parametrize("gate", ["none", "one", "zero", "channel", "token", "all"])
+@pytest.mark.parametrize("post,int8", [(True, "both"), (False, False)])
+@pytest.mark.parametrize("H", [512, 333])
+def test_gates(ops, gate, post, int8, H):
+    _check_norm(ops, 37, H, post, gate, 0.22, False, int8, bias=False, offset=1.0)
+
+
+@pytest.mark.parametrize("at", [1, 8])
+def test_norms_of_rows_that_begin_inside_a_buffer(ops, at):
+    _check_norm(ops, 200, 256, True, "channel", 1.0, True, True, at=at)
+
+
+@pytest.mark.parametrize("H", [64, 65])
+def test_rows_of_zeros_and_numbers_that_are_not_finite_stay_in_their_rows(ops, H):
+    g = _gen(H)
+    y, res, w = _randn(g, 6, H), _randn(g, 6, H), _randn(g, H)
+    y[0] = 0
+    res[0] = 0
+    y[2, 3] = float("nan")
+    res[3, 4] = float("inf")
+    y[4, 5] = float("inf")
+    h = torch.empty_like(res)
+    for int8 in (False, True):
+        x = ops.norm_block(y, res, w, 1e-6, residual_out=h, int8=int8)
+        bad = x.scale.isnan() if int8 else x.isnan().any(1)
+        assert bad.tolist() == [False, False, True, True, True, False]
+        assert ((x.q if int8 else x)[0] == 0).all()
+    assert torch.equal(h.isfinite().all(1), torch.tensor([True, True, False, False, False, True], device="cuda"))
+    # a gate of zero leaves a row as it is, unless what it shuts out is not finite
+    gate = torch.zeros(6, 1, device="cuda", dtype=BF)
+    ops.norm_block(y, res, w, 1e-6, gate=gate, residual_out=h)
+    assert torch.equal(h[[0, 1, 3, 5]], res[[0, 1, 3, 5]]) and h[2, 3].isnan() and h[4, 5].isnan()
+
+
+def test_large_means_do_not_cost_a_layer_norm_its_precision(ops):
+    """Squares are taken of what the mean leaves: 1000 +- 4 in bf16 is 1000 and its neighbours."""
+    res = 1000 + _randn(_gen(1), 4, 2048, dtype=torch.float32, std=8.0)
+    res = res.to(BF)
+    w = torch.ones(2048, device="cuda", dtype=BF)
+    x = ops.norm_block(None, res, w, 1e-5, layernorm=True)
+    want = torch.nn.functional.layer_norm(res.double(), (2048,), eps=1e-5)
+    # the mean is off by 32 steps of 1000 at most, the values have a deviation of 8
+    assert ((x.double() - want).abs() <= HALF * want.abs() + 64 * E * 1000 / 8).all()
+
+
+# ------------------------------------------------------------------------------------------------ products
+def _check_product(ops, T, N, K, bias=True, at=0, out=None):
+    g = _gen(T, N, K)
+    q, w = _int8(g, T, K, at), _int8(g, N, K, at)
+    xs, ws = torch.rand(T, generator=g, device="cuda") * 0.1, torch.rand(N, generator=g, device="cuda") * 0.01
+    b = _randn(g, N) if bias else None
+    y = ops.gemm_int8(Int8Rows(q, xs), w, ws, bias=b, out=out)
+    s = (q.double() @ w.double().t()) * (xs.double()[:, None] * ws.double())
+    want = s + (0 if b is None else b.double())
+    # the sum to 32 bits, two products, the bias: four roundings; then one to bf16
+    assert y.shape == (T, N) and y.dtype == BF
+    assert ((y.double() - want).abs() <= HALF * want.abs() + 5 * E * (s.abs() + want.abs())).all()
+    return y
+
+
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 33, 64, 65, 128, 137, 200, 256, 257, 300, 513])
+@pytest.mark.parametrize("N,K", [(256, 512), (130, 1021)])
+def test_products(ops, T, N, K):
+    _check_product(ops, T, N, K)
+
+
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 127, 128, 129, 131, 255, 1000, 4099])
+@pytest.mark.parametrize("T,K", [(1, 256), (20, 300)])
+def test_products_of_any_number_of_channels(ops, N, T, K):
+    _check_product(ops, T, N, K, bias=N % 2 == 0)
+
+
+@pytest.mark.parametrize("K", [1, 15, 16, 17, 127, 128, 129, 255, 384, 511, 640, 900, 1100, 2048, 2300, 4096, 8192, 14336])
+@pytest.mark.parametrize("T", [1, 48, 260])
+def test_products_of_any_depth(ops, K, T):
+    """K in one part or shared by up to eight CTAs."""
+    _check_product(ops, T, 192, K, bias=False)
+
+
+@pytest.mark.parametrize("T,N,K", [(1, 6144, 4096), (1, 28672, 4096), (7, 4096, 14336), (64, 28672, 4096), (256, 4096, 14336), (1500, 4096, 4096), (2048, 6144, 1024),
+                                   (700, 11008, 2048), (4001, 2050, 520)])
+def test_large_products(ops, T, N, K):
+    _check_product(ops, T, N, K)
+
+
+@pytest.mark.parametrize("T", [3, 400])
+def test_rows_and_results_in_wider_buffers(ops, T):
+    buf = torch.full((T, 400), 3.0, device="cuda", dtype=BF)
+    for a, n in ((0, 333), (1, 332), (4, 336), (8, 200)):
+        buf.fill_(3.0)
+        _check_product(ops, T, n, 320, at=16, out=buf[:, a:a + n])
+        assert (buf[:, :a] == 3).all() and (buf[:, a + n:] == 3).all()
+
+
+def test_the_longest_sums_are_whole(ops):
+    K = 1 << 17
+    q = torch.full((2, K), -127, device="cuda", dtype=torch.int8)
+    w = torch.full((3, K), -128, device="cuda", dtype=torch.int8)
+    w[1] = 127
+    y = ops.gemm_int8(Int8Rows(q, torch.full((2,), 2.0 ** -31, device="cuda")), w, torch.ones(3, device="cuda"))
+    want = (q.double() @ w.double().t() * 2.0 ** -31).to(BF)
+    assert torch.equal(y, want)
+
+
+def test_rows_behind_the_last_one_are_left_alone(ops):
+    for T in (1, 5, 130, 300):
+        buf = torch.full((T + 3, 256), 9.0, device="cuda", dtype=BF)
+        _check_product(ops, T, 256, 256, out=buf[:T])
+        assert (buf[T:] == 9).all()
+
+
+# ------------------------------------------------------------------------------------------------ together
+def _feed_forward(ops, y, res, w, up, down, I):
+    x = ops.norm_block(y, res, w, 1e-5, post_weight=w, int8=True)
+    h = ops.gemm_int8(x, *up)
+    return h, ops.gemm_int8(ops.act_mul_int8(h, I, "silu"), *down)
+
+
+def _state(T, H, I, seed=0):
+    g = _gen(T, H, I, seed)
+    up = ref.quantize_weight_int8(_randn(g, 2 * I, H, dtype=torch.float32, std=H ** -0.5))
+    down = ref.quantize_weight_int8(_randn(g, H, I, dtype=torch.float32, std=I ** -0.5))
+    return _randn(g, T, H), _randn(g, T, H), 1 + _randn(g, H, std=0.1), up, down, I
+
+
+@pytest.mark.parametrize("T,H,I", [(1, 1024, 2816), (48, 512, 1000), (333, 1032, 520)])
+def test_a_feed_forward(ops, T, H, I):
+    """Norms, product, activation, product: each step against its definition on what the step before it gave, and the whole against the same in bf16 weights."""
+    y, res, w, up, down, I = _state(T, H, I)
+    h0 = res.clone()
+    h, out = _feed_forward(ops, y, h0, w, up, down, I)
+    a = torch.nn.functional.silu(h[:, :I].double()) * h[:, I:].double()
+    whole = a @ (down[0].double() * down[1].double()[:, None]).t()
+    # the rows' rounding: half a step of max / 127, of random sign, over I products of weights of the size I^-0.5; six deviations, and the result's own rounding
+    sd = (a.abs().amax(1) / 127 / 12 ** 0.5)[:, None] * (down[0].double() * down[1].double()[:, None]).square().sum(1).sqrt()
+    assert ((out.double() - whole).abs() <= 6 * sd + HALF * whole.abs()).all()
+
+
+def test_captured_graphs_and_streams(ops):
+    """Two captured passes replayed at the same time on two streams, while a third runs eagerly: none has scratch that another one uses."""
+    states = [_state(T, 1024, 1536, T) for T in (1, 17, 300)]
+    want = [_feed_forward(ops, y, res.clone(), *rest) for y, res, *rest in states]
+    graphs = []
+    for y, res, *rest in states[:2]:
+        r, work = res.clone(), torch.empty_like(res)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            work.copy_(r)
+            _feed_forward(ops, y, work, *rest)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                work.copy_(r)
+                out = _feed_forward(ops, y, work, *rest)
+        graphs.append((g, s, out, r, work))          # (a graph keeps no tensor alive that was made outside)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s, *_ in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+        y, res, *rest = states[2]
+        eager = _feed_forward(ops, y, res.clone(), *rest)
+    torch.cuda.synchronize()
+    for got, w in zip([graphs[0][2], graphs[1][2], eager], want):
+        assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
+
+
+def test_results_do_not_depend_on_other_rows(ops):
+    """A row's sums are whole numbers and its norms its own: alone, and among any number of others, the same bits."""
+    y, res, w, up, down, I = _state(300, 512, 768)
+    h, out = _feed_forward(ops, y, res.clone(), w, up, down, I)
+    for a, b in ((0, 1), (5, 22), (100, 300)):
+        h1, out1 = _feed_forward(ops, y[a:b], res[a:b].clone(), w, up, down, I)
+        assert torch.equal(h1, h[a:b]) and torch.equal(out1, out[a:b])
+
+
+def test_empty_calls_launch_nothing(ops):
+    w, ws = ref.quantize_weight_int8(torch.randn(5, 16, device="cuda"))
+    n = ops.launch_count
+    r = ops.quant_rows_int8(torch.empty(0, 16, device="cuda", dtype=BF))
+    assert ops.gemm_int8(r, w, ws).shape == (0, 5) and ops.launch_count == n
+    assert ops.norm_block(None, torch.empty(0, 16, device="cuda", dtype=BF), torch.ones(16, device="cuda", dtype=BF), 1e-6).shape == (0, 16)
+    assert ops.launch_count == n
