@@ -9,7 +9,7 @@
 // kept in global memory between CTAs, calls or graphs.
 //
 // The reference has no such product (it expands 8-bit integer weights beside bf16 activations, server/lorax_server/layers/eetq.py:1-26).
-#include "common.cuh"
+#include "pair.cuh"
 
 namespace lx {
 
@@ -56,23 +56,71 @@ LX_DEVICE int4 cluster_load_int4(uint32_t smem_addr, uint32_t rank) {
   return v;
 }
 
-// Results of four features of one token.
-LX_DEVICE void int8_store4(const Int8GemmParams& p, int t, int n, int4 s) {
-  const float xs = p.xs[t];
-  const int v[4] = {s.x, s.y, s.z, s.w};
-  float f[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int at = min(n + q, p.N - 1);
-    f[q] = (float)v[q] * p.ws[at] * xs + (p.bias != nullptr ? __bfloat162float(p.bias[at]) : 0.f);
+// A tile's scales and biases in shared memory, fetched while its products are formed: behind them every load would wait for L2.
+struct __align__(16) Int8Scales {
+  float ws[kI8BM], bias[kI8BM], xs[256];
+};
+LX_DEVICE void int8_scales(const Int8GemmParams& p, Int8Scales& sc, int n0, int t0, int thread, int threads) {
+  for (int i = thread; i < kI8BM; i += threads) {
+    const int at = min(n0 + i, p.N - 1);
+    sc.ws[i] = p.ws[at];
+    sc.bias[i] = p.bias != nullptr ? __bfloat162float(p.bias[at]) : 0.f;
   }
-  __nv_bfloat16* o = p.out + (long long)t * p.ldo + n;
-  if (p.wide && n + 4 <= p.N) {
-    *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
-  } else {
+  for (int i = thread; i < p.bn; i += threads) sc.xs[i] = p.xs[min(t0 + i, p.T - 1)];
+}
+
+// A tile's results from its parts' sums ([token][128 features] in the shared memory of the CTAs first, first + stride ... of the cluster; of this one, if there are
+// no others).  A warp takes a token's features, four a lane; the tokens go round the warps of all parts, and the sums of several are on their way at a time: a
+// trip to another CTA's shared memory takes the better part of a microsecond.
+template <int PARTS, int ROWS>
+LX_DEVICE void int8_join(const Int8GemmParams& p, const int* sums, const Int8Scales& sc, int part, uint32_t first, uint32_t stride, int n0, int t0, int live) {
+  const int lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5, step = warps * p.parts, n = n0 + lane * 4;
+  const float4 w4 = *reinterpret_cast<const float4*>(sc.ws + lane * 4), b4 = *reinterpret_cast<const float4*>(sc.bias + lane * 4);
+  const float ws[4] = {w4.x, w4.y, w4.z, w4.w}, bias[4] = {b4.x, b4.y, b4.z, b4.w};
+  const uint32_t at = smem_u32(sums) + (uint32_t)lane * 16;
+  for (int t = (int)(threadIdx.x >> 5) * p.parts + part; t < live; t += ROWS * step) {
+    int4 v[ROWS][PARTS];
+    float xs[ROWS];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (n + q < p.N) o[q] = __float2bfloat16(f[q]);
+    for (int u = 0; u < ROWS; ++u) {
+      const int tu = min(t + u * step, live - 1);
+      xs[u] = sc.xs[tu];
+#pragma unroll
+      for (int r = 0; r < PARTS; ++r) {
+        const uint32_t src = at + (uint32_t)tu * (kI8BM * 4);
+        if (PARTS == 1) v[u][r] = *reinterpret_cast<const int4*>(sums + tu * kI8BM + lane * 4);
+        else if (r < p.parts) v[u][r] = cluster_load_int4(src, first + (uint32_t)r * stride);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      if (t + u * step >= live) break;
+      int4 s = v[u][0];
+#pragma unroll
+      for (int r = 1; r < PARTS; ++r)
+        if (r < p.parts) { s.x += v[u][r].x; s.y += v[u][r].y; s.z += v[u][r].z; s.w += v[u][r].w; }
+      const float f[4] = {(float)s.x * ws[0] * xs[u] + bias[0], (float)s.y * ws[1] * xs[u] + bias[1], (float)s.z * ws[2] * xs[u] + bias[2],
+                          (float)s.w * ws[3] * xs[u] + bias[3]};
+      __nv_bfloat16* row = p.out + (long long)(t0 + t + u * step) * p.ldo + n0;
+      if (p.wide) {
+        if (n + 4 <= p.N) *reinterpret_cast<uint2*>(row + lane * 4) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+        else
+          for (int q = 0; q < 4; ++q)
+            if (n + q < p.N) row[lane * 4 + q] = __float2bfloat16(f[q]);
+      } else {
+        // a row that begins anywhere: 32 neighbours a store, fetched from the lanes that hold them
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float g = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float h = __shfl_sync(0xffffffffu, f[q], 8 * e + (lane >> 2));
+            if ((lane & 3) == q) g = h;
+          }
+          if (n0 + 32 * e + lane < p.N) row[32 * e + lane] = __float2bfloat16(g);
+        }
+      }
+    }
   }
 }
 
@@ -82,7 +130,8 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_bytes = kI8ABytes + p.bn * kI8BK;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
+  Int8Scales& scales = *reinterpret_cast<Int8Scales*>(smem + p.stages * stage_bytes);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(&scales + 1);
   uint64_t* empty_bar = full_bar + kI8MaxStages;
   uint64_t* done_bar = empty_bar + kI8MaxStages;
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
@@ -169,6 +218,8 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       tc_commit(done_bar);
     }
     __syncwarp();
+  } else {
+    int8_scales(p, scales, ta * kI8BM, tb * p.bn, (int)threadIdx.x - 64, 64);
   }
 
   // (done: every load of this CTA has arrived and been read, so the ring is free)
@@ -184,40 +235,268 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   if (ok) {
     tc_fence_after();
     const uint32_t taddr = tmem_d + ((uint32_t)(warp * 32) << 16);
+    int* mine = sums + warp * 32 + lane;
     for (int c = 0; c < live; c += 16) {
       uint32_t r[16];
       tmem_ld_32x32b_x16(taddr + c, r);
       tc_wait_ld();
 #pragma unroll
-      for (int q = 0; q < 16; ++q)
-        if (c + q < live) sums[(c + q) * kI8BM + warp * 32 + lane] = (int)r[q];
+      for (int q = 0; q < 16; ++q) mine[(c + q) * kI8BM] = (int)r[q];      // (rows of the tile behind the last token too: there is room for bn of them)
     }
     tc_fence_before();
   }
   if (p.parts > 1) cluster_sync();
   else __syncthreads();
-  // four features of a token at a time, in turn over the cluster's threads
-  const int4* mine = reinterpret_cast<const int4*>(sums);
-  for (int u = part * kI8Threads + (int)threadIdx.x; u < live * (kI8BM / 4); u += p.parts * kI8Threads) {
-    const int n = ta * kI8BM + u % (kI8BM / 4) * 4;
-    if (n >= p.N) continue;
-    int4 s = make_int4(0, 0, 0, 0);
-    if (p.parts > 1) {
-      int4 v[kI8MaxParts];
-#pragma unroll
-      for (int r = 0; r < kI8MaxParts; ++r)
-        if (r < p.parts) v[r] = cluster_load_int4(smem_u32(mine + u), (uint32_t)r);
-#pragma unroll
-      for (int r = 0; r < kI8MaxParts; ++r)
-        if (r < p.parts) { s.x += v[r].x; s.y += v[r].y; s.z += v[r].z; s.w += v[r].w; }
-    } else {
-      s = mine[u];
-    }
-    if (ok) int8_store4(p, t0 + u / (kI8BM / 4), n, s);
+  if (!*abort_flag) {
+    if (p.parts == 1) int8_join<1, 4>(p, sums, scales, 0, 0, 0, ta * kI8BM, t0, live);
+    else if (p.parts <= 4) int8_join<4, 4>(p, sums, scales, part, 0, 1, ta * kI8BM, t0, live);
+    else int8_join<kI8MaxParts, 2>(p, sums, scales, part, 0, 1, ta * kI8BM, t0, live);
   }
   if (p.parts > 1) cluster_sync();      // nobody leaves while its sums are read
   else __syncthreads();
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_d, (uint32_t)p.tmem_cols); }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Long steps, by pairs of CTAs (cta_group::2): a tile is 256 features x up to 256 tokens, of which each CTA loads 128 rows of the weights and half of
+// the tokens, 32 KB a stage for 4 x 256 x 256 x 32 products, where one CTA on 128 x 256 takes 48 KB for half as many.  What comes in from L2 is what bounds a
+// single CTA at these sizes (some 95 bytes a nanosecond).  One part: persistent pairs, whose accumulators take turns, so that a tile's results are written while
+// the next one is multiplied.  Several: a cluster of pairs shares one tile's K, as above.
+// ------------------------------------------------------------------------------------------------
+constexpr int kI8PairStages = 6;
+constexpr int kI8PairThreads = 192;
+constexpr int kI8PairStageBytes = 2 * kI8ABytes;
+constexpr int kI8PairMaxParts = 4;
+constexpr int kI8TurnBytes = 4 * 16 * 32 * 4;     // a warp's 32 features x 32 tokens in bf16, two tokens a word
+constexpr int kI8PairSmem = kI8PairStages * kI8PairStageBytes + kI8TurnBytes + (int)sizeof(Int8Scales) + 256 + 1024;
+static_assert(kI8PairSmem <= 227 * 1024 && 256 * kI8BM * 4 <= kI8PairStages * kI8PairStageBytes, "the ring holds a tile's sums");
+
+LX_DEVICE void pair_mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// pair_commit of a pair that is not the cluster's first.
+LX_DEVICE void pair_commit_of(uint64_t* bar, uint32_t even) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_u32(bar)), "h"((uint16_t)(3u << even)) : "memory");
+}
+
+__global__ void __launch_bounds__(kI8PairThreads, 1)
+gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8GemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint32_t* turn_all = reinterpret_cast<uint32_t*>(smem + kI8PairStages * kI8PairStageBytes);
+  Int8Scales& scales = *reinterpret_cast<Int8Scales*>(smem + kI8PairStages * kI8PairStageBytes + kI8TurnBytes);    // (of a shared tile)
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(&scales + 1);                                                   // (the even CTA's are used)
+  uint64_t* empty_bar = full_bar + kI8PairStages;
+  uint64_t* tmem_full = empty_bar + kI8PairStages;
+  uint64_t* tmem_empty = tmem_full + 2;                                                                            // (the even CTA's are used)
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_rank(), even = cta & ~1u;
+  const int rank = (int)(cta & 1), part = (int)(cta >> 1);
+  const int tiles_b = (p.T + p.bn - 1) / p.bn;
+  const int num_tiles = (p.N + 2 * kI8BM - 1) / (2 * kI8BM) * tiles_b;
+  const int first = (int)blockIdx.x / (2 * p.parts), step = p.parts > 1 ? num_tiles : (int)gridDim.x / 2;      // (parts: one tile a cluster)
+  const int kblocks = (p.K + kI8BK - 1) / kI8BK;
+  const int kb0 = (int)((long long)kblocks * part / p.parts), kb1 = (int)((long long)kblocks * (part + 1) / p.parts);
+  const int half = p.bn >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kI8PairStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&tmem_full[s], 1); mbar_init(&tmem_empty[s], 8); }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+  }
+  if (warp == 1) pair_tmem_alloc(tmem_base_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                                      // both CTAs' barriers and columns are there
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_slot;
+
+  if (!p.w_const) pdl_wait();
+  const uint32_t bytes = 2u * (uint32_t)(kI8ABytes + half * kI8BK);      // of a stage, in both CTAs
+  int ahead = 0;
+  if (threadIdx.x == 0 && first < num_tiles) {
+    ahead = min(kI8PairStages, kb1 - kb0);
+    for (int s = 0; s < ahead; ++s) {
+      if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
+      pair_load_2d(smem + s * kI8PairStageBytes, &tmap_w, pair_map(&full_bar[s], even), (kb0 + s) * kI8BK, (2 * (first / tiles_b) + rank) * kI8BM);
+    }
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  int loaded = 0;                                      // (of thread 0) stages filled so far
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first; tile < num_tiles && ok; tile += step) {
+        const int i0 = (2 * (tile / tiles_b) + rank) * kI8BM, j0 = tile % tiles_b * p.bn + rank * half;
+        for (int kb = kb0; kb < kb1; ++kb, ++loaded) {
+          const uint32_t bar = pair_map(&full_bar[stage], even);
+          uint8_t* sa = smem + stage * kI8PairStageBytes;
+          if (loaded >= ahead) {
+            if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
+              report_status(p.status, kTimeoutEmptyBarrier, tile);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            if (rank == 0) mbar_expect_tx(&full_bar[stage], bytes);
+            pair_load_2d(sa, &tmap_w, bar, kb * kI8BK, i0);
+          }
+          pair_load_2d(sa + kI8ABytes, &tmap_x, bar, kb * kI8BK, j0);
+          if (++stage == kI8PairStages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      const uint32_t idesc = make_idesc_i8(2 * kI8BM, (uint32_t)p.bn);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase[2] = {0, 0};
+      bool ok = true;
+      for (int tile = first; tile < num_tiles && ok; tile += step) {
+        if (!pair_wait(&tmem_empty[acc], acc_phase[acc] ^ 1, abort_flag)) {
+          report_status(p.status, kTimeoutTmemEmpty, tile);
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t tmem_d = tmem_base + (uint32_t)(acc * 256);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag)) {
+            report_status(p.status, kTimeoutFullBarrier, tile);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * kI8PairStageBytes);
+          const uint64_t da = make_desc_k_sw128(sa), db = make_desc_k_sw128(sa + kI8ABytes);
+#pragma unroll
+          for (int k = 0; k < kI8BK / 32; ++k) pair_mma_i8(tmem_d, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          pair_commit_of(&empty_bar[stage], even);
+          if (++stage == kI8PairStages) { stage = 0; phase ^= 1; }
+        }
+        if (ok) pair_commit_of(&tmem_full[acc], even);
+        acc_phase[acc] ^= 1;
+        acc ^= 1;
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quad = warp & 3;
+    uint32_t* turn = turn_all + quad * (16 * 32);
+    int* sums = reinterpret_cast<int*>(smem);          // [token][128 features], of a shared tile: over the ring, which has been read by then
+    int acc = 0;
+    uint32_t acc_phase[2] = {0, 0};
+    for (int tile = first; tile < num_tiles; tile += step) {
+      const int j0 = tile % tiles_b * p.bn, jend = min(p.T, j0 + p.bn);
+      const int f0 = (2 * (tile / tiles_b) + rank) * kI8BM + quad * 32, fi = min(f0 + lane, p.N - 1);
+      float ws = 0.f, bias = 0.f, xl[8];                // (fetched while the tile's products are formed; xl[i]: the scale of token 32 i + lane)
+      if (p.parts > 1) {
+        int8_scales(p, scales, f0 - quad * 32, j0, (int)threadIdx.x - 64, 128);
+      } else {
+        ws = p.ws[fi];
+        if (p.bias != nullptr) bias = __bfloat162float(p.bias[fi]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xl[i] = p.xs[min(j0 + 32 * i + lane, p.T - 1)];
+      }
+      if (!mbar_wait(&tmem_full[acc], acc_phase[acc], abort_flag)) {
+        report_status(p.status, kTimeoutTmemFull, tile);
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      acc_phase[acc] ^= 1;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * 256);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = 32 * i;
+        if (c >= p.bn || j0 + c >= jend) break;
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(taddr + c, r);
+        tc_wait_ld();
+        if (p.parts > 1) {
+#pragma unroll
+          for (int q = 0; q < 32; ++q) sums[(c + q) * kI8BM + quad * 32 + lane] = (int)r[q];
+          continue;
+        }
+        if (!p.wide) {
+          // rows that begin anywhere: 32 neighbours a store, as they are
+#pragma unroll
+          for (int q = 0; q < 32; ++q) {
+            const float v = (float)(int)r[q] * ws * __shfl_sync(0xffffffffu, xl[i], q) + bias;
+            if (j0 + c + q < jend && f0 + lane < p.N) p.out[(long long)(j0 + c + q) * p.ldo + f0 + lane] = __float2bfloat16(v);
+          }
+          continue;
+        }
+        // a thread holds one feature of 32 tokens; the warp turns its block around, two tokens a word, and a lane stores eight features of two tokens
+#pragma unroll
+        for (int q = 0; q < 32; q += 2) {
+          const float a = (float)(int)r[q] * ws * __shfl_sync(0xffffffffu, xl[i], q) + bias;
+          const float b = (float)(int)r[q + 1] * ws * __shfl_sync(0xffffffffu, xl[i], q + 1) + bias;
+          turn[(q >> 1) * 32 + lane] = pack_bf16x2(a, b);
+        }
+        __syncwarp();
+        const int n = f0 + (lane & 3) * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int pr = h * 8 + (lane >> 2), t = j0 + c + 2 * pr;
+          const uint4 u = *reinterpret_cast<const uint4*>(turn + pr * 32 + (lane & 3) * 8), v = *reinterpret_cast<const uint4*>(turn + pr * 32 + (lane & 3) * 8 + 4);
+          const uint4 lo = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.z, u.w, 0x5410), __byte_perm(v.x, v.y, 0x5410), __byte_perm(v.z, v.w, 0x5410));
+          const uint4 hi = make_uint4(__byte_perm(u.x, u.y, 0x7632), __byte_perm(u.z, u.w, 0x7632), __byte_perm(v.x, v.y, 0x7632), __byte_perm(v.z, v.w, 0x7632));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint4 o = k ? hi : lo;
+            if (t + k >= jend || n >= p.N) continue;
+            __nv_bfloat16* dst = p.out + (long long)(t + k) * p.ldo + n;
+            if (n + 8 <= p.N) {
+              *reinterpret_cast<uint4*>(dst) = o;
+            } else {
+              const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (n + e < p.N) reinterpret_cast<unsigned short*>(dst)[e] = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) pair_arrive(pair_map(&tmem_empty[acc], even));
+      acc ^= 1;
+    }
+    __syncwarp();
+  }
+
+  if (*abort_flag && rank == 0 && threadIdx.x == 0)    // copies still on their way to either CTA arrive before the pair leaves
+    for (int s = 0; s < min(kI8PairStages, loaded); ++s) mbar_wait(&full_bar[s], (uint32_t)((loaded - 1 - s) / kI8PairStages) & 1u, nullptr);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                                      // nothing of this pair is on its way to a CTA that has left; the parts' sums are there
+  if (p.parts > 1) {
+    const int j0 = first % tiles_b * p.bn;
+    if (!*abort_flag)
+      int8_join<kI8PairMaxParts, 4>(p, reinterpret_cast<const int*>(smem), scales, part, (uint32_t)rank, 2, (2 * (first / tiles_b) + rank) * kI8BM, j0, min(p.bn, p.T - j0));
+    __syncwarp();
+    cluster_sync();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    pair_tmem_dealloc(tmem_base, 512);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -250,25 +529,109 @@ static int make_tmap_i8(CUtensorMap* out, const void* base, uint64_t rows, uint6
 }
 
 struct Int8Plan {
-  int bn, stages, parts, tmem_cols, smem;
+  int pairs, bn, stages, parts, tmem_cols, smem;      // pairs: of CTAs that stay, 0: single ones
 };
-static Int8Plan int8_plan(int T, int N, int K, int num_sms) {
+static int int8_up(int a, int b) { return (a + b - 1) / b; }
+
+// By single CTAs: where there are more of them than SMs, or clusters, which leave SMs empty, the ring of small tiles takes half of an SM's shared memory, so
+// that two share an SM; else all of it.
+static Int8Plan int8_single_plan(int T, int N, int K, int bn, int parts, int num_sms) {
   Int8Plan w{};
-  const int t16 = (T + 15) / 16 * 16, token_tiles = (t16 + 255) / 256;
-  w.bn = ((t16 + token_tiles - 1) / token_tiles + 15) / 16 * 16;
-  const int kblocks = (K + kI8BK - 1) / kI8BK;
-  const long long tiles = (long long)((N + kI8BM - 1) / kI8BM) * ((T + w.bn - 1) / w.bn);
-  w.parts = 1;
-  while (w.parts < kI8MaxParts && tiles * w.parts < num_sms && kblocks >= 4 * (w.parts + 1)) ++w.parts;
+  w.bn = bn;
+  w.parts = parts;
   const int stage = kI8ABytes + w.bn * kI8BK;
-  const int room = w.bn <= 64 ? 108 * 1024 : 216 * 1024;      // two CTAs an SM of small tiles, or one
+  const bool share = w.bn <= 64 && (parts > 1 || (long long)int8_up(N, kI8BM) * int8_up(T, bn) > num_sms);
+  const int room = share ? 108 * 1024 : 216 * 1024, most = int8_up(int8_up(K, kI8BK), w.parts);
   w.stages = room / stage < kI8MaxStages ? room / stage : kI8MaxStages;
-  const int most = (kblocks + w.parts - 1) / w.parts;
   if (w.stages > most) w.stages = most > 4 ? most : 4;
   w.tmem_cols = 32;
   while (w.tmem_cols < w.bn) w.tmem_cols *= 2;
-  w.smem = w.stages * stage + (2 * kI8MaxStages + 1) * 8 + 16 + 1024;
+  w.smem = w.stages * stage + (int)sizeof(Int8Scales) + (2 * kI8MaxStages + 1) * 8 + 16 + 1024;
   return w;
+}
+
+// What a plan costs, in ns.  A CTA's time is that of its operands' way in from L2 (98 bytes a nanosecond; a second CTA on the SM adds a third to it) and of its
+// tokens' results; waves of CTAs add a start, parts a join; and no plan is quicker than the weights' way from HBM.  The constants are fitted to 6000 plans of 160
+// shapes (1 to 2048 rows, 390 to 28672 features, K 512 to 14336); the plan with the least cost is 2 % slower than the quickest one on average, at worst 21 %.
+constexpr double kI8Hbm = 6450.0;
+static double int8_single_cost(int T, int N, int K, const Int8Plan& w, int num_sms) {
+  const int blocks = int8_up(int8_up(K, kI8BK), w.parts), live = w.bn < T ? w.bn : T;
+  int fit = 233472 / (w.smem + 1024);                                     // CTAs an SM
+  if (fit > 4) fit = 4;
+  const long long ctas = (long long)int8_up(N, kI8BM) * int8_up(T, w.bn) * w.parts;
+  const long long slots = (long long)(num_sms - (w.parts == 1 ? 0 : w.parts == 2 ? 2 : w.parts == 4 ? 16 : 18)) * fit;      // (clusters leave some SMs empty)
+  const long long waves = (ctas + (slots > 0 ? slots : 1) - 1) / (slots > 0 ? slots : 1);
+  long long together = (ctas + num_sms - 1) / num_sms;
+  if (together > fit) together = fit;
+  const double fill = blocks * (double)(kI8ABytes + kI8BK * w.bn) * (1 + 0.33 * (double)(together - 1)) / 98.0;
+  const double t = 1410.0 + (double)waves * (fill + 1820.0 + 15.0 * live * (double)together) + (w.parts > 1 ? 1000.0 + 5.2 * live : 0.0);
+  const double hbm = 3230.0 + ((double)N * K + (double)T * K) / kI8Hbm;
+  return t > hbm ? t : hbm;
+}
+static double int8_pair_cost(int T, int N, int K, int bn, int parts, int clusters) {
+  const int blocks = int8_up(int8_up(K, kI8BK), parts), live = bn < T ? bn : T;
+  const long long tiles = (long long)int8_up(N, 2 * kI8BM) * int8_up(T, bn), waves = (tiles + clusters - 1) / clusters;
+  const double in = (kI8ABytes + kI8BK / 2 * bn) / 80.0, mma = 0.67 * bn;
+  const double t = 3040.0 + (double)waves * (blocks * (in > mma ? in : mma) + 720.0) + 17.5 * live + (parts > 1 ? 630.0 + 2.3 * live : 0.0);
+  const double hbm = 3760.0 + ((double)N * K + (double)T * K) / kI8Hbm;
+  return t > hbm ? t : hbm;
+}
+
+// clusters[parts]: clusters of `parts` pairs that run at the same time.
+static Int8Plan int8_plan(int T, int N, int K, int num_sms, const int* clusters) {
+  Int8Plan best{};
+  double least = 1e30;
+  const int kblocks = int8_up(K, kI8BK);
+  for (int most = 256; most >= 16; most -= most > 64 ? 32 : 16) {
+    const int tiles = int8_up(T, most);
+    if (most < 256 && tiles == int8_up(T, most + (most >= 64 ? 32 : 16))) continue;      // (the same tiles, evened out)
+    if (most < 256 && tiles > 64) break;
+    const int bn = int8_up(int8_up(T, tiles), 16) * 16, bn2 = int8_up(bn, 32) * 32;
+    for (int parts : {1, 2, 3, 4, 8}) {
+      if (parts > kblocks) break;
+      const Int8Plan w = int8_single_plan(T, N, K, bn, parts, num_sms);
+      const double c = int8_single_cost(T, N, K, w, num_sms);
+      if (c < least) { least = c; best = w; }
+    }
+    for (int parts = 1; T > 32 && bn2 <= 256 && parts <= kI8PairMaxParts && parts <= kblocks; ++parts) {
+      if (clusters[parts] < 1 || (parts > 1 && (long long)int8_up(N, 2 * kI8BM) * int8_up(T, bn2) > clusters[parts])) break;
+      const double c = int8_pair_cost(T, N, K, bn2, parts, clusters[parts]);
+      if (c < least) {
+        least = c;
+        best = Int8Plan{clusters[1], bn2, 0, parts, 0, kI8PairSmem};
+      }
+    }
+  }
+  return best;
+}
+
+// Clusters of `parts` pairs that run at the same time on the current device (none of a size that no part of the device holds), or a query's negative error,
+// which the next call makes again.
+static int int8_clusters(int parts) {
+  static int known[64][kI8PairMaxParts + 1] = {{0}};
+  int dev = 0, n = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64)) return 0;
+  if (e == cudaSuccess && known[dev][parts] != 0) return known[dev][parts] - 1;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(gemm_int8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8PairSmem);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2u * (unsigned)parts);
+    cfg.blockDim = dim3(kI8PairThreads);
+    cfg.dynamicSmemBytes = kI8PairSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2u * (unsigned)parts; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&n, gemm_int8_pair_kernel, &cfg);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return -(int)e;
+  }
+  known[dev][parts] = n + 1;
+  return n;
 }
 
 }  // namespace lx
@@ -277,15 +640,51 @@ extern "C" {
 
 int lx_gemm_int8_max_k() { return 1 << 17; }
 
-// out[T, N] (bf16) = xq[T, K] wq[N, K]^T * xs[T] * ws[N] + bias[N].  Rows of xq and wq are ldq and ldw bytes apart (multiples of 16).
-// w_const: the kernel in front on the stream does not write wq.
+// The plan that a product takes where `clusters` (of 1, 2, 3, 4 pairs) run at the same time: out[0] pairs of CTAs (0: single ones), out[1] tokens a tile,
+// out[2] CTAs or pairs that share a tile's K, out[3] stages of a single CTA's ring.
+int lx_gemm_int8_plan(int T, int N, int K, int num_sms, const int* clusters, int* out) {
+  using namespace lx;
+  if (T <= 0 || N <= 0 || K <= 0 || K > lx_gemm_int8_max_k()) return -1000;
+  const int fit[kI8PairMaxParts + 1] = {0, clusters[0], clusters[1], clusters[2], clusters[3]};
+  const Int8Plan w = int8_plan(T, N, K, num_sms, fit);
+  out[0] = w.pairs; out[1] = w.bn; out[2] = w.parts; out[3] = w.stages;
+  return 0;
+}
+
+int lx_gemm_int8_clusters(int parts) { return parts < 1 || parts > lx::kI8PairMaxParts ? -1 : lx::int8_clusters(parts); }
+
+// out[T, N] (bf16) = xq[T, K] wq[N, K]^T * ws[N] * xs[T] + bias[N].  Rows of xq and wq are ldq and ldw bytes apart (multiples of 16).
+// w_const: the kernel in front on the stream does not write wq.  force (0: none): 1 + pairs + 2 * (parts | bn << 8), to measure a plan.
 int lx_gemm_int8(const void* xq, long long ldq, const void* xs, const void* wq, long long ldw, const void* ws, const void* bias, void* out, long long ldo,
-                 int T, int N, int K, int w_const, int* status, int num_sms, void* stream) {
+                 int T, int N, int K, int w_const, int* status, int num_sms, int force, void* stream_) {
   using namespace lx;
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K > lx_gemm_int8_max_k() || ldq % 16 != 0 || ldw % 16 != 0) return -1000;
-  const Int8Plan w = int8_plan(T, N, K, num_sms);
-  const long long ctas = (long long)((N + kI8BM - 1) / kI8BM) * ((T + w.bn - 1) / w.bn) * w.parts;
+  int clusters[kI8PairMaxParts + 1] = {0};
+  for (int parts = 1; parts <= kI8PairMaxParts; ++parts) {
+    const int n = int8_clusters(parts);
+    if (n < 0) return n;
+    clusters[parts] = pairs_on(num_sms / parts, n);
+  }
+  Int8Plan w;
+  if (force) {
+    const int pairs = (force - 1) & 1, parts = ((force - 1) >> 1) & 255, bn = (force - 1) >> 9;
+    if (bn < 16 || bn > 256 || bn % (pairs ? 32 : 16) != 0 || parts < 1 || parts > (pairs ? kI8PairMaxParts : kI8MaxParts) || parts > int8_up(K, kI8BK) ||
+        (pairs && clusters[parts] < 1))
+      return -1004;
+    w = pairs ? Int8Plan{clusters[1], bn, 0, parts, 0, kI8PairSmem} : int8_single_plan(T, N, K, bn, parts, num_sms);
+  } else {
+    // a plan takes some microseconds to choose and goes by sizes alone: the last ones of a thread are kept
+    struct Known { int T, N, K, sms, dev; Int8Plan w; };
+    static thread_local Known known[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return -3;
+    Known& k = known[((unsigned)T * 31u + (unsigned)N * 7u + (unsigned)K) % 64u];
+    if (k.T != T || k.N != N || k.K != K || k.sms != num_sms || k.dev != dev) k = Known{T, N, K, num_sms, dev, int8_plan(T, N, K, num_sms, clusters)};
+    w = k.w;
+  }
+  const long long tiles = (long long)((N + (w.pairs ? 2 : 1) * kI8BM - 1) / ((w.pairs ? 2 : 1) * kI8BM)) * ((T + w.bn - 1) / w.bn);
+  const long long ctas = !w.pairs ? tiles * w.parts : 2 * (w.parts > 1 ? tiles * w.parts : tiles < w.pairs ? tiles : w.pairs);
   if (ctas > 0x7fffffffll) return -1001;
   Int8GemmParams p{};
   p.N = N; p.T = T; p.K = K;
@@ -294,22 +693,27 @@ int lx_gemm_int8(const void* xq, long long ldq, const void* xs, const void* wq, 
   p.xs = reinterpret_cast<const float*>(xs); p.ws = reinterpret_cast<const float*>(ws);
   p.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
   p.out = reinterpret_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  p.wide = reinterpret_cast<uintptr_t>(out) % 8 == 0 && ldo % 4 == 0;
+  const int wide = w.pairs && w.parts == 1 ? 8 : 4;      // values that a thread stores at once
+  p.wide = reinterpret_cast<uintptr_t>(out) % (2 * wide) == 0 && ldo % wide == 0;
   p.status = status;
   p.w_const = w_const;
   CUtensorMap tw, tx;
   if (make_tmap_i8(&tw, wq, N, K, ldw, kI8BM)) return -1002;
-  if (make_tmap_i8(&tx, xq, T, K, ldq, w.bn)) return -1003;
+  if (make_tmap_i8(&tx, xq, T, K, ldq, w.pairs ? w.bn / 2 : w.bn)) return -1003;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  if (w.pairs) {
+    launch_pdl_cluster(gemm_int8_pair_kernel, dim3((unsigned)ctas), dim3(kI8PairThreads), dim3(2u * (unsigned)w.parts), (size_t)w.smem, stream, tw, tx, p);
+    return -(int)cudaGetLastError();
+  }
   static bool set[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   if (!set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm_int8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    const cudaError_t e = cudaFuncSetAttribute(gemm_int8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024);
     if (e != cudaSuccess) return -(int)e;
     set[dev] = true;
   }
-  launch_pdl_cluster(gemm_int8_kernel, dim3((unsigned)ctas), dim3(kI8Threads), dim3((unsigned)w.parts), (size_t)w.smem,
-                     reinterpret_cast<cudaStream_t>(stream), tw, tx, p);
+  launch_pdl_cluster(gemm_int8_kernel, dim3((unsigned)ctas), dim3(kI8Threads), dim3((unsigned)w.parts), (size_t)w.smem, stream, tw, tx, p);
   return -(int)cudaGetLastError();
 }
 

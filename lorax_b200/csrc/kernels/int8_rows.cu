@@ -8,11 +8,20 @@ namespace lx {
 
 enum RowsAct : int { kRowsPlain = -1, kRowsSilu = 0, kRowsGelu = 1, kRowsGeluTanh = 2, kRowsRelu = 3, kRowsRelu2 = 4 };
 
+// x / (1 + exp(-x)) = x * s for x >= 0, x * a * s below, with a = exp(-|x|), s = 1 / (1 + a): nothing overflows, small results keep their digits, and
+// the reciprocal's argument lies in [1, 2], where the approximate one is within one last place.  A NaN stays one.
+LX_DEVICE float times_sigmoid(float x, float z) {
+  const float a = __expf(-fabsf(z));
+  float s;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + a));
+  return x * (z < 0.f ? a : 1.f) * s;
+}
+
 template <int ACT>
 LX_DEVICE float rows_act(float x) {
-  if (ACT == kRowsSilu) return x / (1.f + __expf(-x));
+  if (ACT == kRowsSilu) return times_sigmoid(x, x);
   if (ACT == kRowsGelu) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-  if (ACT == kRowsGeluTanh) return 0.5f * x * (1.f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
+  if (ACT == kRowsGeluTanh) return times_sigmoid(x, 1.5957691216057308f * (x + 0.044715f * x * x * x));      // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
   if (ACT == kRowsRelu || ACT == kRowsRelu2) {
     const float r = x <= 0.f ? 0.f : x;      // (a NaN stays one)
     return ACT == kRowsRelu2 ? r * r : r;
@@ -53,15 +62,14 @@ __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kerne
   __shared__ uint32_t red[32];
   const long long t = blockIdx.x;
   const __nv_bfloat16* row = p.x + t * p.ldx;
-  uint32_t m = 0;
+  float m = 0.f;
   constexpr int KEEP = NV > 0 ? NV : 1;
   float f[KEEP][8];
   const int passes = NV > 0 ? NV : (p.n + (int)blockDim.x * 8 - 1) / ((int)blockDim.x * 8);
 #pragma unroll
   for (int it = 0; it < (NV > 0 ? NV : passes); ++it) {
     rows_values<ACT, WIDE>(p, row, it, f[NV > 0 ? it : 0]);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) m = larger_magnitude(m, f[NV > 0 ? it : 0][q]);
+    m = largest_magnitude(m, f[NV > 0 ? it : 0]);
   }
   const RowScale s = row_scale(block_max(m, red));
   if (threadIdx.x == 0) p.scale[t] = s.scale;

@@ -54,31 +54,38 @@ LX_DEVICE void row_store(__nv_bfloat16* row, int it, int n, const float (&f)[8])
   }
 }
 
-// The larger magnitude, as the bits of a 32-bit number: those order as the magnitudes do, infinity above all numbers and NaN above infinity.
-LX_DEVICE uint32_t larger_magnitude(uint32_t m, float v) { return max(m, __float_as_uint(v) & 0x7fffffffu); }
-
-// Over a block of up to 1024 threads, for all of them.  `red` holds 32 words; a barrier stands between two uses of the same ones.
-LX_DEVICE float block_sum(float v, float* red) {
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int warps = (int)blockDim.x >> 5;
-  float s = 0.f;
-  for (int i = 0; i < warps; ++i) s += red[i];
-  return s;
+// The largest magnitude of eight values and one that stands already; a NaN among them stays one.
+LX_DEVICE float larger_of(float m, float a, float b) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(a), "f"(b));
+  return d;
 }
-LX_DEVICE uint32_t block_max(uint32_t v, uint32_t* red) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int warps = (int)blockDim.x >> 5;
-  uint32_t m = 0;
-  for (int i = 0; i < warps; ++i) m = max(m, red[i]);
+LX_DEVICE float largest_magnitude(float m, const float (&f)[8]) {
+#pragma unroll
+  for (int q = 0; q < 8; q += 2) m = larger_of(m, f[q], f[q + 1]);
   return m;
 }
 
+// Over a block of up to 1024 threads, for all of them.  `red` holds 32 words; a barrier stands between two uses of the same ones.  (Every warp joins the warps'
+// parts by itself, a lane each: a loop over them was a quarter of the norms' instructions.)
+LX_DEVICE float block_sum(float v, float* red) {
+  const int lane = threadIdx.x & 31;
+  v = warp_sum(v);
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_sum(lane < ((int)blockDim.x >> 5) ? red[lane] : 0.f);
+}
+// Of magnitudes.  Their bits order as they do, infinity above all numbers and NaN above infinity.
+LX_DEVICE uint32_t block_max(float magnitude, uint32_t* red) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t v = __reduce_max_sync(0xffffffffu, __float_as_uint(magnitude) & 0x7fffffffu);
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return __reduce_max_sync(0xffffffffu, lane < ((int)blockDim.x >> 5) ? red[lane] : 0u);
+}
+
 struct RowScale {
-  float scale, inv;      // inv: about 1 / scale, 0 where all of the row's q are 0
+  float scale, inv;      // inv: 1 / scale, rounded; 0 where all of the row's q are 0
 };
 LX_DEVICE RowScale row_scale(uint32_t magnitude) {
   RowScale s;
@@ -92,41 +99,57 @@ LX_DEVICE RowScale row_scale(uint32_t magnitude) {
   return s;
 }
 
-// v / scale to the nearest integer.  v * inv is off by 2^-16 at most (|q| <= 127, two roundings of 2^-24 each, one of the scale), so only quotients that near
-// to a border need more: there v - q * scale is exact (a multiple of the smaller last place of v and scale, no larger than the scale), and is
-// compared with half the scale.  inv is infinite for scales below 2^-128: quotients of those rows all go through the division.
-LX_DEVICE int row_quotient(float v, const RowScale& s) {
-  constexpr float kWhole = 12582912.f;                       // 1.5 * 2^23: the sum's last place is 1
-  const float t = v * s.inv;
-  float q = __fsub_rn(__fadd_rn(t, kWhole), kWhole);
-  if (!(fabsf(t - q) < 0.4998f)) {
-    if (s.inv == 0.f) return 0;
-    if (!(fabsf(t) < 256.f)) q = rintf(__fdiv_rn(v, s.scale));
-    const float r = fmaf(-q, s.scale, v), a = fabsf(r), rest = s.scale - a;      // (a > rest: over half; exact, both are within a factor of two)
-    const float step = r > 0.f ? 1.f : -1.f;
-    if (a > rest || (a == rest && (((int)q) & 1))) q += step;
+// Quotients of rows whose scale is below 2^-128, where 1 / scale passes what 32 bits hold.
+static __device__ __noinline__ int tiny_quotient(float v, float scale) { return (int)rint((double)v / (double)scale); }
+
+// Eight quotients as bytes.  v * inv, unrounded, is off from v / scale by 127 * 2^-24 = 7.6e-6 at most (inv's rounding; |v| <= 127 scales), and its distance from the
+// integer by 2^-26 more, so that only a quotient within 1e-5 of a border may have gone to the wrong side.  Groups with such a one compare what is left with half the
+// scale: r = v - q * scale is exact there, a multiple of the smaller last place of v and scale and no larger than the scale.  Rows of bf16 numbers hold ties by the
+// hundred (their quotients are 127 times ratios of 8-bit numbers), so that the comparison has to be short.
+LX_DEVICE uint2 row_quotients(const float (&f)[8], const RowScale& s) {
+  constexpr float kWhole = 12582912.f;                       // 1.5 * 2^23: a sum's last place is 1, and its low byte the integer's
+  float u[8], far = 0.f;
+#pragma unroll
+  for (int q = 0; q < 8; q += 2) {
+    u[q] = fmaf(f[q], s.inv, kWhole);
+    u[q + 1] = fmaf(f[q + 1], s.inv, kWhole);
+    far = larger_of(far, fmaf(f[q], s.inv, -__fsub_rn(u[q], kWhole)), fmaf(f[q + 1], s.inv, -__fsub_rn(u[q + 1], kWhole)));
   }
-  return (int)fminf(fmaxf(q, -127.f), 127.f);
+  if (!(far < 0.49999f)) {
+    if (s.inv == 0.f) return make_uint2(0, 0);
+    if (s.inv > 3e38f) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) u[q] = __int_as_float(tiny_quotient(f[q], s.scale));
+    } else {
+      const float half = 0.5f * s.scale;                     // (exact: the scale is 2^-128 at least)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float r = fmaf(-__fsub_rn(u[q], kWhole), s.scale, f[q]);
+        // over half, or a tie at an odd integer: the neighbour on r's side
+        if (fabsf(r) > half || (fabsf(r) == half && (__float_as_int(u[q]) & 1))) u[q] += r > 0.f ? 1.f : -1.f;
+      }
+    }
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    w[h] = __byte_perm(__byte_perm(__float_as_uint(u[4 * h]), __float_as_uint(u[4 * h + 1]), 0x0040),
+                       __byte_perm(__float_as_uint(u[4 * h + 2]), __float_as_uint(u[4 * h + 3]), 0x0040), 0x5410);
+  return make_uint2(w[0], w[1]);
 }
 
 // A thread's eight quotients to its row's bytes.
 template <bool WIDE>
 LX_DEVICE void row_store_int8(int8_t* row, int it, int n, const float (&f)[8], const RowScale& s) {
+  if (WIDE && row_at<true>(it, 0) >= n) return;
+  const uint2 w = row_quotients(f, s);
   if (WIDE) {
-    const int c = row_at<true>(it, 0);
-    if (c >= n) return;
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int a = row_quotient(f[4 * h], s), b = row_quotient(f[4 * h + 1], s), d = row_quotient(f[4 * h + 2], s), e = row_quotient(f[4 * h + 3], s);
-      w[h] = __byte_perm(__byte_perm((uint32_t)a, (uint32_t)b, 0x0040), __byte_perm((uint32_t)d, (uint32_t)e, 0x0040), 0x5410);
-    }
-    *reinterpret_cast<uint2*>(row + c) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(row + row_at<true>(it, 0)) = w;
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const int c = row_at<false>(it, q);
-      if (c < n) row[c] = (int8_t)row_quotient(f[q], s);
+      if (c < n) row[c] = (int8_t)((q < 4 ? w.x : w.y) >> (8 * (q & 3)));
     }
   }
 }

@@ -18,13 +18,15 @@ struct NormBlockParams {
   const __nv_bfloat16* w;              // [H]
   const __nv_bfloat16* b;              // [H] or null
   const __nv_bfloat16* gate;           // or null
-  long long gate_t, gate_h;            // elements between two rows' and two channels' gates (0: the same)
+  long long gate_t;                    // elements between two rows' gates (0: the same)
+  int gate_h, gate_wide;               // 1: every channel has its own, 0: a row has one; rows of gates begin at 16 bytes
   __nv_bfloat16* out;                  // [T, H] or null
   int8_t* q;                           // [T, H] or null
   float* q_scale;
   long long ldy, ldr, ldro, ldo, ldq;
-  int H;
+  int H, T;
   float eps, w_offset, scale;
+  int* status;
 };
 
 // Sums over the block of up to three norms' passes, each with words of its own.
@@ -44,7 +46,7 @@ LX_DEVICE void norm_rows(float (&f)[NV][8], int H, float eps, float (*red)[32]) 
   for (int it = 0; it < NV; ++it)
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      f[it][q] = row_at<WIDE>(it, q) < H ? f[it][q] - mean : 0.f;
+      if (LAYERNORM) f[it][q] = (WIDE ? row_at<true>(it, 0) : row_at<false>(it, q)) < H ? f[it][q] - mean : 0.f;
       s = fmaf(f[it][q], f[it][q], s);
     }
   const float r = rsqrtf(block_sum(s, red[1]) / H + eps);
@@ -66,6 +68,24 @@ LX_DEVICE void scale_rows(float (&f)[NV][8], int H, const __nv_bfloat16* w, cons
       row_load<WIDE>(b, it, H, g);
 #pragma unroll
       for (int q = 0; q < 8; ++q) f[it][q] += g[q];
+    }
+  }
+}
+
+template <bool WIDE>
+LX_DEVICE void gates(const NormBlockParams& p, long long t, int it, float (&g)[8]) {
+  const __nv_bfloat16* gate = p.gate + t * p.gate_t;
+  if (p.gate_h == 0) {
+    const float one = __bfloat162float(*gate);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) g[q] = one;
+  } else if (WIDE && p.gate_wide) {
+    row_load<true>(gate, it, p.H, g);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int c = row_at<WIDE>(it, q);
+      g[q] = c < p.H ? __bfloat162float(gate[c]) : 0.f;
     }
   }
 }
@@ -92,24 +112,17 @@ __global__ void __launch_bounds__(kRowThreads4) norm_block_kernel(const NormBloc
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
       if (p.gate != nullptr) {
-        const __nv_bfloat16* gate = p.gate + t * p.gate_t;
         float g[8];
-        if (p.gate_h == 0) {
-          const float one = __bfloat162float(*gate);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) g[q] = one;
-        } else {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int c = row_at<WIDE>(it, q);
-            g[q] = c < p.H ? __bfloat162float(gate[c * p.gate_h]) : 0.f;
-          }
-        }
+        gates<WIDE>(p, t, it, g);
 #pragma unroll
         for (int q = 0; q < 8; ++q) y[it][q] *= g[q];
       }
 #pragma unroll
-      for (int q = 0; q < 8; ++q) h[it][q] = __bfloat162float(__float2bfloat16(fmaf(p.scale, y[it][q], h[it][q])));
+      for (int q = 0; q < 8; q += 2) {
+        const float2 r = unpack_bf16x2(pack_bf16x2(fmaf(p.scale, y[it][q], h[it][q]), fmaf(p.scale, y[it][q + 1], h[it][q + 1])));
+        h[it][q] = r.x;
+        h[it][q + 1] = r.y;
+      }
     }
   }
   if (p.residual_out != nullptr) {
@@ -123,17 +136,190 @@ __global__ void __launch_bounds__(kRowThreads4) norm_block_kernel(const NormBloc
     for (int it = 0; it < NV; ++it) row_store<WIDE>(p.out + t * p.ldo, it, p.H, h[it]);
   }
   if (p.q != nullptr) {
-    uint32_t m = 0;
+    float m = 0.f;
 #pragma unroll
-    for (int it = 0; it < NV; ++it)
+    for (int it = 0; it < NV; ++it) {
+      if (!WIDE) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
-        if (row_at<WIDE>(it, q) < p.H) m = larger_magnitude(m, h[it][q]);
+        for (int q = 0; q < 8; ++q)
+          if (row_at<WIDE>(it, q) >= p.H) h[it][q] = 0.f;
+      }
+      if (!WIDE || row_at<true>(it, 0) < p.H) m = largest_magnitude(m, h[it]);
+    }
     const RowScale s = row_scale(block_max(m, red_max));
     if (threadIdx.x == 0) p.q_scale[t] = s.scale;
 #pragma unroll
     for (int it = 0; it < NV; ++it) row_store_int8<WIDE>(p.q + t * p.ldq, it, p.H, h[it], s);
   }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Many rows: blocks that stay, with the next row of y and of the residual on its way by bulk copies (no registers, no waiting warps) while one is normed.
+// Rows are read from shared memory as often as a pass needs them, so that a thread holds the values of one row only, and the norms' weights for all rows.
+// ------------------------------------------------------------------------------------------------
+constexpr int kNormStages = 2;
+constexpr int kNormRingRows = 4;      // rows an SM from which they are worth it
+
+template <int NV>
+LX_DEVICE void unpack8(const uint4& v, float (&f)[NV][8], int it) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float2 t = unpack_bf16x2(w[q]);
+    f[it][2 * q] = t.x;
+    f[it][2 * q + 1] = t.y;
+  }
+}
+
+template <bool LAYERNORM, int NV>
+__global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring_kernel(const NormBlockParams p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kNormStages];
+  __shared__ float red[2][4][32];
+  __shared__ uint32_t red_max[2][32];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int H = p.H, nvec = H / 8, step = (int)gridDim.x;
+  const uint32_t row_bytes = (uint32_t)H * 2, stage_bytes = row_bytes * (p.y != nullptr ? 2 : 1);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kNormStages; ++s) mbar_init(&full[s], 1);
+    abort_word = 0;
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  const auto fetch = [&](int t, int s) {
+    mbar_expect_tx(&full[s], stage_bytes);
+    bulk_load_1d(ring + s * stage_bytes, p.residual + t * p.ldr, row_bytes, &full[s]);
+    if (p.y != nullptr) bulk_load_1d(ring + s * stage_bytes + row_bytes, p.y + t * p.ldy, row_bytes, &full[s]);
+  };
+  if (threadIdx.x == 0)
+    for (int s = 0; s < kNormStages && (int)blockIdx.x + s * step < p.T; ++s) fetch((int)blockIdx.x + s * step, s);
+  uint4 wv[NV], pv[NV];
+#pragma unroll
+  for (int it = 0; it < NV; ++it) {
+    const int v = it * (int)blockDim.x + (int)threadIdx.x;
+    wv[it] = pv[it] = make_uint4(0, 0, 0, 0);
+    if (v < nvec) {
+      wv[it] = reinterpret_cast<const uint4*>(p.w)[v];
+      if (p.post_w != nullptr) pv[it] = reinterpret_cast<const uint4*>(p.post_w)[v];
+    }
+  }
+  int i = 0;
+  for (int row = (int)blockIdx.x; row < p.T; row += step, ++i) {
+    const long long t = row;
+    const int s = i % kNormStages;
+    float(*sums)[32] = red[i & 1];
+    if (!mbar_wait(&full[s], (uint32_t)(i / kNormStages) & 1u, abort_flag)) {      // (every thread goes on to the block's barriers all the same)
+      report_status(p.status, kTimeoutFullBarrier, row);
+      *abort_flag = 1;
+    }
+    const uint4* rs = reinterpret_cast<const uint4*>(ring + s * stage_bytes);
+    const uint4* ys = reinterpret_cast<const uint4*>(ring + s * stage_bytes + row_bytes);
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    float h[NV][8];
+    if (p.y == nullptr) {
+#pragma unroll
+      for (int it = 0; it < NV; ++it) {
+        const int v = it * (int)blockDim.x + (int)threadIdx.x;
+        unpack8<NV>(v < nvec ? rs[v] : zero, h, it);
+      }
+    } else {
+#pragma unroll
+      for (int it = 0; it < NV; ++it) {
+        const int v = it * (int)blockDim.x + (int)threadIdx.x;
+        unpack8<NV>(v < nvec ? ys[v] : zero, h, it);
+      }
+      if (p.post_w != nullptr) {
+        norm_rows<LAYERNORM, NV, true>(h, H, p.eps, sums);
+#pragma unroll
+        for (int it = 0; it < NV; ++it) {
+          float g[1][8];
+          unpack8<1>(pv[it], g, 0);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) h[it][q] *= g[0][q] + p.w_offset;
+          if (p.post_b != nullptr) {
+            float b[8];
+            row_load<true>(p.post_b, it, H, b);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) h[it][q] += b[q];
+          }
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < NV; ++it) {
+        const int v = it * (int)blockDim.x + (int)threadIdx.x;
+        if (p.gate != nullptr) {
+          float g[8];
+          gates<true>(p, t, it, g);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) h[it][q] *= g[q];
+        }
+        float r[1][8];
+        unpack8<1>(v < nvec ? rs[v] : zero, r, 0);
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          w[q] = pack_bf16x2(fmaf(p.scale, h[it][2 * q], r[0][2 * q]), fmaf(p.scale, h[it][2 * q + 1], r[0][2 * q + 1]));
+          const float2 u = unpack_bf16x2(w[q]);
+          h[it][2 * q] = u.x;
+          h[it][2 * q + 1] = u.y;
+        }
+        if (v < nvec) reinterpret_cast<uint4*>(p.residual_out + t * p.ldro)[v] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    norm_rows<LAYERNORM, NV, true>(h, H, p.eps, sums + 2);
+    // (a barrier has passed since the row was read last: its stage takes the one after the next)
+    if (threadIdx.x == 0 && row + kNormStages * step < p.T) fetch(row + kNormStages * step, s);
+#pragma unroll
+    for (int it = 0; it < NV; ++it) {
+      float g[1][8];
+      unpack8<1>(wv[it], g, 0);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) h[it][q] *= g[0][q] + p.w_offset;
+      if (p.b != nullptr) {
+        float b[8];
+        row_load<true>(p.b, it, H, b);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) h[it][q] += b[q];
+      }
+      if (p.out != nullptr) row_store<true>(p.out + t * p.ldo, it, H, h[it]);
+    }
+    if (p.q != nullptr) {
+      float m = 0.f;
+#pragma unroll
+      for (int it = 0; it < NV; ++it)
+        if (row_at<true>(it, 0) < H) m = largest_magnitude(m, h[it]);
+      const RowScale sc = row_scale(block_max(m, red_max[i & 1]));
+      if (threadIdx.x == 0) p.q_scale[t] = sc.scale;
+#pragma unroll
+      for (int it = 0; it < NV; ++it) row_store_int8<true>(p.q + t * p.ldq, it, H, h[it], sc);
+    }
+  }
+}
+
+// Blocks that an SM holds at a time go by their registers (64 a thread, 128 with four groups) and their stages.
+template <bool LAYERNORM, int NV>
+static int launch_norm_ring(const NormBlockParams& p, int num_sms, cudaStream_t s) {
+  const int need = p.H / 8, threads = ((need + NV - 1) / NV + 31) / 32 * 32;
+  const int smem = kNormStages * p.H * 2 * (p.y != nullptr ? 2 : 1);
+  static bool set[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+  if (!set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(norm_block_ring_kernel<LAYERNORM, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormStages * 2 * 2 * kRowThreads4 * 8 * NV);
+    if (e != cudaSuccess) return -(int)e;
+    set[dev] = true;
+  }
+  int blocks = 65536 / (threads * (NV == 4 ? 128 : 64));
+  if (blocks > 220 * 1024 / (smem + 4096)) blocks = 220 * 1024 / (smem + 4096);
+  if (blocks > 32) blocks = 32;
+  if (blocks < 1) blocks = 1;
+  const int grid = p.T < num_sms * blocks ? p.T : num_sms * blocks;
+  launch_pdl(norm_block_ring_kernel<LAYERNORM, NV>, dim3((unsigned)grid), dim3((unsigned)threads), (size_t)smem, s, p);
+  return -(int)cudaGetLastError();
 }
 
 template <bool LAYERNORM, bool WIDE>
@@ -150,21 +336,27 @@ extern "C" {
 
 int lx_norm_block_max_width() { return lx::kRowThreads4 * 4 * 8; }
 
+// ring: -1 the library's choice, 0 or 1 (where rows begin at 16 bytes) a block per row or blocks that stay, to measure each.
 int lx_norm_block(const void* y, long long ldy, const void* residual, long long ldr, void* residual_out, long long ldro, const void* post_w,
-                  const void* post_b, const void* w, const void* b, const void* gate, long long gate_t, long long gate_h, void* out, long long ldo, void* q,
-                  long long ldq, void* q_scale, int T, int H, float eps, float w_offset, float scale, int layernorm, int num_sms, void* stream) {
+                  const void* post_b, const void* w, const void* b, const void* gate, long long gate_t, int gate_h, void* out, long long ldo, void* q,
+                  long long ldq, void* q_scale, int T, int H, float eps, float w_offset, float scale, int layernorm, int* status, int num_sms, int ring, void* stream) {
   using namespace lx;
   if (T <= 0) return 0;
   if (H <= 0 || H > lx_norm_block_max_width()) return -1;
   const auto bf = [](const void* a) { return reinterpret_cast<const __nv_bfloat16*>(a); };
-  NormBlockParams p{bf(y), bf(residual), reinterpret_cast<__nv_bfloat16*>(residual_out), bf(post_w), bf(post_b), bf(w), bf(b), bf(gate), gate_t, gate_h,
-                    reinterpret_cast<__nv_bfloat16*>(out), reinterpret_cast<int8_t*>(q), reinterpret_cast<float*>(q_scale), ldy, ldr, ldro, ldo, ldq, H, eps,
-                    w_offset, scale};
+  NormBlockParams p{bf(y), bf(residual), reinterpret_cast<__nv_bfloat16*>(residual_out), bf(post_w), bf(post_b), bf(w), bf(b), bf(gate), gate_t, gate_h, reinterpret_cast<uintptr_t>(gate) % 16 == 0 && gate_t % 8 == 0,
+                    reinterpret_cast<__nv_bfloat16*>(out), reinterpret_cast<int8_t*>(q), reinterpret_cast<float*>(q_scale), ldy, ldr, ldro, ldo, ldq, H, T, eps,
+                    w_offset, scale, status};
   uintptr_t bits = 0;
   for (const void* a : {y, residual, static_cast<const void*>(residual_out), post_w, post_b, w, b, static_cast<const void*>(out)}) bits |= reinterpret_cast<uintptr_t>(a);
   const bool wide = H % 8 == 0 && bits % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && (ldy | ldr | ldro | ldo | ldq) % 8 == 0;
   const RowShape r = row_shape(T, H, num_sms, kRowThreads4);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (wide && (ring < 0 ? T >= kNormRingRows * num_sms : ring)) {
+    const bool two = H <= 2 * 8 * kRowThreads4;
+    if (layernorm) return two ? launch_norm_ring<true, 2>(p, num_sms, s) : launch_norm_ring<true, 4>(p, num_sms, s);
+    return two ? launch_norm_ring<false, 2>(p, num_sms, s) : launch_norm_ring<false, 4>(p, num_sms, s);
+  }
   if (layernorm) {
     if (wide) launch_norm_block<true, true>(p, T, r, s);
     else launch_norm_block<true, false>(p, T, r, s);

@@ -20,10 +20,12 @@ P, I, L, F = c_void_p, c_int, c_longlong, c_float
 
 SIGNATURES = {
     "lx_norm_block_max_width": ([], I),
-    "lx_norm_block": ([P, L, P, L, P, L, P, P, P, P, P, L, L, P, L, P, L, P, I, I, F, F, F, I, I, P], I),
+    "lx_norm_block": ([P, L, P, L, P, L, P, P, P, P, P, L, I, P, L, P, L, P, I, I, F, F, F, I, P, I, I, P], I),
     "lx_rows_int8": ([P, L, P, L, P, P, L, I, I, I, I, I, P], I),
     "lx_gemm_int8_max_k": ([], I),
-    "lx_gemm_int8": ([P, L, P, P, L, P, P, P, L, I, I, I, I, P, I, P], I),
+    "lx_gemm_int8_plan": ([I, I, I, I, P, P], I),
+    "lx_gemm_int8_clusters": ([I], I),
+    "lx_gemm_int8": ([P, L, P, P, L, P, P, P, L, I, I, I, I, P, I, I, P], I),
 }
 
 
@@ -39,6 +41,18 @@ def _bf16(op: str, t: torch.Tensor):
         raise ValueError(f"{op}: the kernels are bf16; got {t.dtype}")
 
 
+_devices = {}
+
+
+def _device(at: int):
+    """(SMs, status words' address) of a device, which live as long as its workspace."""
+    known = _devices.get(at)
+    if known is None:
+        ws = nv.workspace(torch.device("cuda", at))
+        known = _devices[at] = (ws.num_sms, ws.status.data_ptr())
+    return known
+
+
 def _pitch(t: Optional[torch.Tensor]) -> int:
     """Elements between two rows (one row's own stride says nothing)."""
     return 0 if t is None else t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
@@ -49,7 +63,7 @@ def _rows(x: torch.Tensor, T: int, n: int, act: int, gated: bool, out: Optional[
     r = empty_int8_rows(T, n, x.device)
     if T:
         rc = nv.load().lx_rows_int8(x.data_ptr(), _pitch(x), r.q.data_ptr(), _pitch(r.q), r.scale.data_ptr(), nv._ptr(out), _pitch(out), T, n, act,
-                                    int(gated), nv.workspace(x.device).num_sms, stream)
+                                    int(gated), _device(x.get_device())[0], stream)
         nv._check(rc, "lx_rows_int8")
     return r
 
@@ -82,7 +96,7 @@ def norm_block(y: Optional[torch.Tensor], residual: torch.Tensor, weight: torch.
 
 
 @_on_its_device
-def _norm_block(residual, y, weight, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, to, out, int8):
+def _norm_block(residual, y, weight, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, to, out, int8, ring=-1):
     T, H = residual.shape
     stream = _stream_of(residual)
     if out is None and not int8:
@@ -90,10 +104,11 @@ def _norm_block(residual, y, weight, eps, post_weight, gate, scale, bias, post_b
     r = empty_int8_rows(T, H, residual.device) if int8 else None
     if T:
         q, q_scale = r if int8 else (None, None)
+        sms, status = _device(residual.get_device())
         rc = nv.load().lx_norm_block(nv._ptr(y), _pitch(y), residual.data_ptr(), _pitch(residual), nv._ptr(to), _pitch(to), nv._ptr(post_weight),
                                      nv._ptr(post_bias), weight.data_ptr(), nv._ptr(bias), nv._ptr(gate), 0 if gate is None or T == 1 else gate.stride(0),
                                      0 if gate is None or H == 1 else gate.stride(1), nv._ptr(out), _pitch(out), nv._ptr(q), _pitch(q), nv._ptr(q_scale),
-                                     T, H, eps, weight_offset, scale, int(layernorm), nv.workspace(residual.device).num_sms, stream)
+                                     T, H, eps, weight_offset, scale, int(layernorm), status, sms, ring, stream)
         nv._check(rc, "lx_norm_block")
     return r if int8 else out
 
@@ -109,14 +124,16 @@ def gemm_int8(x: Int8Rows, w: torch.Tensor, w_scale: torch.Tensor, bias: Optiona
 
 
 @_on_its_device
-def _gemm_int8(q, scale, w, w_scale, bias, out, w_const):
+def _gemm_int8(q, scale, w, w_scale, bias, out, w_const, plan=None):
+    """`plan`: (by pairs of CTAs, token tile, parts of K) in place of the library's choice, to measure and test each."""
     (T, K), N = q.shape, w.shape[0]
     stream = _stream_of(q)
     if out is None:
         out = torch.empty(T, N, dtype=torch.bfloat16, device=q.device)
     if T and N:
-        ws = nv.workspace(q.device)
+        sms, status = _device(q.get_device())
+        force = 0 if plan is None else 1 + int(plan[0]) + 2 * (plan[2] | plan[1] << 8)
         rc = nv.load().lx_gemm_int8(q.data_ptr(), _pitch(q), scale.data_ptr(), w.data_ptr(), _pitch(w), w_scale.data_ptr(), nv._ptr(bias), out.data_ptr(),
-                                    out.stride(0) if T > 1 else N, T, N, K, int(w_const), ws.status.data_ptr(), ws.num_sms, stream)
+                                    out.stride(0) if T > 1 else N, T, N, K, int(w_const), status, sms, force, stream)
         nv._check(rc, "lx_gemm_int8")
     return out

@@ -1227,7 +1227,7 @@ class Int8Rows(NamedTuple):
 
 
 def empty_int8_rows(T: int, K: int, device) -> Int8Rows:
-    return Int8Rows(torch.empty(T, (K + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :K], torch.empty(T, dtype=torch.float32, device=device))
+    return Int8Rows(torch.empty_strided((T, K), ((K + 15) // 16 * 16, 1), dtype=torch.int8, device=device), torch.empty(T, dtype=torch.float32, device=device))
 
 
 def _to_int8_rows(v) -> Int8Rows:
@@ -1259,33 +1259,41 @@ def quantize_weight_int8(w: torch.Tensor):
 
 
 def _span(t):
-    """First byte, bytes of a row, bytes between two rows, rows."""
-    size = t.element_size()
-    if t.dim() < 2 or t.shape[0] == 1 or t.is_contiguous():
-        return t.data_ptr(), t.numel() * size, t.numel() * size, 1
-    return t.data_ptr(), t.shape[1] * size, t.stride(0) * size, t.shape[0]
+    """First byte, the byte behind the last one."""
+    n, at = t.element_size(), t.data_ptr()
+    for size, step in zip(t.shape, t.stride()):
+        if size == 0:
+            return at, at
+        n += (size - 1) * step * t.element_size()
+    return at, at + n
 
 
-def _apart(a, b) -> bool:
-    """Whether no byte of one tensor (rows without gaps in them) is one of the other's, as far as their strides say: rows of the same distance may take turns, others
-    have to lie one tensor behind the other."""
-    if a is None or b is None or not a.numel() or not b.numel():
-        return True
-    (pa, na, sa, ra), (pb, nb, sb, rb) = _span(a), _span(b)
-    if pa + sa * (ra - 1) + na <= pb or pb + sb * (rb - 1) + nb <= pa:
-        return True
-    if sa != sb or ra == 1 or rb == 1:
+def _turns(a, b) -> bool:
+    """Whether two matrices of overlapping extents share no byte: their rows, of the same distance, take turns in one buffer."""
+    if a.dim() != 2 or b.dim() != 2 or a.shape[0] == 1 or b.shape[0] == 1:
         return False
-    d = (pb - pa) % sa
+    (na, sa), (nb, sb) = ((t.shape[1] * t.element_size(), t.stride(0) * t.element_size()) for t in (a, b))
+    d = (b.data_ptr() - a.data_ptr()) % sa if sa == sb and sa > 0 else 0
     return d >= na and sa - d >= nb
 
 
-def _same(a, b) -> bool:
-    return b is not None and a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
+def _apart(a, others) -> bool:
+    """Whether no byte of `a` is one of the others', as far as their extents and the distances of their rows say."""
+    lo, hi = _span(a)
+    for b in others:
+        if b is not None:
+            p, q = _span(b)
+            if lo < q and p < hi and not _turns(a, b):
+                return False
+    return True
 
 
 def _rows_fit(t, T: int, n: int) -> bool:
-    return t.dim() == 2 and t.shape == (T, n) and (n <= 1 or t.stride(1) == 1) and (T <= 1 or t.stride(0) >= n)
+    """[T, n], the values of a row neighbours, the rows one behind the other."""
+    if t.shape != (T, n):
+        return False
+    s0, s1 = t.stride()
+    return (s1 == 1 or n <= 1) and (s0 >= n or T <= 1)
 
 
 def check_quant_rows_int8(x):
@@ -1311,7 +1319,7 @@ def check_act_mul_int8(x, inter, act, gated, out):
         raise ValueError(f"act_mul_int8: rows of {n} neighbouring values; got {tuple(x.shape)}, strides {x.stride()}")
     if act not in INT8_ACTS:
         raise ValueError(f"act_mul_int8: activation {act!r}")
-    if out is not None and not (out.dtype == x.dtype and out.device == x.device and _rows_fit(out, T, inter) and _apart(out, x)):
+    if out is not None and not (out.dtype == x.dtype and out.device == x.device and _rows_fit(out, T, inter) and _apart(out, (x,))):
         raise ValueError("act_mul_int8: out [T, features] is of x's type and device, and lies apart from it")
     return T
 
@@ -1332,44 +1340,58 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
     """-> (T, H, gate as [T, H] or None, what h is written to or None)."""
     if not (isinstance(residual, torch.Tensor) and residual.dim() == 2 and residual.is_floating_point()):
         raise ValueError("norm_block: residual [T, H] of numbers")
-    T, H = residual.shape
+    if residual_out is residual:
+        residual_out = None
+    shape, dtype, at, size = residual.shape, residual.dtype, residual.get_device(), residual.element_size()
+    T, H = shape
     if not 1 <= H <= NORM_BLOCK_MAX_WIDTH:
         raise ValueError(f"norm_block: rows of 1 to {NORM_BLOCK_MAX_WIDTH} values; got {H}")
-    rows = {"y": y, "residual": residual, "residual_out": residual_out, "out": out}
-    for name, t in rows.items():
-        if t is not None and not (t.dtype == residual.dtype and t.device == residual.device and _rows_fit(t, T, H)):
-            raise ValueError(f"norm_block: {name} is [T, H] with neighbouring values in a row, of the residual's type and device")
-    if y is None and not (post_weight is None and gate is None and scale == 1.0 and residual_out is None):
-        raise ValueError("norm_block: without y there is nothing to norm, gate, scale or write back")
-    if post_bias is not None and post_weight is None:
-        raise ValueError("norm_block: post_bias without post_weight")
-    vectors = {"weight": weight, "post_weight": post_weight, "bias": bias, "post_bias": post_bias}
-    for name, t in vectors.items():
-        if t is None and name != "weight":
-            continue
-        if not (isinstance(t, torch.Tensor) and t.shape == (H,) and t.is_contiguous() and t.dtype == residual.dtype and t.device == residual.device):
-            raise ValueError(f"norm_block: {name} is [H], contiguous, of the residual's type and device")
-    given = gate
-    if gate is not None:
-        if not (gate.dtype == residual.dtype and gate.device == residual.device and gate.dim() <= 2):
-            raise ValueError("norm_block: gate is of the residual's type and device")
-        try:
-            gate = gate.expand(T, H)
-        except RuntimeError:
-            raise ValueError(f"norm_block: a gate of {tuple(gate.shape)} for rows of {(T, H)}: one, [H], [T, 1] or [T, H]") from None
-    to = None if y is None else residual if residual_out is None else residual_out
-    for name, t in (("residual_out", to), ("out", out)):
+    spans = {}                                       # of what is read and written: first byte, the byte behind the last one
+    for name, t in (("y", y), ("residual", residual), ("residual_out", residual_out), ("out", out)):
         if t is None:
             continue
-        # a row's values are read before they are written, at the same places
-        if not (all(_apart(t, v) for v in vectors.values()) and all(_same(t, v) or _apart(t, v) for v in (y, residual))
-                and _apart(t, given)):
-            raise ValueError(f"norm_block: {name} lies apart from the inputs, or is y or the residual itself")
-    if gate is not None and H > 1 and T > 0 and gate.stride(1) not in (0, 1):
-        raise ValueError("norm_block: a row's gates are neighbours, or one for all")
-    if to is not None and out is not None and not _apart(to, out):
-        raise ValueError("norm_block: out and the residual lie apart")
-    return T, H, gate, to
+        if not (t.shape == shape and t.dtype == dtype and t.get_device() == at):
+            raise ValueError(f"norm_block: {name} is [T, H], of the residual's type and device")
+        s0, s1 = t.stride()
+        if (s1 != 1 and H > 1) or (s0 < H and T > 1):
+            raise ValueError(f"norm_block: {name} has neighbouring values in a row, and rows one behind the other")
+        p = t.data_ptr()
+        spans[name] = (p, p + ((T - 1) * s0 + H) * size if T else p, t)
+    for name, t in (("weight", weight), ("post_weight", post_weight), ("bias", bias), ("post_bias", post_bias)):
+        if t is None and name != "weight":
+            continue
+        if not (isinstance(t, torch.Tensor) and t.dim() == 1 and t.shape[0] == H and t.is_contiguous() and t.dtype == dtype and t.get_device() == at):
+            raise ValueError(f"norm_block: {name} is [H], contiguous, of the residual's type and device")
+        p = t.data_ptr()
+        spans[name] = (p, p + H * size, t)
+    if post_bias is not None and post_weight is None:
+        raise ValueError("norm_block: post_bias without post_weight")
+    if y is None:
+        if not (post_weight is None and gate is None and scale == 1.0 and residual_out is None):
+            raise ValueError("norm_block: without y there is nothing to norm, gate, scale or write back")
+        to = None
+    else:
+        to = residual if residual_out is None else residual_out
+    gates = None
+    if gate is not None:
+        if not (gate.dtype == dtype and gate.get_device() == at and gate.dim() <= 2):
+            raise ValueError("norm_block: gate is of the residual's type and device")
+        try:
+            gates = gate.expand(T, H)
+        except RuntimeError:
+            raise ValueError(f"norm_block: a gate of {tuple(gate.shape)} for rows of {(T, H)}: one, [H], [T, 1] or [T, H]") from None
+        if H > 1 and T > 0 and gates.stride(1) not in (0, 1):
+            raise ValueError("norm_block: a row's gates are neighbours, or one for all")
+        spans["gate"] = (*_span(gate), gate)
+    # a row's values are read before they are written, at the same places: a result may be y or the residual itself
+    written = ("residual",) if to is residual else ("residual_out",) if to is not None else ()
+    for name in written if out is None else (*written, "out"):
+        lo, hi, a = spans[name]
+        for other, (p, q, b) in spans.items():
+            if lo < q and p < hi and other != name and not _turns(a, b) and not (
+                    p == lo and b.shape == a.shape and b.stride() == a.stride() and other in ("y", "residual") and (other not in written)):
+                raise ValueError(f"norm_block: {name} lies on {other} (results lie apart from each other and from the inputs, or are y or the residual itself)")
+    return T, H, gates, to
 
 
 def norm_block(y, residual, weight, eps, post_weight=None, gate=None, scale: float = 1.0, bias=None, post_bias=None, weight_offset: float = 0.0,
@@ -1405,20 +1427,23 @@ def check_gemm_int8(x, w, w_scale, bias, out, dtype):
     if not isinstance(x, Int8Rows):
         raise ValueError("gemm_int8: x is the Int8Rows of a quantiser")
     q, scale = x
-    if not (q.dim() == 2 and w.dim() == 2 and q.dtype == w.dtype == torch.int8 and q.shape[1] == w.shape[1]):
+    if not (q.dim() == 2 and w.dim() == 2 and q.dtype == torch.int8 and w.dtype == torch.int8 and q.shape[1] == w.shape[1]):
         raise ValueError(f"gemm_int8: int8 rows [T, K] and weights [N, K]; got {tuple(q.shape)} {q.dtype}, {tuple(w.shape)} {w.dtype}")
-    (T, K), N = q.shape, w.shape[0]
+    (T, K), N, at = q.shape, w.shape[0], q.get_device()
     if not (1 <= K <= INT8_MAX_K):
         raise ValueError(f"gemm_int8: K from 1 to {INT8_MAX_K}, whose sums stay whole; got {K}")
     for name, t, n in (("rows", q, T), ("weights", w, N)):
-        if not ((K == 1 or t.stride(1) == 1) and (n <= 1 or (t.stride(0) >= K and t.stride(0) % 16 == 0)) and (n == 0 or t.data_ptr() % 16 == 0)):
+        s0, s1 = t.stride()
+        if not ((K == 1 or s1 == 1) and (n <= 1 or (s0 >= K and s0 % 16 == 0)) and (n == 0 or t.data_ptr() % 16 == 0)):
             raise ValueError(f"gemm_int8: {name} begin at 16 bytes and lie a multiple of 16 bytes apart; got strides {t.stride()}")
     for name, t, n in (("the rows' scales", scale, T), ("w_scale", w_scale, N)):
-        if not (t.shape == (n,) and t.dtype == torch.float32 and t.is_contiguous() and t.device == q.device):
-            raise ValueError(f"gemm_int8: {name} are [{n}] fp32 on the rows' device")
-    if not (w.device == q.device and (bias is None or (bias.shape == (N,) and bias.dtype == dtype and bias.is_contiguous() and bias.device == q.device))):
-        raise ValueError(f"gemm_int8: weights and bias [{N}] {dtype} on the rows' device")
-    if out is not None and not (out.dtype == dtype and out.device == q.device and _rows_fit(out, T, N) and all(_apart(out, t) for t in (q, scale, w, w_scale, bias))):
+        if not (t.dim() == 1 and t.shape[0] == n and t.dtype == torch.float32 and t.is_contiguous() and t.get_device() == at):
+            raise ValueError(f"gemm_int8: {name} are [{n}] fp32, contiguous, on the rows' device")
+    if bias is not None and not (bias.shape == (N,) and bias.dtype == dtype and bias.is_contiguous() and bias.get_device() == at):
+        raise ValueError(f"gemm_int8: bias is [{N}] {dtype}, contiguous, on the rows' device")
+    if w.get_device() != at:
+        raise ValueError("gemm_int8: weights on the rows' device")
+    if out is not None and not (out.dtype == dtype and out.get_device() == at and _rows_fit(out, T, N) and _apart(out, (q, scale, w, w_scale, bias))):
         raise ValueError(f"gemm_int8: out is [T, N] {dtype} on the rows' device, apart from the inputs")
     return T, N, K
 

@@ -130,7 +130,7 @@ def test_norms_that_are_refused(change):
 def test_results_on_top_of_inputs():
     """y and the residual may be written over, value by value; anything else may not, and rows of one buffer may take turns."""
     buf = torch.zeros(3, 32, dtype=BF)
-    ok = [dict(out=NORM["y"]), dict(residual_out=NORM["y"]), dict(y=buf[:, :16], residual=buf[:, 16:]), dict(y=buf[:, :16], residual=buf[:, 16:], out=buf[:, :16])]
+    ok = [dict(residual_out=NORM["residual"]), dict(y=NORM["residual"]), dict(out=NORM["y"]), dict(residual_out=NORM["y"]), dict(y=buf[:, :16], residual=buf[:, 16:]), dict(y=buf[:, :16], residual=buf[:, 16:], out=buf[:, :16])]
     for change in ok:
         ref.norm_block(**{**NORM, **change})
     vec = torch.ones(48, dtype=BF)

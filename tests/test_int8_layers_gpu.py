@@ -4,6 +4,7 @@ Tolerances.  A result in bf16 is rounded once: 2^-8 of it.  What is computed in 
 import pytest
 import torch
 
+from lorax_b200.ops import native, native_int8  # noqa: F401  (the bindings of every operator first)
 from lorax_b200.ops import reference as ref
 from lorax_b200.ops.reference import Int8Rows
 
@@ -130,7 +131,12 @@ def _norm64(v, w, b, eps, offset, layernorm):
     return y, slack
 
 
-def _check_norm(ops, T, H, post, gate, scale, layernorm, int8, bias=True, offset=0.0, eps=1e-5, at=0):
+def _check_norm(ops, T, H, post, gate, scale, layernorm, int8, bias=True, offset=0.0, eps=1e-5, at=0, ring=-1):
+    def call(y, res, w, eps, post_weight=None, gate=None, scale=1.0, bias=None, post_bias=None, weight_offset=0.0, layernorm=False, residual_out=None, out=None, int8=False):
+        if ring < 0:
+            return ops.norm_block(y, res, w, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, residual_out, out, int8)
+        _, _, gate, to = ref.check_norm_block(y, res, w, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
+        return native_int8._norm_block(res, y, w, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, to, out, int8, ring=ring)
     g = _gen(T, H, post, scale, layernorm)
     wide = H + at
     y, res = _randn(g, T, wide)[:, at:], _randn(g, T, wide, std=3.0)[:, at:]
@@ -142,7 +148,7 @@ def _check_norm(ops, T, H, post, gate, scale, layernorm, int8, bias=True, offset
     keep = res.clone()
     kw = dict(post_weight=pw if post else None, gate=gate, scale=scale, bias=b, post_bias=pb if post else None, weight_offset=offset, layernorm=layernorm)
     out = torch.full((T, H), 5.0, device="cuda", dtype=BF) if int8 == "both" else None
-    x = ops.norm_block(y, res, w, eps, residual_out=h, out=out, int8=bool(int8), **kw)
+    x = call(y, res, w, eps, residual_out=h, out=out, int8=bool(int8), **kw)
     assert torch.equal(res, keep)
     part, slack = (y.double(), 0.0) if not post else _norm64(y.double(), pw, kw["post_bias"], eps, offset, layernorm)
     f = scale * (1.0 if gate is None else gate.double())
@@ -157,7 +163,7 @@ def _check_norm(ops, T, H, post, gate, scale, layernorm, int8, bias=True, offset
     if value is not None:
         assert ((value.double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
     # in place, the same bits
-    again = ops.norm_block(y, res, w, eps, int8=bool(int8), **kw)
+    again = call(y, res, w, eps, int8=bool(int8), **kw)
     assert torch.equal(res, h) and (torch.equal(again.q, x.q) and torch.equal(again.scale, x.scale) if int8 else torch.equal(again, x))
 
 
@@ -173,6 +179,24 @@ def test_norms(ops, T, H, layernorm, int8):
 @pytest.mark.parametrize("H", [512, 333])
 def test_gates(ops, gate, post, int8, H):
     _check_norm(ops, 37, H, post, gate, 0.22, False, int8, bias=False, offset=1.0)
+
+
+@pytest.mark.parametrize("gate", ["none", "one", "channel", "token", "all"])
+@pytest.mark.parametrize("T,H", [(1, 8), (3, 256), (700, 64), (1300, 1000), (700, 4096), (301, 8192), (300, 16384)])
+@pytest.mark.parametrize("layernorm", [False, True])
+def test_both_forms_of_norms(ops, gate, T, H, layernorm):
+    """A block per row, and blocks that stay."""
+    for ring in (0, 1):
+        _check_norm(ops, T, H, gate != "one", gate, 0.5, layernorm, "both" if gate in ("token", "all") else gate == "none", ring=ring, bias=layernorm)
+
+
+def test_a_norm_without_a_block_in_front_by_both_forms(ops):
+    g = _gen(9)
+    res, w = _randn(g, 700, 512), _randn(g, 512)
+    a, b = (native_int8._norm_block(res, None, w, 1e-5, None, None, 1.0, None, None, 0.0, False, None, None, False, ring=ring) for ring in (0, 1))
+    want, slack = _norm64(res.double(), w, None, 1e-5, 0.0, False)
+    for x in (a, b, ops.norm_block(None, res, w, 1e-5)):
+        assert ((x.double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
 
 
 @pytest.mark.parametrize("at", [1, 8])
@@ -214,12 +238,15 @@ def test_large_means_do_not_cost_a_layer_norm_its_precision(ops):
 
 
 # ------------------------------------------------------------------------------------------------ products
-def _check_product(ops, T, N, K, bias=True, at=0, out=None):
+def _check_product(ops, T, N, K, bias=True, at=0, out=None, plan=None):
     g = _gen(T, N, K)
     q, w = _int8(g, T, K, at), _int8(g, N, K, at)
     xs, ws = torch.rand(T, generator=g, device="cuda") * 0.1, torch.rand(N, generator=g, device="cuda") * 0.01
     b = _randn(g, N) if bias else None
-    y = ops.gemm_int8(Int8Rows(q, xs), w, ws, bias=b, out=out)
+    if plan is None:
+        y = ops.gemm_int8(Int8Rows(q, xs), w, ws, bias=b, out=out)
+    else:
+        y = native_int8._gemm_int8(q, xs, w, ws, b, out, False, plan=plan)
     s = (q.double() @ w.double().t()) * (xs.double()[:, None] * ws.double())
     want = s + (0 if b is None else b.double())
     # the sum to 32 bits, two products, the bias: four roundings; then one to bf16
@@ -251,6 +278,20 @@ def test_products_of_any_depth(ops, K, T):
                                    (700, 11008, 2048), (4001, 2050, 520)])
 def test_large_products(ops, T, N, K):
     _check_product(ops, T, N, K)
+
+
+@pytest.mark.parametrize("pairs,bn,parts", [(False, 16, 1), (False, 48, 8), (False, 128, 3), (False, 256, 5), (True, 32, 1), (True, 96, 1), (True, 256, 1), (True, 64, 2),
+                                            (True, 256, 3), (True, 160, 4)])
+@pytest.mark.parametrize("T,N,K", [(1, 300, 1100), (33, 129, 1024), (520, 1000, 1030), (300, 2050, 2048)])
+def test_every_plan(ops, pairs, bn, parts, T, N, K):
+    """Single CTAs and pairs, every share of K, tiles that end behind the last token and channel."""
+    _check_product(ops, T, N, K, plan=(pairs, bn, parts))
+
+
+def test_plans_that_do_not_exist_are_refused(ops):
+    for plan in ((False, 8, 1), (False, 272, 1), (False, 24, 1), (True, 48, 1), (True, 64, 5), (False, 64, 9), (False, 64, 0), (False, 64, 3)):
+        with pytest.raises(ops.NativeError):
+            _check_product(ops, 3, 64, 256, plan=plan)
 
 
 @pytest.mark.parametrize("T", [3, 400])
