@@ -45,7 +45,7 @@ const Flag kFlags[] = {
     {"adapter-source", "ADAPTER_SOURCE", "hub", "default adapter source"},
     {"revision", "REVISION", "", "model revision"},
     {"num-shard", "NUM_SHARD", "", "number of tensor-parallel shards"},
-    {"quantize", "QUANTIZE", "", "fp8 | gptq | awq | eetq | bitsandbytes ..."},
+    {"quantize", "QUANTIZE", "", "fp8 | w8a8 | gptq | awq | eetq | bitsandbytes ..."},
     {"dtype", "DTYPE", "", "float16 | bfloat16"},
     {"compile", "COMPILE", "true", "capture decode steps in CUDA graphs"},
     {"skip-download", "SKIP_DOWNLOAD", "false", "do not run the download-weights step before the shards start"},

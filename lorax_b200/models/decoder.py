@@ -16,7 +16,7 @@ from __future__ import annotations
 import os
 import math
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional
+from typing import Dict, List, NamedTuple, Optional
 
 import torch
 
@@ -56,6 +56,23 @@ class Fp8Weight:
     @property
     def shape(self):
         return self.q.shape
+
+
+@dataclass
+class Int8Weight:
+    """A projection matrix in 8-bit integers [N, K] with an fp32 scale for each output feature, for products with rows in 8 bits."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+
+class RowsInt8(NamedTuple):
+    """What a norm or an activation hands to a product in 8-bit integers: its rows, and the same in the model's dtype where adapters read them."""
+    rows: reference.Int8Rows
+    x: Optional[torch.Tensor]
 
 
 @dataclass
@@ -435,13 +452,31 @@ class DecoderModel:
         self.quantized = "fp8"
         self._native = None
 
+    def quantize_w8a8(self):
+        """Replace the dense projection matrices of every layer by 8-bit integers with a scale for each output feature.  Their products take activations in 8-bit
+        integers too, with a scale for each token, which the norms and the activations in front of them write (`ops.norm_block`, `ops.act_mul_int8`);
+        embeddings, norms, the lm_head, MoE experts and every LoRA adapter stay as they are."""
+        if self.mixed:
+            raise ValueError(f"quantisation of {self.config.model_type} is not supported")
+        for lw in self.layers:
+            for name in ("qkv_w", "o_w", "gate_up_w", "down_w"):
+                w = getattr(lw, name)
+                if isinstance(w, torch.Tensor) and w.dim() == 2:
+                    setattr(lw, name, Int8Weight(*reference.quantize_weight_int8(w)))
+                elif w is not None:
+                    raise ValueError("w8a8 takes dense projections; the checkpoint holds packed ones")
+        self.quantized = "w8a8"
+        self._native = None
+
     def quantize(self, method: str, group: int = 128):
         """Weight-only quantisation of the dense projection matrices on load (`--quantize` of the reference's shard CLI,
         cli.py:15-28): 4-bit groups (`gptq`, `awq`, `int4`), int8 per channel (`eetq`, `bitsandbytes`, `int8`), the nf4 / fp4
-        code books (`bitsandbytes-nf4`, `bitsandbytes-fp4`) and HQQ at 4 / 3 / 2 bits.  Matrices the checkpoint already
+        code books (`bitsandbytes-nf4`, `bitsandbytes-fp4`) and HQQ at 4 / 3 / 2 bits; `fp8` and `w8a8` quantise the activations too.  Matrices the checkpoint already
         holds in packed form are left as loaded."""
         if method == "fp8":
             return self.quantize_fp8()
+        if method == "w8a8":
+            return self.quantize_w8a8()
         if self.mixed:
             raise ValueError(f"quantisation of {self.config.model_type} is not supported")
         from ..utils.quant_formats import quantize_weight
@@ -478,6 +513,8 @@ class DecoderModel:
         """Base GEMM plus the multi-adapter LoRA delta for the projection group.  On a GPU with the rows grouped by adapter
         that is ONE launch (shrink items, base tiles, expand UMMAs); otherwise a shrink launch, the GEMM and an expand launch."""
         ts = tok_slot if tok_slot is not None else inp.tok_slot
+        if isinstance(w, Int8Weight):
+            return self._linear_int8(x, w, b, group, layer, inp, ts)
         epi = None
         if (self.fused_lora and x.shape[0] <= self.fused_lora_max_tokens and self.adapters is not None and ts is not None
                 and inp.lora_tiles is not None and x.is_cuda and x.dtype == torch.bfloat16):
@@ -502,9 +539,26 @@ class DecoderModel:
         self.adapters.expand(self.ops, epi, y, tiles=inp.lora_tiles)
         return y
 
+    def _linear_int8(self, x, w: Int8Weight, b, group: str, layer: int, inp: StepInputs, ts):
+        """The product in 8-bit integers plus the adapters' delta, which comes from the rows in the model's dtype."""
+        rows, x = x if isinstance(x, RowsInt8) else (self.ops.quant_rows_int8(x), x)
+        epi = None
+        if self.adapters is not None and ts is not None and x is not None:
+            epi = self.adapters.shrink(self.ops, x, ts, group, layer, tiles=inp.lora_tiles)
+        y = self.ops.gemm_int8(rows, w.q, w.scale, bias=b, dtype=self.dtype, w_const=True)
+        if epi is not None:
+            self.adapters.expand(self.ops, epi, y, tiles=inp.lora_tiles)
+        return y
+
+    def _adapters_read(self, inp: StepInputs) -> bool:
+        return self.adapters is not None and self.adapters.max_rank > 0 and inp.tok_slot is not None
+
     def _row_parallel(self, x, w, b, group: str, layer: int, inp: StepInputs):
         """Row-parallel projection + all-reduce.  With the NVLink kernels enabled and a decode-sized batch this is one
         fused GEMM -> reduce-scatter -> all-gather kernel; the rank's partial LoRA delta is reduced with it."""
+        if isinstance(w, Int8Weight):
+            out = self._linear(x, w, b, group, layer, inp)
+            return self.tp.all_reduce(out) if self.tp.world_size > 1 else out
         fused = self.tp.fused if self.tp.world_size > 1 else None
         if (fused is not None and x.is_cuda and x.shape[0] <= min(fused.MAX_TOKENS, fused.max_fused_tokens) and b is None
                 and not self.config.parallel_residual and isinstance(w, torch.Tensor)):
@@ -565,6 +619,8 @@ class DecoderModel:
             h = h + self.pos_embed[inp.positions.long() + c.position_offset]
         if self.embed_norm is not None:
             h = self._norm(h, None, self.embed_norm, self.embed_norm_b)
+        if self.quantized == "w8a8":
+            return self._score(self._layers_int8(h, inp, kv_cache), inp)
         residual = h
         pending = None      # output of the previous block that still has to be added to the residual stream
         rm = c.residual_multiplier
@@ -592,6 +648,32 @@ class DecoderModel:
             pending = self._moe(normed2, lw, li, inp) if c.is_moe else self._mlp(normed2, lw, li, inp)
         hidden = self._norm(pending, residual, self.final_norm, self.final_norm_b, x_scale=rm)
         return self._score(hidden, inp)
+
+    def _layers_int8(self, residual, inp: StepInputs, kv_cache) -> torch.Tensor:
+        """The layers with projections in 8-bit integers -> the normed stream.  One launch adds what a block gave to the stream (behind its own norm and times the
+        residual multiplier, where the model has them), norms it for the next block and leaves rows in 8 bits."""
+        c, ops = self.config, self.ops
+
+        def norm(y, w, b=None, post=None, int8=True):
+            out = torch.empty_like(residual) if int8 and self._adapters_read(inp) else None
+            r = ops.norm_block(y, residual, w, c.rms_norm_eps, post_weight=post, scale=c.residual_multiplier if y is not None and post is None else 1.0, bias=b,
+                               weight_offset=c.norm_weight_offset, layernorm=c.norm_type.startswith("layernorm"), out=out, int8=int8)
+            return RowsInt8(r, out) if int8 else r
+        pending = post = None      # output of the block in front that is not yet part of the stream, and the weight of its own norm
+        for li, lw in enumerate(self.layers):
+            normed = norm(pending, lw.input_norm, lw.input_norm_b, post)
+            attn_out = self._attention(normed, lw, li, inp, kv_cache[li])
+            post = None
+            if c.parallel_residual:
+                mlp_in = normed if lw.post_norm is None else norm(None, lw.post_norm, lw.post_norm_b)
+                pending = attn_out + self._mlp(mlp_in, lw, li, inp)
+            elif lw.post_ffn_norm is not None:
+                pending, post = self._mlp(norm(attn_out, lw.pre_ffn_norm, post=lw.post_norm), lw, li, inp), lw.post_ffn_norm
+            elif c.is_moe:
+                pending = self._moe(norm(attn_out, lw.post_norm, lw.post_norm_b, int8=False), lw, li, inp)
+            else:
+                pending = self._mlp(norm(attn_out, lw.post_norm, lw.post_norm_b), lw, li, inp)
+        return norm(pending, self.final_norm, self.final_norm_b, post, int8=False)
 
     def _forward_post(self, inp: StepInputs, kv_cache) -> torch.Tensor:
         """Layers that read the fp32 stream itself: every addition to the stream also leaves its copy in the model's dtype."""
@@ -688,6 +770,10 @@ class DecoderModel:
     def _mlp(self, x, lw: LayerWeights, li: int, inp: StepInputs):
         c, ops = self.config, self.ops
         gu = self._linear(x, lw.gate_up_w, lw.gate_up_b, "gate_up", li, inp)
+        if isinstance(lw.down_w, Int8Weight):
+            out = torch.empty(gu.shape[0], self.inter, dtype=gu.dtype, device=gu.device) if self._adapters_read(inp) else None
+            act = RowsInt8(ops.act_mul_int8(gu, self.inter, c.hidden_act, gated=self.gated, out=out), out)
+            return self._row_parallel(act, lw.down_w, lw.down_b, "down", li, inp)
         act = ops.act_mul(gu, self.inter, c.hidden_act, gated=self.gated, ahead=True)
         return self._row_parallel(act, lw.down_w, lw.down_b, "down", li, inp)
 

@@ -113,14 +113,14 @@ def _norm_block(residual, y, weight, eps, post_weight, gate, scale, bias, post_b
     return r if int8 else out
 
 
-def gemm_int8(x: Int8Rows, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, lora=None,
+def gemm_int8(x: Int8Rows, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
               dtype: torch.dtype = torch.bfloat16, w_const: bool = False) -> torch.Tensor:
-    """out[T, N] = (x.q @ w^T) * w_scale[n] * x.scale[t] + bias[n], the sums whole numbers, rounded to bf16 once (`reference.gemm_int8`).  `lora`, `w_const` as for
-    `gemm_wq`: (what the shrink returned, the step's tile table), added to the result by a launch of its own; the kernel in front writes no weights."""
+    """out[T, N] = (x.q @ w^T) * w_scale[n] * x.scale[t] + bias[n], the sums whole numbers, rounded to bf16 once (`reference.gemm_int8`).  `w_const` as for `gemm`: the
+    kernel in front on the stream does not write `w`."""
     check_gemm_int8(x, w, w_scale, bias, out, dtype)
     if dtype != torch.bfloat16:
         raise ValueError(f"gemm_int8: the kernels are bf16; got {dtype}")
-    return nv._lora_expand(_gemm_int8(x.q, x.scale, w, w_scale, bias, out, w_const), lora)
+    return _gemm_int8(x.q, x.scale, w, w_scale, bias, out, w_const)
 
 
 @_on_its_device

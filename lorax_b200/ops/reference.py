@@ -1448,7 +1448,7 @@ def check_gemm_int8(x, w, w_scale, bias, out, dtype):
     return T, N, K
 
 
-def gemm_int8(x: Int8Rows, w, w_scale, bias=None, out=None, lora=None, dtype=torch.bfloat16, w_const: bool = False):
+def gemm_int8(x: Int8Rows, w, w_scale, bias=None, out=None, dtype=torch.bfloat16, w_const: bool = False):
     """out[t, n] = (sum over k of x.q[t, k] * w[n, k]) * w_scale[n] * x.scale[t] + bias[n]: the sums whole, the rest in 32 bits, one rounding to `dtype`."""
     T, N, K = check_gemm_int8(x, w, w_scale, bias, out, dtype)
     y = (x.q.double() @ w.double().t()).float() * w_scale * x.scale[:, None]

@@ -12,7 +12,7 @@ import sys
 import threading
 import time
 
-QUANTIZE_CHOICES = ["bitsandbytes", "bitsandbytes-nf4", "bitsandbytes-fp4", "gptq", "awq", "eetq", "hqq-4bit", "hqq-3bit", "hqq-2bit", "fp8", "fp8-kv"]
+QUANTIZE_CHOICES = ["bitsandbytes", "bitsandbytes-nf4", "bitsandbytes-fp4", "gptq", "awq", "eetq", "hqq-4bit", "hqq-3bit", "hqq-2bit", "fp8", "fp8-kv", "w8a8"]
 
 
 def _log(level: str, msg: str, as_json: bool):

@@ -203,3 +203,54 @@ def test_limits_of_the_library_and_of_python_agree(monkeypatch):
         with pytest.raises(native.NativeError, match="C\\+\\+ says"):
             native_int8.check_limits(native.load())
         monkeypatch.undo()
+
+
+# ------------------------------------------------------------------------------------------------ models
+def _step(model, T=9):
+    from lorax_b200.models.decoder import StepInputs
+    c = model.config
+    kv = [torch.zeros(2, model.nkv, 2, 32, model.d, dtype=model.dtype) for _ in range(c.num_hidden_layers)]
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    seq, q0 = ref.prefill_tiles([T])
+    inp = StepInputs(input_ids=torch.arange(3, 3 + T, dtype=torch.int32), positions=torch.arange(T, dtype=torch.int32), slots=torch.arange(32, 32 + T, dtype=torch.int32),
+                     is_prefill=True, block_tables=i32(1).view(1, 1), cu_q=i32(0, T), cache_lens=i32(0), tile_seq=torch.as_tensor(seq, dtype=torch.int32),
+                     tile_q0=torch.as_tensor(q0, dtype=torch.int32))
+    return model.forward(inp, kv)
+
+
+@pytest.mark.parametrize("kind", ["llama", "gemma2", "granite", "gpt_neox", "cohere", "gpt2", "mixtral"])
+def test_a_model_in_8_bit_integers_is_near_the_same_in_32_bits(kind):
+    """Norms on both sides (gemma2), residual multiplier (granite), parallel blocks with one norm or two (cohere, gpt_neox), layer norms and biases (gpt2), experts."""
+    from lorax_b200.config import ModelConfig
+    from lorax_b200.models.decoder import DecoderModel, Int8Weight
+    more = dict(gemma2=dict(norm_weight_offset=1.0, tie_word_embeddings=True, hidden_act="gelu_pytorch_tanh"), granite=dict(residual_multiplier=0.22),
+                gpt_neox=dict(parallel_residual=True, norm_type="layernorm", hidden_act="gelu"), cohere=dict(parallel_residual=True, norm_type="layernorm_nobias"),
+                gpt2=dict(norm_type="layernorm", learned_positions=True, mlp_bias=True, attention_bias=True, hidden_act="gelu_new"),
+                mixtral=dict(num_local_experts=4, num_experts_per_tok=2)).get(kind, {})
+    c = ModelConfig(model_type=kind, hidden_size=64, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=4 if kind == "gpt2" else 2, intermediate_size=96, vocab_size=128,
+                    head_dim=16, max_position_embeddings=64, **more)
+    dense = DecoderModel.random_init(c, "cpu", torch.float32, seed=3, std=0.1)
+    small = DecoderModel.random_init(c, "cpu", torch.float32, seed=3, std=0.1)
+    small.quantize("w8a8")
+    assert small.quantized == "w8a8" and all(isinstance(lw.qkv_w, Int8Weight) and isinstance(lw.o_w, Int8Weight) for lw in small.layers)
+    a, b = _step(dense), _step(small)
+    assert torch.isfinite(b).all()
+    # twelve products, each off by two roundings of a 127th of a row's largest value (some 3 deviations), 0.29 / 127 * 3 = 0.7 % of a result twice, of random
+    # sign: 0.01 * sqrt(12) = 3.4 %; twice that for what attention and norms make of it
+    assert (a - b).norm() / a.norm() < 0.07
+    again = DecoderModel.random_init(c, "cpu", torch.float32, seed=3, std=0.1)
+    again.quantize("w8a8")
+    assert torch.equal(_step(again), b)
+
+
+def test_layer_by_layer_designs_are_not_quantised():
+    from lorax_b200.models.decoder import DecoderModel
+    m = DecoderModel.__new__(DecoderModel)
+    m.mixed, m.config = True, type("C", (), dict(model_type="x"))()
+    with pytest.raises(ValueError, match="not supported"):
+        m.quantize("w8a8")
+
+
+def test_w8a8_is_a_name_of_the_shard_s_quantize_flag():
+    from lorax_b200.server.cli import QUANTIZE_CHOICES
+    assert "w8a8" in QUANTIZE_CHOICES
