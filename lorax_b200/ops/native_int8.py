@@ -12,7 +12,6 @@ from typing import Optional, Union
 import torch
 
 from . import native as nv
-from .native_steps import _on_its_device, _stream_of
 from .reference import (INT8_MAX_K, NORM_BLOCK_MAX_WIDTH, Int8Rows, check_act_mul_int8, check_gemm_int8, check_norm_block, check_quant_rows_int8,
                         empty_int8_rows)
 
@@ -36,11 +35,6 @@ def check_limits(lib):
             raise nv.NativeError(f"{name}: C++ says {said()}, Python says {here}")
 
 
-def _bf16(op: str, t: torch.Tensor):
-    if t.dtype != torch.bfloat16:
-        raise ValueError(f"{op}: the kernels are bf16; got {t.dtype}")
-
-
 _devices = {}
 
 
@@ -53,36 +47,46 @@ def _device(at: int):
     return known
 
 
-def _pitch(t: Optional[torch.Tensor]) -> int:
+def _on(t: torch.Tensor, call, *args):
+    """`call` with `t`'s device as the current one: launches go to the current device."""
+    at = t.get_device()
+    if at < 0:
+        raise ValueError(f"tensors on {t.device}: the kernels take those of a CUDA device")
+    if at == torch._C._cuda_getDevice():
+        return call(at, torch._C._cuda_getCurrentRawStream(at), *args)
+    with torch.cuda.device(at):
+        return call(at, torch._C._cuda_getCurrentRawStream(at), *args)
+
+
+def _pitch(t: torch.Tensor) -> int:
     """Elements between two rows (one row's own stride says nothing)."""
-    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
-def _rows(x: torch.Tensor, T: int, n: int, act: int, gated: bool, out: Optional[torch.Tensor]) -> Int8Rows:
-    stream = _stream_of(x)
+def _rows(at: int, stream: int, x: torch.Tensor, T: int, n: int, act: int, gated: bool, out: Optional[torch.Tensor]) -> Int8Rows:
     r = empty_int8_rows(T, n, x.device)
     if T:
-        rc = nv.load().lx_rows_int8(x.data_ptr(), _pitch(x), r.q.data_ptr(), _pitch(r.q), r.scale.data_ptr(), nv._ptr(out), _pitch(out), T, n, act,
-                                    int(gated), _device(x.get_device())[0], stream)
+        rc = nv.load().lx_rows_int8(x.data_ptr(), _pitch(x), r.q.data_ptr(), (n + 15) // 16 * 16, r.scale.data_ptr(), None if out is None else out.data_ptr(),
+                                    0 if out is None else _pitch(out), T, n, act, gated, _device(at)[0], stream)
         nv._check(rc, "lx_rows_int8")
     return r
 
 
-@_on_its_device
 def quant_rows_int8(x: torch.Tensor) -> Int8Rows:
     """Rows x [T, K] in 8-bit integers, with a scale for each row (`reference.quant_rows_int8` states the numbers)."""
     T, K = check_quant_rows_int8(x)
-    _bf16("quant_rows_int8", x)
-    return _rows(x, T, K, -1, False, None)
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"quant_rows_int8: the kernels are bf16; got {x.dtype}")
+    return _on(x, _rows, x, T, K, -1, False, None)
 
 
-@_on_its_device
 def act_mul_int8(x: torch.Tensor, inter: int, act: str = "silu", gated: bool = True, out: Optional[torch.Tensor] = None) -> Int8Rows:
     """act(gate) * up of rows [gate | up], or act(gate), in 8-bit integers with a scale for each row; `out` takes the values in bf16 too
     (`reference.act_mul_int8`)."""
     T = check_act_mul_int8(x, inter, act, gated, out)
-    _bf16("act_mul_int8", x)
-    return _rows(x, T, inter, nv._ACTS[act], gated, out)
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"act_mul_int8: the kernels are bf16; got {x.dtype}")
+    return _on(x, _rows, x, T, inter, nv._ACTS[act], gated, out)
 
 
 def norm_block(y: Optional[torch.Tensor], residual: torch.Tensor, weight: torch.Tensor, eps: float, post_weight: Optional[torch.Tensor] = None,
@@ -90,25 +94,33 @@ def norm_block(y: Optional[torch.Tensor], residual: torch.Tensor, weight: torch.
                weight_offset: float = 0.0, layernorm: bool = False, residual_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                int8: bool = False) -> Union[torch.Tensor, Int8Rows]:
     """Norms on both sides of a block with its gate and scale, the residual stream between them, in one pass (`reference.norm_block` states them)."""
-    T, H, gate, to = check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
-    _bf16("norm_block", residual)
-    return _norm_block(residual, y, weight, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, to, out, int8)
+    checked = check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
+    if residual.dtype != torch.bfloat16:
+        raise ValueError(f"norm_block: the kernels are bf16; got {residual.dtype}")
+    return _on(residual, _norm_block, checked, eps, scale, weight_offset, layernorm, out, int8)
 
 
-@_on_its_device
-def _norm_block(residual, y, weight, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, to, out, int8, ring=-1):
-    T, H = residual.shape
-    stream = _stream_of(residual)
+_NONE = (None, 0, None, 0)
+
+
+def _norm_block(at: int, stream: int, checked, eps: float, scale: float, weight_offset: float, layernorm: bool, out, int8: bool, ring: int = -1):
+    """`ring`: 0 or 1 in place of the library's choice between a block per row and blocks that stay, to measure and test each."""
+    T, H, gate, to, spans = checked
+    residual = spans["residual"]
     if out is None and not int8:
-        out = torch.empty(T, H, dtype=residual.dtype, device=residual.device)
-    r = empty_int8_rows(T, H, residual.device) if int8 else None
+        out = torch.empty_strided((T, H), (H, 1), dtype=torch.bfloat16, device=residual[2].device)
+        o, ldo = out.data_ptr(), H
+    else:
+        o, _, _, ldo = spans.get("out", _NONE)
+    r = empty_int8_rows(T, H, residual[2].device) if int8 else None
     if T:
-        q, q_scale = r if int8 else (None, None)
-        sms, status = _device(residual.get_device())
-        rc = nv.load().lx_norm_block(nv._ptr(y), _pitch(y), residual.data_ptr(), _pitch(residual), nv._ptr(to), _pitch(to), nv._ptr(post_weight),
-                                     nv._ptr(post_bias), weight.data_ptr(), nv._ptr(bias), nv._ptr(gate), 0 if gate is None or T == 1 else gate.stride(0),
-                                     0 if gate is None or H == 1 else gate.stride(1), nv._ptr(out), _pitch(out), nv._ptr(q), _pitch(q), nv._ptr(q_scale),
-                                     T, H, eps, weight_offset, scale, int(layernorm), status, sms, ring, stream)
+        y, p = spans.get("y", _NONE), spans.get
+        h = _NONE if to is None else p("residual_out", residual)
+        sms, status = _device(at)
+        rc = nv.load().lx_norm_block(y[0], y[3], residual[0], residual[3], h[0], h[3], p("post_weight", _NONE)[0], p("post_bias", _NONE)[0], p("weight")[0],
+                                     p("bias", _NONE)[0], p("gate", _NONE)[0], 0 if gate is None or T == 1 else gate.stride(0),
+                                     0 if gate is None or H == 1 else gate.stride(1), o, ldo, r.q.data_ptr() if int8 else None, (H + 15) // 16 * 16,
+                                     r.scale.data_ptr() if int8 else None, T, H, eps, weight_offset, scale, layernorm, status, sms, ring, stream)
         nv._check(rc, "lx_norm_block")
     return r if int8 else out
 
@@ -116,24 +128,25 @@ def _norm_block(residual, y, weight, eps, post_weight, gate, scale, bias, post_b
 def gemm_int8(x: Int8Rows, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
               dtype: torch.dtype = torch.bfloat16, w_const: bool = False) -> torch.Tensor:
     """out[T, N] = (x.q @ w^T) * w_scale[n] * x.scale[t] + bias[n], the sums whole numbers, rounded to bf16 once (`reference.gemm_int8`).  `w_const` as for `gemm`: the
-    kernel in front on the stream does not write `w`."""
-    check_gemm_int8(x, w, w_scale, bias, out, dtype)
+    kernel in front on the stream does not write `w`.  Rows of a result that the call allocates lie a multiple of 16 bytes apart."""
+    T, N, K = check_gemm_int8(x, w, w_scale, bias, out, dtype)
     if dtype != torch.bfloat16:
         raise ValueError(f"gemm_int8: the kernels are bf16; got {dtype}")
-    return _gemm_int8(x.q, x.scale, w, w_scale, bias, out, w_const)
+    return _on(w, _gemm_int8, x, w, w_scale, bias, out, T, N, K, w_const)
 
 
-@_on_its_device
-def _gemm_int8(q, scale, w, w_scale, bias, out, w_const, plan=None):
+def _gemm_int8(at: int, stream: int, x: Int8Rows, w, w_scale, bias, out, T: int, N: int, K: int, w_const: bool, plan=None):
     """`plan`: (by pairs of CTAs, token tile, parts of K) in place of the library's choice, to measure and test each."""
-    (T, K), N = q.shape, w.shape[0]
-    stream = _stream_of(q)
     if out is None:
-        out = torch.empty(T, N, dtype=torch.bfloat16, device=q.device)
+        # (rows of a multiple of 8: written 16 bytes at a time, over thousands of rows up to twice as quick as rows that begin anywhere)
+        ldo = (N + 7) // 8 * 8
+        out = torch.empty_strided((T, N), (ldo, 1), dtype=torch.bfloat16, device=w.device)
+    else:
+        ldo = _pitch(out)
     if T and N:
-        sms, status = _device(q.get_device())
+        sms, status = _device(at)
         force = 0 if plan is None else 1 + int(plan[0]) + 2 * (plan[2] | plan[1] << 8)
-        rc = nv.load().lx_gemm_int8(q.data_ptr(), _pitch(q), scale.data_ptr(), w.data_ptr(), _pitch(w), w_scale.data_ptr(), nv._ptr(bias), out.data_ptr(),
-                                    out.stride(0) if T > 1 else N, T, N, K, int(w_const), status, sms, force, stream)
+        rc = nv.load().lx_gemm_int8(x.q.data_ptr(), _pitch(x.q), x.scale.data_ptr(), w.data_ptr(), _pitch(w), w_scale.data_ptr(),
+                                    None if bias is None else bias.data_ptr(), out.data_ptr(), ldo, T, N, K, w_const, status, sms, force, stream)
         nv._check(rc, "lx_gemm_int8")
     return out

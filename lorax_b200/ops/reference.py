@@ -1337,7 +1337,7 @@ def act_mul_int8(x, inter: int, act: str = "silu", gated: bool = True, out=None)
 
 
 def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8):
-    """-> (T, H, gate as [T, H] or None, what h is written to or None)."""
+    """-> (T, H, gate as [T, H] or None, what h is written to or None, {name: (address, end, tensor, elements between rows)} of what is given)."""
     if not (isinstance(residual, torch.Tensor) and residual.dim() == 2 and residual.is_floating_point()):
         raise ValueError("norm_block: residual [T, H] of numbers")
     if residual_out is residual:
@@ -1356,14 +1356,14 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
         if (s1 != 1 and H > 1) or (s0 < H and T > 1):
             raise ValueError(f"norm_block: {name} has neighbouring values in a row, and rows one behind the other")
         p = t.data_ptr()
-        spans[name] = (p, p + ((T - 1) * s0 + H) * size if T else p, t)
+        spans[name] = (p, p + ((T - 1) * s0 + H) * size, t, s0) if T > 1 else (p, p + T * H * size, t, (H + 15) // 16 * 16)      # (one row's own distance says nothing)
     for name, t in (("weight", weight), ("post_weight", post_weight), ("bias", bias), ("post_bias", post_bias)):
         if t is None and name != "weight":
             continue
         if not (isinstance(t, torch.Tensor) and t.dim() == 1 and t.shape[0] == H and t.is_contiguous() and t.dtype == dtype and t.get_device() == at):
             raise ValueError(f"norm_block: {name} is [H], contiguous, of the residual's type and device")
         p = t.data_ptr()
-        spans[name] = (p, p + H * size, t)
+        spans[name] = (p, p + H * size, t, 0)
     if post_bias is not None and post_weight is None:
         raise ValueError("norm_block: post_bias without post_weight")
     if y is None:
@@ -1382,16 +1382,16 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
             raise ValueError(f"norm_block: a gate of {tuple(gate.shape)} for rows of {(T, H)}: one, [H], [T, 1] or [T, H]") from None
         if H > 1 and T > 0 and gates.stride(1) not in (0, 1):
             raise ValueError("norm_block: a row's gates are neighbours, or one for all")
-        spans["gate"] = (*_span(gate), gate)
+        spans["gate"] = (*_span(gate), gate, 0)
     # a row's values are read before they are written, at the same places: a result may be y or the residual itself
     written = ("residual",) if to is residual else ("residual_out",) if to is not None else ()
     for name in written if out is None else (*written, "out"):
-        lo, hi, a = spans[name]
-        for other, (p, q, b) in spans.items():
+        lo, hi, a, _ = spans[name]
+        for other, (p, q, b, _) in spans.items():
             if lo < q and p < hi and other != name and not _turns(a, b) and not (
                     p == lo and b.shape == a.shape and b.stride() == a.stride() and other in ("y", "residual") and (other not in written)):
                 raise ValueError(f"norm_block: {name} lies on {other} (results lie apart from each other and from the inputs, or are y or the residual itself)")
-    return T, H, gates, to
+    return T, H, gates, to, spans
 
 
 def norm_block(y, residual, weight, eps, post_weight=None, gate=None, scale: float = 1.0, bias=None, post_bias=None, weight_offset: float = 0.0,
@@ -1400,7 +1400,7 @@ def norm_block(y, residual, weight, eps, post_weight=None, gate=None, scale: flo
     was written.  N is the RMS norm, or the layer norm, times (weight + weight_offset), plus the bias; N_post is left out without a `post_weight`, h is the residual
     without y.  `gate` is one value, [H], [T, 1] or [T, H].  Returns N(h) in the residual's type (in `out` where given), or with `int8` as `Int8Rows` made from the
     32-bit values, and then writes `out` too where it is given."""
-    T, H, gate, to = check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
+    T, H, gate, to, _ = check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
 
     def norm(v, w, b):
         if layernorm:

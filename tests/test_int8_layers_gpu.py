@@ -131,12 +131,17 @@ def _norm64(v, w, b, eps, offset, layernorm):
     return y, slack
 
 
+def _norm_by(ring, y, res, w, eps, post_weight=None, gate=None, scale=1.0, bias=None, post_bias=None, weight_offset=0.0, layernorm=False, residual_out=None, out=None,
+             int8=False):
+    checked = ref.check_norm_block(y, res, w, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
+    return native_int8._on(res, native_int8._norm_block, checked, eps, scale, weight_offset, layernorm, out, int8, ring)
+
+
 def _check_norm(ops, T, H, post, gate, scale, layernorm, int8, bias=True, offset=0.0, eps=1e-5, at=0, ring=-1):
     def call(y, res, w, eps, post_weight=None, gate=None, scale=1.0, bias=None, post_bias=None, weight_offset=0.0, layernorm=False, residual_out=None, out=None, int8=False):
         if ring < 0:
             return ops.norm_block(y, res, w, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, residual_out, out, int8)
-        _, _, gate, to = ref.check_norm_block(y, res, w, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
-        return native_int8._norm_block(res, y, w, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, to, out, int8, ring=ring)
+        return _norm_by(ring, y, res, w, eps, post_weight, gate, scale, bias, post_bias, weight_offset, layernorm, residual_out, out, int8)
     g = _gen(T, H, post, scale, layernorm)
     wide = H + at
     y, res = _randn(g, T, wide)[:, at:], _randn(g, T, wide, std=3.0)[:, at:]
@@ -193,7 +198,7 @@ def test_both_forms_of_norms(ops, gate, T, H, layernorm):
 def test_a_norm_without_a_block_in_front_by_both_forms(ops):
     g = _gen(9)
     res, w = _randn(g, 700, 512), _randn(g, 512)
-    a, b = (native_int8._norm_block(res, None, w, 1e-5, None, None, 1.0, None, None, 0.0, False, None, None, False, ring=ring) for ring in (0, 1))
+    a, b = (_norm_by(ring, None, res, w, 1e-5) for ring in (0, 1))
     want, slack = _norm64(res.double(), w, None, 1e-5, 0.0, False)
     for x in (a, b, ops.norm_block(None, res, w, 1e-5)):
         assert ((x.double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
@@ -246,7 +251,7 @@ def _check_product(ops, T, N, K, bias=True, at=0, out=None, plan=None):
     if plan is None:
         y = ops.gemm_int8(Int8Rows(q, xs), w, ws, bias=b, out=out)
     else:
-        y = native_int8._gemm_int8(q, xs, w, ws, b, out, False, plan=plan)
+        y = native_int8._on(w, native_int8._gemm_int8, Int8Rows(q, xs), w, ws, b, out, T, N, K, False, plan)
     s = (q.double() @ w.double().t()) * (xs.double()[:, None] * ws.double())
     want = s + (0 if b is None else b.double())
     # the sum to 32 bits, two products, the bias: four roundings; then one to bf16
