@@ -9,6 +9,8 @@
 // kept in global memory between CTAs, calls or graphs.
 //
 // The reference has no such product (it expands 8-bit integer weights beside bf16 activations, server/lorax_server/layers/eetq.py:1-26).
+#include <math.h>
+
 #include "pair.cuh"
 
 namespace lx {
@@ -550,31 +552,35 @@ static Int8Plan int8_single_plan(int T, int N, int K, int bn, int parts, int num
   return w;
 }
 
-// What a plan costs, in ns.  A CTA's time is that of its operands' way in from L2 (98 bytes a nanosecond; a second CTA on the SM adds a third to it) and of its
-// tokens' results; waves of CTAs add a start, parts a join; and no plan is quicker than the weights' way from HBM.  The constants are fitted to 6000 plans of 160
-// shapes (1 to 2048 rows, 390 to 28672 features, K 512 to 14336); the plan with the least cost is 2 % slower than the quickest one on average, at worst 21 %.
-constexpr double kI8Hbm = 6450.0;
+// What a plan costs, in ns.  A CTA's time is that of its operands' way in from L2 (100 bytes a nanosecond, 84 where all SMs work in pairs; a second CTA on an SM
+// adds a quarter) and of its tokens' results; waves of CTAs add a start, parts a join; and the weights come from HBM meanwhile, and all operands through L2: the fourth powers of both
+// times add up, so that the smaller one counts where they are near.  The constants are fitted to 7000 plans of 209 shapes (1 to 3900 rows, 144 to 28672 features,
+// K 159 to 14336): the plan of least cost is 3 % slower than the quickest one on average, at worst 23 % (7.5 us where 6.1 are possible).
+static double int8_beside(double t, double hbm) {
+  const double a = t * t, b = hbm * hbm;
+  return sqrt(sqrt(a * a + b * b));
+}
 static double int8_single_cost(int T, int N, int K, const Int8Plan& w, int num_sms) {
   const int blocks = int8_up(int8_up(K, kI8BK), w.parts), live = w.bn < T ? w.bn : T;
   int fit = 233472 / (w.smem + 1024);                                     // CTAs an SM
   if (fit > 4) fit = 4;
   const long long ctas = (long long)int8_up(N, kI8BM) * int8_up(T, w.bn) * w.parts;
-  const long long slots = (long long)(num_sms - (w.parts == 1 ? 0 : w.parts == 2 ? 2 : w.parts == 4 ? 16 : 18)) * fit;      // (clusters leave some SMs empty)
-  const long long waves = (ctas + (slots > 0 ? slots : 1) - 1) / (slots > 0 ? slots : 1);
+  long long slots = (long long)(num_sms - (w.parts == 1 ? 0 : w.parts == 2 ? 2 : w.parts == 8 ? 18 : 16)) * fit;      // (clusters leave some SMs empty)
+  if (slots < 1) slots = 1;
+  const long long waves = (ctas + slots - 1) / slots;
   long long together = (ctas + num_sms - 1) / num_sms;
   if (together > fit) together = fit;
-  const double fill = blocks * (double)(kI8ABytes + kI8BK * w.bn) * (1 + 0.33 * (double)(together - 1)) / 98.0;
-  const double t = 1410.0 + (double)waves * (fill + 1820.0 + 15.0 * live * (double)together) + (w.parts > 1 ? 1000.0 + 5.2 * live : 0.0);
-  const double hbm = 3230.0 + ((double)N * K + (double)T * K) / kI8Hbm;
-  return t > hbm ? t : hbm;
+  const double fill = blocks * (double)(kI8ABytes + kI8BK * w.bn) * (1 + 0.27 * (double)(together - 1)) / 100.8;
+  const double t = 1510.0 + (double)waves * (fill + 1358.0 + 20.4 * live * (double)together) + (w.parts > 1 ? 846.0 + 2.5 * live : 0.0);
+  const double hbm = ((double)N * K + (double)T * K) / 4810.0, l2 = (double)ctas * blocks * (kI8ABytes + kI8BK * w.bn) / 16500.0;
+  return int8_beside(t, 2868.0 + (hbm > l2 ? hbm : l2));
 }
 static double int8_pair_cost(int T, int N, int K, int bn, int parts, int clusters) {
   const int blocks = int8_up(int8_up(K, kI8BK), parts), live = bn < T ? bn : T;
   const long long tiles = (long long)int8_up(N, 2 * kI8BM) * int8_up(T, bn), waves = (tiles + clusters - 1) / clusters;
-  const double in = (kI8ABytes + kI8BK / 2 * bn) / 80.0, mma = 0.67 * bn;
-  const double t = 3040.0 + (double)waves * (blocks * (in > mma ? in : mma) + 720.0) + 17.5 * live + (parts > 1 ? 630.0 + 2.3 * live : 0.0);
-  const double hbm = 3760.0 + ((double)N * K + (double)T * K) / kI8Hbm;
-  return t > hbm ? t : hbm;
+  const double in = (kI8ABytes + kI8BK / 2 * bn) / 84.1, mma = 1.48 * bn;
+  const double t = 2022.0 + (double)waves * (blocks * (in > mma ? in : mma) + 1329.0) + 21.95 * live + (parts > 1 ? 374.0 + 1.6 * live : 0.0);
+  return int8_beside(t, 3351.0 + ((double)N * K + (double)T * K) / 4810.0);
 }
 
 // clusters[parts]: clusters of `parts` pairs that run at the same time.
@@ -589,6 +595,8 @@ static Int8Plan int8_plan(int T, int N, int K, int num_sms, const int* clusters)
     const int bn = int8_up(int8_up(T, tiles), 16) * 16, bn2 = int8_up(bn, 32) * 32;
     for (int parts : {1, 2, 3, 4, 8}) {
       if (parts > kblocks) break;
+      // (three, whose CTAs would have an SM and half its shared memory each: 64 rows of 6144 features 10.9 us, by four 9.1; two an SM, one row of 11008: 9.7, by two 11.4)
+      if (parts == 3 && (long long)int8_up(N, kI8BM) * int8_up(T, bn) * parts <= num_sms) continue;
       const Int8Plan w = int8_single_plan(T, N, K, bn, parts, num_sms);
       const double c = int8_single_cost(T, N, K, w, num_sms);
       if (c < least) { least = c; best = w; }

@@ -205,6 +205,45 @@ def test_limits_of_the_library_and_of_python_agree(monkeypatch):
         monkeypatch.undo()
 
 
+def _plan(T, N, K, sms=148, clusters=(74, 33, 22, 15)):
+    import ctypes
+
+    from lorax_b200.ops import native
+    out = (ctypes.c_int * 4)()
+    assert native.load().lx_gemm_int8_plan(T, N, K, sms, (ctypes.c_int * 4)(*clusters), out) == 0
+    return tuple(out)
+
+
+@pytest.mark.parametrize("sms,clusters", [(148, (74, 33, 22, 15)), (148, (0, 0, 0, 0)), (20, (10, 4, 2, 1)), (1, (0, 0, 0, 0))])
+def test_plans_stay_within_what_tiles_and_clusters_allow(sms, clusters):
+    rng = __import__("random").Random(7)
+    sizes = [(1, 1, 1), (1 << 20, 1, 1), (1, 1 << 20, 128), (4001, 28672, 4096), (300, 100, 1 << 17)]
+    sizes += [tuple(int(2 ** rng.uniform(0, top)) for top in (13, 15, 15)) for _ in range(400)]
+    for T, N, K in sizes:
+        pairs, bn, parts, stages = _plan(T, N, K, sms, clusters)
+        blocks = -(-K // 128)
+        assert 1 <= parts <= blocks and 16 <= bn <= 256
+        if pairs:
+            assert bn % 32 == 0 and parts <= 4 and clusters[parts - 1] > 0 and T > 32
+            assert parts == 1 or -(-N // 256) * -(-T // bn) <= clusters[parts - 1]      # a cluster has one tile, and all run at the same time
+        else:
+            # the ring holds a tile's sums, and fits beside scales and barriers
+            assert bn % 16 == 0 and parts <= 8 and 4 <= stages <= 16 and stages * (128 + bn) * 128 >= bn * 512 and stages * (128 + bn) * 128 <= 216 * 1024
+
+
+@pytest.mark.parametrize("size,pairs,parts", [
+    ((1, 28672, 4096), False, 1),       # 20.2 us; shared by two CTAs 25.6
+    ((1, 4096, 14336), False, 8),       # 12.1; by four 14.7, alone 34.5
+    ((48, 6144, 4096), False, 4),       # 9.0; alone 14
+    ((256, 4096, 14336), False, 4),     # 21.2; pairs sharing by three 21.6
+    ((512, 4096, 14336), True, 2),      # 27.3; single CTAs 30.3, pairs alone 42
+    ((256, 28672, 4096), True, 1),      # 32.4; single CTAs 42.2
+    ((4001, 28672, 4096), True, 1)])
+def test_plans_that_measured_quickest(size, pairs, parts):
+    got = _plan(*size)
+    assert (got[0] > 0, got[2]) == (pairs, parts)
+
+
 # ------------------------------------------------------------------------------------------------ models
 def _step(model, T=9):
     from lorax_b200.models.decoder import StepInputs
