@@ -6,6 +6,10 @@
 
 namespace lx {
 
+constexpr int kRowStages = 3;
+constexpr int kRowRing = 108 * 1024;      // bytes of a block's stages, so that two blocks share an SM
+constexpr int kRowRingRows = 4;           // rows an SM from which blocks that stay are worth it
+
 enum RowsAct : int { kRowsPlain = -1, kRowsSilu = 0, kRowsGelu = 1, kRowsGeluTanh = 2, kRowsRelu = 3, kRowsRelu2 = 4 };
 
 // x / (1 + exp(-x)) = x * s for x >= 0, x * a * s below, with a = exp(-|x|), s = 1 / (1 + a): nothing overflows, small results keep their digits, and
@@ -37,7 +41,8 @@ struct RowsInt8Params {
   float* scale;                // [T]
   __nv_bfloat16* out;          // [T, n] the values themselves, or null
   long long ldo;
-  int n, gated;
+  int n, gated, T, stages;
+  int* status;
 };
 
 template <int ACT, bool WIDE>
@@ -81,44 +86,119 @@ __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kerne
   }
 }
 
+// Many rows: blocks that stay, whose next rows come by bulk copies while one is quantised; a row's values stand in registers from its maximum to its quotients,
+// so that its stage is free between the two.
+template <int ACT, int NV>
+__global__ void __launch_bounds__(kRowThreads4, 2) rows_int8_ring_kernel(const RowsInt8Params p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kRowStages];
+  __shared__ uint32_t red[2][32];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int step = (int)gridDim.x;
+  const uint32_t stage_bytes = (uint32_t)p.n * (p.gated ? 4 : 2);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    abort_word = 0;
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  const auto fetch = [&](int t, int s) {
+    mbar_expect_tx(&full[s], stage_bytes);
+    bulk_load_1d(ring + s * stage_bytes, p.x + t * p.ldx, stage_bytes, &full[s]);
+  };
+  if (threadIdx.x == 0)
+    for (int s = 0; s < p.stages && (int)blockIdx.x + s * step < p.T; ++s) fetch((int)blockIdx.x + s * step, s);
+  int s = 0;
+  uint32_t phase = 0;
+  for (int row = (int)blockIdx.x, i = 0; row < p.T; row += step, ++i) {
+    const long long t = row;
+    if (!mbar_wait(&full[s], phase, abort_flag)) {      // (every thread goes on to the block's barriers all the same)
+      report_status(p.status, kTimeoutFullBarrier, row);
+      *abort_flag = 1;
+    }
+    float f[NV][8], m = 0.f;
+#pragma unroll
+    for (int it = 0; it < NV; ++it) {
+      rows_values<ACT, true>(p, reinterpret_cast<const __nv_bfloat16*>(ring + s * stage_bytes), it, f[it]);
+      m = largest_magnitude(m, f[it]);
+    }
+    const RowScale sc = row_scale(block_max(m, red[i & 1]));
+    if (threadIdx.x == 0) {
+      p.scale[t] = sc.scale;
+      if (row + p.stages * step < p.T) fetch(row + p.stages * step, s);
+    }
+#pragma unroll
+    for (int it = 0; it < NV; ++it) {
+      row_store_int8<true>(p.q + t * p.ldq, it, p.n, f[it], sc);
+      if (p.out != nullptr) row_store<true>(p.out + t * p.ldo, it, p.n, f[it]);
+    }
+    if (++s == p.stages) { s = 0; phase ^= 1; }
+  }
+}
+
+// Two blocks an SM by their registers; as many stages as fit then, up to three.
+template <int ACT, int NV>
+static int launch_rows_ring(RowsInt8Params p, int num_sms, cudaStream_t s) {
+  const int threads = ((p.n / 8 + NV - 1) / NV + 31) / 32 * 32, stage = p.n * (p.gated ? 4 : 2);
+  static bool set[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+  if (!set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(rows_int8_ring_kernel<ACT, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowRing);
+    if (e != cudaSuccess) return -(int)e;
+    set[dev] = true;
+  }
+  int blocks = 1024 / threads;
+  if (blocks > 16) blocks = 16;
+  p.stages = kRowRing / ((blocks + 1) / 2 * stage);
+  p.stages = p.stages > kRowStages ? kRowStages : p.stages < 1 ? 1 : p.stages;
+  const int grid = p.T < num_sms * blocks ? p.T : num_sms * blocks;
+  launch_pdl(rows_int8_ring_kernel<ACT, NV>, dim3((unsigned)grid), dim3((unsigned)threads), (size_t)p.stages * stage, s, p);
+  return -(int)cudaGetLastError();
+}
+
 template <int ACT, bool WIDE>
-static void launch_rows(const RowsInt8Params& p, int T, const RowShape& r, cudaStream_t s) {
-  const dim3 grid((unsigned)T), block((unsigned)r.threads);
+static int launch_rows(const RowsInt8Params& p, int num_sms, int ring, cudaStream_t s) {
+  if (WIDE && p.n <= kRowThreads4 * 4 * 8 && (ring < 0 ? p.T >= kRowRingRows * num_sms : ring))
+    return p.n <= kRowThreads4 * 2 * 8 ? launch_rows_ring<ACT, 2>(p, num_sms, s) : launch_rows_ring<ACT, 4>(p, num_sms, s);
+  const RowShape r = row_shape(p.T, p.n, num_sms, 1024);
+  const dim3 grid((unsigned)p.T), block((unsigned)r.threads);
   if (r.groups == 1) launch_pdl(rows_int8_kernel<ACT, 1, WIDE>, grid, block, 0, s, p);
   else if (r.groups == 2) launch_pdl(rows_int8_kernel<ACT, 2, WIDE>, grid, block, 0, s, p);
   else if (r.groups == 4) launch_pdl(rows_int8_kernel<ACT, 4, WIDE>, grid, block, 0, s, p);
   else launch_pdl(rows_int8_kernel<ACT, 0, WIDE>, grid, block, 0, s, p);
+  return -(int)cudaGetLastError();
 }
 
 }  // namespace lx
 
 extern "C" {
 
-// act < 0: x [T, n] as it is; else act(x[:, :n]), times x[:, n : 2 n] where gated.  out (bf16) may be null.
-int lx_rows_int8(const void* x, long long ldx, void* q, long long ldq, void* scale, void* out, long long ldo, int T, int n, int act, int gated, int num_sms,
-                 void* stream) {
+// ring as for lx_norm_block.  act < 0: x [T, n] as it is; else act(x[:, :n]), times x[:, n : 2 n] where gated.  out (bf16) may be null.
+int lx_rows_int8(const void* x, long long ldx, void* q, long long ldq, void* scale, void* out, long long ldo, int T, int n, int act, int gated, int* status,
+                 int num_sms, int ring, void* stream) {
   using namespace lx;
   if (T <= 0) return 0;
   if (n <= 0) return -1;
   RowsInt8Params p{reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<int8_t*>(q), ldq, reinterpret_cast<float*>(scale),
-                   reinterpret_cast<__nv_bfloat16*>(out), ldo, n, gated};
+                   reinterpret_cast<__nv_bfloat16*>(out), ldo, n, gated, T, 0, status};
   const auto at = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
   const bool wide = n % 8 == 0 && at(x) % 16 == 0 && ldx % 8 == 0 && at(q) % 8 == 0 && ldq % 8 == 0 && at(out) % 16 == 0 && ldo % 8 == 0;
-  const RowShape r = row_shape(T, n, num_sms, 1024);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define LX_ROWS(A)                          \
-  if (wide) launch_rows<A, true>(p, T, r, s); \
-  else launch_rows<A, false>(p, T, r, s)
+#define LX_ROWS(A) return wide ? launch_rows<A, true>(p, num_sms, ring, s) : launch_rows<A, false>(p, num_sms, ring, s)
   switch (act) {
-    case kRowsSilu: LX_ROWS(kRowsSilu); break;
-    case kRowsGelu: LX_ROWS(kRowsGelu); break;
-    case kRowsGeluTanh: LX_ROWS(kRowsGeluTanh); break;
-    case kRowsRelu: LX_ROWS(kRowsRelu); break;
-    case kRowsRelu2: LX_ROWS(kRowsRelu2); break;
-    default: LX_ROWS(kRowsPlain); break;
+    case kRowsSilu: LX_ROWS(kRowsSilu);
+    case kRowsGelu: LX_ROWS(kRowsGelu);
+    case kRowsGeluTanh: LX_ROWS(kRowsGeluTanh);
+    case kRowsRelu: LX_ROWS(kRowsRelu);
+    case kRowsRelu2: LX_ROWS(kRowsRelu2);
+    default: LX_ROWS(kRowsPlain);
   }
 #undef LX_ROWS
-  return -(int)cudaGetLastError();
 }
 
 }  // extern "C"

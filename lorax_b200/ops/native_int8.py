@@ -20,7 +20,7 @@ P, I, L, F = c_void_p, c_int, c_longlong, c_float
 SIGNATURES = {
     "lx_norm_block_max_width": ([], I),
     "lx_norm_block": ([P, L, P, L, P, L, P, P, P, P, P, L, I, P, L, P, L, P, I, I, F, F, F, I, P, I, I, P], I),
-    "lx_rows_int8": ([P, L, P, L, P, P, L, I, I, I, I, I, P], I),
+    "lx_rows_int8": ([P, L, P, L, P, P, L, I, I, I, I, P, I, I, P], I),
     "lx_gemm_int8_max_k": ([], I),
     "lx_gemm_int8_plan": ([I, I, I, I, P, P], I),
     "lx_gemm_int8_clusters": ([I], I),
@@ -63,11 +63,13 @@ def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
-def _rows(at: int, stream: int, x: torch.Tensor, T: int, n: int, act: int, gated: bool, out: Optional[torch.Tensor]) -> Int8Rows:
+def _rows(at: int, stream: int, x: torch.Tensor, T: int, n: int, act: int, gated: bool, out: Optional[torch.Tensor], ring: int = -1) -> Int8Rows:
+    """`ring` as for `_norm_block`."""
     r = empty_int8_rows(T, n, x.device)
     if T:
+        sms, status = _device(at)
         rc = nv.load().lx_rows_int8(x.data_ptr(), _pitch(x), r.q.data_ptr(), (n + 15) // 16 * 16, r.scale.data_ptr(), None if out is None else out.data_ptr(),
-                                    0 if out is None else _pitch(out), T, n, act, gated, _device(at)[0], stream)
+                                    0 if out is None else _pitch(out), T, n, act, gated, status, sms, ring, stream)
         nv._check(rc, "lx_rows_int8")
     return r
 

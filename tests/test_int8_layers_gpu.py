@@ -108,6 +108,21 @@ def test_activations(ops, act, T, I, gated):
     assert torch.equal(ops.act_mul_int8(x, I, act, gated).q, r.q)
 
 
+@pytest.mark.parametrize("T,n", [(1, 8), (5, 64), (700, 256), (1300, 1000), (601, 4096), (300, 8192), (301, 14336), (200, 16384)])
+@pytest.mark.parametrize("act,gated", [(None, False), ("silu", True), ("relu2", False)])
+def test_both_forms_of_quantisers(ops, T, n, act, gated):
+    """A block per row, and blocks that stay: the same bits, since a row's maximum and quotients depend on no order."""
+    x = _randn(_gen(T, n), T, 2 * n if gated else n, std=2.0)
+    x[T // 2] = 0
+    x[T // 3, 5] = float("nan")
+    outs = [torch.full((T, n), 7.0, device="cuda", dtype=BF) for _ in range(2)]
+    a, b = (native_int8._on(x, native_int8._rows, x, T, n, native._ACTS[act] if act else -1, gated, o, ring) for ring, o in enumerate(outs))
+    assert torch.equal(a.q, b.q) and torch.equal(a.scale.view(torch.int32), b.scale.view(torch.int32)) and torch.equal(outs[0].view(torch.int16), outs[1].view(torch.int16))
+    if act is None:
+        want = ref.quant_rows_int8(x.cpu())
+        assert torch.equal(b.q.cpu(), want.q) and (outs[1] == x)[x == x].all()
+
+
 def test_activations_keep_what_is_not_a_number(ops):
     x = _randn(_gen(3), 4, 64)
     x[1, 3] = float("nan")
