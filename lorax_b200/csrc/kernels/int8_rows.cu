@@ -45,12 +45,13 @@ struct RowsInt8Params {
   int* status;
 };
 
-template <int ACT, bool WIDE>
-LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, int it, float (&f)[8]) {
-  row_load<WIDE>(row, it, p.n, f);
+// (M of rows that begin anywhere is kRowsShifted with a shift of 0: their bytes begin at 16, and that is where groups do)
+template <int ACT, int M>
+LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, const VectorRaw& gate, const VectorRaw& up, int it, float (&f)[8]) {
+  vector_take<M>(gate, row, it, p.n, f);
   if (ACT == kRowsPlain) return;
   float u[8];
-  if (p.gated) row_load<WIDE>(row + p.n, it, p.n, u);
+  if (p.gated) vector_take<M>(up, row + p.n, it, p.n, u);
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     f[q] = rows_act<ACT>(f[q]);
@@ -58,9 +59,15 @@ LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, in
   }
 }
 
+template <int ACT, int M>
+LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, int it, float (&f)[8]) {
+  const VectorRaw g = vector_fetch<M>(row, it, p.n);
+  rows_values<ACT, M>(p, row, g, ACT != kRowsPlain && p.gated ? vector_fetch<M>(row + p.n, it, p.n) : g, it, f);
+}
+
 // One block per row.  NV: groups of eight that a thread keeps in registers between the pass for the maximum and the quotients; 0: any number, read and
 // computed again (from L2: a row was read a moment ago).
-template <int ACT, int NV, bool WIDE>
+template <int ACT, int NV, int M>
 __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kernel(const RowsInt8Params p) {
   pdl_wait();
   pdl_trigger();
@@ -71,18 +78,39 @@ __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kerne
   constexpr int KEEP = NV > 0 ? NV : 1;
   float f[KEEP][8];
   const int passes = NV > 0 ? NV : (p.n + (int)blockDim.x * 8 - 1) / ((int)blockDim.x * 8);
+  if (NV > 0) {
+    VectorRaw g[KEEP], u[KEEP];
 #pragma unroll
-  for (int it = 0; it < (NV > 0 ? NV : passes); ++it) {
-    rows_values<ACT, WIDE>(p, row, it, f[NV > 0 ? it : 0]);
-    m = largest_magnitude(m, f[NV > 0 ? it : 0]);
+    for (int it = 0; it < KEEP; ++it) {
+      g[it] = vector_fetch<M>(row, it, p.n);
+      if (ACT != kRowsPlain && p.gated) u[it] = vector_fetch<M>(row + p.n, it, p.n);
+    }
+#pragma unroll
+    for (int it = 0; it < KEEP; ++it) {
+      rows_values<ACT, M>(p, row, g[it], u[it], it, f[it]);
+      m = largest_magnitude(m, f[it]);
+    }
+  } else {
+    for (int it = 0; it < passes; ++it) {
+      rows_values<ACT, M>(p, row, it, f[0]);
+      m = largest_magnitude(m, f[0]);
+    }
   }
   const RowScale s = row_scale(block_max(m, red));
   if (threadIdx.x == 0) p.scale[t] = s.scale;
 #pragma unroll
   for (int it = 0; it < (NV > 0 ? NV : passes); ++it) {
-    if (NV == 0) rows_values<ACT, WIDE>(p, row, it, f[0]);
-    row_store_int8<WIDE>(p.q + t * p.ldq, it, p.n, f[NV > 0 ? it : 0], s);
-    if (p.out != nullptr) row_store<WIDE>(p.out + t * p.ldo, it, p.n, f[NV > 0 ? it : 0]);
+    if (NV == 0) rows_values<ACT, M>(p, row, it, f[0]);
+    row_store_int8<M>(p.q + t * p.ldq, it, p.n, f[NV > 0 ? it : 0], s);
+    if (p.out != nullptr) {
+      if (M == kRowsWide) {
+        row_store<kRowsWide>(p.out + t * p.ldo, it, p.n, f[NV > 0 ? it : 0]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (row_has<M>(it, q, p.n, 0)) p.out[t * p.ldo + row_at<M>(it, q)] = __float2bfloat16(f[NV > 0 ? it : 0][q]);
+      }
+    }
   }
 }
 
@@ -123,7 +151,7 @@ __global__ void __launch_bounds__(kRowThreads4, 2) rows_int8_ring_kernel(const R
     float f[NV][8], m = 0.f;
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
-      rows_values<ACT, true>(p, reinterpret_cast<const __nv_bfloat16*>(ring + s * stage_bytes), it, f[it]);
+      rows_values<ACT, kRowsWide>(p, reinterpret_cast<const __nv_bfloat16*>(ring + s * stage_bytes), it, f[it]);
       m = largest_magnitude(m, f[it]);
     }
     const RowScale sc = row_scale(block_max(m, red[i & 1]));
@@ -133,8 +161,8 @@ __global__ void __launch_bounds__(kRowThreads4, 2) rows_int8_ring_kernel(const R
     }
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
-      row_store_int8<true>(p.q + t * p.ldq, it, p.n, f[it], sc);
-      if (p.out != nullptr) row_store<true>(p.out + t * p.ldo, it, p.n, f[it]);
+      row_store_int8<kRowsWide>(p.q + t * p.ldq, it, p.n, f[it], sc);
+      if (p.out != nullptr) row_store<kRowsWide>(p.out + t * p.ldo, it, p.n, f[it]);
     }
     if (++s == p.stages) { s = 0; phase ^= 1; }
   }
@@ -161,16 +189,16 @@ static int launch_rows_ring(RowsInt8Params p, int num_sms, cudaStream_t s) {
   return -(int)cudaGetLastError();
 }
 
-template <int ACT, bool WIDE>
+template <int ACT, int M>
 static int launch_rows(const RowsInt8Params& p, int num_sms, int ring, cudaStream_t s) {
-  if (WIDE && p.n <= kRowThreads4 * 4 * 8 && (ring < 0 ? p.T >= kRowRingRows * num_sms : ring))
+  if (M == kRowsWide && p.n <= kRowThreads4 * 4 * 8 && (ring < 0 ? p.T >= kRowRingRows * num_sms : ring))
     return p.n <= kRowThreads4 * 2 * 8 ? launch_rows_ring<ACT, 2>(p, num_sms, s) : launch_rows_ring<ACT, 4>(p, num_sms, s);
   const RowShape r = row_shape(p.T, p.n, num_sms, 1024);
   const dim3 grid((unsigned)p.T), block((unsigned)r.threads);
-  if (r.groups == 1) launch_pdl(rows_int8_kernel<ACT, 1, WIDE>, grid, block, 0, s, p);
-  else if (r.groups == 2) launch_pdl(rows_int8_kernel<ACT, 2, WIDE>, grid, block, 0, s, p);
-  else if (r.groups == 4) launch_pdl(rows_int8_kernel<ACT, 4, WIDE>, grid, block, 0, s, p);
-  else launch_pdl(rows_int8_kernel<ACT, 0, WIDE>, grid, block, 0, s, p);
+  if (r.groups == 1) launch_pdl(rows_int8_kernel<ACT, 1, M>, grid, block, 0, s, p);
+  else if (r.groups == 2) launch_pdl(rows_int8_kernel<ACT, 2, M>, grid, block, 0, s, p);
+  else if (r.groups == 4) launch_pdl(rows_int8_kernel<ACT, 4, M>, grid, block, 0, s, p);
+  else launch_pdl(rows_int8_kernel<ACT, 0, M>, grid, block, 0, s, p);
   return -(int)cudaGetLastError();
 }
 
@@ -189,7 +217,7 @@ int lx_rows_int8(const void* x, long long ldx, void* q, long long ldq, void* sca
   const auto at = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
   const bool wide = n % 8 == 0 && at(x) % 16 == 0 && ldx % 8 == 0 && at(q) % 8 == 0 && ldq % 8 == 0 && at(out) % 16 == 0 && ldo % 8 == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define LX_ROWS(A) return wide ? launch_rows<A, true>(p, num_sms, ring, s) : launch_rows<A, false>(p, num_sms, ring, s)
+#define LX_ROWS(A) return wide ? launch_rows<A, kRowsWide>(p, num_sms, ring, s) : launch_rows<A, kRowsShifted>(p, num_sms, ring, s)
   switch (act) {
     case kRowsSilu: LX_ROWS(kRowsSilu);
     case kRowsGelu: LX_ROWS(kRowsGelu);

@@ -9,48 +9,130 @@
 
 namespace lx {
 
-// Position of a thread's value q of its `it`-th group of eight: eight neighbours (16-byte loads), or values a block's width apart where rows do not
-// begin at 16 bytes or their length is no multiple of eight (a warp's loads are then still of neighbours).
-template <bool WIDE>
-LX_DEVICE int row_at(int it, int q) {
-  return WIDE ? (it * (int)blockDim.x + (int)threadIdx.x) * 8 + q : (it * 8 + q) * (int)blockDim.x + (int)threadIdx.x;
+// How a thread's groups of eight lie in a row.  kRowsWide: eight neighbours, rows of a multiple of eight that begin at 16 bytes.  kRowsShifted: eight
+// neighbours that begin at 16 bytes, wherever the row does: `shift` values in front of it, so that all groups but a row's first and last are loaded and stored at
+// once.  kRowsApart: values a block's width apart, for rows of which every tensor begins elsewhere (a warp's loads are still of neighbours).
+enum RowsMode : int { kRowsApart = 0, kRowsWide = 1, kRowsShifted = 2 };
+
+template <int M>
+LX_DEVICE int row_at(int it, int q, int shift = 0) {
+  return M == kRowsApart ? (it * 8 + q) * (int)blockDim.x + (int)threadIdx.x : (it * (int)blockDim.x + (int)threadIdx.x) * 8 + q - (M == kRowsShifted ? shift : 0);
+}
+template <int M>
+LX_DEVICE bool row_has(int it, int q, int n, int shift) {
+  const int c = row_at<M>(it, M == kRowsWide ? 0 : q, shift);
+  return c < n && (M != kRowsShifted || c >= 0);
+}
+// Whether the group lies in the row as a whole.
+template <int M>
+LX_DEVICE bool row_whole(int it, int n, int shift) {
+  const int c = row_at<M>(it, 0, shift);
+  return M == kRowsWide ? c < n : M == kRowsShifted && c >= 0 && c + 8 <= n;
 }
 
-// A thread's eight values of a row (0 behind its end), in 32 bits.
-template <bool WIDE>
-LX_DEVICE void row_load(const __nv_bfloat16* row, int it, int n, float (&f)[8]) {
-  if (WIDE) {
-    const int c = row_at<true>(it, 0);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (c < n) v = *reinterpret_cast<const uint4*>(row + c);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+LX_DEVICE void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 t = unpack_bf16x2(w[q]);
-      f[2 * q] = t.x;
-      f[2 * q + 1] = t.y;
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int c = row_at<false>(it, q);
-      f[q] = c < n ? __bfloat162float(row[c]) : 0.f;
-    }
+  for (int q = 0; q < 4; ++q) {
+    const float2 t = unpack_bf16x2(w[q]);
+    f[2 * q] = t.x;
+    f[2 * q + 1] = t.y;
   }
 }
 
-template <bool WIDE>
-LX_DEVICE void row_store(__nv_bfloat16* row, int it, int n, const float (&f)[8]) {
-  if (WIDE) {
-    const int c = row_at<true>(it, 0);
-    if (c < n)
-      *reinterpret_cast<uint4*>(row + c) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  } else {
+// The values of a group that lie in the row, one by one, and zeros.
+template <int M>
+LX_DEVICE uint4 row_pieces(const __nv_bfloat16* row, int it, int n, int shift) {
+  uint32_t w[4];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int c = row_at<false>(it, q);
-      if (c < n) row[c] = __float2bfloat16(f[q]);
-    }
+  for (int q = 0; q < 4; ++q) {
+    const unsigned short* v = reinterpret_cast<const unsigned short*>(row);
+    const uint32_t a = row_has<M>(it, 2 * q, n, shift) ? v[row_at<M>(it, 2 * q, shift)] : 0u, b = row_has<M>(it, 2 * q + 1, n, shift) ? v[row_at<M>(it, 2 * q + 1, shift)] : 0u;
+    w[q] = a | b << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Where the elements of a tensor of rows lie: from `lo` up to `hi`.
+struct Extent {
+  const __nv_bfloat16 *lo, *hi;
+};
+LX_DEVICE Extent extent(const __nv_bfloat16* base, long long ld, int rows, int n) { return Extent{base, base + (rows - 1) * ld + n}; }
+
+// A thread's eight values of a row (0 outside it), in two steps: loads, all of them on their way before the first is waited for, and what becomes of them.  A shifted
+// row's first and last 16 bytes are loaded as a whole where they lie in the tensor, and what belongs to its neighbours is cut off.
+template <int M>
+LX_DEVICE uint4 row_fetch(const __nv_bfloat16* row, int it, int n, int shift, const Extent& e) {
+  if (M == kRowsApart) return row_pieces<M>(row, it, n, shift);
+  const int c = row_at<M>(it, 0, shift);
+  const __nv_bfloat16* a = row + c;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  const bool some = c < n && c + 8 > 0, inside = M == kRowsWide || (a >= e.lo && a + 8 <= e.hi);
+  if (some && inside) v = *reinterpret_cast<const uint4*>(a);
+  if (M == kRowsShifted && some && !inside) v = row_pieces<M>(row, it, n, shift);
+  return v;
+}
+template <int M>
+LX_DEVICE void row_take(const uint4& v, int it, int n, float (&f)[8], int shift) {
+  unpack8(v, f);
+  if (M == kRowsShifted && !row_whole<M>(it, n, shift)) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (!row_has<M>(it, q, n, shift)) f[q] = 0.f;
+  }
+}
+
+// The same of a vector that begins anywhere: two 16-byte loads and a shift where both lie inside the vector.
+struct VectorRaw {
+  uint4 lo, hi;
+};
+template <int M>
+LX_DEVICE int vector_in(const __nv_bfloat16* v, int it, int n, int shift) {      // values of the first 16 bytes in front of the group; -1: its pieces were loaded
+  if (M != kRowsShifted) return row_whole<M>(it, n, shift) ? 0 : -1;
+  const int c = row_at<M>(it, 0, shift), in = (int)((reinterpret_cast<uintptr_t>(v + c) & 15) >> 1);
+  return c - in >= 0 && c - in + 16 <= n ? in : -1;
+}
+template <int M>
+LX_DEVICE VectorRaw vector_fetch(const __nv_bfloat16* v, int it, int n, int shift = 0) {
+  VectorRaw r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  const int in = vector_in<M>(v, it, n, shift);
+  if (in >= 0) {
+    const uint4* a = reinterpret_cast<const uint4*>(v + (row_at<M>(it, 0, shift) - in));
+    r.lo = a[0];
+    if (M == kRowsShifted) r.hi = a[1];
+  } else if (M != kRowsWide) {
+    r.lo = row_pieces<M>(v, it, n, shift);
+  }
+  return r;
+}
+template <int M>
+LX_DEVICE void vector_take(const VectorRaw& r, const __nv_bfloat16* v, int it, int n, float (&f)[8], int shift = 0) {
+  uint32_t w[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
+  if (M == kRowsShifted) {
+    const int in = max(vector_in<M>(v, it, n, shift), 0);
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = in & 4 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = in & 2 ? w[i + 1] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (in & 1) * 16);
+  }
+  unpack8(make_uint4(w[0], w[1], w[2], w[3]), f);
+}
+template <int M>
+LX_DEVICE void vector_load(const __nv_bfloat16* v, int it, int n, float (&f)[8], int shift = 0) {
+  vector_take<M>(vector_fetch<M>(v, it, n, shift), v, it, n, f, shift);
+}
+
+template <int M>
+LX_DEVICE void row_store(__nv_bfloat16* row, int it, int n, const float (&f)[8], int shift = 0) {
+  if (row_whole<M>(it, n, shift)) {
+    *reinterpret_cast<uint4*>(row + row_at<M>(it, 0, shift)) =
+        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  } else if (M != kRowsWide) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (row_has<M>(it, q, n, shift)) row[row_at<M>(it, q, shift)] = __float2bfloat16(f[q]);
   }
 }
 
@@ -138,19 +220,17 @@ LX_DEVICE uint2 row_quotients(const float (&f)[8], const RowScale& s) {
   return make_uint2(w[0], w[1]);
 }
 
-// A thread's eight quotients to its row's bytes.
-template <bool WIDE>
-LX_DEVICE void row_store_int8(int8_t* row, int it, int n, const float (&f)[8], const RowScale& s) {
-  if (WIDE && row_at<true>(it, 0) >= n) return;
+// A thread's eight quotients to its row's bytes, which begin at 16 bytes.
+template <int M>
+LX_DEVICE void row_store_int8(int8_t* row, int it, int n, const float (&f)[8], const RowScale& s, int shift = 0) {
+  if (M == kRowsWide && !row_whole<M>(it, n, 0)) return;
   const uint2 w = row_quotients(f, s);
-  if (WIDE) {
-    *reinterpret_cast<uint2*>(row + row_at<true>(it, 0)) = w;
+  if (M != kRowsApart && (row_at<M>(it, 0, shift) & 7) == 0 && row_whole<M>(it, n, shift)) {
+    *reinterpret_cast<uint2*>(row + row_at<M>(it, 0, shift)) = w;
   } else {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int c = row_at<false>(it, q);
-      if (c < n) row[c] = (int8_t)((q < 4 ? w.x : w.y) >> (8 * (q & 3)));
-    }
+    for (int q = 0; q < 8; ++q)
+      if (row_has<M>(it, q, n, shift)) row[row_at<M>(it, q, shift)] = (int8_t)((q < 4 ? w.x : w.y) >> (8 * (q & 3)));
   }
 }
 
@@ -168,6 +248,12 @@ inline RowShape row_shape(int rows, int n, int num_sms, int most) {
     if (threads <= (g == 4 ? kRowThreads4 : most)) return RowShape{threads, g};
   }
   return RowShape{1024, 0};
+}
+// For kRowsShifted, whose groups take more registers: one a thread, or two in blocks of up to 768.
+constexpr int kRowShifted2 = 768;
+inline RowShape row_shape_shifted(int n) {
+  const int need = (n + 7) / 8, g = need <= 1024 ? 1 : 2;
+  return RowShape{((need + g - 1) / g + 31) / 32 * 32, g};
 }
 
 }  // namespace lx

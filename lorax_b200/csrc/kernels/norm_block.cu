@@ -30,8 +30,8 @@ struct NormBlockParams {
 };
 
 // Sums over the block of up to three norms' passes, each with words of its own.
-template <bool LAYERNORM, int NV, bool WIDE>
-LX_DEVICE void norm_rows(float (&f)[NV][8], int H, float eps, float (*red)[32]) {
+template <bool LAYERNORM, int NV, int M>
+LX_DEVICE void norm_rows(float (&f)[NV][8], int H, float eps, float (*red)[32], int shift = 0) {
   float mean = 0.f;
   if (LAYERNORM) {
     float s = 0.f;
@@ -46,7 +46,7 @@ LX_DEVICE void norm_rows(float (&f)[NV][8], int H, float eps, float (*red)[32]) 
   for (int it = 0; it < NV; ++it)
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      if (LAYERNORM) f[it][q] = (WIDE ? row_at<true>(it, 0) : row_at<false>(it, q)) < H ? f[it][q] - mean : 0.f;
+      if (LAYERNORM) f[it][q] = row_has<M>(it, q, H, shift) ? f[it][q] - mean : 0.f;
       s = fmaf(f[it][q], f[it][q], s);
     }
   const float r = rsqrtf(block_sum(s, red[1]) / H + eps);
@@ -56,64 +56,76 @@ LX_DEVICE void norm_rows(float (&f)[NV][8], int H, float eps, float (*red)[32]) 
     for (int q = 0; q < 8; ++q) f[it][q] *= r;
 }
 
-template <int NV, bool WIDE>
-LX_DEVICE void scale_rows(float (&f)[NV][8], int H, const __nv_bfloat16* w, const __nv_bfloat16* b, float offset) {
+template <int NV, int M>
+LX_DEVICE void scale_rows(float (&f)[NV][8], int H, const VectorRaw (&raw)[NV], const __nv_bfloat16* w, const __nv_bfloat16* b, float offset, int shift) {
 #pragma unroll
   for (int it = 0; it < NV; ++it) {
     float g[8];
-    row_load<WIDE>(w, it, H, g);
+    vector_take<M>(raw[it], w, it, H, g, shift);
 #pragma unroll
     for (int q = 0; q < 8; ++q) f[it][q] *= g[q] + offset;
     if (b != nullptr) {
-      row_load<WIDE>(b, it, H, g);
+      vector_load<M>(b, it, H, g, shift);
 #pragma unroll
       for (int q = 0; q < 8; ++q) f[it][q] += g[q];
     }
   }
 }
 
-template <bool WIDE>
-LX_DEVICE void gates(const NormBlockParams& p, long long t, int it, float (&g)[8]) {
+template <int M>
+LX_DEVICE void gates(const NormBlockParams& p, long long t, int it, float (&g)[8], int shift = 0) {
   const __nv_bfloat16* gate = p.gate + t * p.gate_t;
   if (p.gate_h == 0) {
     const float one = __bfloat162float(*gate);
 #pragma unroll
     for (int q = 0; q < 8; ++q) g[q] = one;
-  } else if (WIDE && p.gate_wide) {
-    row_load<true>(gate, it, p.H, g);
+  } else if (M != kRowsWide || p.gate_wide) {
+    vector_load<M>(gate, it, p.H, g, shift);
   } else {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int c = row_at<WIDE>(it, q);
-      g[q] = c < p.H ? __bfloat162float(gate[c]) : 0.f;
-    }
+    for (int q = 0; q < 8; ++q) g[q] = row_has<M>(it, q, p.H, shift) ? __bfloat162float(gate[row_at<M>(it, q, shift)]) : 0.f;
   }
 }
 
 // One block per row; NV groups of eight a thread, all in registers.
-template <bool LAYERNORM, int NV, bool WIDE>
-__global__ void __launch_bounds__(kRowThreads4) norm_block_kernel(const NormBlockParams p) {
+template <bool LAYERNORM, int NV, int M>
+__global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? 1024 : kRowShifted2) norm_block_kernel(const NormBlockParams p) {
   pdl_wait();
   pdl_trigger();
   __shared__ float red[4][32];
   __shared__ uint32_t red_max[32];
   const long long t = blockIdx.x;
+  const int H = p.H, shift = M == kRowsShifted ? (int)((reinterpret_cast<uintptr_t>(p.residual + t * p.ldr) & 15) >> 1) : 0;
+  const __nv_bfloat16 *res = p.residual + t * p.ldr, *block = p.y + t * p.ldy;
+  const Extent res_at = extent(p.residual, p.ldr, p.T, H), block_at = extent(p.y, p.ldy, p.T, H);
+  uint4 hr[NV], yr[NV];
+  VectorRaw wr[NV], pr[NV];
+#pragma unroll
+  for (int it = 0; it < NV; ++it) {
+    hr[it] = row_fetch<M>(res, it, H, shift, res_at);
+    if (p.y != nullptr) yr[it] = row_fetch<M>(block, it, H, shift, block_at);
+  }
+#pragma unroll
+  for (int it = 0; it < NV; ++it) {
+    if (p.post_w != nullptr) pr[it] = vector_fetch<M>(p.post_w, it, H, shift);
+    wr[it] = vector_fetch<M>(p.w, it, H, shift);
+  }
   float h[NV][8];
 #pragma unroll
-  for (int it = 0; it < NV; ++it) row_load<WIDE>(p.residual + t * p.ldr, it, p.H, h[it]);
+  for (int it = 0; it < NV; ++it) row_take<M>(hr[it], it, H, h[it], shift);
   if (p.y != nullptr) {
     float y[NV][8];
 #pragma unroll
-    for (int it = 0; it < NV; ++it) row_load<WIDE>(p.y + t * p.ldy, it, p.H, y[it]);
+    for (int it = 0; it < NV; ++it) row_take<M>(yr[it], it, H, y[it], shift);
     if (p.post_w != nullptr) {
-      norm_rows<LAYERNORM, NV, WIDE>(y, p.H, p.eps, red);
-      scale_rows<NV, WIDE>(y, p.H, p.post_w, p.post_b, p.w_offset);
+      norm_rows<LAYERNORM, NV, M>(y, H, p.eps, red, shift);
+      scale_rows<NV, M>(y, H, pr, p.post_w, p.post_b, p.w_offset, shift);
     }
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
       if (p.gate != nullptr) {
         float g[8];
-        gates<WIDE>(p, t, it, g);
+        gates<M>(p, t, it, g, shift);
 #pragma unroll
         for (int q = 0; q < 8; ++q) y[it][q] *= g[q];
       }
@@ -127,29 +139,29 @@ __global__ void __launch_bounds__(kRowThreads4) norm_block_kernel(const NormBloc
   }
   if (p.residual_out != nullptr) {
 #pragma unroll
-    for (int it = 0; it < NV; ++it) row_store<WIDE>(p.residual_out + t * p.ldro, it, p.H, h[it]);
+    for (int it = 0; it < NV; ++it) row_store<M>(p.residual_out + t * p.ldro, it, H, h[it], shift);
   }
-  norm_rows<LAYERNORM, NV, WIDE>(h, p.H, p.eps, red + 2);
-  scale_rows<NV, WIDE>(h, p.H, p.w, p.b, p.w_offset);
+  norm_rows<LAYERNORM, NV, M>(h, H, p.eps, red + 2, shift);
+  scale_rows<NV, M>(h, H, wr, p.w, p.b, p.w_offset, shift);
   if (p.out != nullptr) {
 #pragma unroll
-    for (int it = 0; it < NV; ++it) row_store<WIDE>(p.out + t * p.ldo, it, p.H, h[it]);
+    for (int it = 0; it < NV; ++it) row_store<M>(p.out + t * p.ldo, it, H, h[it], shift);
   }
   if (p.q != nullptr) {
     float m = 0.f;
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
-      if (!WIDE) {
+      if (!row_whole<M>(it, H, shift)) {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-          if (row_at<WIDE>(it, q) >= p.H) h[it][q] = 0.f;
+          if (!row_has<M>(it, q, H, shift)) h[it][q] = 0.f;      // (0 times a row's infinite or NaN factors)
       }
-      if (!WIDE || row_at<true>(it, 0) < p.H) m = largest_magnitude(m, h[it]);
+      m = largest_magnitude(m, h[it]);
     }
     const RowScale s = row_scale(block_max(m, red_max));
     if (threadIdx.x == 0) p.q_scale[t] = s.scale;
 #pragma unroll
-    for (int it = 0; it < NV; ++it) row_store_int8<WIDE>(p.q + t * p.ldq, it, p.H, h[it], s);
+    for (int it = 0; it < NV; ++it) row_store_int8<M>(p.q + t * p.ldq, it, H, h[it], s, shift);
   }
 }
 
@@ -158,18 +170,9 @@ __global__ void __launch_bounds__(kRowThreads4) norm_block_kernel(const NormBloc
 // Rows are read from shared memory as often as a pass needs them, so that a thread holds the values of one row only, and the norms' weights for all rows.
 // ------------------------------------------------------------------------------------------------
 constexpr int kNormStages = 2;
-constexpr int kNormRingRows = 4;      // rows an SM from which they are worth it
-
-template <int NV>
-LX_DEVICE void unpack8(const uint4& v, float (&f)[NV][8], int it) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float2 t = unpack_bf16x2(w[q]);
-    f[it][2 * q] = t.x;
-    f[it][2 * q + 1] = t.y;
-  }
-}
+// Values of the stream an SM has to norm from which they are worth it (us, a block per row and blocks that stay): 200 rows of 4096 3.9 and 4.3, 444 6.7 and 6.3, 4001 32 and 26;
+// 148 of 8192 4.6 and 5.0, 200 7.3 and 6.3, 4001 70 and 49; 600 of 1024 3.0 and 3.7, 8192 16.4 and 14.9.
+constexpr int kNormRingValues = 9600;
 
 template <bool LAYERNORM, int NV>
 __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring_kernel(const NormBlockParams p) {
@@ -224,25 +227,25 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
 #pragma unroll
       for (int it = 0; it < NV; ++it) {
         const int v = it * (int)blockDim.x + (int)threadIdx.x;
-        unpack8<NV>(v < nvec ? rs[v] : zero, h, it);
+        unpack8(v < nvec ? rs[v] : zero, h[it]);
       }
     } else {
 #pragma unroll
       for (int it = 0; it < NV; ++it) {
         const int v = it * (int)blockDim.x + (int)threadIdx.x;
-        unpack8<NV>(v < nvec ? ys[v] : zero, h, it);
+        unpack8(v < nvec ? ys[v] : zero, h[it]);
       }
       if (p.post_w != nullptr) {
-        norm_rows<LAYERNORM, NV, true>(h, H, p.eps, sums);
+        norm_rows<LAYERNORM, NV, kRowsWide>(h, H, p.eps, sums);
 #pragma unroll
         for (int it = 0; it < NV; ++it) {
-          float g[1][8];
-          unpack8<1>(pv[it], g, 0);
+          float g[8];
+          unpack8(pv[it], g);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) h[it][q] *= g[0][q] + p.w_offset;
+          for (int q = 0; q < 8; ++q) h[it][q] *= g[q] + p.w_offset;
           if (p.post_b != nullptr) {
             float b[8];
-            row_load<true>(p.post_b, it, H, b);
+            vector_load<kRowsWide>(p.post_b, it, H, b);
 #pragma unroll
             for (int q = 0; q < 8; ++q) h[it][q] += b[q];
           }
@@ -253,16 +256,16 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
         const int v = it * (int)blockDim.x + (int)threadIdx.x;
         if (p.gate != nullptr) {
           float g[8];
-          gates<true>(p, t, it, g);
+          gates<kRowsWide>(p, t, it, g);
 #pragma unroll
           for (int q = 0; q < 8; ++q) h[it][q] *= g[q];
         }
-        float r[1][8];
-        unpack8<1>(v < nvec ? rs[v] : zero, r, 0);
+        float r[8];
+        unpack8(v < nvec ? rs[v] : zero, r);
         uint32_t w[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          w[q] = pack_bf16x2(fmaf(p.scale, h[it][2 * q], r[0][2 * q]), fmaf(p.scale, h[it][2 * q + 1], r[0][2 * q + 1]));
+          w[q] = pack_bf16x2(fmaf(p.scale, h[it][2 * q], r[2 * q]), fmaf(p.scale, h[it][2 * q + 1], r[2 * q + 1]));
           const float2 u = unpack_bf16x2(w[q]);
           h[it][2 * q] = u.x;
           h[it][2 * q + 1] = u.y;
@@ -270,32 +273,32 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
         if (v < nvec) reinterpret_cast<uint4*>(p.residual_out + t * p.ldro)[v] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    norm_rows<LAYERNORM, NV, true>(h, H, p.eps, sums + 2);
+    norm_rows<LAYERNORM, NV, kRowsWide>(h, H, p.eps, sums + 2);
     // (a barrier has passed since the row was read last: its stage takes the one after the next)
     if (threadIdx.x == 0 && row + kNormStages * step < p.T) fetch(row + kNormStages * step, s);
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
-      float g[1][8];
-      unpack8<1>(wv[it], g, 0);
+      float g[8];
+      unpack8(wv[it], g);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) h[it][q] *= g[0][q] + p.w_offset;
+      for (int q = 0; q < 8; ++q) h[it][q] *= g[q] + p.w_offset;
       if (p.b != nullptr) {
         float b[8];
-        row_load<true>(p.b, it, H, b);
+        vector_load<kRowsWide>(p.b, it, H, b);
 #pragma unroll
         for (int q = 0; q < 8; ++q) h[it][q] += b[q];
       }
-      if (p.out != nullptr) row_store<true>(p.out + t * p.ldo, it, H, h[it]);
+      if (p.out != nullptr) row_store<kRowsWide>(p.out + t * p.ldo, it, H, h[it]);
     }
     if (p.q != nullptr) {
       float m = 0.f;
 #pragma unroll
       for (int it = 0; it < NV; ++it)
-        if (row_at<true>(it, 0) < H) m = largest_magnitude(m, h[it]);
+        if (row_whole<kRowsWide>(it, H, 0)) m = largest_magnitude(m, h[it]);
       const RowScale sc = row_scale(block_max(m, red_max[i & 1]));
       if (threadIdx.x == 0) p.q_scale[t] = sc.scale;
 #pragma unroll
-      for (int it = 0; it < NV; ++it) row_store_int8<true>(p.q + t * p.ldq, it, H, h[it], sc);
+      for (int it = 0; it < NV; ++it) row_store_int8<kRowsWide>(p.q + t * p.ldq, it, H, h[it], sc);
     }
   }
 }
@@ -322,12 +325,12 @@ static int launch_norm_ring(const NormBlockParams& p, int num_sms, cudaStream_t 
   return -(int)cudaGetLastError();
 }
 
-template <bool LAYERNORM, bool WIDE>
+template <bool LAYERNORM, int M>
 static void launch_norm_block(const NormBlockParams& p, int T, const RowShape& r, cudaStream_t s) {
   const dim3 grid((unsigned)T), block((unsigned)r.threads);
-  if (r.groups == 1) launch_pdl(norm_block_kernel<LAYERNORM, 1, WIDE>, grid, block, 0, s, p);
-  else if (r.groups == 2) launch_pdl(norm_block_kernel<LAYERNORM, 2, WIDE>, grid, block, 0, s, p);
-  else launch_pdl(norm_block_kernel<LAYERNORM, 4, WIDE>, grid, block, 0, s, p);
+  if (r.groups == 1) launch_pdl(norm_block_kernel<LAYERNORM, 1, M>, grid, block, 0, s, p);
+  else if (r.groups == 2) launch_pdl(norm_block_kernel<LAYERNORM, 2, M>, grid, block, 0, s, p);
+  else if (M != kRowsShifted) launch_pdl(norm_block_kernel<LAYERNORM, M == kRowsShifted ? 2 : 4, M>, grid, block, 0, s, p);
 }
 
 }  // namespace lx
@@ -350,19 +353,27 @@ int lx_norm_block(const void* y, long long ldy, const void* residual, long long 
   uintptr_t bits = 0;
   for (const void* a : {y, residual, static_cast<const void*>(residual_out), post_w, post_b, w, b, static_cast<const void*>(out)}) bits |= reinterpret_cast<uintptr_t>(a);
   const bool wide = H % 8 == 0 && bits % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && (ldy | ldr | ldro | ldo | ldq) % 8 == 0;
-  const RowShape r = row_shape(T, H, num_sms, kRowThreads4);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (wide && (ring < 0 ? T >= kNormRingRows * num_sms : ring)) {
+  if (wide && (ring < 0 ? T > num_sms && (long long)T * H >= (long long)kNormRingValues * num_sms : ring)) {
     const bool two = H <= 2 * 8 * kRowThreads4;
     if (layernorm) return two ? launch_norm_ring<true, 2>(p, num_sms, s) : launch_norm_ring<true, 4>(p, num_sms, s);
     return two ? launch_norm_ring<false, 2>(p, num_sms, s) : launch_norm_ring<false, 4>(p, num_sms, s);
   }
+  // every row of every tensor as far from 16 bytes as the residual's?
+  bool alike = H + 7 <= kRowShifted2 * 2 * 8;
+  const auto as_residual = [&](const void* a, long long ld) {
+    return a == nullptr || ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(residual)) % 16 == 0 && (T == 1 || (ld - ldr) % 8 == 0));
+  };
+  alike = alike && as_residual(y, ldy) && as_residual(residual_out, ldro) && as_residual(out, ldo) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
+  const RowShape r = wide || !alike ? row_shape(0, H, num_sms, kRowThreads4) : row_shape_shifted(H + 7);
   if (layernorm) {
-    if (wide) launch_norm_block<true, true>(p, T, r, s);
-    else launch_norm_block<true, false>(p, T, r, s);
+    if (wide) launch_norm_block<true, kRowsWide>(p, T, r, s);
+    else if (alike) launch_norm_block<true, kRowsShifted>(p, T, r, s);
+    else launch_norm_block<true, kRowsApart>(p, T, r, s);
   } else {
-    if (wide) launch_norm_block<false, true>(p, T, r, s);
-    else launch_norm_block<false, false>(p, T, r, s);
+    if (wide) launch_norm_block<false, kRowsWide>(p, T, r, s);
+    else if (alike) launch_norm_block<false, kRowsShifted>(p, T, r, s);
+    else launch_norm_block<false, kRowsApart>(p, T, r, s);
   }
   return -(int)cudaGetLastError();
 }

@@ -69,6 +69,21 @@ def test_rows_of_a_wider_buffer(ops, at, wide):
     assert torch.equal(r.scale.cpu(), want.scale) and torch.equal(r.q.cpu(), want.q)
 
 
+@pytest.mark.parametrize("K", [1, 5, 9, 16, 23, 1000, 1001, 4099])
+@pytest.mark.parametrize("at", [0, 1, 2, 3, 5, 8])
+def test_rows_that_begin_anywhere(ops, K, at):
+    x = _randn(_gen(K, at), 11, 2 * K + 11)
+    r, want = ops.quant_rows_int8(x[:, at:at + K]), ref.quant_rows_int8(x[:, at:at + K].cpu())
+    assert torch.equal(r.scale.cpu(), want.scale) and torch.equal(r.q.cpu(), want.q)
+    v = x[:, at:at + 2 * K]
+    out = torch.full((11, K + 1), 3.0, device="cuda", dtype=BF)
+    r = ops.act_mul_int8(v, K, "relu", out=out[:, 1:])
+    v = v[:, :K].double().clamp_min(0) * v[:, K:].double()
+    # (one rounding of the product)
+    _check_rows(r, v, 1)
+    assert ((out[:, 1:].double() - v).abs() <= HALF * v.abs() + 2 * E * v.abs()).all() and (out[:, 0] == 3).all()
+
+
 @pytest.mark.parametrize("K", [24, 25])
 def test_rows_without_a_scale(ops, K):
     x = _randn(_gen(K), 9, K)
@@ -217,6 +232,22 @@ def test_a_norm_without_a_block_in_front_by_both_forms(ops):
     want, slack = _norm64(res.double(), w, None, 1e-5, 0.0, False)
     for x in (a, b, ops.norm_block(None, res, w, 1e-5)):
         assert ((x.double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
+
+
+@pytest.mark.parametrize("H", [1, 2, 6, 7, 9, 15, 17, 257, 1001, 2049, 4095, 8190, 16377])
+@pytest.mark.parametrize("layernorm,int8", [(False, "both"), (True, False), (True, True)])
+def test_rows_of_any_width_in_tensors_without_gaps(ops, H, layernorm, int8):
+    """Every distance of a row from 16 bytes, the same in all tensors, and rows of which each tensor's begin elsewhere."""
+    _check_norm(ops, 17, H, True, "channel", 0.5, layernorm, int8)
+    g = _gen(H)
+    y, res, w = _randn(g, 17, H + 3)[:, 1:H + 1], _randn(g, 17, H), 1 + _randn(g, H, std=0.1)
+    out = torch.full((17, H + 5), 5.0, device="cuda", dtype=BF)
+    h = torch.empty_like(res)
+    ops.norm_block(y, res, w, 1e-5, residual_out=h, out=out[:, 2:H + 2], layernorm=layernorm)
+    want = res.double() + y.double()
+    assert ((h.double() - want).abs() <= HALF * want.abs() + 2 * E * want.abs()).all() and (out[:, :2] == 5).all() and (out[:, H + 2:] == 5).all()
+    want, slack = _norm64(h.double(), w, None, 1e-5, 0.0, layernorm)
+    assert ((out[:, 2:H + 2].double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
 
 
 @pytest.mark.parametrize("at", [1, 8])
