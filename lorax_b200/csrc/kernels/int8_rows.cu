@@ -2,6 +2,8 @@
 // gate and up halves, which then pass through memory once, as bytes, instead of being written in bf16 and read again.
 //
 // The reference has no such layers (its 8-bit integer weights meet bf16 activations, server/lorax_server/layers/eetq.py:1-26).
+#include <string.h>
+
 #include "int8_rows.cuh"
 
 namespace lx {
@@ -206,19 +208,38 @@ static int launch_rows(const RowsInt8Params& p, int num_sms, int ring, cudaStrea
 
 extern "C" {
 
-// ring as for lx_norm_block.  act < 0: x [T, n] as it is; else act(x[:, :n]), times x[:, n : 2 n] where gated.  out (bf16) may be null.
-int lx_rows_int8(const void* x, long long ldx, void* q, long long ldq, void* scale, void* out, long long ldo, int T, int n, int act, int gated, int* status,
-                 int num_sms, int ring, void* stream) {
+// In one block, as for lx_gemm_int8.
+struct LxRowsInt8Args {
+  const void* x;              // act < 0: [T, n] as it is; else act(x[:, :n]), times x[:, n : 2 n] where gated
+  long long ldx;
+  void* q;
+  long long ldq;
+  float* scale;
+  void* out;                  // [T, n] bf16 or null
+  long long ldo, T, n, act, gated;
+  int* status;
+  long long num_sms;
+  long long ring;             // as of lx_norm_block
+  void* stream;
+};
+int lx_rows_int8_bytes() { return (int)sizeof(LxRowsInt8Args); }
+
+int lx_rows_int8(const char* args) {
   using namespace lx;
-  if (T <= 0) return 0;
-  if (n <= 0) return -1;
-  RowsInt8Params p{reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<int8_t*>(q), ldq, reinterpret_cast<float*>(scale),
-                   reinterpret_cast<__nv_bfloat16*>(out), ldo, n, gated, T, 0, status};
-  const auto at = [](const void* a) { return reinterpret_cast<uintptr_t>(a); };
+  LxRowsInt8Args a;
+  memcpy(&a, args, sizeof(a));
+  if (a.T <= 0) return 0;
+  if (a.n <= 0 || a.n > (1 << 30) || a.T > 0x7fffffff) return -1;
+  const void *x = a.x, *q = a.q, *out = a.out;
+  const long long ldx = a.ldx, ldq = a.ldq, ldo = a.ldo;
+  const int n = (int)a.n, num_sms = (int)a.num_sms, ring = (int)a.ring;
+  RowsInt8Params p{reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<int8_t*>(a.q), ldq, a.scale, reinterpret_cast<__nv_bfloat16*>(a.out), ldo, n,
+                   (int)a.gated, (int)a.T, 0, a.status};
+  const auto at = [](const void* v) { return reinterpret_cast<uintptr_t>(v); };
   const bool wide = n % 8 == 0 && at(x) % 16 == 0 && ldx % 8 == 0 && at(q) % 8 == 0 && ldq % 8 == 0 && at(out) % 16 == 0 && ldo % 8 == 0;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(a.stream);
 #define LX_ROWS(A) return wide ? launch_rows<A, kRowsWide>(p, num_sms, ring, s) : launch_rows<A, kRowsShifted>(p, num_sms, ring, s)
-  switch (act) {
+  switch (a.act) {
     case kRowsSilu: LX_ROWS(kRowsSilu);
     case kRowsGelu: LX_ROWS(kRowsGelu);
     case kRowsGeluTanh: LX_ROWS(kRowsGeluTanh);

@@ -5,6 +5,8 @@
 // with a scale for each row (int8_rows.cuh), from the same 32-bit values, or both.
 //
 // The reference norms and adds in separate kernels (server/lorax_server/models/custom_modeling/flash_gemma2_modeling.py:355-396).
+#include <string.h>
+
 #include "int8_rows.cuh"
 
 namespace lx {
@@ -339,21 +341,48 @@ extern "C" {
 
 int lx_norm_block_max_width() { return lx::kRowThreads4 * 4 * 8; }
 
-// ring: -1 the library's choice, 0 or 1 (where rows begin at 16 bytes) a block per row or blocks that stay, to measure each.
-int lx_norm_block(const void* y, long long ldy, const void* residual, long long ldr, void* residual_out, long long ldro, const void* post_w,
-                  const void* post_b, const void* w, const void* b, const void* gate, long long gate_t, int gate_h, void* out, long long ldo, void* q,
-                  long long ldq, void* q_scale, int T, int H, float eps, float w_offset, float scale, int layernorm, int* status, int num_sms, int ring, void* stream) {
+// In one block, as for lx_gemm_int8.
+struct LxNormBlockArgs {
+  const void* y;              // [T, H] or null
+  long long ldy;
+  const void* residual;
+  long long ldr;
+  void* residual_out;         // or null
+  long long ldro;
+  const void *post_w, *post_b, *w, *b, *gate;
+  long long gate_t, gate_h;   // elements between two rows' gates, two channels' (0 or 1)
+  void* out;                  // [T, H] bf16 or null
+  long long ldo;
+  void* q;                    // [T, H] int8 or null
+  long long ldq;
+  void* q_scale;
+  long long T, H, layernorm;
+  int* status;
+  long long num_sms;
+  long long ring;             // -1: the library's choice; 0 or 1 (where rows begin at 16 bytes): a block per row or blocks that stay, to measure each
+  void* stream;
+  double eps, w_offset, scale;
+};
+int lx_norm_block_bytes() { return (int)sizeof(LxNormBlockArgs); }
+
+int lx_norm_block(const char* args) {
   using namespace lx;
-  if (T <= 0) return 0;
-  if (H <= 0 || H > lx_norm_block_max_width()) return -1;
-  const auto bf = [](const void* a) { return reinterpret_cast<const __nv_bfloat16*>(a); };
-  NormBlockParams p{bf(y), bf(residual), reinterpret_cast<__nv_bfloat16*>(residual_out), bf(post_w), bf(post_b), bf(w), bf(b), bf(gate), gate_t, gate_h, reinterpret_cast<uintptr_t>(gate) % 16 == 0 && gate_t % 8 == 0,
-                    reinterpret_cast<__nv_bfloat16*>(out), reinterpret_cast<int8_t*>(q), reinterpret_cast<float*>(q_scale), ldy, ldr, ldro, ldo, ldq, H, T, eps,
-                    w_offset, scale, status};
+  LxNormBlockArgs a;
+  memcpy(&a, args, sizeof(a));
+  if (a.T <= 0) return 0;
+  if (a.H <= 0 || a.H > lx_norm_block_max_width() || a.T > 0x7fffffff) return -1;
+  const void *y = a.y, *residual = a.residual, *residual_out = a.residual_out, *out = a.out, *q = a.q, *gate = a.gate;
+  const long long ldy = a.ldy, ldr = a.ldr, ldro = a.ldro, ldo = a.ldo, ldq = a.ldq, gate_t = a.gate_t;
+  const int T = (int)a.T, H = (int)a.H, num_sms = (int)a.num_sms, ring = (int)a.ring, layernorm = (int)a.layernorm;
+  const auto bf = [](const void* v) { return reinterpret_cast<const __nv_bfloat16*>(v); };
+  NormBlockParams p{bf(y), bf(residual), reinterpret_cast<__nv_bfloat16*>(a.residual_out), bf(a.post_w), bf(a.post_b), bf(a.w), bf(a.b), bf(gate), gate_t,
+                    (int)a.gate_h, reinterpret_cast<uintptr_t>(gate) % 16 == 0 && gate_t % 8 == 0, reinterpret_cast<__nv_bfloat16*>(a.out),
+                    reinterpret_cast<int8_t*>(a.q), reinterpret_cast<float*>(a.q_scale), ldy, ldr, ldro, ldo, ldq, H, T, (float)a.eps, (float)a.w_offset,
+                    (float)a.scale, a.status};
   uintptr_t bits = 0;
-  for (const void* a : {y, residual, static_cast<const void*>(residual_out), post_w, post_b, w, b, static_cast<const void*>(out)}) bits |= reinterpret_cast<uintptr_t>(a);
+  for (const void* v : {y, residual, residual_out, a.post_w, a.post_b, a.w, a.b, out}) bits |= reinterpret_cast<uintptr_t>(v);
   const bool wide = H % 8 == 0 && bits % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && (ldy | ldr | ldro | ldo | ldq) % 8 == 0;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(a.stream);
   if (wide && (ring < 0 ? T > num_sms && (long long)T * H >= (long long)kNormRingValues * num_sms : ring)) {
     const bool two = H <= 2 * 8 * kRowThreads4;
     if (layernorm) return two ? launch_norm_ring<true, 2>(p, num_sms, s) : launch_norm_ring<true, 4>(p, num_sms, s);
@@ -361,8 +390,8 @@ int lx_norm_block(const void* y, long long ldy, const void* residual, long long 
   }
   // every row of every tensor as far from 16 bytes as the residual's?
   bool alike = H + 7 <= kRowShifted2 * 2 * 8;
-  const auto as_residual = [&](const void* a, long long ld) {
-    return a == nullptr || ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(residual)) % 16 == 0 && (T == 1 || (ld - ldr) % 8 == 0));
+  const auto as_residual = [&](const void* v, long long ld) {
+    return v == nullptr || ((reinterpret_cast<uintptr_t>(v) ^ reinterpret_cast<uintptr_t>(residual)) % 16 == 0 && (T == 1 || (ld - ldr) % 8 == 0));
   };
   alike = alike && as_residual(y, ldy) && as_residual(residual_out, ldro) && as_residual(out, ldo) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
   const RowShape r = wide || !alike ? row_shape(0, H, num_sms, kRowThreads4) : row_shape_shifted(H + 7);

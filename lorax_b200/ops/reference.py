@@ -1226,8 +1226,9 @@ class Int8Rows(NamedTuple):
     scale: torch.Tensor            # [T] fp32
 
 
-def empty_int8_rows(T: int, K: int, device) -> Int8Rows:
-    return Int8Rows(torch.empty_strided((T, K), ((K + 15) // 16 * 16, 1), dtype=torch.int8, device=device), torch.empty(T, dtype=torch.float32, device=device))
+def empty_int8_rows(T: int, K: int, like) -> Int8Rows:
+    """Rows for T x K numbers on the device of `like`."""
+    return Int8Rows(like.new_empty_strided((T, K), ((K + 15) // 16 * 16, 1), dtype=torch.int8), like.new_empty_strided((T,), (1,), dtype=torch.float32))
 
 
 def _to_int8_rows(v) -> Int8Rows:
@@ -1237,7 +1238,7 @@ def _to_int8_rows(v) -> Int8Rows:
     scale = torch.where(top.isfinite(), top / torch.full_like(top, 127.0), torch.full_like(top, float("nan")))      # (a division, not a product)
     some = (scale > 0)[:, None]
     q = torch.where(some, v.double() / torch.where(some, scale[:, None], 1.0).double(), 0.0)      # (64 bits: which of two integers is nearer)
-    r = empty_int8_rows(*v.shape, v.device)
+    r = empty_int8_rows(*v.shape, v)
     r.q.copy_(q.round().clamp(-127, 127))
     r.scale.copy_(scale)
     return r
@@ -1248,7 +1249,7 @@ def quantize_weight_int8(w: torch.Tensor):
     parts = [_to_int8_rows(p.float()) for p in w.split(max(1, (1 << 26) // max(1, w.shape[1])))]
     if len(parts) == 1:
         return tuple(parts[0])
-    whole = empty_int8_rows(*w.shape, w.device)
+    whole = empty_int8_rows(*w.shape, w)
     at = 0
     for p in parts:
         n = p.q.shape[0]
@@ -1423,21 +1424,25 @@ def norm_block(y, residual, weight, eps, post_weight=None, gate=None, scale: flo
 
 
 def check_gemm_int8(x, w, w_scale, bias, out, dtype):
-    """-> (T, N, K)."""
+    """-> (T, N, K, bytes between two rows, between two rows of the weights)."""
     if not isinstance(x, Int8Rows):
         raise ValueError("gemm_int8: x is the Int8Rows of a quantiser")
     q, scale = x
-    if not (q.dim() == 2 and w.dim() == 2 and q.dtype == torch.int8 and w.dtype == torch.int8 and q.shape[1] == w.shape[1]):
+    if not (q.dim() == 2 and w.dim() == 2 and q.dtype == torch.int8 and w.dtype == torch.int8):
         raise ValueError(f"gemm_int8: int8 rows [T, K] and weights [N, K]; got {tuple(q.shape)} {q.dtype}, {tuple(w.shape)} {w.dtype}")
-    (T, K), N, at = q.shape, w.shape[0], q.get_device()
-    if not (1 <= K <= INT8_MAX_K):
-        raise ValueError(f"gemm_int8: K from 1 to {INT8_MAX_K}, whose sums stay whole; got {K}")
+    (T, K), (N, K2), at = q.shape, w.shape, q.get_device()
+    if not (K == K2 and 1 <= K <= INT8_MAX_K):
+        raise ValueError(f"gemm_int8: rows and weights of the same K, from 1 to {INT8_MAX_K}, whose sums stay whole; got {K}, {K2}")
+    pitches = []
     for name, t, n in (("rows", q, T), ("weights", w, N)):
         s0, s1 = t.stride()
-        if not ((K == 1 or s1 == 1) and (n <= 1 or (s0 >= K and s0 % 16 == 0)) and (n == 0 or t.data_ptr() % 16 == 0)):
+        if n <= 1:
+            s0 = (K + 15) // 16 * 16                 # (one row's own distance says nothing)
+        if (s1 != 1 and K > 1) or s0 < K or s0 % 16 or (n and t.data_ptr() % 16):
             raise ValueError(f"gemm_int8: {name} begin at 16 bytes and lie a multiple of 16 bytes apart; got strides {t.stride()}")
+        pitches.append(s0)
     for name, t, n in (("the rows' scales", scale, T), ("w_scale", w_scale, N)):
-        if not (t.dim() == 1 and t.shape[0] == n and t.dtype == torch.float32 and t.is_contiguous() and t.get_device() == at):
+        if not (t.dtype == torch.float32 and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.get_device() == at):
             raise ValueError(f"gemm_int8: {name} are [{n}] fp32, contiguous, on the rows' device")
     if bias is not None and not (bias.shape == (N,) and bias.dtype == dtype and bias.is_contiguous() and bias.get_device() == at):
         raise ValueError(f"gemm_int8: bias is [{N}] {dtype}, contiguous, on the rows' device")
@@ -1445,12 +1450,12 @@ def check_gemm_int8(x, w, w_scale, bias, out, dtype):
         raise ValueError("gemm_int8: weights on the rows' device")
     if out is not None and not (out.dtype == dtype and out.get_device() == at and _rows_fit(out, T, N) and _apart(out, (q, scale, w, w_scale, bias))):
         raise ValueError(f"gemm_int8: out is [T, N] {dtype} on the rows' device, apart from the inputs")
-    return T, N, K
+    return T, N, K, pitches[0], pitches[1]
 
 
 def gemm_int8(x: Int8Rows, w, w_scale, bias=None, out=None, dtype=torch.bfloat16, w_const: bool = False):
     """out[t, n] = (sum over k of x.q[t, k] * w[n, k]) * w_scale[n] * x.scale[t] + bias[n]: the sums whole, the rest in 32 bits, one rounding to `dtype`."""
-    T, N, K = check_gemm_int8(x, w, w_scale, bias, out, dtype)
+    check_gemm_int8(x, w, w_scale, bias, out, dtype)
     y = (x.q.double() @ w.double().t()).float() * w_scale * x.scale[:, None]
     if bias is not None:
         y = y + bias.float()

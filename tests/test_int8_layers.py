@@ -106,7 +106,7 @@ def test_empty_calls():
 
 
 def _rows(T, K):
-    return ref.empty_int8_rows(T, K, "cpu")
+    return ref.empty_int8_rows(T, K, torch.empty(0))
 
 
 NORM = dict(y=torch.zeros(3, 16, dtype=BF), residual=torch.zeros(3, 16, dtype=BF), weight=torch.ones(16, dtype=BF), eps=1e-6)
@@ -198,8 +198,9 @@ def test_the_bindings_take_bf16_on_a_gpu():
 def test_limits_of_the_library_and_of_python_agree(monkeypatch):
     from lorax_b200.ops import native, native_int8
     native_int8.check_limits(native.load())
-    for name in ("NORM_BLOCK_MAX_WIDTH", "INT8_MAX_K"):
-        monkeypatch.setattr(native_int8, name, getattr(ref, name) + 1)
+    for name, value in (("NORM_BLOCK_MAX_WIDTH", ref.NORM_BLOCK_MAX_WIDTH + 1), ("INT8_MAX_K", ref.INT8_MAX_K + 1), ("_NORM", native_int8._GEMM), ("_ROWS", native_int8._GEMM),
+                        ("_GEMM", native_int8._ROWS)):
+        monkeypatch.setattr(native_int8, name, value)
         with pytest.raises(native.NativeError, match="C\\+\\+ says"):
             native_int8.check_limits(native.load())
         monkeypatch.undo()

@@ -297,7 +297,8 @@ def _check_product(ops, T, N, K, bias=True, at=0, out=None, plan=None):
     if plan is None:
         y = ops.gemm_int8(Int8Rows(q, xs), w, ws, bias=b, out=out)
     else:
-        y = native_int8._on(w, native_int8._gemm_int8, Int8Rows(q, xs), w, ws, b, out, T, N, K, False, plan)
+        x = Int8Rows(q, xs)
+        y = native_int8._on(w, native_int8._gemm_int8, x, w, ws, b, out, ref.check_gemm_int8(x, w, ws, b, out, BF), False, plan)
     s = (q.double() @ w.double().t()) * (xs.double()[:, None] * ws.double())
     want = s + (0 if b is None else b.double())
     # the sum to 32 bits, two products, the bias: four roundings; then one to bf16
