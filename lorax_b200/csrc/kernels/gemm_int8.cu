@@ -226,13 +226,10 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   }
 
   // (done: every load of this CTA has arrived and been read, so the ring is free)
-  bool ok = mbar_wait(done_bar, 0, abort_flag);
+  const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag));
   if (!ok) {
     report_status(p.status, kTimeoutTmemFull, item);
     *abort_flag = 1;
-    // copies still on their way arrive before this CTA leaves
-    if (threadIdx.x == 0)
-      for (int s = 0; s < min(p.stages, loaded); ++s) mbar_wait(&full_bar[s], (uint32_t)((loaded - 1 - s) / p.stages) & 1u, nullptr);
   }
   const int t0 = tb * p.bn, live = min(p.bn, p.T - t0);
   if (ok) {
@@ -250,11 +247,14 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   }
   if (p.parts > 1) cluster_sync();
   else __syncthreads();
-  if (!*abort_flag) {
+  if (__syncthreads_or(*abort_flag) == 0) {
     if (p.parts == 1) int8_join<1, 4>(p, sums, scales, 0, 0, 0, ta * kI8BM, t0, live);
     else if (p.parts <= 4) int8_join<4, 4>(p, sums, scales, part, 0, 1, ta * kI8BM, t0, live);
     else int8_join<kI8MaxParts, 2>(p, sums, scales, part, 0, 1, ta * kI8BM, t0, live);
   }
+  if (*abort_flag && threadIdx.x == 0)  // copies still on their way arrive before this CTA leaves
+    for (int s = 0; s < min(p.stages, loaded); ++s) mbar_wait(&full_bar[s], (uint32_t)((loaded - 1 - s) / p.stages) & 1u, nullptr);
+  __syncwarp();
   if (p.parts > 1) cluster_sync();      // nobody leaves while its sums are read
   else __syncthreads();
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_d, (uint32_t)p.tmem_cols); }
@@ -415,7 +415,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 #pragma unroll
         for (int i = 0; i < 8; ++i) xl[i] = p.xs[min(j0 + 32 * i + lane, p.T - 1)];
       }
-      if (!mbar_wait(&tmem_full[acc], acc_phase[acc], abort_flag)) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_phase[acc], abort_flag))) {
         report_status(p.status, kTimeoutTmemFull, tile);
         *abort_flag = 1;
         break;
@@ -486,12 +486,13 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 
   if (*abort_flag && rank == 0 && threadIdx.x == 0)    // copies still on their way to either CTA arrive before the pair leaves
     for (int s = 0; s < min(kI8PairStages, loaded); ++s) mbar_wait(&full_bar[s], (uint32_t)((loaded - 1 - s) / kI8PairStages) & 1u, nullptr);
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   cluster_sync();                                      // nothing of this pair is on its way to a CTA that has left; the parts' sums are there
   if (p.parts > 1) {
     const int j0 = first % tiles_b * p.bn;
-    if (!*abort_flag)
+    if (__syncthreads_or(*abort_flag) == 0)
       int8_join<kI8PairMaxParts, 4>(p, reinterpret_cast<const int*>(smem), scales, part, (uint32_t)rank, 2, (2 * (first / tiles_b) + rank) * kI8BM, j0, min(p.bn, p.T - j0));
     __syncwarp();
     cluster_sync();

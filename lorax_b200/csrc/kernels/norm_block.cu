@@ -370,7 +370,7 @@ int lx_norm_block(const char* args) {
   LxNormBlockArgs a;
   memcpy(&a, args, sizeof(a));
   if (a.T <= 0) return 0;
-  if (a.H <= 0 || a.H > lx_norm_block_max_width() || a.T > 0x7fffffff) return -1;
+  if (a.H <= 0 || a.H > lx_norm_block_max_width() || a.T > 0x7fffffff || (a.y != nullptr && a.residual_out == nullptr)) return -1;
   const void *y = a.y, *residual = a.residual, *residual_out = a.residual_out, *out = a.out, *q = a.q, *gate = a.gate;
   const long long ldy = a.ldy, ldr = a.ldr, ldro = a.ldro, ldo = a.ldo, ldq = a.ldq, gate_t = a.gate_t;
   const int T = (int)a.T, H = (int)a.H, num_sms = (int)a.num_sms, ring = (int)a.ring, layernorm = (int)a.layernorm;

@@ -1351,7 +1351,7 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
     for name, t in (("y", y), ("residual", residual), ("residual_out", residual_out), ("out", out)):
         if t is None:
             continue
-        if not (t.shape == shape and t.dtype == dtype and t.get_device() == at):
+        if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.get_device() == at):
             raise ValueError(f"norm_block: {name} is [T, H], of the residual's type and device")
         s0, s1 = t.stride()
         if (s1 != 1 and H > 1) or (s0 < H and T > 1):
@@ -1375,8 +1375,8 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
         to = residual if residual_out is None else residual_out
     gates = None
     if gate is not None:
-        if not (gate.dtype == dtype and gate.get_device() == at and gate.dim() <= 2):
-            raise ValueError("norm_block: gate is of the residual's type and device")
+        if not (isinstance(gate, torch.Tensor) and gate.dtype == dtype and gate.get_device() == at and gate.dim() <= 2):
+            raise ValueError("norm_block: gate is a tensor of the residual's type and device")
         try:
             gates = gate.expand(T, H)
         except RuntimeError:
@@ -1428,6 +1428,8 @@ def check_gemm_int8(x, w, w_scale, bias, out, dtype):
     if not isinstance(x, Int8Rows):
         raise ValueError("gemm_int8: x is the Int8Rows of a quantiser")
     q, scale = x
+    if not all(isinstance(t, torch.Tensor) for t in (q, scale, w, w_scale)):
+        raise ValueError("gemm_int8: rows, weights and their scales are tensors")
     if not (q.dim() == 2 and w.dim() == 2 and q.dtype == torch.int8 and w.dtype == torch.int8):
         raise ValueError(f"gemm_int8: int8 rows [T, K] and weights [N, K]; got {tuple(q.shape)} {q.dtype}, {tuple(w.shape)} {w.dtype}")
     (T, K), (N, K2), at = q.shape, w.shape, q.get_device()

@@ -117,7 +117,7 @@ _BUF = torch.zeros(3, 64, dtype=BF)
     dict(y=torch.zeros(2, 16, dtype=BF)), dict(y=torch.zeros(3, 16)), dict(residual=torch.zeros(16, dtype=BF)), dict(y=torch.zeros(16, 3, dtype=BF).t()),
     dict(weight=torch.ones(8, dtype=BF)), dict(weight=torch.ones(16)), dict(weight=torch.ones(32, dtype=BF)[::2]), dict(weight=None),
     dict(post_bias=torch.zeros(16, dtype=BF)), dict(post_weight=torch.ones(1, dtype=BF)), dict(gate=torch.ones(3, dtype=BF)), dict(gate=torch.ones(16)),
-    dict(gate=torch.ones(3, 32, dtype=BF)[:, ::2]), dict(gate=torch.ones(1, 1, 16, dtype=BF)), dict(y=None, scale=0.5), dict(y=None, gate=torch.ones(1, dtype=BF)),
+    dict(gate=torch.ones(3, 32, dtype=BF)[:, ::2]), dict(gate=0.5), dict(y=1.0), dict(gate=torch.ones(1, 1, 16, dtype=BF)), dict(y=None, scale=0.5), dict(y=None, gate=torch.ones(1, dtype=BF)),
     dict(y=None, post_weight=torch.ones(16, dtype=BF)), dict(y=None, residual_out=torch.zeros(3, 16, dtype=BF)),
     dict(y=_BUF[:, :16], residual=_BUF[:, 8:24]), dict(y=_BUF[:, :16], residual_out=_BUF[:, 8:24]), dict(residual_out=torch.zeros(3, 16)),
     dict(residual=torch.zeros(2, 16385, dtype=BF), y=torch.zeros(2, 16385, dtype=BF), weight=torch.zeros(16385, dtype=BF)), dict(out=torch.zeros(3, 17, dtype=BF))])
@@ -149,7 +149,7 @@ GEMM = dict(x=_rows(3, 32), w=torch.zeros(5, 32, dtype=torch.int8), w_scale=torc
     dict(x=torch.zeros(3, 32, dtype=torch.int8)), dict(x=_rows(3, 48)), dict(x=Int8Rows(torch.zeros(3, 32), torch.ones(3))), dict(x=Int8Rows(_rows(3, 32).q, torch.ones(4))),
     dict(x=Int8Rows(torch.zeros(3, 40, dtype=torch.int8)[:, :32], torch.ones(3))), dict(x=Int8Rows(torch.zeros(3, 48, dtype=torch.int8)[:, 8:40], torch.ones(3))),
     dict(x=Int8Rows(_rows(3, 32).q, torch.ones(3, dtype=torch.float64))), dict(w=torch.zeros(5, 32)), dict(w=torch.zeros(32, 5, dtype=torch.int8).t()),
-    dict(w_scale=torch.ones(5, 1)), dict(w_scale=torch.ones(10)[::2]), dict(bias=torch.ones(5)), dict(bias=torch.ones(4, dtype=BF)),
+    dict(w_scale=torch.ones(5, 1)), dict(w_scale=0.5), dict(w=None), dict(w_scale=torch.ones(10)[::2]), dict(bias=torch.ones(5)), dict(bias=torch.ones(4, dtype=BF)),
     dict(out=torch.zeros(3, 6, dtype=BF)), dict(out=torch.zeros(3, 5)), dict(out=torch.zeros(5, 3, dtype=BF).t()), dict(x=_rows(3, 0), w=torch.zeros(5, 0, dtype=torch.int8)),
     dict(x=_rows(1, (1 << 17) + 16), w=torch.zeros(1, (1 << 17) + 16, dtype=torch.int8), w_scale=torch.ones(1))])
 def test_products_that_are_refused(change):
