@@ -176,7 +176,7 @@ constexpr int kNormStages = 2;
 // 148 of 8192 4.6 and 5.0, 200 7.3 and 6.3, 4001 70 and 49; 600 of 1024 3.0 and 3.7, 8192 16.4 and 14.9.
 constexpr int kNormRingValues = 9600;
 
-template <bool LAYERNORM, int NV>
+template <bool LAYERNORM, int NV, bool INT8>
 __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring_kernel(const NormBlockParams p) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t full[kNormStages];
@@ -202,14 +202,17 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
   };
   if (threadIdx.x == 0)
     for (int s = 0; s < kNormStages && (int)blockIdx.x + s * step < p.T; ++s) fetch((int)blockIdx.x + s * step, s);
+  // The norms' weights stay in registers, or in L1 where the quotients need the registers.
   uint4 wv[NV], pv[NV];
-#pragma unroll
-  for (int it = 0; it < NV; ++it) {
+  const auto weight = [&](const __nv_bfloat16* w, int it) {
     const int v = it * (int)blockDim.x + (int)threadIdx.x;
-    wv[it] = pv[it] = make_uint4(0, 0, 0, 0);
-    if (v < nvec) {
-      wv[it] = reinterpret_cast<const uint4*>(p.w)[v];
-      if (p.post_w != nullptr) pv[it] = reinterpret_cast<const uint4*>(p.post_w)[v];
+    return v < nvec ? reinterpret_cast<const uint4*>(w)[v] : make_uint4(0, 0, 0, 0);
+  };
+  if (!INT8) {
+#pragma unroll
+    for (int it = 0; it < NV; ++it) {
+      wv[it] = weight(p.w, it);
+      if (p.post_w != nullptr) pv[it] = weight(p.post_w, it);
     }
   }
   int i = 0;
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
 #pragma unroll
         for (int it = 0; it < NV; ++it) {
           float g[8];
-          unpack8(pv[it], g);
+          unpack8(INT8 ? weight(p.post_w, it) : pv[it], g);
 #pragma unroll
           for (int q = 0; q < 8; ++q) h[it][q] *= g[q] + p.w_offset;
           if (p.post_b != nullptr) {
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
       float g[8];
-      unpack8(wv[it], g);
+      unpack8(INT8 ? weight(p.w, it) : wv[it], g);
 #pragma unroll
       for (int q = 0; q < 8; ++q) h[it][q] *= g[q] + p.w_offset;
       if (p.b != nullptr) {
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
       }
       if (p.out != nullptr) row_store<kRowsWide>(p.out + t * p.ldo, it, H, h[it]);
     }
-    if (p.q != nullptr) {
+    if (INT8) {
       float m = 0.f;
 #pragma unroll
       for (int it = 0; it < NV; ++it)
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
 }
 
 // Blocks that an SM holds at a time go by their registers (64 a thread, 128 with four groups) and their stages.
-template <bool LAYERNORM, int NV>
+template <bool LAYERNORM, int NV, bool INT8>
 static int launch_norm_ring(const NormBlockParams& p, int num_sms, cudaStream_t s) {
   const int need = p.H / 8, threads = ((need + NV - 1) / NV + 31) / 32 * 32;
   const int smem = kNormStages * p.H * 2 * (p.y != nullptr ? 2 : 1);
@@ -314,7 +317,7 @@ static int launch_norm_ring(const NormBlockParams& p, int num_sms, cudaStream_t 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   if (!set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(norm_block_ring_kernel<LAYERNORM, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormStages * 2 * 2 * kRowThreads4 * 8 * NV);
+    const cudaError_t e = cudaFuncSetAttribute(norm_block_ring_kernel<LAYERNORM, NV, INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormStages * 2 * 2 * kRowThreads4 * 8 * NV);
     if (e != cudaSuccess) return -(int)e;
     set[dev] = true;
   }
@@ -323,7 +326,7 @@ static int launch_norm_ring(const NormBlockParams& p, int num_sms, cudaStream_t 
   if (blocks > 32) blocks = 32;
   if (blocks < 1) blocks = 1;
   const int grid = p.T < num_sms * blocks ? p.T : num_sms * blocks;
-  launch_pdl(norm_block_ring_kernel<LAYERNORM, NV>, dim3((unsigned)grid), dim3((unsigned)threads), (size_t)smem, s, p);
+  launch_pdl(norm_block_ring_kernel<LAYERNORM, NV, INT8>, dim3((unsigned)grid), dim3((unsigned)threads), (size_t)smem, s, p);
   return -(int)cudaGetLastError();
 }
 
@@ -384,9 +387,12 @@ int lx_norm_block(const char* args) {
   const bool wide = H % 8 == 0 && bits % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && (ldy | ldr | ldro | ldo | ldq) % 8 == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(a.stream);
   if (wide && (ring < 0 ? T > num_sms && (long long)T * H >= (long long)kNormRingValues * num_sms : ring)) {
-    const bool two = H <= 2 * 8 * kRowThreads4;
-    if (layernorm) return two ? launch_norm_ring<true, 2>(p, num_sms, s) : launch_norm_ring<true, 4>(p, num_sms, s);
-    return two ? launch_norm_ring<false, 2>(p, num_sms, s) : launch_norm_ring<false, 4>(p, num_sms, s);
+#define LX_RING(LN, Q) return H <= 2 * 8 * kRowThreads4 ? launch_norm_ring<LN, 2, Q>(p, num_sms, s) : launch_norm_ring<LN, 4, Q>(p, num_sms, s)
+    if (layernorm && q != nullptr) LX_RING(true, true);
+    if (layernorm) LX_RING(true, false);
+    if (q != nullptr) LX_RING(false, true);
+    LX_RING(false, false);
+#undef LX_RING
   }
   // every row of every tensor as far from 16 bytes as the residual's?
   bool alike = H + 7 <= kRowShifted2 * 2 * 8;
