@@ -1,14 +1,12 @@
 // Products of 8-bit integers with a scale for each token and each output channel, on the 5th-generation tensor cores:
 //   out[t, n] = (sum_k xq[t, k] * wq[n, k]) * ws[n] * xs[t] + bias[n]
-// The sums are whole numbers in 32 bits (tcgen05.mma.kind::i8, exact for K up to 2^17: 2^17 * 127 * 128 < 2^31), so that no order in which parts of
+// The sums are whole numbers in 32 bits (tcgen05.mma.kind::i8, exact for K below 2^17: 128 * 128 * (2^17 - 1) < 2^31), so that no order in which parts of
 // K are added changes a result; scales and bias are applied in 32-bit floating point, the
 // weights' first (rows of any size then overflow only where their results do), and the result is rounded to bf16 once.
 //
 // Weights take the UMMA M side, 128 output features a tile; tokens the N side in steps of 16.  A stage of the ring is 128 bytes of K of both.
 // Where there are fewer tiles than SMs the CTAs of a cluster share a tile's K and add their sums up through each other's shared memory: nothing is
 // kept in global memory between CTAs, calls or graphs.
-//
-// The reference has no such product (it expands 8-bit integer weights beside bf16 activations, server/lorax_server/layers/eetq.py:1-26).
 #include <math.h>
 #include <string.h>
 
@@ -648,7 +646,7 @@ static int int8_clusters(int parts) {
 
 extern "C" {
 
-int lx_gemm_int8_max_k() { return 1 << 17; }
+int lx_gemm_int8_max_k() { return (1 << 17) - 1; }
 
 // The plan that a product takes where `clusters` (of 1, 2, 3, 4 pairs) run at the same time: out[0] pairs of CTAs (0: single ones), out[1] tokens a tile,
 // out[2] CTAs or pairs that share a tile's K, out[3] stages of a single CTA's ring.

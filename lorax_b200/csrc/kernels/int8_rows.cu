@@ -1,7 +1,5 @@
 // Quantisers of rows for products in 8-bit integers (int8_rows.cuh states the numbers): rows as they are, or the activations of a feed-forward's
 // gate and up halves, which then pass through memory once, as bytes, instead of being written in bf16 and read again.
-//
-// The reference has no such layers (its 8-bit integer weights meet bf16 activations, server/lorax_server/layers/eetq.py:1-26).
 #include <string.h>
 
 #include "int8_rows.cuh"

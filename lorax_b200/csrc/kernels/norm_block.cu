@@ -3,8 +3,6 @@
 //   x = N(h),  N(v) = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * (w + offset) + b      (RMS norm: without the means)
 // h replaces the residual (or is written elsewhere) in bf16, and N reads the rounded h, as whoever reads the stream later does.  x leaves in bf16, in 8 bits
 // with a scale for each row (int8_rows.cuh), from the same 32-bit values, or both.
-//
-// The reference norms and adds in separate kernels (server/lorax_server/models/custom_modeling/flash_gemma2_modeling.py:355-396).
 #include <string.h>
 
 #include "int8_rows.cuh"

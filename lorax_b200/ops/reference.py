@@ -1214,7 +1214,7 @@ def token_scores(logits, targets=None, k: int = 0, softcap: float = 0.0, entropy
 
 
 # ------------------------------------------------------------------------------------------------ layers in 8-bit integers
-INT8_MAX_K = 1 << 17               # products whose sums stay below 2^31
+INT8_MAX_K = (1 << 17) - 1         # products whose sums stay below 2^31
 NORM_BLOCK_MAX_WIDTH = 16384
 ROWS_INT8_MAX = 1 << 30            # values of a row
 INT8_ACTS = ("silu", "swish", "gelu", "gelu_new", "gelu_pytorch_tanh", "gelu_fast", "gelu_tanh", "relu", "relu2")

@@ -151,7 +151,7 @@ GEMM = dict(x=_rows(3, 32), w=torch.zeros(5, 32, dtype=torch.int8), w_scale=torc
     dict(x=Int8Rows(_rows(3, 32).q, torch.ones(3, dtype=torch.float64))), dict(w=torch.zeros(5, 32)), dict(w=torch.zeros(32, 5, dtype=torch.int8).t()),
     dict(w_scale=torch.ones(5, 1)), dict(w_scale=0.5), dict(w=None), dict(w_scale=torch.ones(10)[::2]), dict(bias=torch.ones(5)), dict(bias=torch.ones(4, dtype=BF)),
     dict(out=torch.zeros(3, 6, dtype=BF)), dict(out=torch.zeros(3, 5)), dict(out=torch.zeros(5, 3, dtype=BF).t()), dict(x=_rows(3, 0), w=torch.zeros(5, 0, dtype=torch.int8)),
-    dict(x=_rows(1, (1 << 17) + 16), w=torch.zeros(1, (1 << 17) + 16, dtype=torch.int8), w_scale=torch.ones(1))])
+    dict(x=_rows(1, 1 << 17), w=torch.zeros(1, 1 << 17, dtype=torch.int8), w_scale=torch.ones(1))])
 def test_products_that_are_refused(change):
     for ops in _ops():
         with pytest.raises(ValueError, match="gemm_int8"):
@@ -218,7 +218,7 @@ def _plan(T, N, K, sms=148, clusters=(74, 33, 22, 15)):
 @pytest.mark.parametrize("sms,clusters", [(148, (74, 33, 22, 15)), (148, (0, 0, 0, 0)), (20, (10, 4, 2, 1)), (1, (0, 0, 0, 0))])
 def test_plans_stay_within_what_tiles_and_clusters_allow(sms, clusters):
     rng = __import__("random").Random(7)
-    sizes = [(1, 1, 1), (1 << 20, 1, 1), (1, 1 << 20, 128), (4001, 28672, 4096), (300, 100, 1 << 17)]
+    sizes = [(1, 1, 1), (1 << 20, 1, 1), (1, 1 << 20, 128), (4001, 28672, 4096), (300, 100, (1 << 17) - 1)]
     sizes += [tuple(int(2 ** rng.uniform(0, top)) for top in (13, 15, 15)) for _ in range(400)]
     for T, N, K in sizes:
         pairs, bn, parts, stages = _plan(T, N, K, sms, clusters)
@@ -294,3 +294,77 @@ def test_layer_by_layer_designs_are_not_quantised():
 def test_w8a8_is_a_name_of_the_shard_s_quantize_flag():
     from lorax_b200.server.cli import QUANTIZE_CHOICES
     assert "w8a8" in QUANTIZE_CHOICES
+
+
+# ------------------------------------------------------------------------------------------------ devices
+def test_operators_run_on_their_tensors_device_whichever_is_current(monkeypatch):
+    """Tensors of a second device while the first is current: launches, with the second device's stream, while it is the current one."""
+    from lorax_b200.ops import native, native_int8
+    current, launches = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Library:
+        def __getattr__(self, name):
+            at = dict(lx_norm_block=(native_int8._NORM, 24), lx_rows_int8=(native_int8._ROWS, 14), lx_gemm_int8=(native_int8._GEMM, 16))[name]
+            return lambda block: (launches.append((name, current[0], at[0].unpack(block)[at[1]])), 0)[1]
+
+    class Space:
+        status, num_sms = torch.zeros(1, dtype=torch.int32), 148
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 100 + d, raising=False)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1)
+    monkeypatch.setattr(native_int8, "_devices", {})
+    monkeypatch.setattr(native_int8.nv, "load", Library)
+    monkeypatch.setattr(native_int8.nv, "workspace", lambda d: Space())
+    x = torch.zeros(3, 32, dtype=BF)
+    native.quant_rows_int8(x)
+    native.act_mul_int8(x, inter=16)
+    native.norm_block(None, residual=x, weight=x[0], eps=1e-6)
+    native.gemm_int8(**GEMM)
+    assert launches == [(n, 1, 101) for n in ("lx_rows_int8", "lx_rows_int8", "lx_norm_block", "lx_gemm_int8")] and current == [0]
+    current[0] = 1
+    native.quant_rows_int8(x)
+    assert launches[-1] == ("lx_rows_int8", 1, 101) and current == [1]
+
+
+def test_what_a_launch_gets(monkeypatch):
+    """The packed blocks, field by field: addresses, distances (a single row's own says nothing), sizes and flags."""
+    from lorax_b200.ops import native, native_int8
+    got = {}
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda block: (got.update({name: block}), 0)[1]
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 7, raising=False)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(native_int8, "_devices", {0: (148, 5)})
+    monkeypatch.setattr(native_int8.nv, "load", Library)
+    y, res, w, pw, b, pb = (torch.zeros(*s, dtype=BF) for s in ((3, 40), (3, 24), (24,), (24,), (24,), (24,)))
+    gate, h, out = torch.zeros(3, 1, dtype=BF), torch.zeros(3, 24, dtype=BF), torch.zeros(3, 32, dtype=BF)
+    r = native.norm_block(y[:, 8:32], res, w, 1e-5, post_weight=pw, gate=gate, scale=0.5, bias=b, post_bias=pb, weight_offset=1.0, layernorm=True, residual_out=h, out=out[:, :24],
+                          int8=True)
+    f = native_int8._NORM.unpack(got["lx_norm_block"])
+    assert f[:25] == (y.data_ptr() + 16, 40, res.data_ptr(), 24, h.data_ptr(), 24, pw.data_ptr(), pb.data_ptr(), w.data_ptr(), b.data_ptr(), gate.data_ptr(), 1, 0, out.data_ptr(), 32,
+                      r.q.data_ptr(), 32, r.scale.data_ptr(), 3, 24, 1, 5, 148, -1, 7) and f[25:] == (1e-5, 1.0, 0.5)
+    x = native.norm_block(None, res[:1], w, 1e-5)
+    f = native_int8._NORM.unpack(got["lx_norm_block"])
+    assert f[:6] == (0, 0, res.data_ptr(), 32, 0, 0) and f[13:18] == (x.data_ptr(), 24, 0, 32, 0) and x.shape == (1, 24)
+    native.norm_block(y[:, 8:32], res, w, 1e-5)
+    assert native_int8._NORM.unpack(got["lx_norm_block"])[4:6] == (res.data_ptr(), 24)          # in place
+    v = native.act_mul_int8(y, 20, "relu2", out=out[:, 1:21])
+    assert native_int8._ROWS.unpack(got["lx_rows_int8"]) == (y.data_ptr(), 40, v.q.data_ptr(), 32, v.scale.data_ptr(), out.data_ptr() + 2, 32, 3, 20, 4, 1, 5, 148, -1, 7)
+    wq, ws = ref.quantize_weight_int8(torch.randn(5, 20))
+    z = native.gemm_int8(v, wq, ws, bias=b[:5], w_const=True)
+    assert z.shape == (3, 5) and z.stride() == (8, 1)
+    assert native_int8._GEMM.unpack(got["lx_gemm_int8"]) == (v.q.data_ptr(), 32, v.scale.data_ptr(), wq.data_ptr(), 32, ws.data_ptr(), b.data_ptr(), z.data_ptr(), 8, 3, 5, 20, 1, 5, 148, 0, 7)

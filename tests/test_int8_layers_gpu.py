@@ -356,9 +356,10 @@ def test_rows_and_results_in_wider_buffers(ops, T):
 
 
 def test_the_longest_sums_are_whole(ops):
-    K = 1 << 17
-    q = torch.full((2, K), -127, device="cuda", dtype=torch.int8)
-    w = torch.full((3, K), -128, device="cuda", dtype=torch.int8)
+    K = ref.INT8_MAX_K
+    q = torch.full((2, K + 1), -127, device="cuda", dtype=torch.int8)[:, :K]
+    q[1] = -128
+    w = torch.full((3, K + 1), -128, device="cuda", dtype=torch.int8)[:, :K]
     w[1] = 127
     y = ops.gemm_int8(Int8Rows(q, torch.full((2,), 2.0 ** -31, device="cuda")), w, torch.ones(3, device="cuda"))
     want = (q.double() @ w.double().t() * 2.0 ** -31).to(BF)
@@ -370,6 +371,56 @@ def test_rows_behind_the_last_one_are_left_alone(ops):
         buf = torch.full((T + 3, 256), 9.0, device="cuda", dtype=BF)
         _check_product(ops, T, 256, 256, out=buf[:T])
         assert (buf[T:] == 9).all()
+
+
+def test_offsets_past_32_bits(ops):
+    """Tensors of more than 2^31 numbers: the first and the last rows."""
+    T, K = 140000, 16384
+    x = torch.zeros(T, K, device="cuda", dtype=BF)
+    g = _gen(11)
+    ends = torch.tensor([0, 1, T // 2, T - 2, T - 1], device="cuda")
+    x[ends] = _randn(g, 5, K)
+    r = ops.quant_rows_int8(x)
+    want = ref.quant_rows_int8(x[ends].cpu())
+    assert torch.equal(r.q[ends].cpu(), want.q) and torch.equal(r.scale[ends].cpu(), want.scale) and not r.scale[2:T // 2].any()
+    w = 1 + _randn(g, K, std=0.1)
+    before = x[ends]
+    small = ops.norm_block(before.clone(), before.clone(), w, 1e-5)
+    big = ops.norm_block(x, x, w, 1e-5)             # (y and the residual are one tensor, which the sum replaces)
+    assert torch.equal(x[ends], 2 * before) and ((big[ends].double() - small.double()).abs() <= 2 * HALF * small.double().abs()).all()
+    del big, x
+    wq, ws = ref.quantize_weight_int8(_randn(g, 16384, 64, dtype=torch.float32))
+    rows = Int8Rows(r.q[:, :64], r.scale)
+    y = ops.gemm_int8(rows, wq, ws)
+    part = ops.gemm_int8(Int8Rows(r.q[ends, :64].contiguous(), r.scale[ends]), wq, ws)
+    assert torch.equal(y[ends], part)
+
+
+def test_the_same_tensor_twice(ops):
+    """y as the residual, one weight for both norms, a gate that is the weight, rows that are both operands of a product."""
+    x, w = _randn(_gen(2), 40, 256), 1 + _randn(_gen(3), 256, std=0.1)
+    h = torch.empty_like(x)
+    a = ops.norm_block(x, x, w, 1e-5, post_weight=w, gate=w, residual_out=h)
+    b = ops.norm_block(x.clone(), x.clone(), w.clone(), 1e-5, post_weight=w.clone(), gate=w.clone())
+    assert torch.equal(a, b)
+    keep = x.clone()
+    ops.norm_block(x, x, w, 1e-5, post_weight=w, gate=w)
+    assert torch.equal(x, h)
+    r = ops.quant_rows_int8(keep)
+    y = ops.gemm_int8(r, r.q, r.scale)
+    want = (r.q.double() @ r.q.double().t()) * r.scale.double()[:, None] * r.scale.double()
+    assert ((y.double() - want).abs() <= (HALF + 6 * E) * want.abs()).all()
+
+
+def test_calls_on_another_stream_than_the_default(ops):
+    y, res, w, up, down, I = _state(65, 512, 640)
+    want = _feed_forward(ops, y, res.clone(), w, up, down, I)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = [_feed_forward(ops, y, res.clone(), w, up, down, I) for _ in range(5)]
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
 
 
 # ------------------------------------------------------------------------------------------------ together
