@@ -47,11 +47,11 @@ struct RowsInt8Params {
 
 // (M of rows that begin anywhere is kRowsShifted with a shift of 0: their bytes begin at 16, and that is where groups do)
 template <int ACT, int M>
-LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, const VectorRaw& gate, const VectorRaw& up, int it, float (&f)[8]) {
-  vector_take<M>(gate, row, it, p.n, f);
+LX_DEVICE void rows_values(const RowsInt8Params& p, const VectorRaw& gate, const VectorRaw& up, int it, float (&f)[8], int in, int in_up) {
+  vector_take<M>(gate, it, p.n, f, 0, in);
   if (ACT == kRowsPlain) return;
   float u[8];
-  if (p.gated) vector_take<M>(up, row + p.n, it, p.n, u);
+  if (p.gated) vector_take<M>(up, it, p.n, u, 0, in_up);
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     f[q] = rows_act<ACT>(f[q]);
@@ -60,9 +60,9 @@ LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, co
 }
 
 template <int ACT, int M>
-LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, int it, float (&f)[8]) {
-  const VectorRaw g = vector_fetch<M>(row, it, p.n);
-  rows_values<ACT, M>(p, row, g, ACT != kRowsPlain && p.gated ? vector_fetch<M>(row + p.n, it, p.n) : g, it, f);
+LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, int it, float (&f)[8], int in = 0, int in_up = 0) {
+  const VectorRaw g = vector_fetch<M>(row, it, p.n, 0, in);
+  rows_values<ACT, M>(p, g, ACT != kRowsPlain && p.gated ? vector_fetch<M>(row + p.n, it, p.n, 0, in_up) : g, it, f, in, in_up);
 }
 
 // One block per row.  NV: groups of eight that a thread keeps in registers between the pass for the maximum and the quotients; 0: any number, read and
@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kerne
   const long long t = blockIdx.x;
   const __nv_bfloat16* row = p.x + t * p.ldx;
   float m = 0.f;
+  const int in = M == kRowsShifted ? vector_in(row, 0) : 0, in_up = M == kRowsShifted ? vector_in(row + p.n, 0) : 0;
   constexpr int KEEP = NV > 0 ? NV : 1;
   float f[KEEP][8];
   const int passes = NV > 0 ? NV : (p.n + (int)blockDim.x * 8 - 1) / ((int)blockDim.x * 8);
@@ -82,17 +83,17 @@ __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kerne
     VectorRaw g[KEEP], u[KEEP];
 #pragma unroll
     for (int it = 0; it < KEEP; ++it) {
-      g[it] = vector_fetch<M>(row, it, p.n);
-      if (ACT != kRowsPlain && p.gated) u[it] = vector_fetch<M>(row + p.n, it, p.n);
+      g[it] = vector_fetch<M>(row, it, p.n, 0, in);
+      if (ACT != kRowsPlain && p.gated) u[it] = vector_fetch<M>(row + p.n, it, p.n, 0, in_up);
     }
 #pragma unroll
     for (int it = 0; it < KEEP; ++it) {
-      rows_values<ACT, M>(p, row, g[it], u[it], it, f[it]);
+      rows_values<ACT, M>(p, g[it], u[it], it, f[it], in, in_up);
       m = largest_magnitude(m, f[it]);
     }
   } else {
     for (int it = 0; it < passes; ++it) {
-      rows_values<ACT, M>(p, row, it, f[0]);
+      rows_values<ACT, M>(p, row, it, f[0], in, in_up);
       m = largest_magnitude(m, f[0]);
     }
   }
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kerne
   if (threadIdx.x == 0) p.scale[t] = s.scale;
 #pragma unroll
   for (int it = 0; it < (NV > 0 ? NV : passes); ++it) {
-    if (NV == 0) rows_values<ACT, M>(p, row, it, f[0]);
+    if (NV == 0) rows_values<ACT, M>(p, row, it, f[0], in, in_up);
     row_store_int8<M>(p.q + t * p.ldq, it, p.n, f[NV > 0 ? it : 0], s);
     if (p.out != nullptr) {
       if (M == kRowsWide) {

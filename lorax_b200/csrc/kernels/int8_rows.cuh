@@ -82,22 +82,22 @@ LX_DEVICE void row_take(const uint4& v, int it, int n, float (&f)[8], int shift)
   }
 }
 
-// The same of a vector that begins anywhere: two 16-byte loads and a shift where both lie inside the vector.
+// The same of a vector whose first 16 bytes lie elsewhere in its groups: two 16-byte loads and a shift where both lie inside the vector, else its pieces.  `in`: values
+// of the first load in front of a group, the same for all groups.
 struct VectorRaw {
   uint4 lo, hi;
 };
+LX_DEVICE int vector_in(const __nv_bfloat16* v, int shift) { return (int)((reinterpret_cast<uintptr_t>(v - shift) & 15) >> 1); }
 template <int M>
-LX_DEVICE int vector_in(const __nv_bfloat16* v, int it, int n, int shift) {      // values of the first 16 bytes in front of the group; -1: its pieces were loaded
-  if (M != kRowsShifted) return row_whole<M>(it, n, shift) ? 0 : -1;
-  const int c = row_at<M>(it, 0, shift), in = (int)((reinterpret_cast<uintptr_t>(v + c) & 15) >> 1);
-  return c - in >= 0 && c - in + 16 <= n ? in : -1;
+LX_DEVICE bool vector_whole(int it, int n, int shift, int in) {
+  const int a = row_at<M>(it, 0, shift) - in;
+  return M != kRowsShifted ? row_whole<M>(it, n, shift) : a >= 0 && a + 16 <= n;
 }
 template <int M>
-LX_DEVICE VectorRaw vector_fetch(const __nv_bfloat16* v, int it, int n, int shift = 0) {
+LX_DEVICE VectorRaw vector_fetch(const __nv_bfloat16* v, int it, int n, int shift, int in) {
   VectorRaw r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  const int in = vector_in<M>(v, it, n, shift);
-  if (in >= 0) {
-    const uint4* a = reinterpret_cast<const uint4*>(v + (row_at<M>(it, 0, shift) - in));
+  if (vector_whole<M>(it, n, shift, in)) {
+    const uint4* a = reinterpret_cast<const uint4*>(v + (row_at<M>(it, 0, shift) - (M == kRowsShifted ? in : 0)));
     r.lo = a[0];
     if (M == kRowsShifted) r.hi = a[1];
   } else if (M != kRowsWide) {
@@ -106,10 +106,10 @@ LX_DEVICE VectorRaw vector_fetch(const __nv_bfloat16* v, int it, int n, int shif
   return r;
 }
 template <int M>
-LX_DEVICE void vector_take(const VectorRaw& r, const __nv_bfloat16* v, int it, int n, float (&f)[8], int shift = 0) {
+LX_DEVICE void vector_take(const VectorRaw& r, int it, int n, float (&f)[8], int shift, int in) {
   uint32_t w[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
   if (M == kRowsShifted) {
-    const int in = max(vector_in<M>(v, it, n, shift), 0);
+    if (!vector_whole<M>(it, n, shift, in)) in = 0;      // (pieces stand where they belong)
 #pragma unroll
     for (int i = 0; i < 6; ++i) w[i] = in & 4 ? w[i + 2] : w[i];
 #pragma unroll
@@ -120,8 +120,8 @@ LX_DEVICE void vector_take(const VectorRaw& r, const __nv_bfloat16* v, int it, i
   unpack8(make_uint4(w[0], w[1], w[2], w[3]), f);
 }
 template <int M>
-LX_DEVICE void vector_load(const __nv_bfloat16* v, int it, int n, float (&f)[8], int shift = 0) {
-  vector_take<M>(vector_fetch<M>(v, it, n, shift), v, it, n, f, shift);
+LX_DEVICE void vector_load(const __nv_bfloat16* v, int it, int n, float (&f)[8], int shift = 0, int in = 0) {
+  vector_take<M>(vector_fetch<M>(v, it, n, shift, in), it, n, f, shift, in);
 }
 
 template <int M>

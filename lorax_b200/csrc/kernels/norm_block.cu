@@ -57,15 +57,15 @@ LX_DEVICE void norm_rows(float (&f)[NV][8], int H, float eps, float (*red)[32], 
 }
 
 template <int NV, int M>
-LX_DEVICE void scale_rows(float (&f)[NV][8], int H, const VectorRaw (&raw)[NV], const __nv_bfloat16* w, const __nv_bfloat16* b, float offset, int shift) {
+LX_DEVICE void scale_rows(float (&f)[NV][8], int H, const VectorRaw (&raw)[NV], const __nv_bfloat16* b, float offset, int shift, int in) {
 #pragma unroll
   for (int it = 0; it < NV; ++it) {
     float g[8];
-    vector_take<M>(raw[it], w, it, H, g, shift);
+    vector_take<M>(raw[it], it, H, g, shift, in);
 #pragma unroll
     for (int q = 0; q < 8; ++q) f[it][q] *= g[q] + offset;
     if (b != nullptr) {
-      vector_load<M>(b, it, H, g, shift);
+      vector_load<M>(b, it, H, g, shift, in);
 #pragma unroll
       for (int q = 0; q < 8; ++q) f[it][q] += g[q];
     }
@@ -80,7 +80,7 @@ LX_DEVICE void gates(const NormBlockParams& p, long long t, int it, float (&g)[8
 #pragma unroll
     for (int q = 0; q < 8; ++q) g[q] = one;
   } else if (M != kRowsWide || p.gate_wide) {
-    vector_load<M>(gate, it, p.H, g, shift);
+    vector_load<M>(gate, it, p.H, g, shift, M == kRowsShifted ? vector_in(gate, shift) : 0);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q) g[q] = row_has<M>(it, q, p.H, shift) ? __bfloat162float(gate[row_at<M>(it, q, shift)]) : 0.f;
@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? 1
   __shared__ uint32_t red_max[32];
   const long long t = blockIdx.x;
   const int H = p.H, shift = M == kRowsShifted ? (int)((reinterpret_cast<uintptr_t>(p.residual + t * p.ldr) & 15) >> 1) : 0;
+  const int in = (8 - shift) & 7;                // (the vectors begin at 16 bytes)
   const __nv_bfloat16 *res = p.residual + t * p.ldr, *block = p.y + t * p.ldy;
   const Extent res_at = extent(p.residual, p.ldr, p.T, H), block_at = extent(p.y, p.ldy, p.T, H);
   uint4 hr[NV], yr[NV];
@@ -107,8 +108,8 @@ __global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? 1
   }
 #pragma unroll
   for (int it = 0; it < NV; ++it) {
-    if (p.post_w != nullptr) pr[it] = vector_fetch<M>(p.post_w, it, H, shift);
-    wr[it] = vector_fetch<M>(p.w, it, H, shift);
+    if (p.post_w != nullptr) pr[it] = vector_fetch<M>(p.post_w, it, H, shift, in);
+    wr[it] = vector_fetch<M>(p.w, it, H, shift, in);
   }
   float h[NV][8];
 #pragma unroll
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? 1
     for (int it = 0; it < NV; ++it) row_take<M>(yr[it], it, H, y[it], shift);
     if (p.post_w != nullptr) {
       norm_rows<LAYERNORM, NV, M>(y, H, p.eps, red, shift);
-      scale_rows<NV, M>(y, H, pr, p.post_w, p.post_b, p.w_offset, shift);
+      scale_rows<NV, M>(y, H, pr, p.post_b, p.w_offset, shift, in);
     }
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? 1
     for (int it = 0; it < NV; ++it) row_store<M>(p.residual_out + t * p.ldro, it, H, h[it], shift);
   }
   norm_rows<LAYERNORM, NV, M>(h, H, p.eps, red + 2, shift);
-  scale_rows<NV, M>(h, H, wr, p.w, p.b, p.w_offset, shift);
+  scale_rows<NV, M>(h, H, wr, p.b, p.w_offset, shift, in);
   if (p.out != nullptr) {
 #pragma unroll
     for (int it = 0; it < NV; ++it) row_store<M>(p.out + t * p.ldo, it, H, h[it], shift);
@@ -392,11 +393,12 @@ int lx_norm_block(const char* args) {
     LX_RING(false, false);
 #undef LX_RING
   }
-  // every row of every tensor as far from 16 bytes as the residual's?
+  // every row of every tensor as far from 16 bytes as the residual's, and the vectors at 16 bytes?
   bool alike = H + 7 <= kRowShifted2 * 2 * 8;
   const auto as_residual = [&](const void* v, long long ld) {
     return v == nullptr || ((reinterpret_cast<uintptr_t>(v) ^ reinterpret_cast<uintptr_t>(residual)) % 16 == 0 && (T == 1 || (ld - ldr) % 8 == 0));
   };
+  for (const void* v : {a.post_w, a.post_b, a.w, a.b}) alike = alike && reinterpret_cast<uintptr_t>(v) % 16 == 0;
   alike = alike && as_residual(y, ldy) && as_residual(residual_out, ldro) && as_residual(out, ldo) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
   const RowShape r = wide || !alike ? row_shape(0, H, num_sms, kRowThreads4) : row_shape_shifted(H + 7);
   if (layernorm) {

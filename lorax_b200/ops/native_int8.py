@@ -112,7 +112,7 @@ _NONE = (0, 0, None, 0)
 
 def _norm_block(at: int, stream: int, checked, eps: float, scale: float, weight_offset: float, layernorm: bool, out, int8: bool, ring: int = -1):
     """`ring`: 0 or 1 in place of the library's choice between a block per row and blocks that stay, to measure and test each."""
-    T, H, gate, to, spans = checked
+    T, H, gate, to, spans = checked              # (gate: its strides)
     get = spans.get
     residual = spans["residual"]
     q = q_scale = 0
@@ -131,8 +131,8 @@ def _norm_block(at: int, stream: int, checked, eps: float, scale: float, weight_
         h = _NONE if to is None else get("residual_out", residual)
         sms, status = _device(at)
         rc = nv.load().lx_norm_block(_NORM.pack(y[0], y[3], residual[0], residual[3], h[0], h[3], get("post_weight", _NONE)[0], get("post_bias", _NONE)[0],
-                                                spans["weight"][0], get("bias", _NONE)[0], get("gate", _NONE)[0], 0 if gate is None else gate.stride(0),
-                                                0 if gate is None or H == 1 else gate.stride(1), o, ldo, q, (H + 15) // 16 * 16, q_scale, T, H, bool(layernorm),
+                                                spans["weight"][0], get("bias", _NONE)[0], get("gate", _NONE)[0], gate[0],
+                                                gate[1], o, ldo, q, (H + 15) // 16 * 16, q_scale, T, H, bool(layernorm),
                                                 status, sms, ring, stream, eps, weight_offset, scale))
         nv._check(rc, "lx_norm_block")
     return r

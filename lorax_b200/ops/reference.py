@@ -1337,8 +1337,19 @@ def act_mul_int8(x, inter: int, act: str = "silu", gated: bool = True, out=None)
     return _to_int8_rows(v)
 
 
+def _gate_strides(gate, T: int, H: int):
+    """Elements between two rows' gates and two channels' (0 or 1), for a gate that broadcasts to [T, H]; None where it does not."""
+    size, step = gate.shape, gate.stride()
+    if len(size) > 2:
+        return None
+    rows, channels = (1, 1, *size)[-2:]
+    if not (rows in (1, T) and channels in (1, H)):
+        return None
+    return (0 if rows == 1 else step[-2]), (0 if channels == 1 else step[-1])
+
+
 def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8):
-    """-> (T, H, gate as [T, H] or None, what h is written to or None, {name: (address, end, tensor, elements between rows)} of what is given)."""
+    """-> (T, H, the gate's `_gate_strides`, what h is written to or None, {name: (address, end, tensor, elements between rows)} of what is given)."""
     if not (isinstance(residual, torch.Tensor) and residual.dim() == 2 and residual.is_floating_point()):
         raise ValueError("norm_block: residual [T, H] of numbers")
     if residual_out is residual:
@@ -1351,7 +1362,7 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
     for name, t in (("y", y), ("residual", residual), ("residual_out", residual_out), ("out", out)):
         if t is None:
             continue
-        if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.get_device() == at):
+        if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.get_device() == at):
             raise ValueError(f"norm_block: {name} is [T, H], of the residual's type and device")
         s0, s1 = t.stride()
         if (s1 != 1 and H > 1) or (s0 < H and T > 1):
@@ -1361,7 +1372,7 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
     for name, t in (("weight", weight), ("post_weight", post_weight), ("bias", bias), ("post_bias", post_bias)):
         if t is None and name != "weight":
             continue
-        if not (isinstance(t, torch.Tensor) and t.dim() == 1 and t.shape[0] == H and t.is_contiguous() and t.dtype == dtype and t.get_device() == at):
+        if not (isinstance(t, torch.Tensor) and t.numel() == H and t.dim() == 1 and t.is_contiguous() and t.dtype is dtype and t.get_device() == at):
             raise ValueError(f"norm_block: {name} is [H], contiguous, of the residual's type and device")
         p = t.data_ptr()
         spans[name] = (p, p + H * size, t, 0)
@@ -1373,17 +1384,19 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
         to = None
     else:
         to = residual if residual_out is None else residual_out
-    gates = None
+    strides = (0, 0)
     if gate is not None:
-        if not (isinstance(gate, torch.Tensor) and gate.dtype == dtype and gate.get_device() == at and gate.dim() <= 2):
+        if not (isinstance(gate, torch.Tensor) and gate.dtype is dtype and gate.get_device() == at):
             raise ValueError("norm_block: gate is a tensor of the residual's type and device")
-        try:
-            gates = gate.expand(T, H)
-        except RuntimeError:
-            raise ValueError(f"norm_block: a gate of {tuple(gate.shape)} for rows of {(T, H)}: one, [H], [T, 1] or [T, H]") from None
-        if H > 1 and T > 0 and gates.stride(1) not in (0, 1):
+        strides = _gate_strides(gate, T, H)
+        if strides is None:
+            raise ValueError(f"norm_block: a gate of {tuple(gate.shape)} for rows of {(T, H)}: one, [H], [T, 1] or [T, H]")
+        if strides[1] not in (0, 1) or strides[0] < 0:
             raise ValueError("norm_block: a row's gates are neighbours, or one for all")
-        spans["gate"] = (*_span(gate), gate, 0)
+        p, n = gate.data_ptr(), 1
+        for k, step in zip(gate.shape, gate.stride()):
+            n += (k - 1) * step
+        spans["gate"] = (p, p + n * size, gate, 0)
     # a row's values are read before they are written, at the same places: a result may be y or the residual itself
     written = ("residual",) if to is residual else ("residual_out",) if to is not None else ()
     for name in written if out is None else (*written, "out"):
@@ -1392,7 +1405,7 @@ def check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_b
             if lo < q and p < hi and other != name and not _turns(a, b) and not (
                     p == lo and b.shape == a.shape and b.stride() == a.stride() and other in ("y", "residual") and (other not in written)):
                 raise ValueError(f"norm_block: {name} lies on {other} (results lie apart from each other and from the inputs, or are y or the residual itself)")
-    return T, H, gates, to, spans
+    return T, H, strides, to, spans
 
 
 def norm_block(y, residual, weight, eps, post_weight=None, gate=None, scale: float = 1.0, bias=None, post_bias=None, weight_offset: float = 0.0,
@@ -1401,7 +1414,7 @@ def norm_block(y, residual, weight, eps, post_weight=None, gate=None, scale: flo
     was written.  N is the RMS norm, or the layer norm, times (weight + weight_offset), plus the bias; N_post is left out without a `post_weight`, h is the residual
     without y.  `gate` is one value, [H], [T, 1] or [T, H].  Returns N(h) in the residual's type (in `out` where given), or with `int8` as `Int8Rows` made from the
     32-bit values, and then writes `out` too where it is given."""
-    T, H, gate, to, _ = check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
+    _, _, _, to, _ = check_norm_block(y, residual, weight, post_weight, gate, scale, bias, post_bias, residual_out, out, int8)
 
     def norm(v, w, b):
         if layernorm:

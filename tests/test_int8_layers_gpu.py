@@ -250,6 +250,25 @@ def test_rows_of_any_width_in_tensors_without_gaps(ops, H, layernorm, int8):
     assert ((out[:, 2:H + 2].double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
 
 
+@pytest.mark.parametrize("H", [5, 64, 1001, 2048])
+@pytest.mark.parametrize("at", [1, 4, 8])
+def test_vectors_that_begin_anywhere(ops, H, at):
+    """Weights, biases and gates inside a larger buffer."""
+    g = _gen(H, at)
+    buf = 1 + _randn(g, 5 * (H + 16), std=0.2)
+    w, pw, b, pb, gate = (buf[i * (H + 16) + at:i * (H + 16) + at + H] for i in range(5))
+    y, res = _randn(g, 33, H), _randn(g, 33, H)
+    for layernorm in (False, True):
+        for vectors in ((w, pw, b, pb, gate), (w.clone(), pw, b, pb.clone(), gate.clone()), (w.clone(), pw.clone(), b.clone(), pb.clone(), gate)):
+            h = torch.empty_like(res)
+            x = ops.norm_block(y, res, vectors[0], 1e-5, post_weight=vectors[1], gate=vectors[4], bias=vectors[2], post_bias=vectors[3], layernorm=layernorm, residual_out=h)
+            part, slack = _norm64(y.double(), pw, pb, 1e-5, 0.0, layernorm)
+            want = res.double() + gate.double() * part
+            assert ((h.double() - want).abs() <= HALF * want.abs() + gate.double().abs() * (slack + 4 * E * part.abs()) + 2 * E * want.abs()).all()
+            want, slack = _norm64(h.double(), w, b, 1e-5, 0.0, layernorm)
+            assert ((x.double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
+
+
 @pytest.mark.parametrize("at", [1, 8])
 def test_norms_of_rows_that_begin_inside_a_buffer(ops, at):
     _check_norm(ops, 200, 256, True, "channel", 1.0, True, True, at=at)
