@@ -24,7 +24,7 @@ LX_DEVICE float times_sigmoid(float x, float z) {
 template <int ACT>
 LX_DEVICE float rows_act(float x) {
   if (ACT == kRowsSilu) return times_sigmoid(x, x);
-  if (ACT == kRowsGelu) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+  if (ACT == kRowsGelu) return 0.5f * x * erfcf(-0.70710678118654752f * x);      // (1 + erf loses the digits of rows whose gates are all shut)
   if (ACT == kRowsGeluTanh) return times_sigmoid(x, 1.5957691216057308f * (x + 0.044715f * x * x * x));      // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
   if (ACT == kRowsRelu || ACT == kRowsRelu2) {
     const float r = x <= 0.f ? 0.f : x;      // (a NaN stays one)

@@ -123,6 +123,26 @@ def test_activations(ops, act, T, I, gated):
     assert torch.equal(ops.act_mul_int8(x, I, act, gated).q, r.q)
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("n", [8, 100])
+def test_rows_whose_gates_are_all_shut_keep_their_digits(ops, act, n):
+    """The largest value of such a row is tiny, and its scale goes by it: what counts is a value's own relative error."""
+    x = (-4 - 8 * torch.rand(60, n, generator=_gen(n), device="cuda")).to(BF)
+    z = x.double()
+    if act == "gelu":
+        v = 0.5 * z * torch.special.erfc(-z * 0.5 ** 0.5)
+        steps = (z * z).amax(1) + 16           # an argument's rounding moves erfc by 2 z^2 = x^2 of its own; erfc's last places, two products
+    else:
+        u = z if act == "silu" else 2 * (2 / torch.pi) ** 0.5 * (z + 0.044715 * z ** 3)
+        v = z * torch.sigmoid(u)
+        steps = 8 * u.abs().amax(1) + 16       # the exponent's roundings (five in the polynomial, two in front of exp2) move the exponential by as much
+    r = ops.act_mul_int8(x, n, act, gated=False)
+    top = v.abs().amax(1)
+    assert ((r.scale.double() - top / 127).abs() <= top / 127 * (steps + 2) * E).all()
+    off = (r.q.double() * r.scale.double()[:, None] - v).abs()
+    assert (off <= r.scale.double()[:, None] * (0.5 + 2.0 ** -20) + (top * steps * E)[:, None]).all()
+
+
 @pytest.mark.parametrize("T,n", [(1, 8), (5, 64), (700, 256), (1300, 1000), (601, 4096), (300, 8192), (301, 14336), (200, 16384)])
 @pytest.mark.parametrize("act,gated", [(None, False), ("silu", True), ("relu2", False)])
 def test_both_forms_of_quantisers(ops, T, n, act, gated):
