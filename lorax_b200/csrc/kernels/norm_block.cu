@@ -87,7 +87,8 @@ LX_DEVICE void gates(const NormBlockParams& p, long long t, int it, float (&g)[8
   }
 }
 
-// One block per row; NV groups of eight a thread, all in registers.
+// One block per row; NV groups of eight a thread, all in registers, with the loads of rows and weights ahead of the first sum.  The chain of loads, sums over the block and
+// stores is the bound: one row of 4096 2.1 us, in 8 bits 2.4; 259 rows 4.1.  Shifted rows are bound by instructions: 1500 of 2049 12 us, as layer norms with gate and biases 19.
 template <bool LAYERNORM, int NV, int M>
 __global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? 1024 : kRowShifted2) norm_block_kernel(const NormBlockParams p) {
   pdl_wait();
@@ -168,7 +169,8 @@ __global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? 1
 
 // ------------------------------------------------------------------------------------------------
 // Many rows: blocks that stay, with the next row of y and of the residual on its way by bulk copies (no registers, no waiting warps) while one is normed.
-// Rows are read from shared memory as often as a pass needs them, so that a thread holds the values of one row only, and the norms' weights for all rows.
+// Rows are read from shared memory as often as a pass needs them, so that a thread holds the values of one row only, and the norms' weights for all rows.  4001 rows of
+// 8192: 43.5 us (6.0 TB/s: HBM), a block per row 70; in 8 bits 55 (issue slots), as layer norms 65 (four sums over the block).
 // ------------------------------------------------------------------------------------------------
 constexpr int kNormStages = 2;
 // Values of the stream an SM has to norm from which they are worth it (us, a block per row and blocks that stay): 200 rows of 4096 3.9 and 4.3, 444 6.7 and 6.3, 4001 32 and 26;
