@@ -16,7 +16,7 @@ namespace lx {
 
 constexpr int kI8BM = 128;                        // output features of a tile
 constexpr int kI8BK = 128;                        // bytes of K in a stage: one row of the 128-byte swizzle
-constexpr int kI8Threads = 128;
+constexpr int kI8Threads = 256;                   // 128 for tiles of 16 tokens, whose results are few: a row of 28672 x 4096 20.1 us, with 256 20.7
 constexpr int kI8MaxStages = 16;
 constexpr int kI8MaxParts = 8;                    // CTAs that share a tile's K: a portable cluster
 constexpr int kI8ABytes = kI8BM * kI8BK;
@@ -125,11 +125,11 @@ LX_DEVICE void int8_join(const Int8GemmParams& p, const int* sums, const Int8Sca
   }
 }
 
-// One tile a cluster, one part of its K a CTA.  Warp 0 loads, warp 1 multiplies, all four write results.  Short steps: the weights' way from HBM is the bound, and
+// One tile a cluster, one part of its K a CTA.  Warp 0 loads, warp 1 multiplies, all (four or eight) write results.  Short steps: the weights' way from HBM is the bound, and
 // two CTAs an SM with six stages of 16 KB each keep enough of them on their way whatever the number of tiles (a persistent CTA an SM would leave the last wave
 // short): one row of 28672 x 4096 20.0 us (5.9 TB/s), 48 rows 21.6.  Narrow layers have fewer tiles than SMs: one row of 4096 x 14336 by eight CTAs a tile 12.1 us, alone 34.5.
 // Middle steps take large tiles, whose operands come from L2 at 100 bytes a nanosecond and SM: 256 rows of 4096 x 14336 20.9 us by four CTAs a tile of 256 tokens.
-__global__ void __launch_bounds__(kI8Threads)
+__global__ void __launch_bounds__(kI8Threads, 3)
 gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -223,7 +223,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     }
     __syncwarp();
   } else {
-    int8_scales(p, scales, ta * kI8BM, tb * p.bn, (int)threadIdx.x - 64, 64);
+    int8_scales(p, scales, ta * kI8BM, tb * p.bn, (int)threadIdx.x - 64, (int)blockDim.x - 64);
   }
 
   // (done: every load of this CTA has arrived and been read, so the ring is free)
@@ -235,9 +235,10 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   const int t0 = tb * p.bn, live = min(p.bn, p.T - t0);
   if (ok) {
     tc_fence_after();
-    const uint32_t taddr = tmem_d + ((uint32_t)(warp * 32) << 16);
-    int* mine = sums + warp * 32 + lane;
-    for (int c = 0; c < live; c += 16) {
+    const int quad = warp & 3;                               // (the lanes that a warp may read; two warps take turns at their columns)
+    const uint32_t taddr = tmem_d + ((uint32_t)(quad * 32) << 16);
+    int* mine = sums + quad * 32 + lane;
+    for (int c = (warp >> 2) * 16; c < live; c += (int)blockDim.x / 8) {
       uint32_t r[16];
       tmem_ld_32x32b_x16(taddr + c, r);
       tc_wait_ld();
@@ -250,8 +251,8 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   else __syncthreads();
   if (__syncthreads_or(*abort_flag) == 0) {
     if (p.parts == 1) int8_join<1, 4>(p, sums, scales, 0, 0, 0, ta * kI8BM, t0, live);
-    else if (p.parts <= 4) int8_join<4, 4>(p, sums, scales, part, 0, 1, ta * kI8BM, t0, live);
-    else int8_join<kI8MaxParts, 2>(p, sums, scales, part, 0, 1, ta * kI8BM, t0, live);
+    else if (p.parts <= 4) int8_join<4, 2>(p, sums, scales, part, 0, 1, ta * kI8BM, t0, live);
+    else int8_join<kI8MaxParts, 1>(p, sums, scales, part, 0, 1, ta * kI8BM, t0, live);
   }
   if (*abort_flag && threadIdx.x == 0)  // copies still on their way arrive before this CTA leaves
     for (int s = 0; s < min(p.stages, loaded); ++s) mbar_wait(&full_bar[s], (uint32_t)((loaded - 1 - s) / p.stages) & 1u, nullptr);
@@ -269,10 +270,11 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 // product 292), the tensor pipe 77 % active at the 1.64 GHz that the power limit leaves, its stages waiting for 32 KB each at 80 bytes a nanosecond.
 // ------------------------------------------------------------------------------------------------
 constexpr int kI8PairStages = 6;
-constexpr int kI8PairThreads = 192;
+constexpr int kI8PairEpiWarps = 8;                // two for each quarter of the features, half of the tokens each
+constexpr int kI8PairThreads = 64 + 32 * kI8PairEpiWarps;
 constexpr int kI8PairStageBytes = 2 * kI8ABytes;
 constexpr int kI8PairMaxParts = 4;
-constexpr int kI8TurnBytes = 4 * 16 * 32 * 4;     // a warp's 32 features x 32 tokens in bf16, two tokens a word
+constexpr int kI8TurnBytes = kI8PairEpiWarps * 16 * 32 * 4;      // a warp's 32 features x 32 tokens in bf16, two tokens a word
 constexpr int kI8PairSmem = kI8PairStages * kI8PairStageBytes + kI8TurnBytes + (int)sizeof(Int8Scales) + 256 + 1024;
 static_assert(kI8PairSmem <= 227 * 1024 && 256 * kI8BM * 4 <= kI8PairStages * kI8PairStageBytes, "the ring holds a tile's sums");
 
@@ -311,7 +313,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kI8PairStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&tmem_full[s], 1); mbar_init(&tmem_empty[s], 8); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&tmem_full[s], 1); mbar_init(&tmem_empty[s], 2 * kI8PairEpiWarps); }
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_w);
@@ -400,22 +402,22 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     }
     __syncwarp();
   } else {
-    const int quad = warp & 3;
-    uint32_t* turn = turn_all + quad * (16 * 32);
+    const int quad = warp & 3, late = (warp - 2) >> 2;      // (late: the warp that takes every other 32 tokens from the second on)
+    uint32_t* turn = turn_all + (warp - 2) * (16 * 32);
     int* sums = reinterpret_cast<int*>(smem);          // [token][128 features], of a shared tile: over the ring, which has been read by then
     int acc = 0;
     uint32_t acc_phase[2] = {0, 0};
     for (int tile = first; tile < num_tiles; tile += step) {
       const int j0 = tile % tiles_b * p.bn, jend = min(p.T, j0 + p.bn);
       const int f0 = (2 * (tile / tiles_b) + rank) * kI8BM + quad * 32, fi = min(f0 + lane, p.N - 1);
-      float ws = 0.f, bias = 0.f, xl[8];                // (fetched while the tile's products are formed; xl[i]: the scale of token 32 i + lane)
+      float ws = 0.f, bias = 0.f, xl[4];                // (fetched while the tile's products are formed; xl[i]: the scale of token 32 (2 i + late) + lane)
       if (p.parts > 1) {
-        int8_scales(p, scales, f0 - quad * 32, j0, (int)threadIdx.x - 64, 128);
+        int8_scales(p, scales, f0 - quad * 32, j0, (int)threadIdx.x - 64, kI8PairThreads - 64);
       } else {
         ws = p.ws[fi];
         if (p.bias != nullptr) bias = __bfloat162float(p.bias[fi]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) xl[i] = p.xs[min(j0 + 32 * i + lane, p.T - 1)];
+        for (int i = 0; i < 4; ++i) xl[i] = p.xs[min(j0 + 32 * (2 * i + late) + lane, p.T - 1)];
       }
       if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_phase[acc], abort_flag))) {
         report_status(p.status, kTimeoutTmemFull, tile);
@@ -426,8 +428,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       acc_phase[acc] ^= 1;
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * 256);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = 32 * i;
+      for (int i = 0; i < 4; ++i) {
+        const int c = 32 * (2 * i + late);
         if (c >= p.bn || j0 + c >= jend) break;
         uint32_t r[32];
         tmem_ld_32x32b_x32(taddr + c, r);
@@ -495,7 +497,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   if (p.parts > 1) {
     const int j0 = first % tiles_b * p.bn;
     if (__syncthreads_or(*abort_flag) == 0)
-      int8_join<kI8PairMaxParts, 4>(p, reinterpret_cast<const int*>(smem), scales, part, (uint32_t)rank, 2, (2 * (first / tiles_b) + rank) * kI8BM, j0, min(p.bn, p.T - j0));
+      int8_join<kI8PairMaxParts, 2>(p, reinterpret_cast<const int*>(smem), scales, part, (uint32_t)rank, 2, (2 * (first / tiles_b) + rank) * kI8BM, j0, min(p.bn, p.T - j0));
     __syncwarp();
     cluster_sync();
   }
@@ -746,7 +748,7 @@ int lx_gemm_int8(const char* args) {
     if (e != cudaSuccess) return -(int)e;
     set[dev] = true;
   }
-  launch_pdl_cluster(gemm_int8_kernel, dim3((unsigned)ctas), dim3(kI8Threads), dim3((unsigned)w.parts), (size_t)w.smem, stream, tw, tx, p);
+  launch_pdl_cluster(gemm_int8_kernel, dim3((unsigned)ctas), dim3(w.bn <= 16 ? kI8Threads / 2 : kI8Threads), dim3((unsigned)w.parts), (size_t)w.smem, stream, tw, tx, p);
   return -(int)cudaGetLastError();
 }
 
