@@ -558,10 +558,10 @@ static Int8Plan int8_single_plan(int T, int N, int K, int bn, int parts, int num
   return w;
 }
 
-// What a plan costs, in ns.  A CTA's time is that of its operands' way in from L2 (100 bytes a nanosecond, 84 where all SMs work in pairs; a second CTA on an SM
-// adds a quarter) and of its tokens' results; waves of CTAs add a start, parts a join; and the weights come from HBM meanwhile, and all operands through L2: the fourth powers of both
+// What a plan costs, in ns.  A CTA's time is that of its operands' way in from L2 (112 bytes a nanosecond, 83 where all SMs work in pairs; a second CTA on an SM
+// adds three eighths) and of its tokens' results; waves of CTAs add a start, parts a join; and the weights come from HBM meanwhile, and all operands through L2: the fourth powers of both
 // times add up, so that the smaller one counts where they are near.  The constants are fitted to 7000 plans of 209 shapes (1 to 3900 rows, 144 to 28672 features,
-// K 159 to 14336): the plan of least cost is 3 % slower than the quickest one on average, at worst 23 % (7.5 us where 6.1 are possible).
+// K 159 to 14336): the plan of least cost is 2 % slower than the quickest one on average, over 10 % in five shapes, at worst 30 % (7.7 us where 5.9 are possible).
 static double int8_beside(double t, double hbm) {
   const double a = t * t, b = hbm * hbm;
   return sqrt(sqrt(a * a + b * b));
@@ -576,17 +576,17 @@ static double int8_single_cost(int T, int N, int K, const Int8Plan& w, int num_s
   const long long waves = (ctas + slots - 1) / slots;
   long long together = (ctas + num_sms - 1) / num_sms;
   if (together > fit) together = fit;
-  const double fill = blocks * (double)(kI8ABytes + kI8BK * w.bn) * (1 + 0.27 * (double)(together - 1)) / 100.8;
-  const double t = 1510.0 + (double)waves * (fill + 1358.0 + 20.4 * live * (double)together) + (w.parts > 1 ? 846.0 + 2.5 * live : 0.0);
-  const double hbm = ((double)N * K + (double)T * K) / 4810.0, l2 = (double)ctas * blocks * (kI8ABytes + kI8BK * w.bn) / 16500.0;
-  return int8_beside(t, 2868.0 + (hbm > l2 ? hbm : l2));
+  const double fill = blocks * (double)(kI8ABytes + kI8BK * w.bn) * (1 + 0.38 * (double)(together - 1)) / 111.7;
+  const double t = 1230.0 + (double)waves * (fill + 1639.0 + 15.7 * live * (double)together) + (w.parts > 1 ? 685.0 + 2.5 * live : 0.0);
+  const double hbm = ((double)N * K + (double)T * K) / 4853.0, l2 = (double)ctas * blocks * (kI8ABytes + kI8BK * w.bn) / 18590.0;
+  return int8_beside(t, 2869.0 + (hbm > l2 ? hbm : l2));
 }
 static double int8_pair_cost(int T, int N, int K, int bn, int parts, int clusters) {
   const int blocks = int8_up(int8_up(K, kI8BK), parts), live = bn < T ? bn : T;
   const long long tiles = (long long)int8_up(N, 2 * kI8BM) * int8_up(T, bn), waves = (tiles + clusters - 1) / clusters;
-  const double in = (kI8ABytes + kI8BK / 2 * bn) / 84.1, mma = 1.48 * bn;
-  const double t = 2022.0 + (double)waves * (blocks * (in > mma ? in : mma) + 1329.0) + 21.95 * live + (parts > 1 ? 374.0 + 1.6 * live : 0.0);
-  return int8_beside(t, 3351.0 + ((double)N * K + (double)T * K) / 4810.0);
+  const double in = (kI8ABytes + kI8BK / 2 * bn) / 83.0, mma = 1.29 * bn;
+  const double t = 2007.0 + (double)waves * (blocks * (in > mma ? in : mma) + 1008.0) + 20.1 * live + (parts > 1 ? 633.0 + 0.8 * live : 0.0);
+  return int8_beside(t, 3015.0 + ((double)N * K + (double)T * K) / 4853.0);
 }
 
 // clusters[parts]: clusters of `parts` pairs that run at the same time.
@@ -619,15 +619,13 @@ static Int8Plan int8_plan(int T, int N, int K, int num_sms, const int* clusters)
   return best;
 }
 
-// Clusters of `parts` pairs that run at the same time on the current device (none of a size that no part of the device holds), or a query's negative error,
-// which the next call makes again.
-static int int8_clusters(int parts) {
+// Clusters of `parts` pairs that run at the same time on `dev`, the current device (none of a size that no part of it holds), or a query's negative error, which the
+// next call makes again.
+static int int8_clusters(int parts, int dev) {
   static int known[64][kI8PairMaxParts + 1] = {{0}};
-  int dev = 0, n = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev < 0 || dev >= 64)) return 0;
-  if (e == cudaSuccess && known[dev][parts] != 0) return known[dev][parts] - 1;
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(gemm_int8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8PairSmem);
+  int n = 0;
+  if (known[dev][parts] != 0) return known[dev][parts] - 1;
+  cudaError_t e = cudaFuncSetAttribute(gemm_int8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8PairSmem);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2u * (unsigned)parts);
@@ -665,7 +663,11 @@ int lx_gemm_int8_plan(int T, int N, int K, int num_sms, const int* clusters, int
   return 0;
 }
 
-int lx_gemm_int8_clusters(int parts) { return parts < 1 || parts > lx::kI8PairMaxParts ? -1 : lx::int8_clusters(parts); }
+int lx_gemm_int8_clusters(int parts) {
+  int dev = 0;
+  if (parts < 1 || parts > lx::kI8PairMaxParts || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  return lx::int8_clusters(parts, dev);
+}
 
 // Arguments in one block of 8-byte fields: a call by ctypes pays for each argument of its own (17 of them 2.4 us, a packed block 0.6).
 struct LxGemmInt8Args {
@@ -695,9 +697,10 @@ int lx_gemm_int8(const char* args) {
   if (a.K <= 0 || a.K > lx_gemm_int8_max_k() || a.ldq % 16 != 0 || a.ldw % 16 != 0 || a.T > 0x7fffffff || a.N > 0x7fffffff) return -1000;
   const int T = (int)a.T, N = (int)a.N, K = (int)a.K, num_sms = (int)a.num_sms;
   const long long force = a.force;
-  int clusters[kI8PairMaxParts + 1] = {0};
+  int dev = 0, clusters[kI8PairMaxParts + 1] = {0};
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   for (int parts = 1; parts <= kI8PairMaxParts; ++parts) {
-    const int n = int8_clusters(parts);
+    const int n = int8_clusters(parts, dev);
     if (n < 0) return n;
     clusters[parts] = pairs_on(num_sms / parts, n);
   }
@@ -712,8 +715,6 @@ int lx_gemm_int8(const char* args) {
     // a plan takes some microseconds to choose and goes by sizes alone: the last ones of a thread are kept
     struct Known { int T, N, K, sms, dev; Int8Plan w; };
     static thread_local Known known[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return -3;
     Known& k = known[((unsigned)T * 31u + (unsigned)N * 7u + (unsigned)K) % 64u];
     if (k.T != T || k.N != N || k.K != K || k.sms != num_sms || k.dev != dev) k = Known{T, N, K, num_sms, dev, int8_plan(T, N, K, num_sms, clusters)};
     w = k.w;
@@ -741,8 +742,6 @@ int lx_gemm_int8(const char* args) {
     return -(int)cudaGetLastError();
   }
   static bool set[64] = {false};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   if (!set[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(gemm_int8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024);
     if (e != cudaSuccess) return -(int)e;
