@@ -127,8 +127,8 @@ LX_DEVICE void int8_join(const Int8GemmParams& p, const int* sums, const Int8Sca
 
 // One tile a cluster, one part of its K a CTA.  Warp 0 loads, warp 1 multiplies, all (four or eight) write results.  Short steps: the weights' way from HBM is the bound, and
 // two CTAs an SM with six stages of 16 KB each keep enough of them on their way whatever the number of tiles (a persistent CTA an SM would leave the last wave
-// short): one row of 28672 x 4096 20.0 us (5.9 TB/s), 48 rows 21.6.  Narrow layers have fewer tiles than SMs: one row of 4096 x 14336 by eight CTAs a tile 12.1 us, alone 34.5.
-// Middle steps take large tiles, whose operands come from L2 at 100 bytes a nanosecond and SM: 256 rows of 4096 x 14336 20.9 us by four CTAs a tile of 256 tokens.
+// short): one row of 28672 x 4096 20.2 us (5.8 TB/s), 48 rows 21.3.  Narrow layers have fewer tiles than SMs: one row of 4096 x 14336 by eight CTAs a tile 12.1 us, alone 34.5.
+// Middle steps take large tiles, whose operands come from L2 at 100 bytes a nanosecond and SM: 256 rows of 4096 x 14336 20.2 us by four CTAs a tile of 256 tokens.
 __global__ void __launch_bounds__(kI8Threads, 3)
 gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8GemmParams p) {
   extern __shared__ uint8_t smem_raw[];

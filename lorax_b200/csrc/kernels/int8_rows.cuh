@@ -249,10 +249,10 @@ inline RowShape row_shape(int rows, int n, int num_sms, int most) {
   }
   return RowShape{1024, 0};
 }
-// For kRowsShifted, whose groups take more registers: one a thread, or two in blocks of up to 768.
-constexpr int kRowShifted2 = 768;
+// For kRowsShifted, whose groups take more registers: one a thread in blocks of up to 576 (56 registers, so that four blocks of 288 share an SM), or two in blocks of up to 768.
+constexpr int kRowShifted1 = 576, kRowShifted2 = 768;
 inline RowShape row_shape_shifted(int n) {
-  const int need = (n + 7) / 8, g = need <= 1024 ? 1 : 2;
+  const int need = (n + 7) / 8, g = need <= kRowShifted1 ? 1 : 2;
   return RowShape{((need + g - 1) / g + 31) / 32 * 32, g};
 }
 

@@ -88,9 +88,9 @@ LX_DEVICE void gates(const NormBlockParams& p, long long t, int it, float (&g)[8
 }
 
 // One block per row; NV groups of eight a thread, all in registers, with the loads of rows and weights ahead of the first sum.  The chain of loads, sums over the block and
-// stores is the bound: one row of 4096 2.1 us, in 8 bits 2.4; 259 rows 4.1.  Shifted rows are bound by instructions: 1500 of 2049 12 us, as layer norms with gate and biases 19.
+// stores is the bound: one row of 4096 2.1 us, in 8 bits 2.4; 259 rows 4.1.  Shifted rows are bound by instructions: 1500 of 2049 12 us, as layer norms with gate and biases 18.
 template <bool LAYERNORM, int NV, int M>
-__global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? 1024 : kRowShifted2) norm_block_kernel(const NormBlockParams p) {
+__global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? kRowShifted1 : kRowShifted2, M == kRowsShifted && NV == 1 ? 2 : 1) norm_block_kernel(const NormBlockParams p) {
   pdl_wait();
   pdl_trigger();
   __shared__ float red[4][32];
