@@ -368,3 +368,33 @@ def test_what_a_launch_gets(monkeypatch):
     z = native.gemm_int8(v, wq, ws, bias=b[:5], w_const=True)
     assert z.shape == (3, 5) and z.stride() == (8, 1)
     assert native_int8._GEMM.unpack(got["lx_gemm_int8"]) == (v.q.data_ptr(), 32, v.scale.data_ptr(), wq.data_ptr(), 32, ws.data_ptr(), b.data_ptr(), z.data_ptr(), 8, 3, 5, 20, 1, 5, 148, 0, 7)
+
+
+def test_a_checkpoint_is_served_in_8_bit_integers(tmp_path):
+    """`--quantize w8a8` of the shard: the dense checkpoint's projections are quantised on load, and a prompt runs through them."""
+    import json
+
+    from safetensors.torch import save_file
+    from tokenizers import Tokenizer, models, pre_tokenizers
+
+    from lorax_b200.config import EngineConfig, tiny_llama
+    from lorax_b200.models.decoder import DecoderModel, Int8Weight
+    from lorax_b200.models.loading import export_hf_state_dict
+    from lorax_b200.server.runtime import build_runtime
+    cfg = tiny_llama()
+    dense = DecoderModel.random_init(cfg, "cpu", torch.float32, seed=1)
+    save_file(export_hf_state_dict(dense), str(tmp_path / "model.safetensors"))
+    (tmp_path / "config.json").write_text(json.dumps({
+        "model_type": "llama", "vocab_size": cfg.vocab_size, "hidden_size": cfg.hidden_size, "intermediate_size": cfg.intermediate_size,
+        "num_hidden_layers": cfg.num_hidden_layers, "num_attention_heads": cfg.num_attention_heads, "num_key_value_heads": cfg.num_key_value_heads,
+        "rms_norm_eps": cfg.rms_norm_eps, "rope_theta": cfg.rope_theta, "max_position_embeddings": 2048, "torch_dtype": "float32"}))
+    tok = Tokenizer(models.WordLevel({f"w{i}": i for i in range(cfg.vocab_size)}, unk_token="w0"))
+    tok.pre_tokenizer = pre_tokenizers.Whitespace()
+    tok.save(str(tmp_path / "tokenizer.json"))
+    (tmp_path / "tokenizer_config.json").write_text(json.dumps({"tokenizer_class": "PreTrainedTokenizerFast", "unk_token": "w0", "eos_token": "w2"}))
+    rt = build_runtime(str(tmp_path), EngineConfig(max_input_length=40, max_total_tokens=64), device="cpu", source="local", quantize="w8a8", num_blocks=32, max_batch=4)
+    model = rt.runner.model if hasattr(rt, "runner") else rt.model
+    assert model.quantized == "w8a8" and isinstance(model.layers[-1].down_w, Int8Weight)
+    want = DecoderModel.random_init(cfg, "cpu", torch.float32, seed=1)
+    want.quantize("w8a8")
+    assert torch.equal(model.layers[0].qkv_w.q, want.layers[0].qkv_w.q) and torch.equal(_step(model), _step(want))
