@@ -862,7 +862,8 @@ _TIMED_OPS = ("gemm", "gemm_fp8", "norm_residual", "rope_kvwrite", "act_mul", "e
               "attn_prefill", "lora_shrink", "lora_expand", "lora_shrink_tiles", "lora_expand_tiles",
               "embed_stream", "norm_stream", "norm_gate", "tanh_", "gemm_heads", "linear_attn", "wkv", "token_shift", "latent_prep", "rope_pairs",
               "latent_attn", "latent_prefill", "norm_add", "qk_norm_kvwrite", "conv_rope_kvwrite", "causal_conv", "ssd",
-              "gate_norm", "gqa_attn", "moe_route", "moe_grouped_gemm", "moe_combine", "step_tables", "moe_few", "token_scores")
+              "gate_norm", "gqa_attn", "moe_route", "moe_grouped_gemm", "moe_combine", "step_tables", "moe_few", "token_scores",
+              "norm_block", "quant_rows_int8", "act_mul_int8", "gemm_int8")
 _timing_records = None
 _timing_originals = {}
 
