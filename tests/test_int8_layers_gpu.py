@@ -245,13 +245,37 @@ def test_both_forms_of_norms(ops, gate, T, H, layernorm):
         _check_norm(ops, T, H, gate != "one", gate, 0.5, layernorm, "both" if gate in ("token", "all") else gate == "none", ring=ring, bias=layernorm)
 
 
-def test_a_norm_without_a_block_in_front_by_both_forms(ops):
-    g = _gen(9)
-    res, w = _randn(g, 700, 512), _randn(g, 512)
-    a, b = (_norm_by(ring, None, res, w, 1e-5) for ring in (0, 1))
-    want, slack = _norm64(res.double(), w, None, 1e-5, 0.0, False)
-    for x in (a, b, ops.norm_block(None, res, w, 1e-5)):
+@pytest.mark.parametrize("T,H", [(1, 512), (700, 512), (33, 511), (1500, 4096)])
+@pytest.mark.parametrize("layernorm", [False, True])
+def test_a_norm_without_a_block_in_front_by_both_forms(ops, T, H, layernorm):
+    g = _gen(9, T, H)
+    res, w, b = _randn(g, T, H), _randn(g, H), _randn(g, H)
+    keep = res.clone()
+    want, slack = _norm64(res.double(), w, b, 1e-5, 0.0, layernorm)
+    for x in (*(_norm_by(ring, None, res, w, 1e-5, bias=b, layernorm=layernorm) for ring in (0, 1)), ops.norm_block(None, res, w, 1e-5, bias=b, layernorm=layernorm)):
         assert ((x.double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
+    out = torch.empty_like(res)
+    r = ops.norm_block(None, res, w, 1e-5, bias=b, layernorm=layernorm, int8=True, out=out)
+    assert torch.equal(out, x) and torch.equal(res, keep)
+    off = (r.q.double() * r.scale.double()[:, None] - want).abs()
+    assert (off <= r.scale.double()[:, None] * (0.5 + 2.0 ** -18) + 2 * slack.amax(1, keepdim=True)).all()
+    assert ops.norm_block(None, res, w, 1e-5, bias=b, layernorm=layernorm, out=res) is res and torch.equal(res, out)      # over the residual itself
+
+
+@pytest.mark.parametrize("T,H", [(2, 100), (700, 2048), (50, 333)])
+def test_results_over_the_inputs(ops, T, H):
+    """Every place that a result may take: over y, over the residual, each over the other's."""
+    g = _gen(4, T, H)
+    y, res, w = _randn(g, T, H), _randn(g, T, H), 1 + _randn(g, H, std=0.1)
+    h, x = torch.empty_like(res), torch.empty_like(res)
+    ops.norm_block(y, res, w, 1e-5, post_weight=w, residual_out=h, out=x)
+    for to, out in (("y", "residual"), ("residual", "y"), ("y", None), (None, "y"), ("residual", None), (None, "residual")):
+        at = dict(y=y.clone(), residual=res.clone())
+        if to != "residual" and out == "residual" and to is None:
+            at["h"] = torch.empty_like(res)
+            to = "h"
+        got = ops.norm_block(at["y"], at["residual"], w, 1e-5, post_weight=w, residual_out=at.get(to), out=at.get(out))
+        assert torch.equal(got, x) and torch.equal(at[to or "residual"], h) and (out is None or got is at[out])
 
 
 @pytest.mark.parametrize("H", [1, 2, 6, 7, 9, 15, 17, 257, 1001, 2049, 4095, 8190, 16377])
@@ -580,6 +604,34 @@ def test_a_model_in_8_bit_integers_matches_the_plain_operators(ops, adapters):
     # bf16 activations and weights (rounded before they are quantised) against 32 bits: what the same model in bf16 weights is allowed (0.03), and the steps of a
     # 127th that fall to the other side on the way, as far off as the rounding to 8 bits itself
     assert (outs[0] - outs[1]).norm() / outs[1].norm() < 0.06
+
+
+@pytest.mark.parametrize("kind", ["gemma2", "granite", "gpt_neox", "cohere", "mixtral"])
+def test_models_of_other_shapes_match_the_plain_operators(ops, kind):
+    """Norms on both sides, a residual multiplier, parallel blocks with two norms or one, experts that stay in bf16."""
+    from lorax_b200.config import ModelConfig
+    from lorax_b200.runtime.kv_cache import KVCache
+    from lorax_b200.runtime.runner import ModelRunner, PrefillItem
+    more = dict(gemma2=dict(norm_weight_offset=1.0, tie_word_embeddings=True, hidden_act="gelu_pytorch_tanh"), granite=dict(residual_multiplier=0.22),
+                gpt_neox=dict(parallel_residual=True, norm_type="layernorm", hidden_act="gelu"), cohere=dict(parallel_residual=True, norm_type="layernorm_nobias"),
+                mixtral=dict(num_local_experts=4, num_experts_per_tok=2))[kind]
+    c = ModelConfig(model_type=kind, hidden_size=256, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, intermediate_size=512, vocab_size=256, head_dim=64,
+                    max_position_embeddings=256, **more)
+    prompts = [torch.randint(0, 256, (n,), generator=torch.Generator().manual_seed(n)).tolist() for n in (5, 70)]
+    outs = []
+    for device, dtype in (("cuda", BF), ("cpu", torch.float32)):
+        m = _model(device, dtype, c)[1] if kind != "mixtral" else _model_of(c, device, dtype)
+        kv = KVCache(c.num_hidden_layers, 16, m.nkv, m.d, m.dtype, m.device)
+        r = ModelRunner(m, kv, max_batch=4, max_seq_tokens=128, max_prefill_tokens=256, use_graphs=False)
+        outs.append(r.prefill([PrefillItem(p, 0, [1 + 3 * i, 2 + 3 * i, 3 + 3 * i], adapter_index=0) for i, p in enumerate(prompts)])[2].float().cpu())
+    assert (outs[0] - outs[1]).norm() / outs[1].norm() < 0.06      # (as for the model above)
+
+
+def _model_of(c, device, dtype):
+    from lorax_b200.models.decoder import DecoderModel
+    m = DecoderModel.random_init(c, device, dtype, seed=0, std=0.05)
+    m.quantize("w8a8")
+    return m
 
 
 def test_generation_with_graphs_is_that_without(ops):
