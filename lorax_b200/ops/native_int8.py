@@ -68,12 +68,13 @@ def _on(t: torch.Tensor, call, *args):
         return call(at, torch._C._cuda_getCurrentRawStream(at), *args)
 
 
-def _rows(at: int, stream: int, x: torch.Tensor, T: int, n: int, act: int, gated: bool, out: Optional[torch.Tensor], ring: int = -1) -> Int8Rows:
+def _rows(at: int, stream: int, x: torch.Tensor, ldx: int, T: int, n: int, act: int, gated: bool, out: Optional[torch.Tensor], ring: int = -1) -> Int8Rows:
     """`ring` as for `_norm_block`."""
     r = empty_int8_rows(T, n, x)
     if T:
         sms, status = _device(at)
-        rc = nv.load().lx_rows_int8(_ROWS.pack(x.data_ptr(), x.stride(0), r.q.data_ptr(), (n + 15) // 16 * 16, r.scale.data_ptr(), 0 if out is None else out.data_ptr(),
+        q, scale = r
+        rc = nv.load().lx_rows_int8(_ROWS.pack(x.data_ptr(), ldx, q.data_ptr(), (n + 15) // 16 * 16, scale.data_ptr(), 0 if out is None else out.data_ptr(),
                                                0 if out is None else out.stride(0), T, n, act, gated, status, sms, ring, stream))
         nv._check(rc, "lx_rows_int8")
     return r
@@ -81,19 +82,19 @@ def _rows(at: int, stream: int, x: torch.Tensor, T: int, n: int, act: int, gated
 
 def quant_rows_int8(x: torch.Tensor) -> Int8Rows:
     """Rows x [T, K] in 8-bit integers, with a scale for each row (`reference.quant_rows_int8` states the numbers)."""
-    T, K = check_quant_rows_int8(x)
+    T, K, ldx = check_quant_rows_int8(x)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"quant_rows_int8: the kernels are bf16; got {x.dtype}")
-    return _on(x, _rows, x, T, K, -1, False, None)
+    return _on(x, _rows, x, ldx, T, K, -1, False, None)
 
 
 def act_mul_int8(x: torch.Tensor, inter: int, act: str = "silu", gated: bool = True, out: Optional[torch.Tensor] = None) -> Int8Rows:
     """act(gate) * up of rows [gate | up], or act(gate), in 8-bit integers with a scale for each row; `out` takes the values in bf16 too
     (`reference.act_mul_int8`)."""
-    T = check_act_mul_int8(x, inter, act, gated, out)
+    T, ldx = check_act_mul_int8(x, inter, act, gated, out)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"act_mul_int8: the kernels are bf16; got {x.dtype}")
-    return _on(x, _rows, x, T, inter, nv._ACTS[act], bool(gated), out)
+    return _on(x, _rows, x, ldx, T, inter, nv._ACTS[act], bool(gated), out)
 
 
 def norm_block(y: Optional[torch.Tensor], residual: torch.Tensor, weight: torch.Tensor, eps: float, post_weight: Optional[torch.Tensor] = None,

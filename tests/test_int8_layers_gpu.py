@@ -151,7 +151,7 @@ def test_both_forms_of_quantisers(ops, T, n, act, gated):
     x[T // 2] = 0
     x[T // 3, 5] = float("nan")
     outs = [torch.full((T, n), 7.0, device="cuda", dtype=BF) for _ in range(2)]
-    a, b = (native_int8._on(x, native_int8._rows, x, T, n, native._ACTS[act] if act else -1, gated, o, ring) for ring, o in enumerate(outs))
+    a, b = (native_int8._on(x, native_int8._rows, x, x.stride(0), T, n, native._ACTS[act] if act else -1, gated, o, ring) for ring, o in enumerate(outs))
     assert torch.equal(a.q, b.q) and torch.equal(a.scale.view(torch.int32), b.scale.view(torch.int32)) and torch.equal(outs[0].view(torch.int16), outs[1].view(torch.int16))
     if act is None:
         want = ref.quant_rows_int8(x.cpu())
