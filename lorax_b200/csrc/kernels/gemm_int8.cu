@@ -20,6 +20,7 @@ constexpr int kI8Threads = 256;                   // 128 for tiles of 16 tokens,
 constexpr int kI8MaxStages = 16;
 constexpr int kI8MaxParts = 8;                    // CTAs that share a tile's K: a portable cluster
 constexpr int kI8ABytes = kI8BM * kI8BK;
+constexpr int kI8Most = 0x7fff0000;               // rows, features: with a tile more they stay below 2^31
 
 struct Int8GemmParams {
   int N, T, K;
@@ -656,7 +657,7 @@ int lx_gemm_int8_max_k() { return (1 << 17) - 1; }
 // out[2] CTAs or pairs that share a tile's K, out[3] stages of a single CTA's ring.
 int lx_gemm_int8_plan(int T, int N, int K, int num_sms, const int* clusters, int* out) {
   using namespace lx;
-  if (T <= 0 || N <= 0 || K <= 0 || K > lx_gemm_int8_max_k()) return -1000;
+  if (T <= 0 || N <= 0 || K <= 0 || K > lx_gemm_int8_max_k() || T > kI8Most || N > kI8Most) return -1000;
   const int fit[kI8PairMaxParts + 1] = {0, clusters[0], clusters[1], clusters[2], clusters[3]};
   const Int8Plan w = int8_plan(T, N, K, num_sms, fit);
   out[0] = w.pairs; out[1] = w.bn; out[2] = w.parts; out[3] = w.stages;
@@ -694,7 +695,7 @@ int lx_gemm_int8(const char* args) {
   LxGemmInt8Args a;
   memcpy(&a, args, sizeof(a));
   if (a.T <= 0 || a.N <= 0) return 0;
-  if (a.K <= 0 || a.K > lx_gemm_int8_max_k() || a.ldq % 16 != 0 || a.ldw % 16 != 0 || a.T > 0x7fffffff || a.N > 0x7fffffff) return -1000;
+  if (a.K <= 0 || a.K > lx_gemm_int8_max_k() || a.ldq % 16 != 0 || a.ldw % 16 != 0 || a.T > kI8Most || a.N > kI8Most) return -1000;
   const int T = (int)a.T, N = (int)a.N, K = (int)a.K, num_sms = (int)a.num_sms;
   const long long force = a.force;
   int dev = 0, clusters[kI8PairMaxParts + 1] = {0};

@@ -125,13 +125,13 @@ __global__ void __launch_bounds__(kRowThreads4, 2) rows_int8_ring_kernel(const R
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t full[kRowStages];
   __shared__ uint32_t red[2][32];
-  __shared__ int abort_word;
+  __shared__ int abort_word, fetched;
   volatile int* abort_flag = &abort_word;
   const int step = (int)gridDim.x;
   const uint32_t stage_bytes = (uint32_t)p.n * (p.gated ? 4 : 2);
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
-    abort_word = 0;
+    abort_word = fetched = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
   }
@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kRowThreads4, 2) rows_int8_ring_kernel(const R
   pdl_wait();
   pdl_trigger();
   const auto fetch = [&](int t, int s) {
+    ++fetched;
     mbar_expect_tx(&full[s], stage_bytes);
     bulk_load_1d(ring + s * stage_bytes, p.x + t * p.ldx, stage_bytes, &full[s]);
   };
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(kRowThreads4, 2) rows_int8_ring_kernel(const R
     const RowScale sc = row_scale(block_max(m, red[i & 1]));
     if (threadIdx.x == 0) {
       p.scale[t] = sc.scale;
-      if (row + p.stages * step < p.T) fetch(row + p.stages * step, s);
+      if (row + p.stages * step < p.T && !*abort_flag) fetch(row + p.stages * step, s);
     }
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
@@ -170,6 +171,8 @@ __global__ void __launch_bounds__(kRowThreads4, 2) rows_int8_ring_kernel(const R
     }
     if (++s == p.stages) { s = 0; phase ^= 1; }
   }
+  if (threadIdx.x == 0 && *abort_flag)      // copies still on their way arrive before the block leaves
+    for (int j = max(0, fetched - p.stages); j < fetched; ++j) mbar_wait(&full[j % p.stages], (uint32_t)(j / p.stages) & 1u, nullptr);
 }
 
 // Two blocks an SM by their registers; as many stages as fit then, up to three.
@@ -231,7 +234,7 @@ int lx_rows_int8(const char* args) {
   LxRowsInt8Args a;
   memcpy(&a, args, sizeof(a));
   if (a.T <= 0) return 0;
-  if (a.n <= 0 || a.n > (1 << 30) || a.T > 0x7fffffff) return -1;
+  if (a.n <= 0 || a.n > (1 << 30) || a.T > kRowsMost) return -1;
   const void *x = a.x, *q = a.q, *out = a.out;
   const long long ldx = a.ldx, ldq = a.ldq, ldo = a.ldo;
   const int n = (int)a.n, num_sms = (int)a.num_sms, ring = (int)a.ring;

@@ -236,6 +236,7 @@ LX_DEVICE void row_store_int8(int8_t* row, int it, int n, const float (&f)[8], c
 
 // Threads of a block and groups of eight that each holds, for rows of n values.  Few rows: as many threads as there are groups (`most`), since the row's own
 // chain of loads, sums and stores is what takes time.  Many: 256 threads and more groups, whose loads are in flight together.
+constexpr int kRowsMost = 0x7fff0000;  // of a call: a row's number and the rows ahead of it stay below 2^31
 constexpr int kRowThreads4 = 512;      // of a block whose threads hold four groups
 struct RowShape {
   int threads, groups;                 // groups: 1, 2, 4; 0: the row is longer than a block's registers hold

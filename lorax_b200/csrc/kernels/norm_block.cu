@@ -183,13 +183,13 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
   __shared__ uint64_t full[kNormStages];
   __shared__ float red[2][4][32];
   __shared__ uint32_t red_max[2][32];
-  __shared__ int abort_word;
+  __shared__ int abort_word, fetched;
   volatile int* abort_flag = &abort_word;
   const int H = p.H, nvec = H / 8, step = (int)gridDim.x;
   const uint32_t row_bytes = (uint32_t)H * 2, stage_bytes = row_bytes * (p.y != nullptr ? 2 : 1);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kNormStages; ++s) mbar_init(&full[s], 1);
-    abort_word = 0;
+    abort_word = fetched = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
   }
@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
   pdl_wait();
   pdl_trigger();
   const auto fetch = [&](int t, int s) {
+    ++fetched;
     mbar_expect_tx(&full[s], stage_bytes);
     bulk_load_1d(ring + s * stage_bytes, p.residual + t * p.ldr, row_bytes, &full[s]);
     if (p.y != nullptr) bulk_load_1d(ring + s * stage_bytes + row_bytes, p.y + t * p.ldy, row_bytes, &full[s]);
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
     }
     norm_rows<LAYERNORM, NV, kRowsWide>(h, H, p.eps, sums + 2);
     // (a barrier has passed since the row was read last: its stage takes the one after the next)
-    if (threadIdx.x == 0 && row + kNormStages * step < p.T) fetch(row + kNormStages * step, s);
+    if (threadIdx.x == 0 && row + kNormStages * step < p.T && !*abort_flag) fetch(row + kNormStages * step, s);
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
       float g[8];
@@ -307,6 +308,8 @@ __global__ void __launch_bounds__(kRowThreads4, NV == 4 ? 1 : 2) norm_block_ring
       for (int it = 0; it < NV; ++it) row_store_int8<kRowsWide>(p.q + t * p.ldq, it, H, h[it], sc);
     }
   }
+  if (threadIdx.x == 0 && *abort_flag)      // copies still on their way arrive before the block leaves
+    for (int j = max(0, fetched - kNormStages); j < fetched; ++j) mbar_wait(&full[j % kNormStages], (uint32_t)(j / kNormStages) & 1u, nullptr);
 }
 
 // Blocks that an SM holds at a time go by their registers (64 a thread, 128 with four groups) and their stages.
@@ -374,7 +377,7 @@ int lx_norm_block(const char* args) {
   LxNormBlockArgs a;
   memcpy(&a, args, sizeof(a));
   if (a.T <= 0) return 0;
-  if (a.H <= 0 || a.H > lx_norm_block_max_width() || a.T > 0x7fffffff || (a.y != nullptr && a.residual_out == nullptr)) return -1;
+  if (a.H <= 0 || a.H > lx_norm_block_max_width() || a.T > kRowsMost || (a.y != nullptr && a.residual_out == nullptr)) return -1;
   const void *y = a.y, *residual = a.residual, *residual_out = a.residual_out, *out = a.out, *q = a.q, *gate = a.gate;
   const long long ldy = a.ldy, ldr = a.ldr, ldro = a.ldro, ldo = a.ldo, ldq = a.ldq, gate_t = a.gate_t;
   const int T = (int)a.T, H = (int)a.H, num_sms = (int)a.num_sms, ring = (int)a.ring, layernorm = (int)a.layernorm;

@@ -206,6 +206,19 @@ def test_limits_of_the_library_and_of_python_agree(monkeypatch):
         monkeypatch.undo()
 
 
+@pytest.mark.parametrize("rows", [(1 << 31) - 1, (1 << 31) - (1 << 16) + 1, 1 << 31, 1 << 40])
+def test_the_library_refuses_rows_whose_numbers_pass_31_bits(rows):
+    """Tiles and rows in flight behind the last one are counted in 32 bits.  (The library says no in front of its first use of a device or of an address.)"""
+    from lorax_b200.ops import native, native_int8
+    lib = native.load()
+    assert lib.lx_norm_block(native_int8._NORM.pack(*([0] * 18), rows, 8, 0, 0, 148, 1, 0, 1e-6, 0.0, 1.0)) < 0
+    assert lib.lx_rows_int8(native_int8._ROWS.pack(*([0] * 7), rows, 8, -1, 0, 0, 148, 1, 0)) < 0
+    for T, N in ((rows, 1), (1, rows)):
+        assert lib.lx_gemm_int8(native_int8._GEMM.pack(0, 16, 0, 0, 16, 0, 0, 0, 8, T, N, 16, 0, 0, 148, 0, 0)) < 0
+        if rows < 1 << 31:
+            assert lib.lx_gemm_int8_plan(T, N, 16, 148, (native_int8.I * 4)(74, 33, 22, 15), (native_int8.I * 4)()) < 0
+
+
 def _plan(T, N, K, sms=148, clusters=(74, 33, 22, 15)):
     import ctypes
 
