@@ -106,7 +106,7 @@ LX_DEVICE VectorRaw vector_fetch(const __nv_bfloat16* v, int it, int n, int shif
   return r;
 }
 template <int M>
-LX_DEVICE void vector_take(const VectorRaw& r, int it, int n, float (&f)[8], int shift, int in) {
+LX_DEVICE uint4 vector_shift(const VectorRaw& r, int it, int n, int shift, int in) {
   uint32_t w[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
   if (M == kRowsShifted) {
     if (!vector_whole<M>(it, n, shift, in)) in = 0;      // (pieces stand where they belong)
@@ -117,7 +117,11 @@ LX_DEVICE void vector_take(const VectorRaw& r, int it, int n, float (&f)[8], int
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (in & 1) * 16);
   }
-  unpack8(make_uint4(w[0], w[1], w[2], w[3]), f);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int M>
+LX_DEVICE void vector_take(const VectorRaw& r, int it, int n, float (&f)[8], int shift, int in) {
+  unpack8(vector_shift<M>(r, it, n, shift, in), f);
 }
 template <int M>
 LX_DEVICE void vector_load(const __nv_bfloat16* v, int it, int n, float (&f)[8], int shift = 0, int in = 0) {

@@ -88,7 +88,7 @@ LX_DEVICE void gates(const NormBlockParams& p, long long t, int it, float (&g)[8
 }
 
 // One block per row; NV groups of eight a thread, all in registers, with the loads of rows and weights ahead of the first sum.  The chain of loads, sums over the block and
-// stores is the bound: one row of 4096 2.1 us, in 8 bits 2.4; 259 rows 4.1.  Shifted rows are bound by instructions: 1500 of 2049 12 us, as layer norms with gate and biases 18.
+// stores is the bound: one row of 4096 2.1 us, in 8 bits 2.4; 259 rows 4.1.  Shifted rows are bound by instructions: 600 of 2049 6.4 us, as layer norms with gate and biases 9.6.
 template <bool LAYERNORM, int NV, int M>
 __global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? kRowShifted1 : kRowShifted2, M == kRowsShifted && NV == 1 ? 2 : 1) norm_block_kernel(const NormBlockParams p) {
   pdl_wait();
@@ -334,6 +334,113 @@ static int launch_norm_ring(const NormBlockParams& p, int num_sms, cudaStream_t 
   return -(int)cudaGetLastError();
 }
 
+// Many shifted rows: blocks that stay, each on rows a multiple of eight apart, which all begin at the same distance from 16 bytes.  The norms' vectors are brought into
+// that place once, to be read from shared memory, and the next row's values are on their way while one is normed.  Bound by instructions and by the chain of a layer norm's sums: 1500
+// layer norms of 2049 with gate and biases 16.1 us, 6000 of 4097 88 (a block per row 18.2 and 123); RMS norms on both sides, 6000 of 4097, 67 (77).
+constexpr int kNormVectors = 5;      // post_w, post_b, w, b, a channel's gate
+template <bool LAYERNORM>
+__global__ void __launch_bounds__(kRowShifted1, 2) norm_block_shifted_kernel(const NormBlockParams p) {
+  constexpr int M = kRowsShifted;
+  extern __shared__ uint4 vectors[];
+  __shared__ float red[2][4][32];
+  __shared__ uint32_t red_max[2][32];
+  pdl_wait();
+  pdl_trigger();
+  const int H = p.H, shift = (int)((reinterpret_cast<uintptr_t>(p.residual + blockIdx.x * p.ldr) & 15) >> 1);
+  uint4* mine = vectors + threadIdx.x;               // (nobody else reads a thread's part)
+  const auto keep = [&](const __nv_bfloat16* v, int k) {
+    if (v == nullptr) return;
+    const int in = vector_in(v, shift);
+    mine[k * (int)blockDim.x] = vector_shift<M>(vector_fetch<M>(v, 0, H, shift, in), 0, H, shift, in);
+  };
+  const bool channels = p.gate != nullptr && p.gate_h != 0 && p.gate_t == 0;
+  keep(p.post_w, 0);
+  keep(p.post_b, 1);
+  keep(p.w, 2);
+  keep(p.b, 3);
+  if (channels) keep(p.gate, 4);
+  const auto scale_by = [&](float (&f)[1][8], int k, const __nv_bfloat16* b) {
+    float g[8];
+    unpack8(mine[k * (int)blockDim.x], g);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[0][q] *= g[q] + p.w_offset;
+    if (b == nullptr) return;
+    unpack8(mine[(k + 1) * (int)blockDim.x], g);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[0][q] += g[q];
+  };
+  const Extent res_at = extent(p.residual, p.ldr, p.T, H), block_at = extent(p.y, p.ldy, p.T, H);
+  uint4 hr = make_uint4(0, 0, 0, 0), yr = hr;          // of the next row
+  const auto fetch = [&](long long t) {
+    hr = row_fetch<M>(p.residual + t * p.ldr, 0, H, shift, res_at);
+    if (p.y != nullptr) yr = row_fetch<M>(p.y + t * p.ldy, 0, H, shift, block_at);
+  };
+  if ((int)blockIdx.x < p.T) fetch(blockIdx.x);
+  int i = 0;
+  for (int row = (int)blockIdx.x; row < p.T; row += (int)gridDim.x, i ^= 1) {
+    const long long t = row;
+    float h[1][8];
+    if (p.y != nullptr) {
+      float r[8];
+      row_take<M>(yr, 0, H, h[0], shift);
+      if (p.post_w != nullptr) {
+        norm_rows<LAYERNORM, 1, M>(h, H, p.eps, red[i], shift);
+        scale_by(h, 0, p.post_b);
+      }
+      if (p.gate != nullptr) {
+        float g[8];
+        if (channels) unpack8(mine[4 * (int)blockDim.x], g);
+        else gates<M>(p, t, 0, g, shift);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) h[0][q] *= g[q];
+      }
+      row_take<M>(hr, 0, H, r, shift);
+#pragma unroll
+      for (int q = 0; q < 8; q += 2) {
+        const float2 u = unpack_bf16x2(pack_bf16x2(fmaf(p.scale, h[0][q], r[q]), fmaf(p.scale, h[0][q + 1], r[q + 1])));
+        h[0][q] = u.x;
+        h[0][q + 1] = u.y;
+      }
+      row_store<M>(p.residual_out + t * p.ldro, 0, H, h[0], shift);
+    } else {
+      row_take<M>(hr, 0, H, h[0], shift);
+    }
+    if (row + (int)gridDim.x < p.T) fetch(row + (int)gridDim.x);
+    norm_rows<LAYERNORM, 1, M>(h, H, p.eps, red[i] + 2, shift);
+    scale_by(h, 2, p.b);
+    if (p.out != nullptr) row_store<M>(p.out + t * p.ldo, 0, H, h[0], shift);
+    if (p.q != nullptr) {
+      if (!row_whole<M>(0, H, shift)) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (!row_has<M>(0, q, H, shift)) h[0][q] = 0.f;      // (0 times a row's infinite or NaN factors)
+      }
+      const RowScale s = row_scale(block_max(largest_magnitude(0.f, h[0]), red_max[i]));
+      if (threadIdx.x == 0) p.q_scale[t] = s.scale;
+      row_store_int8<M>(p.q + t * p.ldq, 0, H, h[0], s, shift);
+    }
+  }
+}
+
+// Blocks that run at the same time, by their registers (56 a thread): a multiple of eight.
+static int norm_shifted_grid(const RowShape& r, int num_sms) {
+  const int fit = 65536 / (r.threads * 56), grid = num_sms * (fit < 32 ? fit : 32) / 8 * 8;
+  return grid < 8 ? 8 : grid;
+}
+// Where each has two rows or more and they are wide, or the norms have several vectors (us, a block per row and blocks that stay).  RMS norms, one vector: 6000 of 1021 19.1 and
+// 20.5, of 2049 31.3 and 28.9, 1500 of 4097 17.8 and 15.7.  Layer norms on both sides, a gate: 1500 of 1021 (one or two rows each) 11.5 and 12.8, 6000 36.8 and 30.9.
+static bool norm_shifted_stays(const NormBlockParams& p, const RowShape& r, int num_sms) {
+  const int kept = 1 + (p.post_w != nullptr) + (p.post_b != nullptr) + (p.b != nullptr) + (p.gate != nullptr && p.gate_h != 0 && p.gate_t == 0);
+  return p.T >= 2ll * norm_shifted_grid(r, num_sms) && (p.H > 2000 || kept >= 3);
+}
+template <bool LAYERNORM>
+static int launch_norm_shifted(const NormBlockParams& p, const RowShape& r, int num_sms, cudaStream_t s) {
+  int grid = norm_shifted_grid(r, num_sms);
+  if (grid > p.T) grid = (p.T + 7) / 8 * 8;      // (of the last eight blocks some have no row)
+  launch_pdl(norm_block_shifted_kernel<LAYERNORM>, dim3((unsigned)grid), dim3((unsigned)r.threads), (size_t)kNormVectors * r.threads * 16, s, p);
+  return -(int)cudaGetLastError();
+}
+
 template <bool LAYERNORM, int M>
 static void launch_norm_block(const NormBlockParams& p, int T, const RowShape& r, cudaStream_t s) {
   const dim3 grid((unsigned)T), block((unsigned)r.threads);
@@ -366,7 +473,7 @@ struct LxNormBlockArgs {
   long long T, H, layernorm;
   int* status;
   long long num_sms;
-  long long ring;             // -1: the library's choice; 0 or 1 (where rows begin at 16 bytes): a block per row or blocks that stay, to measure each
+  long long ring;             // -1: the library's choice; 0 or 1 (where such a kernel takes the rows): a block per row or blocks that stay, to measure each
   void* stream;
   double eps, w_offset, scale;
 };
@@ -406,6 +513,8 @@ int lx_norm_block(const char* args) {
   for (const void* v : {a.post_w, a.post_b, a.w, a.b}) alike = alike && reinterpret_cast<uintptr_t>(v) % 16 == 0;
   alike = alike && as_residual(y, ldy) && as_residual(residual_out, ldro) && as_residual(out, ldo) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
   const RowShape r = wide || !alike ? row_shape(0, H, num_sms, kRowThreads4) : row_shape_shifted(H + 7);
+  if (!wide && alike && r.groups == 1 && (ring < 0 ? norm_shifted_stays(p, r, num_sms) : ring))
+    return layernorm ? launch_norm_shifted<true>(p, r, num_sms, s) : launch_norm_shifted<false>(p, r, num_sms, s);
   if (layernorm) {
     if (wide) launch_norm_block<true, kRowsWide>(p, T, r, s);
     else if (alike) launch_norm_block<true, kRowsShifted>(p, T, r, s);

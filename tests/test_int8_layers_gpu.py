@@ -294,6 +294,31 @@ def test_rows_of_any_width_in_tensors_without_gaps(ops, H, layernorm, int8):
     assert ((out[:, 2:H + 2].double() - want).abs() <= HALF * want.abs() + slack * (1 + HALF)).all()
 
 
+@pytest.mark.parametrize("T,H", [(1, 3), (7, 9), (8, 1), (9, 255), (23, 65), (1500, 65), (700, 1021), (600, 2050), (1300, 2049), (310, 4097), (20, 4601)])
+@pytest.mark.parametrize("layernorm,gate,int8", [(False, "none", False), (False, "token", True), (True, "channel", "both"), (True, "all", False)])
+def test_rows_of_any_width_by_blocks_that_stay(ops, T, H, layernorm, gate, int8):
+    """Blocks on rows of one distance from 16 bytes; fewer rows than blocks, more, and the library's own choice."""
+    for ring in (1, -1):
+        _check_norm(ops, T, H, gate != "all", gate, 0.5, layernorm, int8, bias=layernorm, ring=ring)
+
+
+@pytest.mark.parametrize("H", [15, 2049])
+def test_blocks_that_stay_on_rows_that_are_not_finite(ops, H):
+    """... keep what is not a number in its row, the neighbours' first and last bytes among what a row loads."""
+    g, T = _gen(H), 1600
+    y, res, w = _randn(g, T, H), _randn(g, T, H), 1 + _randn(g, H, std=0.1)
+    at = torch.arange(3, T, 7, device="cuda")
+    y[at[0::4], H - 1], y[at[1::4], 0], res[at[2::4], 0], res[at[3::4], H - 1] = float("nan"), float("inf"), float("-inf"), float("nan")
+    h = torch.empty_like(res)
+    r = _norm_by(1, y, res, w, 1e-5, post_weight=w, residual_out=h, int8=True)
+    bad = torch.zeros(T, dtype=torch.bool, device="cuda")
+    bad[at] = True
+    assert torch.equal(r.scale.isnan(), bad) and (r.q[bad] == 0).all()
+    y, res = y.where(~bad[:, None], 0), res.where(~bad[:, None], 0)
+    good = _norm_by(1, y, res, w, 1e-5, post_weight=w, residual_out=h.clone(), int8=True)
+    assert torch.equal(r.q[~bad], good.q[~bad]) and torch.equal(r.scale[~bad], good.scale[~bad])
+
+
 @pytest.mark.parametrize("H", [5, 64, 1001, 2048])
 @pytest.mark.parametrize("at", [1, 4, 8])
 def test_vectors_that_begin_anywhere(ops, H, at):
