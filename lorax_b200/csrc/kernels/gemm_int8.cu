@@ -540,7 +540,7 @@ static int make_tmap_i8(CUtensorMap* out, const void* base, uint64_t rows, uint6
 struct Int8Plan {
   int pairs, bn, stages, parts, tmem_cols, smem;      // pairs: of CTAs that stay, 0: single ones
 };
-static int int8_up(int a, int b) { return (a + b - 1) / b; }
+static int int8_up(int a, int b) { return (a - 1) / b + 1; }      // of a >= 1, where a + b may pass 31 bits
 
 // By single CTAs: where there are more of them than SMs, or clusters, which leave SMs empty, the ring of small tiles takes half of an SM's shared memory, so
 // that two share an SM; else all of it.
