@@ -620,6 +620,9 @@ static Int8Plan int8_plan(int T, int N, int K, int num_sms, const int* clusters)
   return best;
 }
 
+// Tiles of a product; the kernels count them in 32 bits, with a grid's more.
+static long long int8_tiles(int T, int N, const Int8Plan& w) { return (long long)int8_up(N, w.pairs ? 2 * kI8BM : kI8BM) * int8_up(T, w.bn); }
+
 // Clusters of `parts` pairs that run at the same time on `dev`, the current device (none of a size that no part of it holds), or a query's negative error, which the
 // next call makes again.
 static int int8_clusters(int parts, int dev) {
@@ -660,6 +663,7 @@ int lx_gemm_int8_plan(int T, int N, int K, int num_sms, const int* clusters, int
   if (T <= 0 || N <= 0 || K <= 0 || K > lx_gemm_int8_max_k() || T > kI8Most || N > kI8Most) return -1000;
   const int fit[kI8PairMaxParts + 1] = {0, clusters[0], clusters[1], clusters[2], clusters[3]};
   const Int8Plan w = int8_plan(T, N, K, num_sms, fit);
+  if (int8_tiles(T, N, w) > kI8Most) return -1001;
   out[0] = w.pairs; out[1] = w.bn; out[2] = w.parts; out[3] = w.stages;
   return 0;
 }
@@ -720,9 +724,9 @@ int lx_gemm_int8(const char* args) {
     if (k.T != T || k.N != N || k.K != K || k.sms != num_sms || k.dev != dev) k = Known{T, N, K, num_sms, dev, int8_plan(T, N, K, num_sms, clusters)};
     w = k.w;
   }
-  const long long tiles = (long long)((N + (w.pairs ? 2 : 1) * kI8BM - 1) / ((w.pairs ? 2 : 1) * kI8BM)) * ((T + w.bn - 1) / w.bn);
+  const long long tiles = int8_tiles(T, N, w);
   const long long ctas = !w.pairs ? tiles * w.parts : 2 * (w.parts > 1 ? tiles * w.parts : tiles < w.pairs ? tiles : w.pairs);
-  if (ctas > 0x7fffffffll) return -1001;
+  if (tiles > kI8Most || ctas > 0x7fffffffll) return -1001;
   Int8GemmParams p{};
   p.N = N; p.T = T; p.K = K;
   p.bn = w.bn; p.stages = w.stages; p.parts = w.parts; p.tmem_cols = w.tmem_cols;

@@ -20,3 +20,10 @@ def test_plans_of_rows_and_channels_near_the_most_that_are_taken(T, N, K, cluste
     rc, (pairs, bn, parts, stages) = _plan(T, N, K, clusters=clusters)
     assert rc == 0 and 16 <= bn <= 256 and bn % (32 if pairs else 16) == 0 and 1 <= parts <= -(-K // 128)
     assert pairs >= 0 and (pairs > 0 or 4 <= stages <= 16)
+
+
+def test_tiles_whose_number_passes_31_bits_are_refused():
+    """The kernels count a product's tiles in 32 bits."""
+    for T, N in ((MOST, MOST), (1 << 30, 1 << 28)):
+        assert _plan(T, N, 16)[0] == -1001
+    assert _plan(1 << 20, 1 << 20, 16)[0] == 0                   # 2^16 tiles of 16 rows by 2^13 of channels at most
