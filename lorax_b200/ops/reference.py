@@ -1233,7 +1233,8 @@ def empty_int8_rows(T: int, K: int, like) -> Int8Rows:
 
 
 def _to_int8_rows(v) -> Int8Rows:
-    """scale = max |v| / 127 in 32 bits, q = v / scale to the nearest integer (ties to the even one).  A row whose largest magnitude is not finite has a NaN for
+    """scale = max |v| / 127 in 32 bits, q = v / scale to the nearest integer (ties to the even one), 127 at most (a scale of few units of the least number may be too
+    small by up to half of one).  A row whose largest magnitude is not finite has a NaN for
     its scale; where the scale is zero, as for a row of zeros, and where it is a NaN, q is zero."""
     top = v.abs().amax(1) if v.shape[1] else v.new_zeros(v.shape[0])
     scale = torch.where(top.isfinite(), top / torch.full_like(top, 127.0), torch.full_like(top, float("nan")))      # (a division, not a product)

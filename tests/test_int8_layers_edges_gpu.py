@@ -1,0 +1,63 @@
+"""Operators of layers in 8-bit integers on the GPU: rows at the ends of the numbers' range, and what other rows, forms and plans may change."""
+import pytest
+import torch
+
+from lorax_b200.ops import native, native_int8  # noqa: F401  (the bindings of every operator first)
+from lorax_b200.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from lorax_b200.ops import native
+    native.load()
+    yield native
+    native.workspace().check_status()
+
+
+# A scale of few units of 2^-149 is off from max / 127 by up to half a unit, so that quotients pass 127: of 190 units, whose scale is one, 190.
+TOPS = [1, 63, 64, 100, 127, 128, 129, 150, 190, 191, 255, 256, 300, 400, 513, 1000, 2039, 4000, 5000, 8000, 12345, 16002, 20000, 40000]
+
+
+@pytest.mark.parametrize("I", [8, 100, 1001, 4096, 17000])
+@pytest.mark.parametrize("copies", [1, 30])
+@pytest.mark.parametrize("ring", [0, 1])
+def test_rows_of_few_units_of_the_least_number(ops, I, copies, ring):
+    """Products of two small halves, whole units of 2^-149, by a block per row and by blocks that stay: the bits of the plain form, whose quotients end at 127."""
+    g = torch.Generator().manual_seed(I)
+    tops = torch.tensor(TOPS * copies, dtype=torch.float64)
+    # a unit is 2^-70 of the gate times 2^-79 of the other half; both hold 8 bits, so a row's largest is the nearest such product
+    a = (tops.sqrt().floor()).clamp(1, 255)
+    b = (tops / a).round().clamp(1, 255)
+    up = torch.randint(-255, 256, (len(tops), I), generator=g).double()
+    up = torch.minimum(torch.maximum(up, -b[:, None]), b[:, None])
+    at = torch.arange(len(tops)) % I
+    sign = torch.where(torch.arange(len(tops)) % 2 == 0, 1.0, -1.0).double()
+    up[torch.arange(len(tops)), at] = b * sign
+    x = torch.cat([(a[:, None] * 2.0 ** -70).expand(-1, I), up * 2.0 ** -79], 1).to(BF)
+    want = ref.act_mul_int8(x, I, "relu")
+    x = x.cuda()
+    got = native_int8._on(x, native_int8._rows, x, x.stride(0), len(tops), I, 3, True, None, ring)
+    assert torch.equal(got.scale.cpu(), want.scale) and torch.equal(got.q.cpu(), want.q)
+    pub = ops.act_mul_int8(x, I, "relu")
+    assert torch.equal(pub.q, got.q) and torch.equal(pub.scale, got.scale)
+
+
+@pytest.mark.parametrize("T,H", [(5, 64), (40, 65), (700, 2048), (700, 2049), (6, 16384)])
+@pytest.mark.parametrize("layernorm", [False, True])
+def test_norms_of_few_units_of_the_least_number(ops, T, H, layernorm):
+    """Weights of 2^-133 behind a root of 2^20: a value of the stream of n / 64 is n units of 2^-149, give or take a millionth."""
+    g = torch.Generator().manual_seed(H)
+    n = torch.randint(-90, 91, (T, H), generator=g).double()
+    tops = torch.tensor([100, 128, 150, 190, 255, 64, 129]).double()[torch.arange(T) % 7]
+    n[:, 0] = tops * torch.where(torch.arange(T) % 2 == 0, 1.0, -1.0)
+    n[:, 1] = -n[:, 0]
+    if layernorm:                                  # (a mean of zero, which leaves whole units)
+        n[:, 2::2] = -n[:, 3::2] if H % 2 == 0 else -torch.cat([n[:, 3::2], torch.zeros(T, 1, dtype=torch.float64)], 1)
+    res = (n / 64).to(BF)
+    w = torch.full((H,), 2.0 ** -133, dtype=BF)
+    want = ref.norm_block(None, res, w, 2.0 ** 20, layernorm=layernorm, int8=True)
+    got = ops.norm_block(None, res.cuda(), w.cuda(), 2.0 ** 20, layernorm=layernorm, int8=True)
+    assert torch.equal(got.scale.cpu(), want.scale) and torch.equal(got.q.cpu(), want.q)
