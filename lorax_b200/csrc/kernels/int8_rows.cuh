@@ -185,13 +185,13 @@ LX_DEVICE RowScale row_scale(uint32_t magnitude) {
   return s;
 }
 
-// Quotients of rows whose scale is below 2^-128, where 1 / scale passes what 32 bits hold.  A scale of k units of 2^-149 is off from max / 127 by up to half a unit, so
-// that quotients reach 127 (k + 1/2) / k, and end at 127 as those of all other rows do.
+// Quotients of rows whose scale is below 2^-123: 1 / scale may pass what 32 bits hold, and half the scale fall between two numbers.  A scale of k units of 2^-149 is off
+// from max / 127 by up to half a unit, so that quotients reach 127 (k + 1/2) / k, and end at 127 as those of all other rows do.
+constexpr float kTinyInv = 1e37f;
 static __device__ __noinline__ int tiny_quotient(float v, float scale) { return max(-127, min(127, (int)rint((double)v / (double)scale))); }
 
-// Eight quotients as bytes.  v * inv, unrounded, is off from v / scale by 127 * 2^-24 = 7.6e-6 at most (inv's rounding; |v| is at most 127 scales and the scale's own
-// rounding, some 2^-22 of it where it is not left to tiny_quotient, so that no quotient rounds past 127), and its distance from the integer by 2^-26 more: only a
-// quotient within 1e-5 of a border may have gone to the wrong side.  Groups with such a one compare what is left with half the
+// Eight quotients as bytes.  v * inv, unrounded, is off from v / scale by 127 * 2^-24 = 7.6e-6 at most (inv's rounding; |v| is at most 127 scales and a rounding), and its
+// distance from the integer by 2^-26 more, so that only a quotient within 1e-5 of a border may have gone to the wrong side.  Groups with such a one compare what is left with half the
 // scale: r = v - q * scale is exact there, a multiple of the smaller last place of v and scale and no larger than the scale.  Rows of bf16 numbers hold ties by the
 // hundred (their quotients are 127 times ratios of 8-bit numbers), so that the comparison has to be short.
 LX_DEVICE uint2 row_quotients(const float (&f)[8], const RowScale& s) {
@@ -205,11 +205,11 @@ LX_DEVICE uint2 row_quotients(const float (&f)[8], const RowScale& s) {
   }
   if (!(far < 0.49999f)) {
     if (s.inv == 0.f) return make_uint2(0, 0);
-    if (s.inv > 3e38f) {
+    if (s.inv > kTinyInv) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) u[q] = __int_as_float(tiny_quotient(f[q], s.scale));
     } else {
-      const float half = 0.5f * s.scale;                     // (exact: the scale is 2^-128 at least)
+      const float half = 0.5f * s.scale;                     // (exact: the scale is 1e-37 at least)
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const float r = fmaf(-__fsub_rn(u[q], kWhole), s.scale, f[q]);

@@ -45,6 +45,37 @@ def test_rows_of_few_units_of_the_least_number(ops, I, copies, ring):
     assert torch.equal(pub.q, got.q) and torch.equal(pub.scale, got.scale)
 
 
+def _beside_borders():
+    """(a row's largest value, its scale, a value half a unit from the border between two steps), in units of 2^-149, the values as (a, b, e): a * b * 2^e with a and b of 8
+    bits.  The scales are odd and below 2^24 units, so that half of one lies between two numbers of 32 bits."""
+    halves = {a * b: (a, b) for a in range(1, 256) for b in range(a, 256)}
+    found = []
+    for top in sorted(m for m in halves if m >= 1 << 14):
+        for e in (13, 14, 15, 16):
+            k = ((top << (e + 1)) + 127) // 254
+            if 2500000 < k < 1 << 24 and k % 2:
+                for v in (((2 * q + 1) * k + s) // 2 for q in range(126) for s in (-1, 1)):
+                    z = (v & -v).bit_length() - 1
+                    if v >> z in halves:
+                        found.append(((*halves[top], e), k, (*halves[v >> z], z)))
+    return found
+
+
+@pytest.mark.parametrize("I", [2, 16])
+def test_values_beside_the_border_of_steps_that_are_odd(ops, I):
+    rows = _beside_borders()
+    assert len(rows) > 200
+    x = torch.zeros(len(rows), 2 * I, dtype=torch.float64)
+    for t, (top, _, v) in enumerate(rows):
+        for c, (a, b, e) in enumerate((top, v)):
+            x[t, c], x[t, I + c] = a * 2.0 ** -70, b * 2.0 ** (e - 79)
+    x = x.to(BF)
+    want = ref.act_mul_int8(x, I, "relu")
+    assert (want.scale.double() * 2.0 ** 149).tolist() == [k for _, k, _ in rows]
+    got = ops.act_mul_int8(x.cuda(), I, "relu")
+    assert torch.equal(got.scale.cpu(), want.scale) and torch.equal(got.q.cpu(), want.q)
+
+
 @pytest.mark.parametrize("T,H", [(5, 64), (40, 65), (700, 2048), (700, 2049), (6, 16384)])
 @pytest.mark.parametrize("layernorm", [False, True])
 def test_norms_of_few_units_of_the_least_number(ops, T, H, layernorm):
