@@ -558,7 +558,7 @@ class DecoderModel:
         fused GEMM -> reduce-scatter -> all-gather kernel; the rank's partial LoRA delta is reduced with it."""
         if isinstance(w, Int8Weight):
             out = self._linear(x, w, b, group, layer, inp)
-            return self.tp.all_reduce(out) if self.tp.world_size > 1 else out
+            return self.tp.all_reduce(out.contiguous()) if self.tp.world_size > 1 else out      # (the product's rows lie a multiple of 16 bytes apart)
         fused = self.tp.fused if self.tp.world_size > 1 else None
         if (fused is not None and x.is_cuda and x.shape[0] <= min(fused.MAX_TOKENS, fused.max_fused_tokens) and b is None
                 and not self.config.parallel_residual and isinstance(w, torch.Tensor)):

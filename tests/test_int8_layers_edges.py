@@ -27,3 +27,35 @@ def test_tiles_whose_number_passes_31_bits_are_refused():
     for T, N in ((MOST, MOST), (1 << 30, 1 << 28)):
         assert _plan(T, N, 16)[0] == -1001
     assert _plan(1 << 20, 1 << 20, 16)[0] == 0                   # 2^16 tiles of 16 rows by 2^13 of channels at most
+
+
+def test_rows_that_a_product_left_apart_are_summed_over_ranks_as_one_block():
+    """Results of a number of features that is no multiple of eight lie in wider rows, which a collective does not take."""
+    import torch
+
+    from lorax_b200.models.decoder import DecoderModel, Int8Weight
+    from lorax_b200.ops import reference as ref
+    taken = []
+
+    class Ops:
+        quant_rows_int8 = staticmethod(ref.quant_rows_int8)
+
+        @staticmethod
+        def gemm_int8(x, w, w_scale, bias=None, dtype=None, w_const=False):
+            T, N = x.q.shape[0], w.shape[0]
+            return ref.gemm_int8(x, w, w_scale, bias, out=torch.empty(T, (N + 7) // 8 * 8)[:, :N], dtype=dtype)
+
+    class Ranks:
+        world_size, fused = 2, None
+
+        @staticmethod
+        def all_reduce(x):
+            taken.append(x.is_contiguous())
+            return 2 * x
+    m = DecoderModel.__new__(DecoderModel)
+    m.ops, m.tp, m.adapters, m.dtype = Ops, Ranks, None, torch.float32
+    w, ws = ref.quantize_weight_int8(torch.randn(13, 32))
+    x = torch.randn(3, 32)
+    y = m._row_parallel(x, Int8Weight(w, ws), None, "o", 0, type("Step", (), dict(tok_slot=None, lora_tiles=None))())
+    assert taken == [True]
+    torch.testing.assert_close(y, 2 * ref.gemm_int8(ref.quant_rows_int8(x), w, ws, dtype=torch.float32))
