@@ -92,3 +92,35 @@ def test_norms_of_few_units_of_the_least_number(ops, T, H, layernorm):
     want = ref.norm_block(None, res, w, 2.0 ** 20, layernorm=layernorm, int8=True)
     got = ops.norm_block(None, res.cuda(), w.cuda(), 2.0 ** 20, layernorm=layernorm, int8=True)
     assert torch.equal(got.scale.cpu(), want.scale) and torch.equal(got.q.cpu(), want.q)
+
+
+# ------------------------------------------------------------------------------------------------ other rows, forms and plans
+def _plan(T, N, K, clusters, sms):
+    import ctypes
+    out = (ctypes.c_int * 4)()
+    assert native.load().lx_gemm_int8_plan(T, N, K, sms, (ctypes.c_int * 4)(*clusters), out) == 0
+    return tuple(out)
+
+
+def _clusters():
+    """Clusters of 1 to 4 pairs that run at the same time here, and SMs."""
+    lib = native.load()
+    return tuple(lib.lx_gemm_int8_clusters(p) for p in (1, 2, 3, 4)), native.workspace().num_sms
+
+
+SIZES = [(1, 6144, 4096), (64, 4096, 14336), (256, 4096, 14336), (300, 1024, 8192), (512, 4096, 14336), (700, 4096, 4096), (1500, 2050, 1030), (33, 256, 512)]
+
+
+def test_plans_go_by_the_clusters_that_the_device_runs(ops):
+    clusters, sms = _clusters()
+    assert all(0 <= 2 * p * n <= sms for p, n in enumerate(clusters, 1)) and clusters[0] > 0 and sorted(clusters, reverse=True) == list(clusters)
+    shared = 0
+    for T, N, K in SIZES + [(t, n, k) for t in (40, 130, 260, 520, 1030) for n in (256, 1000, 4096, 6144) for k in (512, 4096, 14336)]:
+        pairs, bn, parts, _ = _plan(T, N, K, clusters, sms)
+        assert pairs <= clusters[0]
+        if pairs and parts > 1:
+            shared += 1
+            assert -(-N // 256) * -(-T // bn) <= clusters[parts - 1]
+    assert shared
+    for bad in (0, 5, -1):
+        assert native.load().lx_gemm_int8_clusters(bad) < 0
