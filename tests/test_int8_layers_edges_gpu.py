@@ -124,3 +124,57 @@ def test_plans_go_by_the_clusters_that_the_device_runs(ops):
     assert shared
     for bad in (0, 5, -1):
         assert native.load().lx_gemm_int8_clusters(bad) < 0
+
+
+@pytest.mark.parametrize("n", [4096, 1001])
+def test_a_row_s_bytes_do_not_depend_on_other_rows_or_the_form(ops, n):
+    """Rows and activations of 700 rows (at a width of a multiple of eight by blocks that stay), and of one row and a few of them by a block per row."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = (torch.randn(700, 2 * n, generator=g, device="cuda") * 3).to(BF)
+    plain, gated = ops.quant_rows_int8(x[:, :n]), ops.act_mul_int8(x, n)
+    for a, b in ((0, 1), (3, 20), (500, 700)):
+        for whole, part in ((plain, ops.quant_rows_int8(x[a:b, :n])), (gated, ops.act_mul_int8(x[a:b], n))):
+            assert torch.equal(part.q, whole.q[a:b]) and torch.equal(part.scale, whole.scale[a:b])
+
+
+@pytest.mark.parametrize("N,K", [(4096, 4096), (1000, 1030)])
+def test_a_row_s_product_does_not_depend_on_other_rows_or_the_plan(ops, N, K):
+    g = torch.Generator(device="cuda").manual_seed(N)
+    x = ops.quant_rows_int8(torch.randn(1500, K, generator=g, device="cuda").to(BF))
+    w, ws = ref.quantize_weight_int8(torch.randn(N, K, generator=g, device="cuda"))
+    b = torch.randn(N, generator=g, device="cuda").to(BF)
+    whole = ops.gemm_int8(x, w, ws, bias=b)
+    clusters, sms = _clusters()
+    plans = {_plan(1500, N, K, clusters, sms)[:3]}
+    for a, e in ((0, 1), (3, 20), (7, 100), (500, 800)):
+        plans.add(_plan(e - a, N, K, clusters, sms)[:3])
+        part = ops.gemm_int8(ref.Int8Rows(x.q[a:e], x.scale[a:e]), w, ws, bias=b)
+        assert torch.equal(part, whole[a:e])
+    assert len(plans) >= 4
+
+
+@pytest.mark.parametrize("H,switch", [(512, False), (4096, True), (2049, True)])
+@pytest.mark.parametrize("layernorm", [False, True])
+def test_a_row_s_norm_differs_by_its_sums_order_alone(ops, H, switch, layernorm):
+    """Of 2500 rows of 4096 and of 2049 the norms come from blocks that stay, of a few rows from a block each (of 512: from a block each, always): the same stream to the bit, as
+    there is no norm in front of it, and the same result but for the order in which 32-bit sums are formed."""
+    g = torch.Generator(device="cuda").manual_seed(H)
+    T = 2500 if switch else 500
+    y, res, w, b = ((torch.randn(*s, generator=g, device="cuda")).to(BF) for s in ((T, H), (T, H), (H,), (H,)))
+    h = torch.empty_like(res)
+    whole = ops.norm_block(y, res, w, 1e-5, bias=b, layernorm=layernorm, residual_out=h)
+    for lo, hi in ((0, 1), (8, 21), (T - 30, T)):
+        part_h = torch.empty_like(res[lo:hi])
+        part = ops.norm_block(y[lo:hi], res[lo:hi], w, 1e-5, bias=b, layernorm=layernorm, residual_out=part_h)
+        assert torch.equal(part_h, h[lo:hi])
+        if not switch:
+            assert torch.equal(part, whole[lo:hi])
+            continue
+        v = h[lo:hi].double()
+        mean = v.mean(1, keepdim=True) if layernorm else 0
+        scaled = (v - mean) / ((v - mean).square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+        # a sum passes 16 values in a thread, 5 and 5 levels of a block: 26 roundings, of the mean and of half the squares' sum; the root, and three factors and the
+        # bias: 45 of 2^-24 for each of the two, the mean's of the row's largest; then a rounding to bf16 each
+        loose = 45 * 2.0 ** -24 * (scaled.abs() + (v.abs().amax(1, keepdim=True) / (v - mean).square().mean(1, keepdim=True).sqrt() * w.double().abs() if layernorm else 0))
+        want = scaled + b.double()
+        assert ((part.double() - whole[lo:hi].double()).abs() <= 2 * (2.0 ** -8 * (want.abs() + loose) + loose)).all()
