@@ -128,8 +128,8 @@ LX_DEVICE void int8_join(const Int8GemmParams& p, const int* sums, const Int8Sca
 
 // One tile a cluster, one part of its K a CTA.  Warp 0 loads, warp 1 multiplies, all (four or eight) write results.  Short steps: the weights' way from HBM is the bound, and
 // two CTAs an SM with six stages of 16 KB each keep enough of them on their way whatever the number of tiles (a persistent CTA an SM would leave the last wave
-// short): one row of 28672 x 4096 20.2 us (5.8 TB/s), 48 rows 21.3.  Narrow layers have fewer tiles than SMs: one row of 4096 x 14336 by eight CTAs a tile 12.1 us, alone 34.5.
-// Middle steps take large tiles, whose operands come from L2 at 100 bytes a nanosecond and SM: 256 rows of 4096 x 14336 20.2 us by four CTAs a tile of 256 tokens.
+// short): one row of 28672 x 4096 20.1 to 21.1 us (5.7 TB/s), 48 rows 22.3.  Narrow layers have fewer tiles than SMs: one row of 4096 x 14336 by eight CTAs a tile 12.9 us, alone 34.5.
+// Middle steps take large tiles, whose operands come from L2 at 100 bytes a nanosecond and SM: 256 rows of 4096 x 14336 20.7 us by four CTAs a tile of 256 tokens.
 __global__ void __launch_bounds__(kI8Threads, 3)
 gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -267,8 +267,8 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 // Long steps, by pairs of CTAs (cta_group::2): a tile is 256 features x up to 256 tokens, of which each CTA loads 128 rows of the weights and half of
 // the tokens, 32 KB a stage for 4 x 256 x 256 x 32 products, where one CTA on 128 x 256 takes 48 KB for half as many.  What comes in from L2 is what bounds a
 // single CTA at these sizes (some 95 bytes a nanosecond).  One part: persistent pairs, whose accumulators take turns, so that a tile's results are written while
-// the next one is multiplied.  Several: a cluster of pairs shares one tile's K, as above.  4001 rows of 28672 x 4096: 318 to 328 us (2.9 POP/s; cuBLAS's integer
-// product 292), the tensor pipe 77 % active at the 1.64 GHz that the power limit leaves, its stages waiting for 32 KB each at 80 bytes a nanosecond.
+// the next one is multiplied.  Several: a cluster of pairs shares one tile's K, as above.  4001 rows of 28672 x 4096: 318 to 332 us (2.9 POP/s; cuBLAS's integer
+// product 293 to 296), the tensor pipe 77 % active at the 1.64 GHz that the power limit leaves, its stages waiting for 32 KB each at 80 bytes a nanosecond.
 // ------------------------------------------------------------------------------------------------
 constexpr int kI8PairStages = 6;
 constexpr int kI8PairEpiWarps = 8;                // two for each quarter of the features, half of the tokens each
@@ -562,7 +562,8 @@ static Int8Plan int8_single_plan(int T, int N, int K, int bn, int parts, int num
 // What a plan costs, in ns.  A CTA's time is that of its operands' way in from L2 (112 bytes a nanosecond, 83 where all SMs work in pairs; a second CTA on an SM
 // adds three eighths) and of its tokens' results; waves of CTAs add a start, parts a join; and the weights come from HBM meanwhile, and all operands through L2: the fourth powers of both
 // times add up, so that the smaller one counts where they are near.  The constants are fitted to 7000 plans of 209 shapes (1 to 3900 rows, 144 to 28672 features,
-// K 159 to 14336): the plan of least cost is 2 % slower than the quickest one on average, over 10 % in five shapes, at worst 30 % (7.7 us where 5.9 are possible).
+// K 159 to 14336): the plan of least cost is 2 % slower than the quickest one on average, over 10 % in five shapes, at worst 30 % (7.7 us where 5.9 are possible).  On 1892 plans
+// of 100 shapes, 64 of them drawn anew: 1.7 % on average, over 10 % in five, at worst 18 % (27 rows of 1034 x 6921).
 static double int8_beside(double t, double hbm) {
   const double a = t * t, b = hbm * hbm;
   return sqrt(sqrt(a * a + b * b));

@@ -8,8 +8,9 @@ namespace lx {
 
 constexpr int kRowStages = 3;
 constexpr int kRowRing = 108 * 1024;      // bytes of a block's stages, so that two blocks share an SM
-// Rows an SM from which blocks that stay are worth it (us, a block per row and blocks that stay): 600 rows of 4096 3.9 and 3.8, 300 2.8 and 3.0; activations of 600 rows of
-// 14336 16.8 and 12.9, of 256 7.2 and 7.6.
+// Rows an SM from which blocks that stay take them.  A compromise (us, a block per row and blocks that stay).  Activations of 14336: 200 rows 8.3 and 7.3, 400 12.6 and 11.8, 592
+// 16.7 and 12.3, 4001 98 and 64; of 8192: 400 6.2 and 7.8, 592 8.1 and 8.3, 1000 11.5 and 12.6, 4001 36.3 and 36.2.  Rows as they are, of 14336: 400 6.8 and 8.5, 592 8.3 and 9.2, 1000
+// 12.5 and 14.0, 4001 42.9 and 40.8; of 4096: 592 3.3 and 3.7, 1000 5.0 and 5.6, 4001 14.4 and 13.7.
 constexpr int kRowRingRows = 4;
 
 enum RowsAct : int { kRowsPlain = -1, kRowsSilu = 0, kRowsGelu = 1, kRowsGeluTanh = 2, kRowsRelu = 3, kRowsRelu2 = 4 };
@@ -67,7 +68,7 @@ LX_DEVICE void rows_values(const RowsInt8Params& p, const __nv_bfloat16* row, in
   rows_values<ACT, M>(p, g, ACT != kRowsPlain && p.gated ? vector_fetch<M>(row + p.n, it, p.n, 0, in_up) : g, it, f, in, in_up);
 }
 
-// One block per row: for few rows, whose own chain of loads, maximum and stores is the bound (one row of 14336 3.0 us, 256 of them 7.2).  NV: groups of eight that a thread keeps in registers between the pass for the maximum and the quotients; 0: any number, read and
+// One block per row: for few rows, whose own chain of loads, maximum and stores is the bound (one row of 14336 3.0 us, 256 of them 4.9, their activations 8.8).  NV: groups of eight that a thread keeps in registers between the pass for the maximum and the quotients; 0: any number, read and
 // computed again (from L2: a row was read a moment ago).
 template <int ACT, int NV, int M>
 __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kernel(const RowsInt8Params p) {
@@ -118,8 +119,8 @@ __global__ void __launch_bounds__(NV == 4 ? kRowThreads4 : 1024) rows_int8_kerne
 }
 
 // Many rows: blocks that stay, whose next rows come by bulk copies while one is quantised; a row's values stand in registers from its maximum to its quotients,
-// so that its stage is free between the two.  Bound by instructions (issue slots 70 to 74 %, two special functions a value of silu): 4001 rows of 14336 38 us (4.5 TB/s;
-// a block per row 43), their activations 61 (4.7 TB/s; 91), 2048 of them 34 (48).
+// so that its stage is free between the two.  Bound by instructions (issue slots 70 to 74 %, two special functions a value of silu): 4001 rows of 14336 41 us (4.2 TB/s;
+// a block per row 43), their activations 63 (4.6 TB/s; 98), 2048 of them 35.5.
 template <int ACT, int NV>
 __global__ void __launch_bounds__(kRowThreads4, 2) rows_int8_ring_kernel(const RowsInt8Params p) {
   extern __shared__ __align__(128) uint8_t ring[];

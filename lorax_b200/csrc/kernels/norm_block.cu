@@ -170,11 +170,12 @@ __global__ void __launch_bounds__(M != kRowsShifted ? kRowThreads4 : NV == 1 ? k
 // ------------------------------------------------------------------------------------------------
 // Many rows: blocks that stay, with the next row of y and of the residual on its way by bulk copies (no registers, no waiting warps) while one is normed.
 // Rows are read from shared memory as often as a pass needs them, so that a thread holds the values of one row only, and the norms' weights for all rows.  4001 rows of
-// 8192: 43.5 us (6.0 TB/s: HBM), a block per row 70; in 8 bits 55 (issue slots), as layer norms 65 (four sums over the block).
+// 8192: 44 us (6.0 TB/s: HBM), a block per row 83; in 8 bits 55 (issue slots), a block per row 90; as layer norms with biases 71 (four sums over the block), a block per row 113.
 // ------------------------------------------------------------------------------------------------
 constexpr int kNormStages = 2;
-// Values of the stream an SM has to norm from which they are worth it (us, a block per row and blocks that stay): 200 rows of 4096 3.9 and 4.3, 444 6.7 and 6.3, 4001 32 and 26;
-// 148 of 8192 4.6 and 5.0, 200 7.3 and 6.3, 4001 70 and 49; 600 of 1024 3.0 and 3.7, 8192 16.4 and 14.9.
+// Values of the stream an SM has to norm from which they are worth it (us, norms on both sides, a block per row and blocks that stay).  In bf16: 1200 rows of 1024 4.3 and 4.7, 1500
+// 6.0 and 5.1; 200 of 4096 4.1 and 3.9, 300 6.0 and 5.2, 400 6.8 and 5.6; 200 of 8192 7.3 and 5.8.  In 8 bits: 4.8 and 5.1, 6.5 and 5.4; 4.4 and 4.7, 6.5 and 5.8, 7.3 and 6.2; 7.8 and
+// 6.5.  Layer norms: 5.4 and 6.3, 7.7 and 6.7; 5.1 and 5.6, 8.1 and 7.3, 9.0 and 7.6; 10.3 and 7.7; in 8 bits 6.0 and 6.5, 8.1 and 6.9; 5.5 and 6.2, 8.7 and 7.5, 9.4 and 7.8; 10.9 and 8.3.
 constexpr int kNormRingValues = 9600;
 
 template <bool LAYERNORM, int NV, bool INT8>
@@ -336,7 +337,7 @@ static int launch_norm_ring(const NormBlockParams& p, int num_sms, cudaStream_t 
 
 // Many shifted rows: blocks that stay, each on rows a multiple of eight apart, which all begin at the same distance from 16 bytes.  The norms' vectors are brought into
 // that place once, to be read from shared memory, and the next row's values are on their way while one is normed.  Bound by instructions and by the chain of a layer norm's sums: 1500
-// layer norms of 2049 with gate and biases 16.1 us, 6000 of 4097 88 (a block per row 18.2 and 123); RMS norms on both sides, 6000 of 4097, 67 (77).
+// layer norms of 2049 with gate and biases 16.4 us, 6000 of 4097 88 (a block per row 18.1 and 124); RMS norms on both sides, 6000 of 4097, 67 (77).
 constexpr int kNormVectors = 5;      // post_w, post_b, w, b, a channel's gate
 template <bool LAYERNORM>
 __global__ void __launch_bounds__(kRowShifted1, 2) norm_block_shifted_kernel(const NormBlockParams p) {
@@ -427,8 +428,9 @@ static int norm_shifted_grid(const RowShape& r, int num_sms) {
   const int fit = 65536 / (r.threads * 56), grid = num_sms * (fit < 32 ? fit : 32) / 8 * 8;
   return grid < 8 ? 8 : grid;
 }
-// Where each has two rows or more and they are wide, or the norms have several vectors (us, a block per row and blocks that stay).  RMS norms, one vector: 6000 of 1021 19.1 and
-// 20.5, of 2049 31.3 and 28.9, 1500 of 4097 17.8 and 15.7.  Layer norms on both sides, a gate: 1500 of 1021 (one or two rows each) 11.5 and 12.8, 6000 36.8 and 30.9.
+// Where each has two rows or more and they are wide, or the norms have several vectors (us, a block per row and blocks that stay).  RMS norms, one vector: 6000 of 1021 19.4 and
+// 20.9, of 1535 25.8 and 26.4, of 1791 30.4 and 28.7 (1500 9.7 and 9.9), of 2049 31.7 and 29.5 (1500 10.2 and 10.5), 1500 of 4097 17.8 and 16.1; norms on both sides, two vectors: 6000 of
+// 1021 23.5 and 25.3, of 1791 37.0 and 34.7, of 2049 38.6 and 36.3.  Layer norms on both sides, a gate: 1500 of 1021 (one or two rows each) 11.8 and 12.8, 6000 37.3 and 31.4.
 static bool norm_shifted_stays(const NormBlockParams& p, const RowShape& r, int num_sms) {
   const int kept = 1 + (p.post_w != nullptr) + (p.post_b != nullptr) + (p.b != nullptr) + (p.gate != nullptr && p.gate_h != 0 && p.gate_t == 0);
   return p.T >= 2ll * norm_shifted_grid(r, num_sms) && (p.H > 2000 || kept >= 3);

@@ -1331,7 +1331,7 @@ def check_act_mul_int8(x, inter, act, gated, out):
 
 def act_mul_int8(x, inter: int, act: str = "silu", gated: bool = True, out=None) -> Int8Rows:
     """act(gate) * up of rows [gate | up], or act(gate), in 8-bit integers with a scale for each row.  `out` [T, inter] takes the values themselves, rounded to x's
-    type."""
+    type.  (Here activations are PyTorch's in 32 bits, whose 1 + erf and 1 + tanh lose the digits of gates that are shut; the kernels keep them.)"""
     check_act_mul_int8(x, inter, act, gated, out)
     v = _act(x[:, :inter].float(), act)
     if gated:
